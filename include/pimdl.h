@@ -355,6 +355,102 @@ PIMDL_API int pimdl_attention(pimdl_ctx* ctx, const float* q, const float* k, co
                               uint32_t batch, uint32_t seq, uint32_t heads, uint32_t head_dim,
                               uint32_t in_stride, uint32_t out_stride, float scale);
 
+/* ---- attention of a window, and over a paged cache ------------------------------------------------
+ * What serving adds to the layer's attention; the reference, which always recomputes whole sequences without a
+ * mask (src/host/transformer_layer.cpp:211-230), has none of it.  Everything here takes DEVICE pointers, is queued
+ * on the context's stream and may be captured into a HIP graph (after one call outside the capture, which sizes the
+ * context's scratch); `starts`, `lengths`, tables and lists are read on the device when the kernels run, so a
+ * captured step follows them from replay to replay.
+ *
+ * A batch is PACKED: sequence b owns rows starts[b] .. starts[b + 1] - 1 of the token buffers ([batch + 1] ascending
+ * numbers; what lies beyond `tokens` is taken for `tokens`).  Rows of no sequence are neither read nor written.
+ * Heads: a row holds head h in columns h * head_dim .. + head_dim - 1, and query head h reads key head
+ * h / (heads / kv_heads), heads a multiple of kv_heads.  head_dim 1 .. 256; 32, 64, 80, 96 and 128 run on the matrix
+ * cores (given 16-byte aligned rows), other sizes on a plain kernel.  Strides are in elements.
+ *
+ * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max_j), over the keys that a query sees.  Scores, maxima,
+ * sums and accumulators are fp32.  With fp32 operands products keep fp32 accuracy (24-bit factors); with 16-bit
+ * operands p_j is rounded to that type once, before it meets v_j.  A query that sees no key, or whose scores are all
+ * -infinity, gives zeros.  Rows of K and V that no query may see (other sequences, behind a length, pages of nobody)
+ * may hold anything, infinities and NaN included. */
+typedef enum pimdl_dtype { PIMDL_F32 = 0, PIMDL_F16 = 1, PIMDL_BF16 = 2 } pimdl_dtype;
+#define PIMDL_UNLIMITED 0xffffffffu
+
+/* Attention within each sequence of the batch, which starts at position 0: position p sees key j if j <= p + right and
+ * (j + left >= p or j < sinks).  left = right = PIMDL_UNLIMITED is pimdl_attention with lengths; right = 0 is causal;
+ * `sinks` keeps the first tokens visible to all. */
+typedef struct pimdl_attention_window_desc {
+    const void *q, *k, *v;   /* [tokens][q_stride], [tokens][kv_stride] twice: column ranges of one buffer are fine */
+    void* out;               /* [tokens][out_stride]; must not overlap q, k or v */
+    const int32_t* starts;   /* [batch + 1] */
+    uint32_t batch, tokens, heads, kv_heads, head_dim;
+    uint32_t q_stride, kv_stride, out_stride;
+    uint32_t left, right, sinks;
+    uint32_t dtype;          /* pimdl_dtype of q, k, v and out */
+    float scale;
+} pimdl_attention_window_desc;
+PIMDL_API int pimdl_attention_window(pimdl_ctx* ctx, const pimdl_attention_window_desc* d);
+
+/* One layer's share of a paged cache.  Position j of sequence s lies in page tables[s][j / page_tokens], row
+ * j % page_tokens.  Positions whose page is not in 0 .. pages - 1 count as not there: nothing is read or written. */
+typedef struct pimdl_paged_cache {
+    void *k, *v;             /* [pages][kv_heads][page_tokens][head_dim] each, 16-byte aligned */
+    const int32_t* tables;   /* [seqs][table_width] */
+    const int32_t* lengths;  /* [seqs]: positions in the cache, those of the call's own tokens included */
+    uint32_t pages, page_tokens; /* page_tokens: a power of two, 16 .. 1024 */
+    uint32_t kv_heads, head_dim;
+    uint32_t seqs, table_width;
+    uint32_t dtype;          /* pimdl_dtype of the cache */
+} pimdl_paged_cache;
+
+/* Attention of the newest tokens of each sequence over its cache: token i of the n that row b of the batch has stands at
+ * position lengths[s] - n + i (s = seqs[b], or b where seqs is NULL) and sees key j if j <= that position and
+ * (j + left >= it or j < sinks).  A single new token per sequence, chunks of prompts and any mixture are one call.
+ * dtype is that of q and out: PIMDL_F32 over a cache of any type, or the cache's own 16-bit type. */
+PIMDL_API int pimdl_attention_paged(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const int32_t* seqs,
+                                    const int32_t* starts, uint32_t batch, uint32_t tokens, const void* q, void* out,
+                                    uint32_t heads, uint32_t q_stride, uint32_t out_stride, uint32_t dtype,
+                                    uint32_t left, uint32_t sinks, float scale);
+/* Writes the new tokens' keys and values ([tokens][kv_stride], rounded to nearest even to the cache's type) at those
+ * positions.  dtype: PIMDL_F32, or the cache's own 16-bit type. */
+PIMDL_API int pimdl_cache_append(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const int32_t* seqs,
+                                 const int32_t* starts, uint32_t batch, uint32_t tokens, const void* k, const void* v,
+                                 uint32_t kv_stride, uint32_t dtype);
+
+/* The pages' bookkeeping lives on the device, so that a step never waits for the host.  Page p is free where refs[p] == 0;
+ * otherwise refs[p] is the number of sequences that hold it.  A sequence holds the first ceil(length / page_tokens) entries of
+ * its table row; the others are -1.  Lists may name a sequence twice: only its first place counts; what is out of range is left
+ * out. */
+typedef struct pimdl_page_book {
+    int32_t* tables;         /* [seqs][table_width] */
+    int32_t* lengths;        /* [seqs] */
+    int32_t* refs;           /* [pages] */
+    int32_t* lacking;        /* [1]: how many pages the last reserve or fork was short of (0: done); -1: a row too short */
+    uint32_t seqs, table_width, pages, page_tokens; /* seqs <= 16384 */
+    void* const* pools;      /* HOST array of the device buffers that hold pages (K, V), each [layers][pages][page_bytes] */
+    uint32_t pool_count;     /* up to 64 */
+    uint32_t layers;
+    uint64_t page_bytes;     /* of one layer's page in one buffer; a multiple of 16 */
+} pimdl_page_book;
+
+/* Makes sequence seqs[i] counts[i] positions longer: new pages are the lowest free ones, in the list's order, then by position.
+ * If they do not suffice, or a row is too short, nothing changes but *lacking. */
+PIMDL_API int pimdl_pages_reserve(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_t* seqs, const int32_t* counts,
+                                  uint32_t n);
+/* Gives the empty sequence children[i] what parents[i] had before the call: whole pages are shared, a partly filled last page is
+ * copied into the lowest free page (in the list's order).  A child that is not empty is left out.  If the pages do not suffice,
+ * nothing changes but *lacking. */
+PIMDL_API int pimdl_pages_fork(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_t* parents, const int32_t* children,
+                               uint32_t n);
+/* Empties the sequences; pages that nobody else holds are free again. */
+PIMDL_API int pimdl_pages_free(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_t* seqs, uint32_t n);
+/* Moves the pages in use to 0 .. L - 1, L being their number: the i-th one from L on goes to the i-th free place below L.  Tables
+ * and refs follow. */
+PIMDL_API int pimdl_pages_compact(pimdl_ctx* ctx, const pimdl_page_book* book);
+/* Copies page src[i] to page dst[i] in every pool (pairs out of range are left out); tables, lengths and refs are neither read nor
+ * written and may be NULL.  No dst may be another pair's dst or src. */
+PIMDL_API int pimdl_pages_copy(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_t* src, const int32_t* dst, uint32_t n);
+
 /* ---- introspection ---------------------------------------------------------------------------
  * No reference counterpart: figures a benchmark needs to place a kernel on its roofline. */
 typedef struct pimdl_device_info {

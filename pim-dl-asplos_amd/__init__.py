@@ -20,6 +20,9 @@ CSRC = os.path.join(_HERE, "csrc")
 LUT_I8, LUT_F32 = 0, 1
 BIAS_ONCE, BIAS_TIMES_CB = 0, 1
 ACT_NONE, ACT_GELU_TANH = 0, 1
+F32, F16, BF16 = 0, 1, 2
+DTYPES = {"f32": F32, "f16": F16, "bf16": BF16}
+UNLIMITED = 0xFFFFFFFF  # of a window: no border on that side
 
 ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = -1, -2, -3
 STATUS = {0: "PIMDL_OK", -1: "PIMDL_ERR_INVALID", -2: "PIMDL_ERR_UNSUPPORTED", -3: "PIMDL_ERR_HIP",
@@ -34,7 +37,9 @@ EXPORTS = ["pimdl_init", "pimdl_destroy", "pimdl_last_error", "pimdl_set_stream"
            "pimdl_diag_mfma_error", "pimdl_amm_group_create", "pimdl_amm_group_run", "pimdl_amm_group_destroy",
            "pimdl_attention", "pimdl_amm_group_fused_cols", "pimdl_amm_group_run_fused", "pimdl_amm_run_noalloc", "pimdl_amm_set_bias",
            "pimdl_amm_create_with", "pimdl_amm_set_tuning", "pimdl_amm_get_tuning", "pimdl_lutgen_mode",
-           "pimdl_diag_mfma_error_crafted", "pimdl_amm_last_gather_kernel", "pimdl_amm_run_breakdown", "pimdl_diag_host_copy"]
+           "pimdl_diag_mfma_error_crafted", "pimdl_amm_last_gather_kernel", "pimdl_amm_run_breakdown", "pimdl_diag_host_copy",
+           "pimdl_attention_window", "pimdl_attention_paged", "pimdl_cache_append", "pimdl_pages_reserve", "pimdl_pages_fork",
+           "pimdl_pages_free", "pimdl_pages_compact", "pimdl_pages_copy"]
 NOALLOC_SCRATCH_BYTES = 8 << 20
 
 
@@ -90,6 +95,27 @@ class AmmGeometry(ctypes.Structure):
 
     def asdict(self):
         return {n: int(getattr(self, n)) for n, _ in self._fields_}
+
+
+class AttentionWindowDesc(ctypes.Structure):
+    """pimdl_attention_window_desc"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "starts")] +
+                [(n, ctypes.c_uint32) for n in ("batch", "tokens", "heads", "kv_heads", "head_dim", "q_stride", "kv_stride",
+                                                "out_stride", "left", "right", "sinks", "dtype")] + [("scale", ctypes.c_float)])
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """pimdl_paged_cache: one layer's share of a paged cache"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "tables", "lengths")] +
+                [(n, ctypes.c_uint32) for n in ("pages", "page_tokens", "kv_heads", "head_dim", "seqs", "table_width", "dtype")])
+
+
+class PageBook(ctypes.Structure):
+    """pimdl_page_book: the bookkeeping of a paged cache and the buffers that hold its pages"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("tables", "lengths", "refs", "lacking")] +
+                [(n, ctypes.c_uint32) for n in ("seqs", "table_width", "pages", "page_tokens")] +
+                [("pools", ctypes.POINTER(ctypes.c_void_p)), ("pool_count", ctypes.c_uint32), ("layers", ctypes.c_uint32),
+                 ("page_bytes", ctypes.c_uint64)])
 
 
 _lib = None
@@ -155,6 +181,15 @@ def lib():
     L.pimdl_amm_group_fused_cols.argtypes = [vp, ctypes.POINTER(u32)]
     L.pimdl_amm_group_run_fused.argtypes = [vp, vp, u32, vp]
     L.pimdl_attention.argtypes = [vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, ctypes.c_float]
+    L.pimdl_attention_window.argtypes = [vp, ctypes.POINTER(AttentionWindowDesc)]
+    L.pimdl_attention_paged.argtypes = [vp, ctypes.POINTER(PagedCacheDesc), vp, vp, u32, u32, vp, vp, u32, u32, u32, u32, u32, u32, ctypes.c_float]
+    L.pimdl_cache_append.argtypes = [vp, ctypes.POINTER(PagedCacheDesc), vp, vp, u32, u32, vp, vp, u32, u32]
+    book = ctypes.POINTER(PageBook)
+    L.pimdl_pages_reserve.argtypes = [vp, book, vp, vp, u32]
+    L.pimdl_pages_fork.argtypes = [vp, book, vp, vp, u32]
+    L.pimdl_pages_free.argtypes = [vp, book, vp, u32]
+    L.pimdl_pages_compact.argtypes = [vp, book]
+    L.pimdl_pages_copy.argtypes = [vp, book, vp, vp, u32]
     for name in EXPORTS:
         if name != "pimdl_last_error":
             getattr(L, name).restype = ctypes.c_int
@@ -294,6 +329,14 @@ class Context:
         self._check(lib().pimdl_attention(self._h, ctypes.c_void_p(q), ctypes.c_void_p(k), ctypes.c_void_p(v),
                                           ctypes.c_void_p(out), batch, seq, heads, head_dim, in_stride, out_stride,
                                           ctypes.c_float(scale)))
+
+    def attention_window_ptr(self, q, k, v, out, starts, batch, tokens, heads, kv_heads, head_dim, q_stride, kv_stride, out_stride,
+                             left, right, sinks, scale, dtype=F32):
+        """Device addresses; attention within each sequence of a packed batch (sequence b owns rows starts[b] .. starts[b + 1] - 1)
+        where position p sees key j if j <= p + right and (j + left >= p or j < sinks); UNLIMITED opens a side.  Strides in elements."""
+        d = AttentionWindowDesc(q, k, v, out, starts, batch, tokens, heads, kv_heads, head_dim, q_stride, kv_stride, out_stride, left, right,
+                                sinks, dtype, scale)
+        self._check(lib().pimdl_attention_window(self._h, ctypes.byref(d)))
 
     def amm_group(self, amms):
         return AmmGroup(self, amms)

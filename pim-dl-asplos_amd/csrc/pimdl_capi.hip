@@ -80,7 +80,7 @@ int allow_dynamic_lds(Ctx* ctx, const void* kernel, int lds_bytes, const char* w
     return rc;
 }
 
-static bool is_device_ptr(const void* p)
+bool is_device_ptr(const void* p)
 {
     hipPointerAttribute_t attr;
     memset(&attr, 0, sizeof(attr));
@@ -125,7 +125,9 @@ static int ensure(Ctx* ctx, T** buf, size_t* have, size_t need, const char* what
     return PIMDL_OK;
 }
 
-static int activate(Ctx* ctx) { return hip_check(ctx, hipSetDevice(ctx->device), "hipSetDevice"); }
+int activate(Ctx* ctx) { return hip_check(ctx, hipSetDevice(ctx->device), "hipSetDevice"); }
+
+int ensure_scratch(Ctx* ctx, char** buf, size_t* have, size_t need, const char* what) { return ensure(ctx, buf, have, need, what); }
 
 // input/output staging common to run / run_debug / the two halves
 struct IoPlan {
@@ -553,7 +555,6 @@ static void move_lut_onehot(const int8_t* from, const AmmGeom& a, int8_t* to, co
 
 using namespace pimdl;
 
-struct pimdl_ctx : Ctx {};
 struct pimdl_amm : Amm {};
 // Operators that read the same input rows, searched by one launch over all their codebooks.
 struct pimdl_amm_group {
@@ -700,6 +701,8 @@ int pimdl_init(int device, pimdl_ctx** out)
     ctx->d_tmp = nullptr; ctx->tmp_bytes = 0;
     ctx->d_lutgen = nullptr; ctx->lutgen_bytes = 0;
     ctx->d_cent = nullptr; ctx->cent_bytes = 0;
+    ctx->d_attn = nullptr; ctx->attn_bytes = 0;
+    ctx->d_book = nullptr; ctx->book_bytes = 0;
     ctx->d_static_scratch = nullptr;
     ctx->pipe = nullptr;
     for (auto& ev : ctx->ev) ev = nullptr;
@@ -737,6 +740,8 @@ int pimdl_destroy(pimdl_ctx* ctx)
     (void)hipFree(ctx->d_tmp);
     (void)hipFree(ctx->d_lutgen);
     (void)hipFree(ctx->d_cent);
+    (void)hipFree(ctx->d_attn);
+    (void)hipFree(ctx->d_book);
     for (void* p : ctx->retired) (void)hipFree(p);
     for (auto& ev : ctx->ev)
         if (ev) (void)hipEventDestroy(ev);

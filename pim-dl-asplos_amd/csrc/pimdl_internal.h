@@ -151,6 +151,10 @@ struct Ctx {
     size_t lutgen_bytes;
     float* d_cent;       // centroids of a context-level pimdl_index_calculation call
     size_t cent_bytes;
+    char* d_attn;        // partial results of attention whose keys are split over workgroups
+    size_t attn_bytes;
+    char* d_book;        // lists of pages that the page book's kernels hand to each other
+    size_t book_bytes;
     hipEvent_t ev[4];
     HostPipe* pipe;      // created by the first call that hands over a host buffer
     std::mutex host_mutex;  // held by a call while it uses `pipe` or d_lutgen: table construction may run beside another thread's calls
@@ -160,6 +164,11 @@ int set_error(Ctx* ctx, int code, const char* fmt, ...);
 int hip_check(Ctx* ctx, hipError_t e, const char* what);
 // Raises a kernel's dynamic LDS limit to `lds_bytes`, once per (device of ctx, kernel); safe from several threads.
 int allow_dynamic_lds(Ctx* ctx, const void* kernel, int lds_bytes, const char* what);
+
+bool is_device_ptr(const void* p);
+int activate(Ctx* ctx);  // makes the context's device the current one
+// grow-only scratch of the context; refused while its stream is being captured
+int ensure_scratch(Ctx* ctx, char** buf, size_t* have, size_t need, const char* what);
 
 // kernels (launchers validate nothing: callers have already checked shapes against AmmGeom)
 // x_cols != 0: the geometry's codebooks are those of several operators that all read rows of x_cols
@@ -234,3 +243,5 @@ bool plan_side_by_side(const Amm& first, uint32_t count, uint32_t max_n, uint32_
 bool apply_runtime_tuning(AmmGeom* g, const pimdl_amm_tuning& t, std::string* why);
 
 }  // namespace pimdl
+
+struct pimdl_ctx : pimdl::Ctx {};

@@ -1,0 +1,694 @@
+"""Attention over a window and over a paged cache, the cache's writes and its pages, on the GPU, against plain float64 (attention) and
+a sequential model of the book (pages).
+
+Tolerances of attention.  With u = 2^-24: a score is a sum of head_dim products of 24-bit factors in fp32, scaled, so it is off by at most
+ds = (head_dim + 8) u scale sum|q||k|, and a probability by a factor of up to exp(2 ds) (its own score and the maximum's), on top
+of 8 u for the exponential.  Numerator and denominator are sums that pass at most keys / 16 + 64 additions.  So out is off by
+(2 expm1(2 ds) + 16 u + 2 (keys / 16 + 64) u) sum p|v| / sum p.  Types of 16 bits: p is rounded once (half a step of it, relative, in
+the numerator), and so is the output."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from __graft_entry__ import load_package
+
+pimdl = load_package()
+from pim_dl_asplos_amd import kvcache as K  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+HALF = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = pimdl.Context(0)
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield c
+    c.close()
+
+
+def starts_of(counts):
+    return torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device="cuda")
+
+
+def gen_of(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(gen, *shape, dtype="f32", scale=1.0):
+    return (torch.randn(shape, device="cuda", generator=gen) * scale).to(TYPES[dtype])
+
+
+def reference(q, k, v, pos0, left, right, sinks, scale, u=U):
+    """q [n][heads][hd], k and v [keys][kv_heads][hd], query i at position pos0 + i: (out, how far fp32 may be off, sum p|v| / sum p)."""
+    n, h, hd = q.shape
+    keys, kv, _ = k.shape
+    q, k, v = (x.double() for x in (q, k, v))
+    p = torch.arange(pos0, pos0 + n, device=q.device)[:, None]
+    j = torch.arange(keys, device=q.device)[None, :]
+    seen = (j <= p + right) & ((j + left >= p) | (j < sinks))
+    out, off, mass = (torch.zeros((n, h, hd), dtype=torch.float64, device=q.device) for _ in range(3))
+    for i in range(h):
+        kh, vh = k[:, i // (h // kv)], v[:, i // (h // kv)]
+        s = (q[:, i] @ kh.t().contiguous()) * scale
+        ds = (hd + 8) * u * abs(scale) * (q[:, i].abs() @ kh.abs().t().contiguous())
+        s = torch.where(seen, s, -math.inf)
+        some = seen.any(-1, keepdim=True)
+        m = torch.where(some, s.amax(-1, keepdim=True) if keys else torch.zeros_like(s[:, :0].sum(-1, keepdim=True)), 0.0)
+        e = torch.exp(s - m)
+        total = torch.where(some, e.sum(-1, keepdim=True), 1.0)
+        d = torch.where(seen, ds, 0.0).amax(-1, keepdim=True) if keys else 0.0
+        out[:, i] = (e / total) @ torch.where(torch.isfinite(vh), vh, 0.0)
+        mass[:, i] = (e / total) @ torch.where(torch.isfinite(vh), vh, 0.0).abs()
+        off[:, i] = (2 * torch.expm1(torch.as_tensor(2 * d)) + 16 * u + 2 * (keys / 16 + 64) * u) * mass[:, i]
+    return out, off, mass
+
+
+def check(got, want, off, mass, dtype):
+    tol = off + HALF[dtype] * mass + HALF[dtype] * want.abs() + 2.0 ** -126
+    bad = (got.double() - want).abs() > tol
+    assert not torch.isnan(got).any()
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}, worst {float(((got.double() - want).abs() / tol).max()):.2f} of the tolerance"
+
+
+# ---------------------------------------------------------------------------------------------- window
+
+def window(ctx, q, k, v, out, counts, heads, kv, hd, left, right, sinks, dtype, tokens=None, scale=None):
+    starts = starts_of(counts)
+    ctx.attention_window_ptr(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), starts.data_ptr(), len(counts), q.shape[0] if tokens is None else tokens,
+                             heads, kv, hd, q.stride(0), k.stride(0), out.stride(0), left, right, sinks, 1 / math.sqrt(hd) if scale is None else scale,
+                             pimdl.DTYPES[dtype])
+
+
+def window_case(ctx, seed, counts, heads, kv, hd, left, right, sinks, dtype, behind=3, scale=None, size=1.0):
+    gen = gen_of(seed)
+    n, d, kd = sum(counts), heads * hd, kv * hd
+    extra = 8 if hd % 8 == 0 else 3  # columns of the rows that belong to nobody
+    buf = randn(gen, n + behind, d + 2 * kd + extra, dtype=dtype, scale=size)
+    buf[n:] = float("nan")
+    buf[:, d + 2 * kd:] = float("inf")
+    out = torch.full((n + behind, d + extra), -5.0, device="cuda", dtype=TYPES[dtype])
+    q, k, v = buf[:, :d], buf[:, d:d + kd], buf[:, d + kd:]
+    window(ctx, q, k, v, out, counts, heads, kv, hd, left, right, sinks, dtype, scale=scale)
+    torch.cuda.synchronize()
+    assert (out[n:] == -5.0).all() and (out[:, d:] == -5.0).all()  # rows behind the last sequence, columns behind the heads
+    at = 0
+    for c in counts:
+        rows = slice(at, at + c)
+        want, off, mass = reference(q[rows].reshape(c, heads, hd), k[rows].reshape(c, kv, hd), buf[rows, d + kd:d + 2 * kd].reshape(c, kv, hd), 0,
+                                    left, right, sinks, 1 / math.sqrt(hd) if scale is None else scale)
+        check(out[rows, :d].reshape(c, heads, hd), want, off, mass, dtype)
+        at += c
+
+
+UNL = pimdl.UNLIMITED
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("counts,heads,kv,hd,left,right,sinks", [
+    ([1], 1, 1, 64, 0, 0, 0),                       # one token sees itself
+    ([5, 1, 0, 70], 2, 2, 64, UNL, UNL, 0),         # the whole sequence; one without tokens
+    ([128], 12, 12, 64, 32, 32, 1),
+    ([129, 31, 64], 4, 2, 64, UNL, 0, 0),           # causal, shared key heads
+    ([300, 17], 4, 1, 128, 100, 0, 4),              # window and sinks, causal
+    ([257], 2, 2, 80, 20, 300, 0),                  # far to the right
+    ([200, 33], 6, 2, 32, 0, 0, 3),                 # nothing but itself and the sinks
+    ([65, 64, 63], 3, 3, 96, 40, 7, 40),            # sinks that reach into the window
+    ([500], 8, 2, 128, 63, 64, 70),
+    ([90, 3], 2, 1, 40, 30, 30, 2),                 # head sizes of the plain kernel
+    ([50], 3, 3, 17, UNL, 0, 0),
+    ([40], 1, 1, 256, 12, 12, 0),
+    ([700, 1100], 2, 2, 64, 129, 0, 1),
+])
+def test_window_against_float64(ctx, dtype, counts, heads, kv, hd, left, right, sinks):
+    window_case(ctx, sum(counts) + hd, counts, heads, kv, hd, left, right, sinks, dtype)
+
+
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 95, 96, 127, 128, 129, 191, 255, 256, 257])
+@pytest.mark.parametrize("left,right,sinks", [(UNL, UNL, 0), (UNL, 0, 0), (33, 0, 5), (31, 31, 0), (64, 1, 33)])
+def test_window_at_the_edges_of_tiles(ctx, n, left, right, sinks):
+    window_case(ctx, n, [n, 3, n], 2, 1, 64, left, right, sinks, "bf16")
+    window_case(ctx, n, [n], 1, 1, 64, left, right, sinks, "f32")
+
+
+@pytest.mark.parametrize("size,scale", [(1e-12, 1e24), (1e3, 1e-7), (30.0, 0.125), (1.0, -0.5), (1.0, 0.0)])
+def test_window_of_small_and_large_values_in_fp32(ctx, size, scale):
+    window_case(ctx, 11, [140, 20], 2, 2, 64, UNL, 0, 0, "f32", size=size, scale=scale)
+
+
+def test_window_token_count_cuts_the_batch(ctx):
+    """Numbers in `starts` beyond `tokens` are taken for `tokens`, negative ones for 0: nothing past the buffers is touched."""
+    gen = gen_of(5)
+    q, k, v = (randn(gen, 40, 64) for _ in range(3))
+    out = torch.full((40, 64), -5.0, device="cuda")
+    starts = torch.tensor([-7, 10, 1 << 30], dtype=torch.int32, device="cuda")
+    ctx.attention_window_ptr(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), starts.data_ptr(), 2, 24, 1, 1, 64, 64, 64, 64, UNL, 0, 0, 0.125, 0)
+    torch.cuda.synchronize()
+    assert (out[24:] == -5.0).all()
+    for a, b in ((0, 10), (10, 24)):
+        want, off, mass = reference(q[a:b, None], k[a:b, None], v[a:b, None], 0, UNL, 0, 0, 0.125)
+        check(out[a:b, None], want, off, mass, "f32")
+
+
+def test_window_of_scores_without_a_finite_one_and_of_infinite_keys_elsewhere(ctx):
+    """All scores -infinity: zeros.  An infinite key or value in a place that the window hides, or in another sequence, changes nothing."""
+    for dtype in ("f32", "bf16"):
+        gen = gen_of(6)
+        q, k, v = (randn(gen, 300, 64, dtype=dtype) for _ in range(3))
+        out = torch.zeros(300, 64, device="cuda", dtype=TYPES[dtype])
+        window(ctx, q, k, v, out, [100, 200], 1, 1, 64, 7, 0, 0, dtype)
+        plain = out.clone()
+        k[40], v[40] = float("inf"), float("nan")  # of sequence 0: seen by its positions 40 .. 47 only
+        out.zero_()
+        window(ctx, q, k, v, out, [100, 200], 1, 1, 64, 7, 0, 0, dtype)
+        torch.cuda.synchronize()
+        assert torch.equal(out[100:], plain[100:])
+        hidden = [i for i in range(100) if not 40 <= i <= 47]
+        assert torch.equal(out[hidden], plain[hidden])
+        q.fill_(1.0)
+        k.fill_(-math.inf)
+        v = torch.randn_like(v)
+        window(ctx, q, k, v, out, [100, 200], 1, 1, 64, 7, 0, 0, dtype)
+        torch.cuda.synchronize()
+        assert (out == 0).all()
+
+
+# ---------------------------------------------------------------------------------------------- paged
+
+class Filled:
+    """A cache with sequences of the given lengths on pages in random order; everything that no sequence holds is NaN or infinite."""
+
+    def __init__(self, ctx, seed, lengths, kv, hd, page_tokens, dtype, layers=1, spare=3, seqs=None, width=None):
+        gen = gen_of(seed)
+        need = [-(-n // page_tokens) for n in lengths]
+        pages = sum(need) + spare
+        seqs, width = seqs or len(lengths), width or max(need + [1])
+        order = np.random.default_rng(seed).permutation(pages)
+        shape = (layers, pages, kv, page_tokens, hd)
+        k, v = (torch.full(shape, bad, device="cuda", dtype=TYPES[dtype]) for bad in (float("nan"), float("inf")))
+        tables = torch.full((seqs, width), -1, dtype=torch.int32)
+        refs = torch.zeros(pages, dtype=torch.int32)
+        self.rows, at = [], 0
+        for s, n in enumerate(lengths):
+            mine = torch.from_numpy(order[at:at + need[s]].copy()).long()
+            at += need[s]
+            tables[s, :need[s]] = mine.int()
+            refs[mine] = 1
+            kk, vv = (randn(gen, layers, n, kv, hd, dtype=dtype) for _ in range(2))
+            self.rows.append((kk, vv))
+            place = torch.arange(n)
+            pg, slot = mine[place // page_tokens].cuda(), (place % page_tokens).cuda()
+            for pool, x in ((k, kk), (v, vv)):
+                for layer in range(layers):
+                    pool[layer, pg, :, slot] = x[layer]
+        all_lengths = torch.zeros(seqs, dtype=torch.int32)
+        all_lengths[:len(lengths)] = torch.tensor(lengths, dtype=torch.int32)
+        self.cache = K.PagedCache.over(ctx, pimdl, k, v, tables.cuda(), all_lengths.cuda(), refs.cuda())
+
+
+def paged_case(ctx, seed, counts, lengths, heads, kv, hd, page_tokens, dtype, cache, left=None, sinks=0, layer=0, layers=1):
+    f = Filled(ctx, seed, lengths, kv, hd, page_tokens, cache, layers=layers)
+    gen, n = gen_of(seed + 1), sum(counts)
+    wide = randn(gen, n + 2, heads * hd + 16, dtype=dtype)
+    wide[n:] = float("nan")
+    q = wide[:n, :heads * hd]
+    out = torch.full((n + 2, heads * hd), -5.0, device="cuda", dtype=TYPES[dtype])
+    f.cache.attend(layer, q, out[:n], starts_of(counts), heads, left=left, sinks=sinks)
+    torch.cuda.synchronize()
+    assert (out[n:] == -5.0).all()
+    at = 0
+    for s, c in enumerate(counts):
+        k, v = (x[layer] for x in f.rows[s])
+        want, off, mass = reference(q[at:at + c].reshape(c, heads, hd), k, v, lengths[s] - c, UNL if left is None else left, 0, sinks, 1 / math.sqrt(hd))
+        check(out[at:at + c].reshape(c, heads, hd), want, off, mass, dtype)
+        at += c
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("counts,lengths,heads,kv,hd,page_tokens,left,sinks", [
+    ([1], [1], 1, 1, 64, 16, None, 0),                                       # the first token of all
+    ([1, 1, 1], [777, 16, 17], 12, 12, 64, 16, None, 0),                     # single tokens
+    ([1] * 5, [100, 2, 1500, 64, 63], 8, 2, 128, 32, None, 0),               # ... of shared key heads
+    ([3, 1, 2], [40, 300, 2], 8, 1, 80, 16, None, 0),                        # a few at a time
+    ([130, 1, 64, 0, 7], [700, 65, 64, 9, 130], 4, 2, 64, 64, None, 0),      # chunks and single tokens in one batch; a row without tokens
+    ([200], [1200], 4, 4, 96, 128, None, 0),
+    ([1, 40], [900, 500], 4, 2, 128, 16, 100, 4),                            # window and sinks
+    ([1, 33], [600, 700], 6, 3, 32, 16, 0, 1),
+    ([9, 3], [4, 0], 2, 2, 64, 16, None, 0),                                 # more tokens than keys: the first ones see nothing
+    ([5, 1], [70, 33], 2, 1, 24, 16, 20, 3),                                 # the plain kernel
+    ([1, 2], [50, 61], 40, 1, 64, 16, None, 0),                              # 40 query heads to a key head
+])
+def test_paged_against_float64(ctx, dtype, cache, counts, lengths, heads, kv, hd, page_tokens, left, sinks):
+    paged_case(ctx, sum(lengths) + hd, counts, lengths, heads, kv, hd, page_tokens, dtype, cache, left, sinks)
+
+
+@pytest.mark.parametrize("length", [1, 15, 16, 17, 31, 32, 33, 47, 48, 63, 64, 65, 127, 128, 129, 255, 256, 257, 1023, 1025])
+def test_paged_single_tokens_at_the_edges_of_pages_and_tiles(ctx, length):
+    paged_case(ctx, length, [1, 1], [length, 2 * length], 4, 2, 64, 16, "f32", "f16")
+    paged_case(ctx, length, [1, 1], [length, 3], 16, 2, 128, 64, "bf16", "bf16", left=length // 2, sinks=2)
+    paged_case(ctx, length, [min(length, 37)], [length], 4, 2, 64, 16, "bf16", "bf16")
+
+
+def test_paged_long_contexts_are_split_and_joined(ctx):
+    """Few rows over many keys; and two calls with different splits one after the other."""
+    paged_case(ctx, 1, [1, 1], [40000, 5], 4, 2, 64, 16, "f16", "f16")
+    paged_case(ctx, 2, [1], [70001], 8, 1, 128, 64, "bf16", "bf16", left=50000, sinks=4)
+    paged_case(ctx, 3, [150], [20000], 2, 1, 64, 32, "f32", "f32")
+    paged_case(ctx, 4, [1], [9000], 2, 2, 80, 16, "f32", "bf16")
+
+
+def test_paged_second_layer_and_listed_sequences(ctx):
+    """Another layer's pages; the rows of the batch are those sequences that `seqs` names, one of them not there."""
+    paged_case(ctx, 7, [2, 1], [100, 50], 4, 2, 64, 16, "bf16", "bf16", layer=2, layers=3)
+    f = Filled(ctx, 8, [64, 100, 7], 2, 64, 16, "f16")
+    q = randn(gen_of(9), 6, 4 * 64)
+    out = torch.full_like(q, -5.0)
+    f.cache.attend(0, q, out, starts_of([2, 1, 3]), 4, seqs=torch.tensor([2, 77, 1], dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    assert (out[2] == 0).all()  # no such sequence: no keys
+    for rows, s, n in ((slice(0, 2), 2, 7), (slice(3, 6), 1, 100)):
+        c = rows.stop - rows.start
+        want, off, mass = reference(q[rows].reshape(c, 4, 64), f.rows[s][0][0], f.rows[s][1][0], n - c, UNL, 0, 0, 0.125)
+        check(out[rows].reshape(c, 4, 64), want, off, mass, "f32")
+
+
+@pytest.mark.parametrize("counts", [[1], [40]])
+def test_paged_positions_without_a_page_are_not_there(ctx, counts):
+    """Entries of the table that are -1 or out of range, and a length past the row: nothing is read for them."""
+    n, c = 200, counts[0]
+    for hd, dtype in ((64, "bf16"), (24, "f32"), (128, "f32")):
+        f = Filled(ctx, 12, [n], 1, hd, 16, dtype, width=13)
+        gone = [1, 4, 11]  # pages of the sequence
+        f.cache.tables[0, 1], f.cache.tables[0, 4], f.cache.tables[0, 11] = -1, 1 << 30, f.cache.k.shape[1]
+        f.cache.lengths[0] = 1 << 30  # the row holds 13 pages
+        f.cache.tables[0, 12] = -3
+        q = randn(gen_of(13), c, 2 * hd, dtype=dtype)
+        out = torch.zeros_like(q)
+        f.cache.attend(0, q, out, starts_of(counts), 2)
+        torch.cuda.synchronize()
+        keep = [j for j in range(n) if j // 16 not in gone and j < 192]
+        k, v = f.rows[0][0][0], f.rows[0][1][0]
+        for i in range(c):
+            p = 13 * 16 - c + i
+            js = [j for j in keep if j <= p]
+            want, off, mass = reference(q[i:i + 1].reshape(1, 2, hd), k[js], v[js], len(js) - 1, UNL, 0, 0, 1 / math.sqrt(hd))
+            check(out[i:i + 1].reshape(1, 2, hd), want, off, mass, dtype)
+
+
+# ---------------------------------------------------------------------------------------------- append
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("counts,lengths,kv,hd,page_tokens", [([1], [1], 1, 64, 16), ([1, 1, 1], [1, 16, 17], 12, 64, 16), ([70, 0, 33], [70, 5, 100], 2, 80, 32),
+                                                              ([20, 3], [30, 2], 3, 17, 16), ([200], [333], 8, 128, 64)])
+def test_append_rounds_and_places(ctx, dtype, cache, counts, lengths, kv, hd, page_tokens):
+    f = Filled(ctx, sum(lengths), lengths, kv, hd, page_tokens, cache)
+    c = f.cache
+    n, gen = sum(counts), gen_of(3)
+    buf = randn(gen, n, 2 * kv * hd + 5, dtype=dtype, scale=3.0)
+    k, v = buf[:, :kv * hd], buf[:, kv * hd:2 * kv * hd]
+    want_k, want_v = c.k.clone(), c.v.clone()
+    at = 0
+    for s, m in enumerate(counts):
+        for i in range(m):
+            pos = lengths[s] - m + i
+            if pos >= 0:  # (more tokens than positions: the first ones have no place)
+                page = int(c.tables[s, pos // page_tokens])
+                want_k[0, page, :, pos % page_tokens] = k[at + i].reshape(kv, hd).to(TYPES[cache])
+                want_v[0, page, :, pos % page_tokens] = v[at + i].reshape(kv, hd).to(TYPES[cache])
+        at += m
+    c.append(0, k, v, starts_of(counts))
+    torch.cuda.synchronize()
+    for got, want in ((c.k, want_k), (c.v, want_v)):
+        bits = torch.int32 if cache == "f32" else torch.int16
+        assert torch.equal(got.view(bits), want.view(bits))
+
+
+def test_append_skips_what_has_no_page(ctx):
+    f = Filled(ctx, 3, [40], 1, 64, 16, "f16", width=3)
+    f.cache.tables[0, 1], f.cache.tables[0, 2] = -1, 1 << 20
+    before = f.cache.k.clone()
+    x = randn(gen_of(1), 40, 64)
+    f.cache.append(0, x, x, starts_of([40]))
+    torch.cuda.synchronize()
+    page = int(f.cache.tables[0, 0])
+    before[0, page, 0] = x[:16].half()
+    assert torch.equal(f.cache.k.view(torch.int16), before.view(torch.int16))
+
+
+# ---------------------------------------------------------------------------------------------- pages
+
+class Model:
+    """The book as a sequential program keeps it."""
+
+    def __init__(self, cache):
+        self.tables, self.lengths, self.refs = (t.cpu().numpy().astype(np.int64) for t in (cache.tables, cache.lengths, cache.refs))
+        self.k, self.v = cache.k.cpu().clone(), cache.v.cpu().clone()
+        self.pt, self.lacking = cache.page_tokens, 0
+
+    def held(self, n):
+        return -(-int(n) // self.pt)
+
+    def first(self, items, ok):
+        seen, out = set(), []
+        for i, s in enumerate(items):
+            if ok(s) and s not in seen:
+                seen.add(s)
+                out.append(i)
+        return out
+
+    def inside(self, s):
+        return 0 <= s < len(self.lengths)
+
+    def reserve(self, seqs, counts):
+        plan = [(seqs[i], max(0, counts[i])) for i in self.first(seqs, self.inside)]
+        if any(self.held(self.lengths[s] + c) > self.tables.shape[1] for s, c in plan):
+            self.lacking = -1
+            return
+        need = [self.held(self.lengths[s] + c) - self.held(self.lengths[s]) for s, c in plan]
+        free = [p for p in range(len(self.refs)) if self.refs[p] == 0]
+        self.lacking = max(0, sum(need) - len(free))
+        if self.lacking:
+            return
+        for (s, c), m in zip(plan, need):
+            at = self.held(self.lengths[s])
+            for j in range(m):
+                self.tables[s, at + j] = free[0]
+                self.refs[free.pop(0)] = 1
+            self.lengths[s] += c
+
+    def fork(self, parents, children):
+        entries = [i for i in self.first(children, self.inside) if self.inside(parents[i]) and self.lengths[children[i]] == 0]
+        part = [i for i in entries if self.lengths[parents[i]] % self.pt]
+        free = [p for p in range(len(self.refs)) if self.refs[p] == 0]
+        self.lacking = max(0, len(part) - len(free))
+        if self.lacking:
+            return
+        before, lens = self.tables.copy(), self.lengths.copy()
+        for i in entries:
+            p, c = parents[i], children[i]
+            whole = lens[p] // self.pt
+            self.tables[c, :whole] = before[p, :whole]
+            self.refs[before[p, :whole]] += 1
+            if lens[p] % self.pt:
+                page = free.pop(0)
+                self.tables[c, whole] = page
+                self.refs[page] = 1
+                for pool in (self.k, self.v):
+                    pool[:, page] = pool[:, before[p, whole]]
+            self.lengths[c] = lens[p]
+
+    def free(self, seqs):
+        for i in self.first(seqs, self.inside):
+            row = self.tables[seqs[i]]
+            self.refs[row[row >= 0]] -= 1
+            row[:] = -1
+            self.lengths[seqs[i]] = 0
+
+    def compact(self):
+        live = [p for p in range(len(self.refs)) if self.refs[p]]
+        holes = [p for p in range(len(live)) if not self.refs[p]]
+        for src, dst in zip([p for p in live if p >= len(live)], holes):
+            for pool in (self.k, self.v):
+                pool[:, dst] = pool[:, src]
+            self.tables[self.tables == src] = dst
+            self.refs[dst], self.refs[src] = self.refs[src], 0
+
+    def same(self, cache):
+        torch.cuda.synchronize()
+        for name in ("tables", "lengths", "refs"):
+            got = getattr(cache, name).cpu().numpy()
+            assert np.array_equal(got, getattr(self, name)), (name, got, getattr(self, name))
+        assert int(cache.lacking) == self.lacking
+        for name in ("k", "v"):
+            assert torch.equal(getattr(cache, name).cpu(), getattr(self, name)), name
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def small_cache(ctx, seed, pages=40, seqs=9, width=8, page_tokens=16, layers=2, dtype="f16"):
+    c = K.PagedCache(ctx, pimdl, layers, pages, 2, 16, page_tokens, dtype, seqs, width * page_tokens)
+    for pool in (c.k, c.v):
+        pool.copy_(randn(gen_of(seed), *pool.shape, dtype=dtype))
+    return c
+
+
+def test_book_against_a_sequential_model(ctx):
+    """A long random life of a cache: every call against the model, over-full ones, sequences listed twice and out of range among them."""
+    rng = np.random.default_rng(0)
+    cache = small_cache(ctx, 1)
+    model = Model(cache)
+    seen = set()
+    for step in range(250):
+        op = rng.choice(["reserve", "reserve", "fork", "free", "compact"])
+        n = int(rng.integers(0, 6))
+        a, b = (rng.integers(-1, 10, n).tolist() for _ in range(2))
+        if op == "reserve":
+            counts = rng.integers(-3, 50, n).tolist()
+            cache.reserve(ints(*a), ints(*counts))
+            model.reserve(a, counts)
+        elif op == "fork":
+            cache.fork(ints(*a), ints(*b))
+            model.fork(a, b)
+        elif op == "free":
+            cache.free(ints(*a))
+            model.free(a)
+        else:
+            cache.compact()
+            model.compact()
+        seen.add((op, model.lacking > 0, model.lacking < 0))
+        model.same(cache)
+    assert {("reserve", True, False), ("reserve", False, True), ("fork", False, False)} <= seen
+
+
+def test_fork_without_enough_pages_changes_nothing(ctx):
+    cache = small_cache(ctx, 2, pages=4, seqs=6, width=4)
+    model = Model(cache)
+    for a, c in (([0, 1], [33, 5]), ):
+        cache.reserve(ints(*a), ints(*c))
+        model.reserve(a, c)
+    model.same(cache)
+    cache.fork(ints(0, 1), ints(2, 3))  # two last pages, none free
+    model.fork([0, 1], [2, 3])
+    assert model.lacking == 2
+    model.same(cache)
+
+
+def test_book_of_many_pages_and_sequences(ctx):
+    """More pages than one step of the scans covers, lists longer than a workgroup, rows of more pages than a block."""
+    pages, seqs, width = 70000, 3000, 1500
+    cache = K.PagedCache(ctx, pimdl, 1, pages, 1, 8, 16, "f16", seqs, width * 16)
+    cache.k.copy_(torch.arange(pages, device="cuda").remainder(2048).half()[None, :, None, None, None].expand_as(cache.k))
+    model = Model(cache)
+    rng = np.random.default_rng(4)
+    lens = rng.integers(0, 400, seqs)
+    lens[5] = width * 16 - 3
+    order = rng.permutation(seqs // 2).tolist()
+    counts = [int(lens[s]) for s in order]
+    cache.reserve(ints(*order), ints(*counts))
+    model.reserve(order, counts)
+    parents, children = rng.integers(0, seqs // 2, 1200).tolist(), (seqs // 2 + rng.permutation(1200)).tolist()
+    parents[0] = 5
+    cache.fork(ints(*parents), ints(*children))
+    model.fork(parents, children)
+    model.same(cache)
+    gone = rng.permutation(seqs)[:1500].tolist()
+    cache.free(ints(*gone))
+    model.free(gone)
+    cache.compact()
+    model.compact()
+    model.same(cache)
+    assert cache.refs[:int((cache.refs > 0).sum())].min() > 0
+
+
+def test_pages_copy(ctx):
+    cache = small_cache(ctx, 3)
+    want_k, want_v = cache.k.clone(), cache.v.clone()
+    src, dst = [0, 0, 39, 7, -1, 40, 3], [5, 6, 8, 7, 9, 10, 40]
+    for s, d in zip(src[:3], dst[:3]):
+        want_k[:, d], want_v[:, d] = want_k[:, s].clone(), want_v[:, s].clone()
+    cache.copy(ints(*src), ints(*dst))
+    torch.cuda.synchronize()
+    assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v)
+
+
+# ---------------------------------------------------------------------------------------------- together
+
+def test_forked_sequences_go_on_from_one_prompt(ctx):
+    """A prompt in chunks, two forks of it, single tokens in all three, a sequence freed, the cache compacted, and on: every attention
+    against float64 over what the sequence has been given."""
+    heads, kv, hd, dtype = 4, 2, 64, "f16"
+    cache = K.PagedCache(ctx, pimdl, 2, 64, kv, hd, 16, dtype, 5, 400)
+    given = {s: ([[], []], [[], []]) for s in range(5)}  # per sequence: keys and values, per layer
+    gen = gen_of(21)
+
+    def step(seqs, counts, left=None, sinks=0):
+        lst, n = ints(*seqs), sum(counts)
+        cache.reserve(lst, ints(*counts))
+        assert int(cache.lacking) == 0
+        starts = starts_of(counts)
+        for layer in range(2):
+            qkv = randn(gen, n, (heads + 2 * kv) * hd)
+            q, k, v = qkv[:, :heads * hd], qkv[:, heads * hd:(heads + kv) * hd], qkv[:, (heads + kv) * hd:]
+            out = torch.zeros(n, heads * hd, device="cuda")
+            cache.append(layer, k, v, starts, lst)
+            cache.attend(layer, q, out, starts, heads, lst, left=left, sinks=sinks)
+            torch.cuda.synchronize()
+            at = 0
+            for s, c in zip(seqs, counts):
+                for store, x in zip(given[s], (k, v)):
+                    store[layer].append(x[at:at + c].half().reshape(c, kv, hd))
+                kk, vv = (torch.cat(store[layer]) for store in given[s])
+                want, off, mass = reference(q[at:at + c].reshape(c, heads, hd), kk, vv, kk.shape[0] - c, UNL if left is None else left, 0, sinks, 0.125)
+                check(out[at:at + c].reshape(c, heads, hd), want, off, mass, "f32")
+                at += c
+
+    step([0, 3], [100, 7])
+    step([0], [41])
+    cache.fork(ints(0, 0), ints(1, 4))
+    for s in (1, 4):
+        given[s] = tuple([list(x) for x in store] for store in given[0])
+    step([4, 0, 1, 3], [1, 1, 1, 1])
+    step([1, 4], [1, 17], left=50, sinks=3)
+    cache.free(ints(0))
+    given[0] = ([[], []], [[], []])
+    cache.compact()
+    live = int((cache.refs > 0).sum())
+    assert (cache.refs[:live] > 0).all() and (cache.refs[live:] == 0).all()
+    step([1, 3, 4], [3, 1, 1])
+    step([0], [70])
+
+
+def test_captured_step_follows_the_lengths(ctx):
+    """A decode step recorded into a graph (lengths + 1, append, attention) and replayed: every replay against the eager calls."""
+    heads, kv, hd = 8, 2, 64
+    own = pimdl.Context(0)
+    side = torch.cuda.Stream()
+    caches = []
+    for c in (ctx, own):
+        cache = K.PagedCache(c, pimdl, 1, 400, kv, hd, 16, "bf16", 3, 2000)
+        cache.reserve(ints(0, 1, 2), ints(500, 30, 1290))
+        for pool, seed in ((cache.k, 1), (cache.v, 2)):
+            pool.copy_(randn(gen_of(seed), *pool.shape, dtype="bf16"))
+        torch.cuda.synchronize()
+        caches.append(cache)
+        own.synchronize()
+    seqs, ones, starts = ints(0, 1, 2), ints(1, 1, 1), starts_of([1, 1, 1])
+    qkv = randn(gen_of(3), 3, (heads + 2 * kv) * hd, dtype="bf16")
+    outs = [torch.zeros(3, heads * hd, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+
+    def step(cache, out):
+        cache.reserve(seqs, ones)
+        cache.append(0, qkv[:, heads * hd:(heads + kv) * hd], qkv[:, (heads + kv) * hd:], starts, seqs)
+        cache.attend(0, qkv[:, :heads * hd], out, starts, heads, seqs)
+
+    torch.cuda.synchronize()
+    own.set_stream(side.cuda_stream)
+    with torch.cuda.stream(side):
+        step(caches[1], outs[1])  # sizes the scratch
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+        step(caches[1], outs[1])
+    step(caches[0], outs[0])
+    for i in range(6):
+        torch.cuda.synchronize()
+        qkv.copy_(randn(gen_of(10 + i), *qkv.shape, dtype="bf16"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        step(caches[0], outs[0])
+        torch.cuda.synchronize()
+        assert torch.equal(caches[0].lengths, caches[1].lengths) and torch.equal(caches[0].tables, caches[1].tables)
+        assert torch.equal(outs[0], outs[1]), i
+    own.close()
+
+
+def test_growing_scratch_is_refused_during_a_capture(ctx):
+    own = pimdl.Context(0)
+    side = torch.cuda.Stream()
+    own.set_stream(side.cuda_stream)
+    cache = K.PagedCache(own, pimdl, 1, 2000, 1, 64, 16, "bf16", 1, 32000)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    keep = torch.zeros(1, device="cuda")
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+        keep.add_(1)
+        with pytest.raises(pimdl.PimdlError) as e:
+            cache.compact()
+    assert e.value.code == pimdl.ERR_INVALID and "captured" in str(e.value)
+    torch.cuda.synchronize()
+    own.close()
+
+
+def test_two_contexts_on_two_streams(ctx):
+    """Two caches, each with its own context and stream, at the same time."""
+    jobs = []
+    for i in range(2):
+        c, st = pimdl.Context(0), torch.cuda.Stream()
+        c.set_stream(st.cuda_stream)
+        f = Filled(c, 30 + i, [3000 + 500 * i, 20], 2, 64, 16, "f16")
+        q = randn(gen_of(40 + i), 2, 8 * 64)
+        jobs.append((c, st, f, q, torch.zeros_like(q), starts_of([1, 1])))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, st, f, q, out, starts in jobs:
+            f.cache.attend(0, q, out, starts, 8)
+    torch.cuda.synchronize()
+    for i, (c, st, f, q, out, starts) in enumerate(jobs):
+        for s, n in enumerate([3000 + 500 * i, 20]):
+            want, off, mass = reference(q[s:s + 1].reshape(1, 8, 64), f.rows[s][0][0], f.rows[s][1][0], n - 1, UNL, 0, 0, 0.125)
+            check(out[s:s + 1].reshape(1, 8, 64), want, off, mass, "f32")
+        c.close()
+
+
+# ---------------------------------------------------------------------------------------------- refusals
+
+def test_wrong_calls_are_refused(ctx):
+    f = Filled(ctx, 50, [40, 9], 2, 64, 16, "f16")
+    c = f.cache
+    q, out, starts = randn(gen_of(1), 2, 256), torch.zeros(2, 256, device="cuda"), starts_of([1, 1])
+    with pytest.raises(ValueError):
+        c.attend(0, q, out, starts, 3)           # columns do not fit the heads
+    with pytest.raises(ValueError):
+        c.attend(0, q, out.half(), starts, 4)
+    with pytest.raises(ValueError):
+        c.attend(0, q, out, starts.long(), 4)
+    with pytest.raises(ValueError):
+        c.attend(0, q, out, starts, 4, seqs=ints(0))
+    with pytest.raises(pimdl.PimdlError):
+        c.attend(0, q.bfloat16(), out.bfloat16(), starts, 4)  # over a cache in halves
+    with pytest.raises(pimdl.PimdlError):
+        c.attend(0, q, out, starts.cpu(), 4)
+    with pytest.raises(pimdl.PimdlError):
+        c.attend(0, q, out, starts, 4, scale=float("nan"))
+    with pytest.raises(pimdl.PimdlError):
+        c.attend(0, q, out, starts_of([1, 1, 0]), 4)  # more rows than sequences
+    with pytest.raises(pimdl.PimdlError):
+        c.attend(0, q[:, :192], out[:, :192], starts, 3)  # 3 heads over 2 key heads
+    with pytest.raises(ValueError):
+        c.append(0, q, q, starts)
+    with pytest.raises(pimdl.PimdlError):
+        c.reserve(ints(0), torch.ones(1, dtype=torch.int32))  # counts in host memory
+    with pytest.raises(ValueError):
+        c.fork(ints(0), ints(1, 1))
+    with pytest.raises(ValueError):
+        K.PagedCache.over(ctx, pimdl, c.k, c.v, c.tables.long(), c.lengths, c.refs)
+    with pytest.raises(pimdl.PimdlError):  # pages of 24 tokens
+        k = torch.zeros(1, 4, 1, 24, 64, device="cuda", dtype=torch.float16)
+        K.PagedCache.over(ctx, pimdl, k, k.clone(), ints(0, 1)[None], ints(5), torch.ones(4, dtype=torch.int32, device="cuda")).attend(
+            0, randn(gen_of(2), 1, 64), torch.zeros(1, 64, device="cuda"), starts_of([1]), 1)
+    x = randn(gen_of(3), 4, 64)
+    for bad in (dict(head_dim=257), dict(heads=2, kv_heads=3), dict(q_stride=63), dict(kv_stride=1), dict(scale=math.inf), dict(dtype=3), dict(kv_heads=0)):
+        a = dict(heads=1, kv_heads=1, head_dim=64, q_stride=64, kv_stride=64, scale=1.0, dtype=0) | bad
+        with pytest.raises(pimdl.PimdlError):
+            ctx.attention_window_ptr(x.data_ptr(), x.data_ptr(), x.data_ptr(), x.data_ptr(), starts.data_ptr(), 2, 4, a["heads"], a["kv_heads"], a["head_dim"],
+                                     a["q_stride"], a["kv_stride"], 64, 1, 1, 0, a["scale"], a["dtype"])
+    # an empty batch is no error
+    c.attend(0, q[:0], out[:0], starts_of([]), 4)
+    c.free(ints())
