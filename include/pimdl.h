@@ -369,10 +369,11 @@ PIMDL_API int pimdl_attention(pimdl_ctx* ctx, const float* q, const float* k, co
  * cores (given 16-byte aligned rows), other sizes on a plain kernel.  Strides are in elements.
  *
  * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max_j), over the keys that a query sees.  Scores, maxima,
- * sums and accumulators are fp32.  With fp32 operands products keep fp32 accuracy (24-bit factors); with 16-bit
- * operands p_j is rounded to that type once, before it meets v_j.  A query that sees no key, or whose scores are all
- * -infinity, gives zeros.  Rows of K and V that no query may see (other sequences, behind a length, pages of nobody)
- * may hold anything, infinities and NaN included. */
+ * sums and accumulators are fp32.  With fp32 operands products keep fp32 accuracy (factors of 24 bits; 22 of q and p over a
+ * cache in halves); with 16-bit operands p_j is rounded to that type once, before it meets v_j.  A query that sees no key gives
+ * zeros.  Rows of K and V that a query does not see -- hidden by the window, behind a length, of other sequences, on pages of
+ * nobody -- do not change its result whatever they hold, infinities and NaN included; an element of its own q or of a row that it
+ * sees which is not finite makes the results it enters infinite or NaN. */
 typedef enum pimdl_dtype { PIMDL_F32 = 0, PIMDL_F16 = 1, PIMDL_BF16 = 2 } pimdl_dtype;
 #define PIMDL_UNLIMITED 0xffffffffu
 

@@ -1,0 +1,766 @@
+// Attention of a ragged batch on the matrix cores (gfx950), for one pair of types; included by a translation unit per pair.
+//
+// Work is cut into tiles of ROWS: row r of a sequence and key head is (token r / group, query head r % group of the key head's
+// group), so query heads that share a key head share what is read of the cache.  A wave holds 32 rows and takes keys 32 at a time.
+// Both products run on v_mfma_f32_32x32x16, transposed, so that a lane keeps to one row and nothing changes lanes in between:
+//   S^T[key][row] = K Q^T:   A = K (32 keys x 16 dims), B = the rows' q.  Lane (row j, half h) gets keys 8 (i / 4) + 4 h + i % 4,
+//                            i = 0 .. 15: a row's maximum and sum are 16 registers and one exchange between halves.
+//   O^T[dim][row] += V^T P^T: the B operand of 16 keys is 8 of those very registers, rounded; the A operand has to hold the same keys in the
+//                            same places, which are two groups of 4 consecutive keys for each half: two transposing reads of LDS
+//                            (ds_read_b64_tr_b16: 16 lanes take 4 rows of 16 columns and get a column of 4 each).
+// Streaming softmax: m is the running maximum of a row's raw scores, p = 2^(c s - c m) with c = scale log2(e), l the sum of p; o and l are
+// multiplied by 2^(c (m - m')) when the maximum rises.
+//
+// fp32 operands are taken apart into 16-bit pieces, so that the products run at the 16-bit rate and keep 24 bits: three bf16
+// pieces by truncation (exact: 8 + 8 + 8 bits), of whose nine products the six that reach 2^-24 are taken; over a cache in halves
+// q (brought to 2^11 .. 2^12 by a power of two of its row) and p (times 2^15) are two halves, 22 bits and nothing subnormal that counts.
+// Against v_mfma_f32_32x32x2_f32, 1 / 16 of the 16-bit rate, that is 6 / 16, 3 / 16 and 2 / 16 of the time.
+#pragma once
+#include <type_traits>
+
+#include "serve_common.h"
+
+namespace pimdl {
+namespace attn {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float INF = __builtin_inff();
+
+// TQ: q and out; TK: keys and values
+template <typename TQ_, typename TK_, int HD_, bool PAGED_>
+struct Config {
+    typedef TQ_ TQ;
+    typedef TK_ TK;
+    static constexpr int HD = HD_;
+    static constexpr bool PAGED = PAGED_;
+    static constexpr bool HALF = std::is_same<TK, _Float16>::value;  // the products' type: halves, or bf16
+    static constexpr int NK = std::is_same<TK, float>::value ? 3 : 1;
+    static constexpr int NQ = std::is_same<TQ, float>::value ? (HALF ? 2 : 3) : 1;
+    static constexpr int KS = HD / 16;          // steps of 16 dims in the first product
+    static constexpr int DT = (HD + 31) / 32;   // tiles of 32 dims in the second (the last one may be half: its other rows are never stored)
+    static constexpr int LB = HD * 2;           // bytes of a row of one piece in LDS
+    static constexpr int PARTS = HD * (int)sizeof(TK) / 16;  // 16-byte parts of a row in memory
+    static constexpr int P_SHIFT = HALF ? 15 : 0;            // p is carried times 2^15 in halves
+};
+
+// Order of a row's 16-byte parts in LDS: part ^ order(row).  Rows of the first product's reads are 32 consecutive ones at one part; the
+// transposing reads take 4 consecutive rows at 4 parts: both meet every bank once per 16 lanes at 32, 64, 96 and 128 dims (80: twice).
+template <int HD>
+__device__ __forceinline__ constexpr uint32_t order(uint32_t row)
+{
+    if (HD == 128) return (row & 3) << 2 | (row >> 2 & 3);
+    if (HD == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    if (HD == 80) return 0;
+    return row >> 2 & 3;
+}
+
+template <bool HALF>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
+{
+    if constexpr (HALF) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t bits(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ __forceinline__ float number(uint32_t x) { return __builtin_bit_cast(float, x); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302); }
+
+// Two floats as N 16-bit pieces each, piece by piece.
+template <bool HALF, int N>
+__device__ __forceinline__ void pieces(float x, float y, uint32_t* out)
+{
+    if constexpr (HALF) {
+        f16x2 a = {(_Float16)x, (_Float16)y};
+        out[0] = __builtin_bit_cast(uint32_t, a);
+        if constexpr (N == 2) {
+            f16x2 b = {(_Float16)(x - (float)a[0]), (_Float16)(y - (float)a[1])};
+            out[1] = __builtin_bit_cast(uint32_t, b);
+        }
+    } else if constexpr (N == 1) {
+        bf16x2 a = {(__bf16)x, (__bf16)y};
+        out[0] = __builtin_bit_cast(uint32_t, a);
+    } else {
+        out[0] = high_halves(bits(x), bits(y));
+        x -= number(bits(x) & 0xffff0000u);
+        y -= number(bits(y) & 0xffff0000u);
+        out[1] = high_halves(bits(x), bits(y));
+        x -= number(bits(x) & 0xffff0000u);
+        y -= number(bits(y) & 0xffff0000u);
+        out[2] = high_halves(bits(x), bits(y));
+    }
+}
+
+__device__ __forceinline__ float other_half(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+    return number((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// 0xffff where a 16-bit element is infinite or NaN
+template <bool HALF>
+__device__ __forceinline__ uint32_t not_finite(uint32_t two)
+{
+    constexpr uint32_t e = HALF ? 0x7c00u : 0x7f80u;
+    return ((two & e) == e ? 0xffffu : 0u) | (((two >> 16) & e) == e ? 0xffff0000u : 0u);
+}
+
+// Where the keys of a tile lie.  A tile begins at a multiple of 16, pages hold multiples of 16: a group of 16 keys has one base address.
+// Keys behind the sequence or on no page are read from an address that exists; `there` has a bit for each group that is.
+template <typename C, int TILE>
+struct Place {
+    static constexpr int GROUPS = C::PAGED ? TILE / 16 : 1;
+    int64_t base[GROUPS];  // elements from k or v
+    uint32_t there;
+};
+
+template <typename C, int TILE>
+__device__ __forceinline__ Place<C, TILE> place(const AttnArgs& a, const Row& r, uint32_t kh, int32_t key0)
+{
+    Place<C, TILE> p;
+    p.there = ~0u;
+    if constexpr (C::PAGED) {
+#pragma unroll
+        for (int g = 0; g < TILE / 16; ++g) {
+            const int32_t key = key0 + 16 * g;
+            int32_t page = key < r.length ? r.table[key >> a.page_shift] : -1;
+            if (page < 0 || (uint32_t)page >= a.pages) {
+                page = 0;
+                p.there &= ~(1u << g);
+            }
+            p.base[g] = ((((int64_t)page * a.kv_heads + kh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * C::HD;
+        }
+    } else {
+        p.base[0] = (int64_t)r.first * a.kv_stride + (int64_t)kh * C::HD;
+    }
+    return p;
+}
+
+// Copies a tile of keys or values by THREADS threads through registers: fetch() asks for it, store() puts it into LDS, piece by piece.
+template <typename C, int TILE, int THREADS>
+struct Stage {
+    static constexpr int TOTAL = TILE * C::PARTS, LOADS = (TOTAL + THREADS - 1) / THREADS;
+    static constexpr int PIECE = TILE * C::LB;                   // bytes of a piece in LDS
+    static constexpr int BYTES = PIECE * C::NK + (C::HD % 32 ? 64 : 0);  // (a half tile of dims reads past the last row)
+    u32x4 x[LOADS];
+
+    __device__ __forceinline__ void fetch(const void* src, const AttnArgs& a, const Row& r, const Place<C, TILE>& p, int32_t key0, uint32_t tid)
+    {
+        const typename C::TK* s = static_cast<const typename C::TK*>(src);
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const uint32_t flat = u * THREADS + tid;
+            uint32_t row = flat / C::PARTS;
+            const uint32_t part = flat % C::PARTS;
+            if (TOTAL % THREADS && row >= TILE) row = TILE - 1;  // (not stored)
+            int64_t at;
+            if constexpr (C::PAGED) {
+                at = p.base[0];
+#pragma unroll
+                for (int g = 1; g < TILE / 16; ++g) at = row >= 16u * g ? p.base[g] : at;
+                at += (row & 15) * C::HD;
+            } else {
+                const int32_t key = key0 + (int32_t)row, k = key < r.length ? key : r.length - 1;
+                at = p.base[0] + (int64_t)k * a.kv_stride;
+            }
+            x[u] = *reinterpret_cast<const u32x4*>(s + at + part * (16 / sizeof(typename C::TK)));
+        }
+    }
+    // whether any of it is infinite or NaN
+    __device__ __forceinline__ bool any_not_finite(uint32_t tid) const
+    {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u)
+            if (TOTAL % THREADS == 0 || u * THREADS + tid < TOTAL) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (C::NK == 3) bad |= (x[u][i] & 0x7f800000u) == 0x7f800000u;
+                    else bad |= not_finite<C::HALF>(x[u][i]);
+                }
+            }
+        return bad != 0;
+    }
+    // CLEAN (fp32): an element that is not finite keeps its first piece (a NaN for a NaN) and has no others
+    template <bool CLEAN>
+    __device__ __forceinline__ void store(char* lds, uint32_t tid) const
+    {
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const uint32_t flat = u * THREADS + tid, row = flat / C::PARTS, part = flat % C::PARTS;
+            if (TOTAL % THREADS && row >= TILE) continue;
+            if constexpr (C::NK == 1) {
+                *reinterpret_cast<u32x4*>(lds + row * C::LB + ((part ^ order<C::HD>(row)) << 4)) = x[u];
+            } else {
+                char* to = lds + row * C::LB + (((part >> 1) ^ order<C::HD>(row)) << 4) + (part & 1) * 8;
+                uint32_t lo[3], hi[3];
+                float f[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = number(x[u][i]);
+                pieces<false, 3>(f[0], f[1], lo);
+                pieces<false, 3>(f[2], f[3], hi);
+                if constexpr (CLEAN) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if ((x[u][i] & 0x7f800000u) == 0x7f800000u) {
+                            uint32_t* w = i < 2 ? lo : hi;
+                            const uint32_t keep = i & 1 ? 0xffffu : 0xffff0000u;
+                            if (f[i] != f[i]) w[0] |= ~keep & 0x7fc07fc0u;
+                            w[1] &= keep;
+                            w[2] &= keep;
+                        }
+                }
+#pragma unroll
+                for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(to + n * PIECE) = (u32x2){lo[n], hi[n]};
+            }
+        }
+    }
+};
+
+// The rows of one wave and what it has of their result.
+template <typename C>
+struct Rows {
+    u32x4 q[C::NQ][C::KS];
+    float c;                  // scores times c are exponents of 2
+    int32_t lo, hi, sinks;    // of this lane's row: keys lo .. hi - 1 and 0 .. sinks - 1 are seen
+    int32_t min_hi, max_hi, min_lo, max_lo;  // over the wave's rows
+    float m, l;
+    f32x16 o[C::DT];
+
+    // row0: first row of the wave, rows: of the sequence and key head
+    __device__ __forceinline__ void begin(const AttnArgs& a, const Row& r, uint32_t kh, uint32_t row0, uint32_t rows)
+    {
+        const uint32_t j = threadIdx.x & 31, h = threadIdx.x >> 5 & 1;
+        const uint32_t row = row0 + j < rows ? row0 + j : rows - 1;  // rows past the last repeat it; they are never stored
+        const uint32_t token = row / a.group, head = kh * a.group + row % a.group;
+        const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;  // c is positive, so that the largest score has the largest exponent
+        c = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * LOG2E;
+        const typename C::TQ* qp = static_cast<const typename C::TQ*>(a.q) + (size_t)(r.first + token) * a.q_stride + (size_t)head * C::HD + 8 * h;
+        if constexpr (C::NQ == 1) {
+#pragma unroll
+            for (int s = 0; s < C::KS; ++s) {
+                u32x4 x = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+                if (sign < 0.0f) x ^= 0x80008000u;
+                if (sign == 0.0f) x = (u32x4){0, 0, 0, 0};
+                q[0][s] = x;
+            }
+        } else {
+            float factor = sign;
+            if constexpr (C::HALF) {  // the row's largest magnitude to 2^11 .. 2^12
+                float big = 0.0f;
+#pragma unroll
+                for (int s = 0; s < C::KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(qp + 16 * s + 4 * i);
+                        big = fmaxf(fmaxf(big, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
+                    }
+                big = fmaxf(big, other_half(big));
+                int e = 11 - ((int)(bits(big) >> 23 & 255) - 127);
+                e = e < -100 ? -100 : e > 100 ? 100 : e;
+                factor *= number((uint32_t)(127 + e) << 23);
+                c *= number((uint32_t)(127 - e) << 23);
+            }
+#pragma unroll
+            for (int s = 0; s < C::KS; ++s) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(qp + 16 * s) * factor, y = *reinterpret_cast<const f32x4*>(qp + 16 * s + 4) * factor;
+                uint32_t w[4][C::NQ];
+                pieces<C::HALF, C::NQ>(x[0], x[1], w[0]);
+                pieces<C::HALF, C::NQ>(x[2], x[3], w[1]);
+                pieces<C::HALF, C::NQ>(y[0], y[1], w[2]);
+                pieces<C::HALF, C::NQ>(y[2], y[3], w[3]);
+#pragma unroll
+                for (int n = 0; n < C::NQ; ++n) q[n][s] = (u32x4){w[0][n], w[1][n], w[2][n], w[3][n]};
+            }
+        }
+        auto border_hi = [&](uint32_t t) {
+            const int64_t e = (int64_t)r.pos0 + t + a.right + 1;
+            return (int32_t)(e < 0 ? 0 : e < r.length ? e : r.length);
+        };
+        auto border_lo = [&](uint32_t t) {
+            const int64_t e = (int64_t)r.pos0 + t - a.left;
+            return (int32_t)(e < 0 ? 0 : e < 0x7fffffff ? e : 0x7fffffff);
+        };
+        sinks = a.sinks < 0x7fffffffu ? (int32_t)a.sinks : 0x7fffffff;
+        hi = border_hi(token);
+        lo = border_lo(token);
+        const uint32_t t0 = row0 / a.group, t1 = (row0 + 32 < rows ? row0 + 31 : rows - 1) / a.group;
+        min_hi = border_hi(t0), max_hi = border_hi(t1), min_lo = border_lo(t0), max_lo = border_lo(t1);
+        m = -INF;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < C::DT; ++d) o[d] = (f32x16)(0.0f);
+    }
+
+    // keys key0 .. key0 + n - 1: whether some row sees some of them, whether every row sees all of them
+    __device__ __forceinline__ bool some(int32_t key0, int32_t n) const { return key0 < max_hi && (key0 + n > min_lo || key0 < sinks); }
+    __device__ __forceinline__ bool all(int32_t key0, int32_t n) const { return key0 + n <= min_hi && (key0 >= max_lo || key0 + n <= sinks); }
+    __device__ __forceinline__ bool sees(int32_t key) const { return key < hi && (key >= lo || key < sinks); }
+    static __device__ __forceinline__ int32_t key_of(int i) { return 8 * (i >> 2) + 4 * (int32_t)(threadIdx.x >> 5 & 1) + (i & 3); }
+
+    // scores of 32 keys, which lie in LDS from `k` on, pieces PIECE bytes apart
+    template <int PIECE>
+    __device__ __forceinline__ f32x16 scores(const char* k) const
+    {
+        const uint32_t j = threadIdx.x & 31, h = threadIdx.x >> 5 & 1;
+        f32x16 s = (f32x16)(0.0f);
+#pragma unroll
+        for (int st = 0; st < C::KS; ++st) {
+            u32x4 x[C::NK];
+#pragma unroll
+            for (int n = 0; n < C::NK; ++n) x[n] = *reinterpret_cast<const u32x4*>(k + n * PIECE + j * C::LB + (((2 * st + h) ^ order<C::HD>(j)) << 4));
+#pragma unroll
+            for (int w = C::NQ + C::NK - 2; w >= 0; --w)  // small products first
+#pragma unroll
+                for (int n = 0; n < C::NK; ++n)
+                    if (w - n >= 0 && w - n < C::NQ && (C::NK == 1 || w < C::NQ)) s = mfma<C::HALF>(x[n], q[w - n][st], s);
+        }
+        return s;
+    }
+
+    // Hides what the row does not see among 32 keys from key0 on; `there`: bits of the two groups of 16 that exist.
+    __device__ __forceinline__ void hide(f32x16& s, int32_t key0, uint32_t there) const
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (!sees(key0 + key_of(i)) || !(there >> (i >> 3) & 1)) s[i] = -INF;
+    }
+
+    // The scores of 32 KT keys become probabilities; o and l follow the maximum.
+    template <int KT>
+    __device__ __forceinline__ void softmax(f32x16* s)
+    {
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+        mx = fmaxf(mx, other_half(mx));
+        if (__any(mx > m)) {
+            const float up = fmaxf(m, mx), base = up == -INF ? 0.0f : up * c;
+            const float alpha = __builtin_amdgcn_exp2f(m * c - base);  // 0 at the first keys
+            m = up;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < C::DT; ++d) o[d] *= alpha;
+        }
+        const float base = (m == -INF ? 0.0f : m * c) - (float)C::P_SHIFT;
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -base));
+                sum += s[t][i];
+            }
+        l += sum;
+    }
+
+    // o += V^T p for 32 keys, which lie in LDS from `v` on.  BAD: V holds elements that are not finite, and some rows do not see some
+    // of its keys: such elements are taken for zeros, and rows that see one get NaN there.
+    template <int PIECE, bool BAD>
+    __device__ __forceinline__ void values(const char* v, const f32x16& p, int32_t key0, uint32_t there)
+    {
+        const uint32_t lane = threadIdx.x & 63, i = lane & 15, side = lane >> 4 & 1, h = lane >> 5;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            uint32_t w[4][C::NQ];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pieces<C::HALF, C::NQ>(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], w[e]);
+            u32x4 b[C::NQ];
+#pragma unroll
+            for (int n = 0; n < C::NQ; ++n) b[n] = (u32x4){w[0][n], w[1][n], w[2][n], w[3][n]};
+            u32x4 see = {0, 0, 0, 0};
+            if constexpr (BAD) {
+                constexpr uint32_t one = C::HALF ? 0x3c00u : 0x3f80u;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (sees(key0 + key_of(8 * st + e)) && (there >> st & 1)) see[e / 2] |= one << 16 * (e & 1);
+            }
+#pragma unroll
+            for (int d = 0; d < C::DT; ++d) {
+                u32x4 x[C::NK];
+#pragma unroll
+                for (int n = 0; n < C::NK; ++n) {
+                    s16x4 half[2];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const uint32_t row = 16 * st + 8 * g + 4 * h + (i >> 2), part = 4 * d + 2 * side + (i >> 1 & 1);
+                        const char* at = v + n * PIECE + row * C::LB + ((part ^ order<C::HD>(row)) << 4) + (i & 1) * 8;
+                        half[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                    }
+                    const u32x2 y = __builtin_bit_cast(u32x2, half[0]), z = __builtin_bit_cast(u32x2, half[1]);
+                    x[n] = (u32x4){y[0], y[1], z[0], z[1]};
+                }
+                if constexpr (BAD) {
+                    constexpr uint32_t ones = C::HALF ? 0x3c003c00u : 0x3f803f80u;
+                    u32x4 bad;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) bad[e] = not_finite<C::HALF>(x[0][e]);
+                    x[0] &= ~bad;
+                    const f32x16 seen = mfma<C::HALF>(bad & ones, see, (f32x16)(0.0f));
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (seen[e] > 0.0f) o[d][e] = __builtin_nanf("");
+                }
+#pragma unroll
+                for (int k = C::NQ + C::NK - 2; k >= 0; --k)
+#pragma unroll
+                    for (int n = 0; n < C::NK; ++n)
+                        if (k - n >= 0 && k - n < C::NQ && (C::NK == 1 || k < C::NQ)) o[d] = mfma<C::HALF>(x[n], b[k - n], o[d]);
+            }
+        }
+    }
+};
+
+// Results of keys that are split over workgroups: per split and row of the output (token, head) the sums, the exponent c m that they are
+// relative to, and l.
+struct Partial {
+    float* o;    // [splits][rows][head_dim]
+    float* ml;   // [splits][rows][2]
+    uint64_t rows;
+};
+
+template <typename TQ>
+__device__ __forceinline__ void store4(TQ* to, f32x4 x)
+{
+    if constexpr (std::is_same<TQ, float>::value) {
+        *reinterpret_cast<f32x4*>(to) = x;
+    } else {
+        struct alignas(8) Four {
+            TQ v[4];
+        } y = {{(TQ)x[0], (TQ)x[1], (TQ)x[2], (TQ)x[3]}};
+        *reinterpret_cast<Four*>(to) = y;
+    }
+}
+
+// The key tiles that a tile of rows has to look at: those of the first `sinks` keys that lie before the window, then the window's.
+struct Span {
+    int32_t first, sinks, total;
+    __device__ __forceinline__ int32_t at(int32_t t) const { return t < sinks ? t : first + (t - sinks); }
+};
+
+__device__ __forceinline__ Span span_of(const AttnArgs& a, const Row& r, uint32_t row0, uint32_t row1, int32_t tile)
+{
+    const int64_t top = (int64_t)r.pos0 + row1 / a.group + a.right + 1, low = (int64_t)r.pos0 + row0 / a.group - a.left;
+    const int32_t hi = (int32_t)(top < 0 ? 0 : top < r.length ? top : r.length), lo = (int32_t)(low < 0 ? 0 : low < hi ? low : hi);
+    Span s;
+    s.first = lo / tile;
+    const int32_t sinks = a.sinks < (uint32_t)lo ? (int32_t)a.sinks : lo, n = (sinks + tile - 1) / tile, last = (hi + tile - 1) / tile;
+    s.sinks = n < s.first ? n : s.first;
+    s.total = s.sinks + (last > s.first ? last - s.first : 0);
+    return s;
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Many rows: a workgroup takes 128 rows of a sequence and key head, its four waves 32 each, and all of them go through the same tiles of keys and
+// values in LDS.  The next tile is on its way in registers while one is worked on.
+// ------------------------------------------------------------------------------------------------------------
+constexpr uint32_t WIDE_ROWS = 128;
+
+template <typename C>
+struct Wide {
+    static constexpr int TILE = C::NK == 1 ? 64 : 32;
+    typedef Stage<C, TILE, 256> S;
+    static constexpr int LDS = 2 * S::BYTES;
+};
+
+// Tiles of rows of all sequences, without knowing their lengths: those of row b begin at slot first_row(b) * group / 128 + b.
+__device__ __forceinline__ uint32_t first_slot(const AttnArgs& a, uint32_t b, uint32_t tokens_before)
+{
+    return (uint32_t)((uint64_t)tokens_before * a.group / WIDE_ROWS) + b;
+}
+
+template <typename C>
+__global__ __launch_bounds__(256, C::NK == 3 && C::HD > 96 ? 1 : 2) void attention_wide_kernel(AttnArgs a, uint32_t slots, uint32_t splits, uint32_t narrow_rows, Partial part)
+{
+    typedef Wide<C> W;
+    constexpr int TILE = W::TILE, KT = TILE / 32;
+    __shared__ __attribute__((aligned(1024))) char lds[W::LDS];
+    __shared__ uint32_t bad[2];
+    char *const lk = lds, *const lv = lds + W::S::BYTES;
+    const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;  // late rows, which see most keys, first
+    uint32_t lo = 0, up = a.batch;
+    while (up - lo > 1) {
+        const uint32_t mid = (lo + up) / 2;
+        if (first_slot(a, mid, clamped_start(a.starts, mid, a.tokens)) <= slot) lo = mid;
+        else up = mid;
+    }
+    const uint32_t b = __builtin_amdgcn_readfirstlane(lo);
+    const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, C::PAGED, b);
+    const uint32_t rows = r.n * a.group, row0 = (slot - first_slot(a, b, r.first)) * WIDE_ROWS;
+    if (slot < first_slot(a, b, r.first) || row0 >= rows || rows <= narrow_rows) return;
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = tid & 31, h = tid >> 5 & 1;
+    const uint32_t end = row0 + WIDE_ROWS < rows ? row0 + WIDE_ROWS : rows, mine = row0 + 32 * wave;
+    const Span span = span_of(a, r, row0, end - 1, TILE);
+    const int32_t per = (span.total + (int32_t)splits - 1) / (int32_t)splits, from = per * (int32_t)split;
+    const int32_t to = from + per < span.total ? from + per : span.total;
+    const bool works = mine < end;
+    Rows<C> w;
+    w.begin(a, r, kh, works ? mine : row0, rows);
+    // whether every row of the workgroup sees all of a tile
+    const int32_t all_hi = [&] {
+        const int64_t e = (int64_t)r.pos0 + row0 / a.group + a.right + 1;
+        return (int32_t)(e < 0 ? 0 : e < r.length ? e : r.length);
+    }();
+    const int64_t all_lo = (int64_t)r.pos0 + (end - 1) / a.group - a.left;
+
+    if (tid < 2) bad[tid] = 0;
+    if (from < to) {
+        typename W::S sk, sv;
+        Place<C, TILE> p = place<C, TILE>(a, r, kh, span.at(from) * TILE);
+        sk.fetch(a.k, a, r, p, span.at(from) * TILE, tid);
+        sv.fetch(a.v, a, r, p, span.at(from) * TILE, tid);
+        for (int32_t t = from; t < to; ++t) {
+            const int32_t key0 = span.at(t) * TILE;
+            const bool mixed = !(key0 + TILE <= all_hi && (key0 >= all_lo || key0 + TILE <= w.sinks)) || p.there != ~0u;
+            __syncthreads();  // everybody is done with the tile before
+            if (tid == 0) bad[(t + 1) & 1] = 0;
+            sk.template store<false>(lk, tid);
+            if (mixed) {
+                if (sv.any_not_finite(tid)) bad[t & 1] = 1;
+                sv.template store<true>(lv, tid);
+            } else {
+                sv.template store<false>(lv, tid);
+            }
+            const uint32_t there = p.there;
+            if (t + 1 < to) {
+                p = place<C, TILE>(a, r, kh, span.at(t + 1) * TILE);
+                sk.fetch(a.k, a, r, p, span.at(t + 1) * TILE, tid);
+                sv.fetch(a.v, a, r, p, span.at(t + 1) * TILE, tid);
+            }
+            __syncthreads();
+            if (!works || !w.some(key0, TILE)) continue;
+            f32x16 s[KT];
+#pragma unroll
+            for (int n = 0; n < KT; ++n) s[n] = w.template scores<W::S::PIECE>(lk + n * 32 * C::LB);
+            if (!w.all(key0, TILE) || there != ~0u) {
+#pragma unroll
+                for (int n = 0; n < KT; ++n) w.hide(s[n], key0 + 32 * n, there >> 2 * n);
+            }
+            w.template softmax<KT>(s);
+            if (mixed && bad[t & 1]) {
+#pragma unroll
+                for (int n = 0; n < KT; ++n) w.template values<W::S::PIECE, true>(lv + n * 32 * C::LB, s[n], key0 + 32 * n, there >> 2 * n);
+            } else {
+#pragma unroll
+                for (int n = 0; n < KT; ++n) w.template values<W::S::PIECE, false>(lv + n * 32 * C::LB, s[n], key0 + 32 * n, there >> 2 * n);
+            }
+        }
+    }
+    if (mine + j >= end || !works) return;
+    const float l = w.l + other_half(w.l);
+    const uint32_t row = mine + j, token = r.first + row / a.group, head = kh * a.group + row % a.group;
+    if (splits == 1) {
+        typename C::TQ* out = static_cast<typename C::TQ*>(a.out) + (size_t)token * a.out_stride + (size_t)head * C::HD;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < C::DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (32 * d + 8 * i < C::HD) store4(out + 32 * d + 8 * i + 4 * h, (f32x4){w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]} * inv);
+    } else {
+        const uint64_t at = (uint64_t)split * part.rows + (uint64_t)token * a.heads + head;
+        if (h == 0) {
+            part.ml[2 * at] = w.m == -INF ? -INF : w.m * w.c;
+            part.ml[2 * at + 1] = l;
+        }
+        if (from >= to) return;  // (the joining kernel does not look at sums whose l is 0)
+#pragma unroll
+        for (int d = 0; d < C::DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (32 * d + 8 * i < C::HD)
+                    store4(part.o + at * C::HD + 32 * d + 8 * i + 4 * h, (f32x4){w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]});
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Few rows (a single new token, mostly): a workgroup takes 32 rows of a sequence and key head at a time; its four waves take the tiles of 32 keys in
+// turn, each through LDS of its own, without barriers, and are joined at the end.
+// ------------------------------------------------------------------------------------------------------------
+constexpr uint32_t NARROW_ROWS = 32;
+
+template <typename C>
+struct Narrow {
+    typedef Stage<C, 32, 64> S;
+    static constexpr int JOIN = 32 * (C::DT * 32 + 1) * 4;  // a wave's sums, rows padded against bank conflicts
+    static constexpr int WAVE = S::BYTES > JOIN ? (S::BYTES + 15) / 16 * 16 : (JOIN + 15) / 16 * 16;
+    static constexpr int LDS = 4 * WAVE;
+};
+
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <typename C>
+__global__ __launch_bounds__(256, C::NK == 3 && C::HD > 64 ? 1 : 2) void attention_narrow_kernel(AttnArgs a, uint32_t splits, uint32_t most_rows, Partial part)
+{
+    typedef Narrow<C> W;
+    __shared__ __attribute__((aligned(1024))) char lds[W::LDS];
+    __shared__ float ml[4][32][2];
+    const uint32_t split = blockIdx.x % splits, rest = blockIdx.x / splits, kh = rest % a.kv_heads, b = rest / a.kv_heads;
+    const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, C::PAGED, b);
+    const uint32_t rows = r.n * a.group;
+    if (rows > most_rows) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 31, h = lane >> 5;
+    char* const mine = lds + wave * W::WAVE;
+    for (uint32_t row0 = 0; row0 < rows; row0 += NARROW_ROWS) {
+        const uint32_t end = row0 + NARROW_ROWS < rows ? row0 + NARROW_ROWS : rows;
+        const Span span = span_of(a, r, row0, end - 1, 32);
+        int32_t per = (span.total + (int32_t)splits - 1) / (int32_t)splits;
+        if (per < 4) per = 4;  // a tile for each wave
+        const int32_t from = per * (int32_t)split, to = from + per < span.total ? from + per : span.total;
+        if (splits > 1 && from >= to) {  // nothing left for this split
+            for (uint32_t row = row0 + tid; row < end; row += 256) {
+                const uint64_t at = (uint64_t)split * part.rows + (uint64_t)(r.first + row / a.group) * a.heads + kh * a.group + row % a.group;
+                part.ml[2 * at] = -INF;
+                part.ml[2 * at + 1] = 0.0f;
+            }
+            continue;
+        }
+        Rows<C> w;
+        w.begin(a, r, kh, row0, rows);
+        int32_t t = from + (int32_t)wave;
+        if (t < to) {
+            typename W::S sk, sv;
+            Place<C, 32> p = place<C, 32>(a, r, kh, span.at(t) * 32);
+            sk.fetch(a.k, a, r, p, span.at(t) * 32, lane);
+            sv.fetch(a.v, a, r, p, span.at(t) * 32, lane);
+            for (; t < to; t += 4) {
+                const int32_t key0 = span.at(t) * 32;
+                const uint32_t there = p.there;
+                const bool mixed = !w.all(key0, 32) || there != ~0u;
+                sk.template store<false>(mine, lane);
+                const bool more = t + 4 < to;
+                if (more) {
+                    p = place<C, 32>(a, r, kh, span.at(t + 4) * 32);
+                    sk.fetch(a.k, a, r, p, span.at(t + 4) * 32, lane);
+                }
+                wave_sync();
+                f32x16 s = w.template scores<W::S::PIECE>(mine);
+                wave_sync();
+                if (mixed) w.hide(s, key0, there);
+                const bool bad = mixed && __any(sv.any_not_finite(lane));
+                if (mixed) sv.template store<true>(mine, lane);
+                else sv.template store<false>(mine, lane);
+                if (more) sv.fetch(a.v, a, r, p, span.at(t + 4) * 32, lane);
+                w.template softmax<1>(&s);
+                wave_sync();
+                if (bad) w.template values<W::S::PIECE, true>(mine, s, key0, there);
+                else w.template values<W::S::PIECE, false>(mine, s, key0, there);
+                wave_sync();
+            }
+        }
+        // join the waves: all relative to the largest exponent
+        const float l = w.l + other_half(w.l);
+        if (h == 0) {
+            ml[wave][j][0] = w.m == -INF ? -INF : w.m * w.c;
+            ml[wave][j][1] = l;
+        }
+        __syncthreads();
+        float top = -INF;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i][j][0]);
+        const float base = top == -INF ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f((w.m == -INF ? -INF : w.m * w.c) - base);
+        float* const sums = reinterpret_cast<float*>(mine);
+        constexpr int PITCH = C::DT * 32 + 1;
+#pragma unroll
+        for (int d = 0; d < C::DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[j * PITCH + 32 * d + w.key_of(i)] = w.o[d][i] * f;
+        __syncthreads();
+        // the row's sums, HD consecutive columns of a row by consecutive threads
+        for (uint32_t x = tid; x < (end - row0) * (C::HD / 4); x += 256) {
+            const uint32_t row = x / (C::HD / 4), col = x % (C::HD / 4) * 4;
+            f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* from_wave = reinterpret_cast<const float*>(lds + i * W::WAVE) + row * PITCH + col;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] += from_wave[e];
+            }
+            float mx = -INF, sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, ml[i][row][0]);
+            const float bs = mx == -INF ? 0.0f : mx;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += ml[i][row][1] * __builtin_amdgcn_exp2f(ml[i][row][0] - bs);
+            const uint32_t token = r.first + (row0 + row) / a.group, head = kh * a.group + (row0 + row) % a.group;
+            if (splits == 1) {
+                store4(static_cast<typename C::TQ*>(a.out) + (size_t)token * a.out_stride + (size_t)head * C::HD + col, sum == 0.0f ? (f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / sum));
+            } else {
+                const uint64_t at = (uint64_t)split * part.rows + (uint64_t)token * a.heads + head;
+                if (col == 0) {
+                    part.ml[2 * at] = mx;
+                    part.ml[2 * at + 1] = sum;
+                }
+                store4(part.o + at * C::HD + col, y);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// What one call launches, decided by launch_attention.
+struct Plan {
+    bool wide, narrow;
+    uint32_t slots;                       // of the wide kernel
+    uint32_t wide_splits, narrow_splits;
+    uint32_t narrow_rows;                 // rows of a sequence and key head up to which the narrow kernel takes them
+    Partial part;
+};
+
+template <typename C>
+int launch(Ctx* ctx, const AttnArgs& a, const Plan& p)
+{
+    int rc = PIMDL_OK;
+    if (p.wide) {
+        hipLaunchKernelGGL((attention_wide_kernel<C>), dim3(p.slots * a.kv_heads * p.wide_splits), dim3(256), 0, ctx->stream, a, p.slots, p.wide_splits,
+                           p.narrow ? p.narrow_rows : 0, p.part);
+        rc = hip_check(ctx, hipGetLastError(), "attention_wide_kernel launch");
+    }
+    if constexpr (C::PAGED) {
+        if (!rc && p.narrow) {
+            hipLaunchKernelGGL((attention_narrow_kernel<C>), dim3(a.batch * a.kv_heads * p.narrow_splits), dim3(256), 0, ctx->stream, a, p.narrow_splits,
+                               p.narrow_rows, p.part);
+            rc = hip_check(ctx, hipGetLastError(), "attention_narrow_kernel launch");
+        }
+    }
+    return rc;
+}
+
+template <typename TQ, typename TK, bool PAGED>
+int launch_heads(Ctx* ctx, const AttnArgs& a, const Plan& p)
+{
+    switch (a.head_dim) {
+    case 32: return launch<Config<TQ, TK, 32, PAGED>>(ctx, a, p);
+    case 64: return launch<Config<TQ, TK, 64, PAGED>>(ctx, a, p);
+    case 80: return launch<Config<TQ, TK, 80, PAGED>>(ctx, a, p);
+    case 96: return launch<Config<TQ, TK, 96, PAGED>>(ctx, a, p);
+    default: return launch<Config<TQ, TK, 128, PAGED>>(ctx, a, p);
+    }
+}
+
+// a translation unit each
+int launch_f32(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_f32_f16(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_f32_bf16(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_f16(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_bf16(Ctx* ctx, const AttnArgs& a, const Plan& p);
+
+}  // namespace attn
+}  // namespace pimdl

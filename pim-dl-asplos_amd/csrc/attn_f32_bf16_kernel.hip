@@ -1,0 +1,7 @@
+// Attention on the matrix cores: fp32 over a cache in bf16.
+#include "attn_body.h"
+
+int pimdl::attn::launch_f32_bf16(Ctx* ctx, const AttnArgs& a, const Plan& p)
+{
+    return launch_heads<float, __bf16, true>(ctx, a, p);  // (a window's tensors have one type)
+}

@@ -1,12 +1,14 @@
 // Attention of a ragged batch over a window or a paged cache for gfx950 (MI355X): see pimdl_attention_window and
 // pimdl_attention_paged.
-#include "serve_common.h"
+#include <algorithm>
+
+#include "attn_body.h"
 
 namespace pimdl {
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
+using attn::LOG2E;
 
 __device__ __forceinline__ float wave_max(float v)
 {
@@ -108,16 +110,133 @@ int launch_plain(Ctx* ctx, const AttnArgs& a)
     return hip_check(ctx, hipGetLastError(), "attention_plain_kernel launch");
 }
 
+// ---------------------------------------------------------------------------------------------
+// Joins what the splits of a row have: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).  A workgroup per token and head; GROUPS
+// of threads take the splits in turn.
+// ---------------------------------------------------------------------------------------------
+template <typename TQ>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::Partial part, uint32_t wide_splits, uint32_t narrow_splits, uint32_t narrow_rows)
+{
+    __shared__ float sums[256][4];
+    __shared__ float red[8];
+    const uint32_t t = blockIdx.x / a.heads, head = blockIdx.x % a.heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t b = row_of_token(a.starts, a.batch, a.tokens, t);
+    const uint32_t first = clamped_start(a.starts, b, a.tokens), end = clamped_start(a.starts, b + 1, a.tokens);
+    if (t < first || t >= end) return;
+    const uint32_t splits = (end - first) * a.group <= narrow_rows ? narrow_splits : wide_splits;
+    if (splits == 1) return;
+    const uint64_t at = (uint64_t)t * a.heads + head;
+    float top = -__builtin_inff();
+    for (uint32_t s = tid; s < splits; s += 256) top = fmaxf(top, part.ml[2 * (s * part.rows + at)]);
+    top = wave_max(top);
+    if (lane == 0) red[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float l = 0.0f;
+    for (uint32_t s = tid; s < splits; s += 256) {
+        const float* ml = part.ml + 2 * (s * part.rows + at);
+        l += ml[1] == 0.0f ? 0.0f : ml[1] * __builtin_amdgcn_exp2f(ml[0] - base);
+    }
+    l = wave_sum(l);
+    if (lane == 0) red[4 + wave] = l;
+    __syncthreads();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    const uint32_t lanes = a.head_dim / 4, groups = 256 / lanes, g = tid / lanes, col = tid % lanes * 4;
+    attn::f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    if (g < groups)
+        for (uint32_t s = g; s < splits; s += groups) {
+            const float* ml = part.ml + 2 * (s * part.rows + at);
+            if (ml[1] != 0.0f) y += *reinterpret_cast<const attn::f32x4*>(part.o + (s * part.rows + at) * a.head_dim + col) * __builtin_amdgcn_exp2f(ml[0] - base);
+        }
+    *reinterpret_cast<attn::f32x4*>(sums[tid]) = y;
+    __syncthreads();
+    if (tid >= lanes) return;
+    for (uint32_t i = 1; i < groups; ++i) y += *reinterpret_cast<const attn::f32x4*>(sums[tid + i * lanes]);
+    attn::store4(static_cast<TQ*>(a.out) + (size_t)t * a.out_stride + (size_t)head * a.head_dim + col, l == 0.0f ? (attn::f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / l));
+}
+
+template <typename TQ>
+int launch_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
+{
+    hipLaunchKernelGGL((attention_join_kernel<TQ>), dim3(a.tokens * a.heads), dim3(256), 0, ctx->stream, a, p.part, p.wide ? p.wide_splits : 1,
+                       p.narrow ? p.narrow_splits : 1, p.narrow ? p.narrow_rows : 0);
+    return hip_check(ctx, hipGetLastError(), "attention_join_kernel launch");
+}
+
+// Whether the matrix-core kernels take the call: head sizes that they are built for, rows of whole 16 bytes.
+bool matrix_form(const AttnArgs& a)
+{
+    if (a.head_dim != 32 && a.head_dim != 64 && a.head_dim != 80 && a.head_dim != 96 && a.head_dim != 128) return false;
+    const uint64_t qe = a.dtype == PIMDL_F32 ? 4 : 2, ke = a.cache_dtype == PIMDL_F32 ? 4 : 2;
+    uint64_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
+    all |= a.q_stride * qe | a.out_stride * qe | (a.paged ? 0 : a.kv_stride * ke);
+    return all % 16 == 0 && (uint64_t)a.tokens * a.group < 1u << 30;
+}
+
+// Which kernels run, and over how many workgroups the keys of a row are split.
+int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
+{
+    *p = {};
+    const uint64_t rows = (uint64_t)a.tokens * a.group, cus = (uint64_t)ctx->prop.multiProcessorCount;
+    // keys that a row may see at most
+    uint64_t keys = a.paged ? (uint64_t)a.table_width << a.page_shift : a.tokens;
+    keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + 1 + a.sinks + attn::WIDE_ROWS);
+    p->narrow = a.paged;
+    p->wide = !a.paged || (a.tokens > a.batch && rows > attn::NARROW_ROWS);
+    p->narrow_rows = p->wide ? attn::NARROW_ROWS : 0xffffffffu;
+    p->wide_splits = p->narrow_splits = 1;
+    p->slots = (uint32_t)(rows / attn::WIDE_ROWS) + a.batch;
+    if (p->narrow) {
+        const uint64_t items = (uint64_t)a.batch * a.kv_heads;
+        p->narrow_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(8 * cus + items - 1) / items, keys / 512, 256}));
+    }
+    if (p->wide) {
+        const uint64_t items = (rows + attn::WIDE_ROWS - 1) / attn::WIDE_ROWS * a.kv_heads;
+        p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + items - 1) / items, keys / 512, 16}));
+    }
+    // what the splits hand over is kept below 128 MiB
+    const uint64_t row_bytes = (uint64_t)(a.head_dim + 2) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
+    p->narrow_splits = (uint32_t)std::min<uint64_t>(p->narrow_splits, most);
+    p->wide_splits = (uint32_t)std::min<uint64_t>(p->wide_splits, most);
+    const uint32_t splits = std::max(p->narrow_splits, p->wide_splits);
+    if ((uint64_t)p->slots * a.kv_heads * p->wide_splits > 1u << 30 || (uint64_t)a.batch * a.kv_heads * p->narrow_splits > 1u << 30 || (uint64_t)a.tokens * a.heads > 1u << 30)
+        return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
+    if (splits > 1) {
+        int rc = ensure_scratch(ctx, &ctx->d_attn, &ctx->attn_bytes, row_bytes * splits, "attention's partial results");
+        if (rc) return rc;
+        p->part.rows = (uint64_t)a.tokens * a.heads;
+        p->part.o = reinterpret_cast<float*>(ctx->d_attn);
+        p->part.ml = p->part.o + p->part.rows * splits * a.head_dim;
+    }
+    return PIMDL_OK;
+}
+
 }  // namespace
 
 int launch_attention(Ctx* ctx, const AttnArgs& a)
 {
     if (a.tokens == 0 || a.batch == 0) return PIMDL_OK;
-    if (a.dtype == PIMDL_BF16) return launch_plain<__bf16, __bf16>(ctx, a);
-    if (a.dtype == PIMDL_F16) return launch_plain<_Float16, _Float16>(ctx, a);
-    if (a.cache_dtype == PIMDL_BF16) return launch_plain<float, __bf16>(ctx, a);
-    if (a.cache_dtype == PIMDL_F16) return launch_plain<float, _Float16>(ctx, a);
-    return launch_plain<float, float>(ctx, a);
+    if (!matrix_form(a)) {
+        if ((uint64_t)a.tokens * a.heads / 4 >= 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
+        if (a.dtype == PIMDL_BF16) return launch_plain<__bf16, __bf16>(ctx, a);
+        if (a.dtype == PIMDL_F16) return launch_plain<_Float16, _Float16>(ctx, a);
+        if (a.cache_dtype == PIMDL_BF16) return launch_plain<float, __bf16>(ctx, a);
+        if (a.cache_dtype == PIMDL_F16) return launch_plain<float, _Float16>(ctx, a);
+        return launch_plain<float, float>(ctx, a);
+    }
+    attn::Plan p;
+    int rc = make_plan(ctx, a, &p);
+    if (rc) return rc;
+    if (a.dtype == PIMDL_BF16) rc = attn::launch_bf16(ctx, a, p);
+    else if (a.dtype == PIMDL_F16) rc = attn::launch_f16(ctx, a, p);
+    else if (a.cache_dtype == PIMDL_BF16) rc = attn::launch_f32_bf16(ctx, a, p);
+    else if (a.cache_dtype == PIMDL_F16) rc = attn::launch_f32_f16(ctx, a, p);
+    else rc = attn::launch_f32(ctx, a, p);
+    if (rc || (p.wide_splits == 1 && p.narrow_splits == 1)) return rc;
+    if (a.dtype == PIMDL_BF16) return launch_join<__bf16>(ctx, a, p);
+    if (a.dtype == PIMDL_F16) return launch_join<_Float16>(ctx, a, p);
+    return launch_join<float>(ctx, a, p);
 }
 
 }  // namespace pimdl

@@ -154,27 +154,40 @@ def test_window_token_count_cuts_the_batch(ctx):
         check(out[a:b, None], want, off, mass, "f32")
 
 
-def test_window_of_scores_without_a_finite_one_and_of_infinite_keys_elsewhere(ctx):
-    """All scores -infinity: zeros.  An infinite key or value in a place that the window hides, or in another sequence, changes nothing."""
-    for dtype in ("f32", "bf16"):
-        gen = gen_of(6)
-        q, k, v = (randn(gen, 300, 64, dtype=dtype) for _ in range(3))
-        out = torch.zeros(300, 64, device="cuda", dtype=TYPES[dtype])
-        window(ctx, q, k, v, out, [100, 200], 1, 1, 64, 7, 0, 0, dtype)
-        plain = out.clone()
-        k[40], v[40] = float("inf"), float("nan")  # of sequence 0: seen by its positions 40 .. 47 only
-        out.zero_()
-        window(ctx, q, k, v, out, [100, 200], 1, 1, 64, 7, 0, 0, dtype)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 80, 20])
+def test_what_the_window_hides_changes_nothing(ctx, dtype, hd):
+    """An infinite key and a value that is infinite or NaN: only the positions that see them have results that are not finite, and of those
+    all columns for the key, its own column for the value."""
+    gen = gen_of(6)
+    q, k, v = (randn(gen, 300, hd, dtype=dtype) for _ in range(3))
+    out = torch.zeros(300, hd, device="cuda", dtype=TYPES[dtype])
+
+    def run():
+        out.fill_(7.0)
+        window(ctx, q, k, v, out, [100, 200], 1, 1, hd, 7, 0, 0, dtype)
         torch.cuda.synchronize()
-        assert torch.equal(out[100:], plain[100:])
-        hidden = [i for i in range(100) if not 40 <= i <= 47]
-        assert torch.equal(out[hidden], plain[hidden])
-        q.fill_(1.0)
-        k.fill_(-math.inf)
-        v = torch.randn_like(v)
-        window(ctx, q, k, v, out, [100, 200], 1, 1, 64, 7, 0, 0, dtype)
-        torch.cuda.synchronize()
-        assert (out == 0).all()
+        return out.clone()
+
+    plain = run()
+    assert torch.isfinite(plain).all()
+    k[40] = float("inf")
+    got = run()
+    seen = torch.zeros(300, dtype=torch.bool, device="cuda")
+    seen[40:48] = True
+    assert torch.equal(got[~seen], plain[~seen])
+    k[40] = 0.5
+    plain = run()
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        v[40, 3], v[41, 9] = bad, bad
+        got = run()
+        for col, rows in ((3, range(40, 48)), (9, range(41, 49))):
+            assert not torch.isfinite(got[list(rows), col]).any()
+            got[list(rows), col] = plain[list(rows), col]
+        v[40, 3], v[41, 9] = 1.0, 1.0
+        v0 = run()
+        got[40:49, 3], got[40:49, 9] = v0[40:49, 3], v0[40:49, 9]
+        assert torch.equal(got, v0)
 
 
 # ---------------------------------------------------------------------------------------------- paged
