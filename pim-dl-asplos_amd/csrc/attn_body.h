@@ -47,8 +47,6 @@ struct Config {
     static constexpr bool HALF = std::is_same<TK, _Float16>::value;  // the products' type: halves, or bf16
     static constexpr int NK = std::is_same<TK, float>::value ? 3 : 1;
     static constexpr int NQ = std::is_same<TQ, float>::value ? (HALF ? 2 : 3) : 1;
-    static constexpr int KS = HD / 16;          // steps of 16 dims in the first product
-    static constexpr int DT = (HD + 31) / 32;   // tiles of 32 dims in the second (the last one may be half: its other rows are never stored)
     static constexpr int LB = HD * 2;           // bytes of a row of one piece in LDS
     static constexpr int PARTS = HD * (int)sizeof(TK) / 16;  // 16-byte parts of a row in memory
     static constexpr int P_SHIFT = HALF ? 15 : 0;            // p is carried times 2^15 in halves
@@ -70,6 +68,12 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c)
 {
     if constexpr (HALF) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <bool HALF>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
+{
+    if constexpr (HALF) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
 __device__ __forceinline__ uint32_t bits(float x) { return __builtin_bit_cast(uint32_t, x); }
@@ -101,10 +105,28 @@ __device__ __forceinline__ void pieces(float x, float y, uint32_t* out)
     }
 }
 
-__device__ __forceinline__ float other_half(float v)
+// maximum and sum over the lanes that share a row: the swapped pair holds both sides' values
+template <int M>
+__device__ __forceinline__ float row_max(float v)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
-    return number((threadIdx.x & 32) ? r[0] : r[1]);
+    v = fmaxf(number(r[0]), number(r[1]));
+    if constexpr (M == 16) {
+        const auto t = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+        v = fmaxf(number(t[0]), number(t[1]));
+    }
+    return v;
+}
+template <int M>
+__device__ __forceinline__ float row_sum(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+    v = number(r[0]) + number(r[1]);
+    if constexpr (M == 16) {
+        const auto t = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+        v = number(t[0]) + number(t[1]);
+    }
+    return v;
 }
 
 // 0xffff where a 16-bit element is infinite or NaN
@@ -117,31 +139,37 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t two)
 
 // Where the keys of a tile lie.  A tile begins at a multiple of 16, pages hold multiples of 16: a group of 16 keys has one base address.
 // Keys behind the sequence or on no page are read from an address that exists; `there` has a bit for each group that is.
-template <typename C, int TILE>
 struct Place {
-    static constexpr int GROUPS = C::PAGED ? TILE / 16 : 1;
-    int64_t base[GROUPS];  // elements from k or v
+    int64_t base, step1, step2, step3;  // elements from k or v: of group 0 (not paged: of the sequence), from each group to the next
     uint32_t there;
 };
 
 template <typename C, int TILE>
-__device__ __forceinline__ Place<C, TILE> place(const AttnArgs& a, const Row& r, uint32_t kh, int32_t key0)
+__device__ __forceinline__ Place place(const AttnArgs& a, const Row& r, uint32_t kh, int32_t key0)
 {
-    Place<C, TILE> p;
+    Place p;
     p.there = ~0u;
+    p.base = p.step1 = p.step2 = p.step3 = 0;
     if constexpr (C::PAGED) {
-#pragma unroll
-        for (int g = 0; g < TILE / 16; ++g) {
+        auto group = [&](int g) -> int64_t {
             const int32_t key = key0 + 16 * g;
             int32_t page = key < r.length ? r.table[key >> a.page_shift] : -1;
             if (page < 0 || (uint32_t)page >= a.pages) {
                 page = 0;
                 p.there &= ~(1u << g);
             }
-            p.base[g] = ((((int64_t)page * a.kv_heads + kh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * C::HD;
+            return ((((int64_t)page * a.kv_heads + kh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * C::HD;
+        };
+        const int64_t g0 = group(0), g1 = group(1);
+        p.base = g0;
+        p.step1 = g1 - g0;
+        if constexpr (TILE == 64) {
+            const int64_t g2 = group(2), g3 = group(3);
+            p.step2 = g2 - g1;
+            p.step3 = g3 - g2;
         }
     } else {
-        p.base[0] = (int64_t)r.first * a.kv_stride + (int64_t)kh * C::HD;
+        p.base = (int64_t)r.first * a.kv_stride + (int64_t)kh * C::HD;
     }
     return p;
 }
@@ -154,7 +182,7 @@ struct Stage {
     static constexpr int BYTES = PIECE * C::NK + (C::HD % 32 ? 64 : 0);  // (a half tile of dims reads past the last row)
     u32x4 x[LOADS];
 
-    __device__ __forceinline__ void fetch(const void* src, const AttnArgs& a, const Row& r, const Place<C, TILE>& p, int32_t key0, uint32_t tid)
+    __device__ __forceinline__ void fetch(const void* src, const AttnArgs& a, const Row& r, const Place& p, int32_t key0, uint32_t tid)
     {
         const typename C::TK* s = static_cast<const typename C::TK*>(src);
 #pragma unroll
@@ -165,122 +193,127 @@ struct Stage {
             if (TOTAL % THREADS && row >= TILE) row = TILE - 1;  // (not stored)
             int64_t at;
             if constexpr (C::PAGED) {
-                at = p.base[0];
-#pragma unroll
-                for (int g = 1; g < TILE / 16; ++g) at = row >= 16u * g ? p.base[g] : at;
-                at += (row & 15) * C::HD;
+                at = p.base + (row & 15) * C::HD;
+                at += row < 16 ? 0 : p.step1;
+                if constexpr (TILE == 64) {
+                    at += row < 32 ? 0 : p.step2;
+                    at += row < 48 ? 0 : p.step3;
+                }
             } else {
                 const int32_t key = key0 + (int32_t)row, k = key < r.length ? key : r.length - 1;
-                at = p.base[0] + (int64_t)k * a.kv_stride;
+                at = p.base + (int64_t)k * a.kv_stride;
             }
             x[u] = *reinterpret_cast<const u32x4*>(s + at + part * (16 / sizeof(typename C::TK)));
         }
     }
-    // whether any of it is infinite or NaN
-    __device__ __forceinline__ bool any_not_finite(uint32_t tid) const
+    // MIXED: elements that are not finite become zeros and get a bit in `marks`, a byte per part of a row; whether there is one
+    template <bool MIXED>
+    __device__ __forceinline__ bool store(char* lds, uint8_t* marks, uint32_t tid)
     {
-        uint32_t bad = 0;
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u)
-            if (TOTAL % THREADS == 0 || u * THREADS + tid < TOTAL) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (C::NK == 3) bad |= (x[u][i] & 0x7f800000u) == 0x7f800000u;
-                    else bad |= not_finite<C::HALF>(x[u][i]);
-                }
-            }
-        return bad != 0;
-    }
-    // CLEAN (fp32): an element that is not finite keeps its first piece (a NaN for a NaN) and has no others
-    template <bool CLEAN>
-    __device__ __forceinline__ void store(char* lds, uint32_t tid) const
-    {
+        uint32_t any = 0;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
             const uint32_t flat = u * THREADS + tid, row = flat / C::PARTS, part = flat % C::PARTS;
             if (TOTAL % THREADS && row >= TILE) continue;
+            if constexpr (MIXED) {
+                uint32_t found = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (C::NK == 3) {
+                        if ((x[u][i] & 0x7f800000u) == 0x7f800000u) {
+                            found |= 1u << i;
+                            x[u][i] = 0;
+                        }
+                    } else {
+                        const uint32_t bad = not_finite<C::HALF>(x[u][i]);
+                        found |= (bad & 1) << 2 * i | (bad >> 31) << (2 * i + 1);
+                        x[u][i] &= ~bad;
+                    }
+                }
+                marks[flat] = (uint8_t)found;
+                any |= found;
+            }
             if constexpr (C::NK == 1) {
                 *reinterpret_cast<u32x4*>(lds + row * C::LB + ((part ^ order<C::HD>(row)) << 4)) = x[u];
             } else {
                 char* to = lds + row * C::LB + (((part >> 1) ^ order<C::HD>(row)) << 4) + (part & 1) * 8;
                 uint32_t lo[3], hi[3];
-                float f[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] = number(x[u][i]);
-                pieces<false, 3>(f[0], f[1], lo);
-                pieces<false, 3>(f[2], f[3], hi);
-                if constexpr (CLEAN) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if ((x[u][i] & 0x7f800000u) == 0x7f800000u) {
-                            uint32_t* w = i < 2 ? lo : hi;
-                            const uint32_t keep = i & 1 ? 0xffffu : 0xffff0000u;
-                            if (f[i] != f[i]) w[0] |= ~keep & 0x7fc07fc0u;
-                            w[1] &= keep;
-                            w[2] &= keep;
-                        }
-                }
+                pieces<false, 3>(number(x[u][0]), number(x[u][1]), lo);
+                pieces<false, 3>(number(x[u][2]), number(x[u][3]), hi);
 #pragma unroll
                 for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(to + n * PIECE) = (u32x2){lo[n], hi[n]};
             }
         }
+        return any != 0;
     }
 };
 
-// The rows of one wave and what it has of their result.
-template <typename C>
+// The M (32 or 16) rows of one wave and what it has of their result.  Lane (row j, group g): j = lane % M, g = lane / M.
+template <typename C, int M>
 struct Rows {
-    u32x4 q[C::NQ][C::KS];
+    static constexpr int GROUPS = 64 / M, REGS = 32 / GROUPS;  // REGS: scores of 32 keys that a lane holds
+    static constexpr int STEP = 8 * GROUPS, KS = (C::HD + STEP - 1) / STEP;  // steps of the first product, in dims; of the last one of 80 dims,
+    static constexpr bool REST = C::HD % STEP != 0;                          // M == 16, groups 2 and 3 repeat the dims of 0 and 1 against zeros of q
+    static constexpr int DT = (C::HD + M - 1) / M;             // tiles of the second (80 dims, M == 32: of the last one only half counts)
+    static constexpr int QUADS = REGS / 4, OREGS = M * M / 64, OQUADS = OREGS / 4;
+    typedef typename std::conditional<M == 32, f32x16, f32x4>::type Acc;
+    static constexpr int KT = M == 32 ? 1 : 2;  // accumulators of 32 keys
+
+    u32x4 q[C::NQ][KS];
     float c;                  // scores times c are exponents of 2
     int32_t lo, hi, sinks;    // of this lane's row: keys lo .. hi - 1 and 0 .. sinks - 1 are seen
     int32_t min_hi, max_hi, min_lo, max_lo;  // over the wave's rows
     float m, l;
-    f32x16 o[C::DT];
+    Acc o[DT];
+
+    static __device__ __forceinline__ uint32_t row() { return threadIdx.x % M; }
+    static __device__ __forceinline__ uint32_t group() { return (threadIdx.x & 63) / M; }
+    // which key of 32, or which dim of a tile, register i of this lane holds
+    static __device__ __forceinline__ int32_t place_of(int i) { return 4 * GROUPS * (i >> 2) + 4 * (int32_t)group() + (i & 3); }
+
+    // the 8 dims that this lane has in step s of the first product
+    static __device__ __forceinline__ uint32_t dims(int s) { return STEP * s + 8 * (REST && s == KS - 1 ? group() & 1 : group()); }
 
     // row0: first row of the wave, rows: of the sequence and key head
     __device__ __forceinline__ void begin(const AttnArgs& a, const Row& r, uint32_t kh, uint32_t row0, uint32_t rows)
     {
-        const uint32_t j = threadIdx.x & 31, h = threadIdx.x >> 5 & 1;
-        const uint32_t row = row0 + j < rows ? row0 + j : rows - 1;  // rows past the last repeat it; they are never stored
-        const uint32_t token = row / a.group, head = kh * a.group + row % a.group;
+        const uint32_t g = group(), mine = row0 + row() < rows ? row0 + row() : rows - 1;  // rows past the last repeat it; they are never stored
+        const uint32_t token = mine / a.group, head = kh * a.group + mine % a.group;
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;  // c is positive, so that the largest score has the largest exponent
         c = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * LOG2E;
-        const typename C::TQ* qp = static_cast<const typename C::TQ*>(a.q) + (size_t)(r.first + token) * a.q_stride + (size_t)head * C::HD + 8 * h;
+        const typename C::TQ* const base = static_cast<const typename C::TQ*>(a.q) + (size_t)(r.first + token) * a.q_stride + (size_t)head * C::HD;
         if constexpr (C::NQ == 1) {
+            const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u, keep = sign == 0.0f ? 0u : ~0u;
 #pragma unroll
-            for (int s = 0; s < C::KS; ++s) {
-                u32x4 x = *reinterpret_cast<const u32x4*>(qp + 16 * s);
-                if (sign < 0.0f) x ^= 0x80008000u;
-                if (sign == 0.0f) x = (u32x4){0, 0, 0, 0};
-                q[0][s] = x;
+            for (int s = 0; s < KS; ++s) {
+                q[0][s] = (*reinterpret_cast<const u32x4*>(base + dims(s)) ^ flip) & keep;
+                if (REST && s == KS - 1 && g >= 2) q[0][s] = (u32x4){0, 0, 0, 0};
             }
         } else {
+            f32x4 x[2 * KS];
+#pragma unroll
+            for (int s = 0; s < 2 * KS; ++s) {
+                x[s] = *reinterpret_cast<const f32x4*>(base + dims(s / 2) + 4 * (s & 1));
+                if (REST && s / 2 == KS - 1 && g >= 2) x[s] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            }
             float factor = sign;
             if constexpr (C::HALF) {  // the row's largest magnitude to 2^11 .. 2^12
                 float big = 0.0f;
 #pragma unroll
-                for (int s = 0; s < C::KS; ++s)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const f32x4 x = *reinterpret_cast<const f32x4*>(qp + 16 * s + 4 * i);
-                        big = fmaxf(fmaxf(big, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
-                    }
-                big = fmaxf(big, other_half(big));
+                for (int s = 0; s < 2 * KS; ++s) big = fmaxf(fmaxf(big, fmaxf(fabsf(x[s][0]), fabsf(x[s][1]))), fmaxf(fabsf(x[s][2]), fabsf(x[s][3])));
+                big = row_max<M>(big);
                 int e = 11 - ((int)(bits(big) >> 23 & 255) - 127);
                 e = e < -100 ? -100 : e > 100 ? 100 : e;
                 factor *= number((uint32_t)(127 + e) << 23);
                 c *= number((uint32_t)(127 - e) << 23);
             }
 #pragma unroll
-            for (int s = 0; s < C::KS; ++s) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(qp + 16 * s) * factor, y = *reinterpret_cast<const f32x4*>(qp + 16 * s + 4) * factor;
-                uint32_t w[4][C::NQ];
-                pieces<C::HALF, C::NQ>(x[0], x[1], w[0]);
-                pieces<C::HALF, C::NQ>(x[2], x[3], w[1]);
-                pieces<C::HALF, C::NQ>(y[0], y[1], w[2]);
-                pieces<C::HALF, C::NQ>(y[2], y[3], w[3]);
+            for (int s = 0; s < 2 * KS; ++s) {
+                uint32_t w[2][C::NQ];
+                pieces<C::HALF, C::NQ>(x[s][0] * factor, x[s][1] * factor, w[0]);
+                pieces<C::HALF, C::NQ>(x[s][2] * factor, x[s][3] * factor, w[1]);
 #pragma unroll
-                for (int n = 0; n < C::NQ; ++n) q[n][s] = (u32x4){w[0][n], w[1][n], w[2][n], w[3][n]};
+                for (int n = 0; n < C::NQ; ++n) q[n][s / 2][2 * (s & 1)] = w[0][n], q[n][s / 2][2 * (s & 1) + 1] = w[1][n];
             }
         }
         auto border_hi = [&](uint32_t t) {
@@ -299,128 +332,134 @@ struct Rows {
         m = -INF;
         l = 0.0f;
 #pragma unroll
-        for (int d = 0; d < C::DT; ++d) o[d] = (f32x16)(0.0f);
+        for (int d = 0; d < DT; ++d) o[d] = (Acc)(0.0f);
     }
 
     // keys key0 .. key0 + n - 1: whether some row sees some of them, whether every row sees all of them
     __device__ __forceinline__ bool some(int32_t key0, int32_t n) const { return key0 < max_hi && (key0 + n > min_lo || key0 < sinks); }
     __device__ __forceinline__ bool all(int32_t key0, int32_t n) const { return key0 + n <= min_hi && (key0 >= max_lo || key0 + n <= sinks); }
     __device__ __forceinline__ bool sees(int32_t key) const { return key < hi && (key >= lo || key < sinks); }
-    static __device__ __forceinline__ int32_t key_of(int i) { return 8 * (i >> 2) + 4 * (int32_t)(threadIdx.x >> 5 & 1) + (i & 3); }
+
+    // of a product of NQ and NK pieces those that reach the last bit of the larger count, small ones first
+    static __device__ __forceinline__ void product(const u32x4* x, const u32x4* y, Acc& sum)
+    {
+#pragma unroll
+        for (int w = C::NK == 1 ? C::NQ - 1 : 2; w >= 0; --w)
+#pragma unroll
+            for (int n = 0; n < C::NK; ++n)
+                if (w - n >= 0 && w - n < C::NQ) sum = mfma<C::HALF>(x[n], y[w - n], sum);
+    }
 
     // scores of 32 keys, which lie in LDS from `k` on, pieces PIECE bytes apart
     template <int PIECE>
-    __device__ __forceinline__ f32x16 scores(const char* k) const
+    __device__ __forceinline__ void scores(const char* k, float* s) const
     {
-        const uint32_t j = threadIdx.x & 31, h = threadIdx.x >> 5 & 1;
-        f32x16 s = (f32x16)(0.0f);
+        const uint32_t j = row();
 #pragma unroll
-        for (int st = 0; st < C::KS; ++st) {
-            u32x4 x[C::NK];
+        for (int t = 0; t < KT; ++t) {
+            Acc acc = (Acc)(0.0f);
+            const char* const at = k + (t * M + j) * C::LB;
 #pragma unroll
-            for (int n = 0; n < C::NK; ++n) x[n] = *reinterpret_cast<const u32x4*>(k + n * PIECE + j * C::LB + (((2 * st + h) ^ order<C::HD>(j)) << 4));
+            for (int st = 0; st < KS; ++st) {
+                u32x4 x[C::NK], y[C::NQ];
 #pragma unroll
-            for (int w = C::NQ + C::NK - 2; w >= 0; --w)  // small products first
+                for (int n = 0; n < C::NK; ++n) x[n] = *reinterpret_cast<const u32x4*>(at + n * PIECE + (((dims(st) / 8) ^ order<C::HD>(t * M + j)) << 4));
 #pragma unroll
-                for (int n = 0; n < C::NK; ++n)
-                    if (w - n >= 0 && w - n < C::NQ && (C::NK == 1 || w < C::NQ)) s = mfma<C::HALF>(x[n], q[w - n][st], s);
+                for (int n = 0; n < C::NQ; ++n) y[n] = q[n][st];
+                product(x, y, acc);
+            }
+#pragma unroll
+            for (int i = 0; i < OREGS; ++i) s[t * OREGS + i] = acc[i];
         }
-        return s;
     }
 
     // Hides what the row does not see among 32 keys from key0 on; `there`: bits of the two groups of 16 that exist.
-    __device__ __forceinline__ void hide(f32x16& s, int32_t key0, uint32_t there) const
+    __device__ __forceinline__ void hide(float* s, int32_t key0, uint32_t there) const
     {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (!sees(key0 + key_of(i)) || !(there >> (i >> 3) & 1)) s[i] = -INF;
+        for (int i = 0; i < REGS; ++i)
+            if (!sees(key0 + place_of(i)) || !(there >> (i / (REGS / 2)) & 1)) s[i] = -INF;
     }
 
-    // The scores of 32 KT keys become probabilities; o and l follow the maximum.
-    template <int KT>
-    __device__ __forceinline__ void softmax(f32x16* s)
+    // The N scores that a lane holds become probabilities; o and l follow the maximum.
+    template <int N>
+    __device__ __forceinline__ void softmax(float* s)
     {
-        float mx = s[0][0];
+        float mx = s[0];
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-        mx = fmaxf(mx, other_half(mx));
+        for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
+        mx = row_max<M>(mx);
         if (__any(mx > m)) {
             const float up = fmaxf(m, mx), base = up == -INF ? 0.0f : up * c;
             const float alpha = __builtin_amdgcn_exp2f(m * c - base);  // 0 at the first keys
             m = up;
             l *= alpha;
 #pragma unroll
-            for (int d = 0; d < C::DT; ++d) o[d] *= alpha;
+            for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
         const float base = (m == -INF ? 0.0f : m * c) - (float)C::P_SHIFT;
         float sum = 0.0f;
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -base));
-                sum += s[t][i];
-            }
+        for (int i = 0; i < N; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base));
+            sum += s[i];
+        }
         l += sum;
     }
 
-    // o += V^T p for 32 keys, which lie in LDS from `v` on.  BAD: V holds elements that are not finite, and some rows do not see some
-    // of its keys: such elements are taken for zeros, and rows that see one get NaN there.
-    template <int PIECE, bool BAD>
-    __device__ __forceinline__ void values(const char* v, const f32x16& p, int32_t key0, uint32_t there)
+    // o += V^T p for 32 keys, which lie in LDS from `v` on
+    template <int PIECE>
+    __device__ __forceinline__ void values(const char* v, const float* p)
     {
-        const uint32_t lane = threadIdx.x & 63, i = lane & 15, side = lane >> 4 & 1, h = lane >> 5;
+        const uint32_t i = threadIdx.x & 15, side = row() / 16, g = group();
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
+        for (int st = 0; st < REGS / 8; ++st) {
             uint32_t w[4][C::NQ];
 #pragma unroll
             for (int e = 0; e < 4; ++e) pieces<C::HALF, C::NQ>(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], w[e]);
             u32x4 b[C::NQ];
 #pragma unroll
             for (int n = 0; n < C::NQ; ++n) b[n] = (u32x4){w[0][n], w[1][n], w[2][n], w[3][n]};
-            u32x4 see = {0, 0, 0, 0};
-            if constexpr (BAD) {
-                constexpr uint32_t one = C::HALF ? 0x3c00u : 0x3f80u;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (sees(key0 + key_of(8 * st + e)) && (there >> st & 1)) see[e / 2] |= one << 16 * (e & 1);
-            }
-#pragma unroll
-            for (int d = 0; d < C::DT; ++d) {
+            for (int d = 0; d < DT; ++d) {
                 u32x4 x[C::NK];
 #pragma unroll
                 for (int n = 0; n < C::NK; ++n) {
-                    s16x4 half[2];
+                    u32x2 half[2];
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const uint32_t row = 16 * st + 8 * g + 4 * h + (i >> 2), part = 4 * d + 2 * side + (i >> 1 & 1);
-                        const char* at = v + n * PIECE + row * C::LB + ((part ^ order<C::HD>(row)) << 4) + (i & 1) * 8;
-                        half[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t key = 4 * GROUPS * (2 * st + e) + 4 * g + (i >> 2), part = M / 8 * d + 2 * side + (i >> 1 & 1);
+                        const char* at = v + n * PIECE + key * C::LB + ((part ^ order<C::HD>(key)) << 4) + (i & 1) * 8;
+                        half[e] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
                     }
-                    const u32x2 y = __builtin_bit_cast(u32x2, half[0]), z = __builtin_bit_cast(u32x2, half[1]);
-                    x[n] = (u32x4){y[0], y[1], z[0], z[1]};
+                    x[n] = (u32x4){half[0][0], half[0][1], half[1][0], half[1][1]};
                 }
-                if constexpr (BAD) {
-                    constexpr uint32_t ones = C::HALF ? 0x3c003c00u : 0x3f803f80u;
-                    u32x4 bad;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) bad[e] = not_finite<C::HALF>(x[0][e]);
-                    x[0] &= ~bad;
-                    const f32x16 seen = mfma<C::HALF>(bad & ones, see, (f32x16)(0.0f));
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (seen[e] > 0.0f) o[d][e] = __builtin_nanf("");
-                }
-#pragma unroll
-                for (int k = C::NQ + C::NK - 2; k >= 0; --k)
-#pragma unroll
-                    for (int n = 0; n < C::NK; ++n)
-                        if (k - n >= 0 && k - n < C::NQ && (C::NK == 1 || k < C::NQ)) o[d] = mfma<C::HALF>(x[n], b[k - n], o[d]);
+                product(x, b, o[d]);
             }
         }
     }
+
+    // NaN where a row sees one of the `n` keys from key0 on whose value is marked.  Keys on no page are seen by nobody.
+    __device__ __forceinline__ void poison(const uint8_t* marks, int32_t key0, int32_t n, uint32_t there)
+    {
+        for (int32_t key = 0; key < n; ++key) {
+            const bool seen = sees(key0 + key) && (there >> (key >> 4) & 1);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < OQUADS; ++i) {
+                    if (M * d + 4 * GROUPS * i >= C::HD) continue;
+                    const uint32_t dim = M * d + place_of(4 * i);
+                    const uint32_t mark = seen ? (uint32_t)marks[key * C::PARTS + dim / (C::NK == 3 ? 4 : 8)] >> (C::NK == 3 ? 0 : dim & 4) : 0u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (mark >> e & 1) o[d][4 * i + e] = __builtin_nanf("");
+                }
+        }
+    }
+
+    __device__ __forceinline__ f32x4 quad(int d, int i) const { return (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}; }
+    __device__ __forceinline__ float exponent() const { return m == -INF ? -INF : m * c; }
 };
 
 // Results of keys that are split over workgroups: per split and row of the output (token, head) the sums, the exponent c m that they are
@@ -482,12 +521,13 @@ __device__ __forceinline__ uint32_t first_slot(const AttnArgs& a, uint32_t b, ui
 }
 
 template <typename C>
-__global__ __launch_bounds__(256, C::NK == 3 && C::HD > 96 ? 1 : 2) void attention_wide_kernel(AttnArgs a, uint32_t slots, uint32_t splits, uint32_t narrow_rows, Partial part)
+__global__ __launch_bounds__(256, (C::NK == 3 || C::NQ > 1) && C::HD > 96 ? 1 : 2) void attention_wide_kernel(AttnArgs a, uint32_t slots, uint32_t splits, uint32_t narrow_rows, Partial part)
 {
     typedef Wide<C> W;
     constexpr int TILE = W::TILE, KT = TILE / 32;
     __shared__ __attribute__((aligned(1024))) char lds[W::LDS];
     __shared__ uint32_t bad[2];
+    __shared__ uint8_t marks[TILE * C::PARTS];
     char *const lk = lds, *const lv = lds + W::S::BYTES;
     const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;  // late rows, which see most keys, first
     uint32_t lo = 0, up = a.batch;
@@ -506,7 +546,7 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 96 ? 1 : 2) void attenti
     const int32_t per = (span.total + (int32_t)splits - 1) / (int32_t)splits, from = per * (int32_t)split;
     const int32_t to = from + per < span.total ? from + per : span.total;
     const bool works = mine < end;
-    Rows<C> w;
+    Rows<C, 32> w;
     w.begin(a, r, kh, works ? mine : row0, rows);
     // whether every row of the workgroup sees all of a tile
     const int32_t all_hi = [&] {
@@ -518,7 +558,7 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 96 ? 1 : 2) void attenti
     if (tid < 2) bad[tid] = 0;
     if (from < to) {
         typename W::S sk, sv;
-        Place<C, TILE> p = place<C, TILE>(a, r, kh, span.at(from) * TILE);
+        Place p = place<C, TILE>(a, r, kh, span.at(from) * TILE);
         sk.fetch(a.k, a, r, p, span.at(from) * TILE, tid);
         sv.fetch(a.v, a, r, p, span.at(from) * TILE, tid);
         for (int32_t t = from; t < to; ++t) {
@@ -526,12 +566,11 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 96 ? 1 : 2) void attenti
             const bool mixed = !(key0 + TILE <= all_hi && (key0 >= all_lo || key0 + TILE <= w.sinks)) || p.there != ~0u;
             __syncthreads();  // everybody is done with the tile before
             if (tid == 0) bad[(t + 1) & 1] = 0;
-            sk.template store<false>(lk, tid);
+            sk.template store<false>(lk, marks, tid);
             if (mixed) {
-                if (sv.any_not_finite(tid)) bad[t & 1] = 1;
-                sv.template store<true>(lv, tid);
+                if (sv.template store<true>(lv, marks, tid)) bad[t & 1] = 1;
             } else {
-                sv.template store<false>(lv, tid);
+                sv.template store<false>(lv, marks, tid);
             }
             const uint32_t there = p.there;
             if (t + 1 < to) {
@@ -541,60 +580,55 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 96 ? 1 : 2) void attenti
             }
             __syncthreads();
             if (!works || !w.some(key0, TILE)) continue;
-            f32x16 s[KT];
+            float s[16 * KT];
 #pragma unroll
-            for (int n = 0; n < KT; ++n) s[n] = w.template scores<W::S::PIECE>(lk + n * 32 * C::LB);
+            for (int n = 0; n < KT; ++n) w.template scores<W::S::PIECE>(lk + n * 32 * C::LB, s + 16 * n);
             if (!w.all(key0, TILE) || there != ~0u) {
 #pragma unroll
-                for (int n = 0; n < KT; ++n) w.hide(s[n], key0 + 32 * n, there >> 2 * n);
+                for (int n = 0; n < KT; ++n) w.hide(s + 16 * n, key0 + 32 * n, there >> 2 * n);
             }
-            w.template softmax<KT>(s);
-            if (mixed && bad[t & 1]) {
+            w.template softmax<16 * KT>(s);
 #pragma unroll
-                for (int n = 0; n < KT; ++n) w.template values<W::S::PIECE, true>(lv + n * 32 * C::LB, s[n], key0 + 32 * n, there >> 2 * n);
-            } else {
-#pragma unroll
-                for (int n = 0; n < KT; ++n) w.template values<W::S::PIECE, false>(lv + n * 32 * C::LB, s[n], key0 + 32 * n, there >> 2 * n);
-            }
+            for (int n = 0; n < KT; ++n) w.template values<W::S::PIECE>(lv + n * 32 * C::LB, s + 16 * n);
+            if (mixed && bad[t & 1]) w.poison(marks, key0, TILE, there);
         }
     }
     if (mine + j >= end || !works) return;
-    const float l = w.l + other_half(w.l);
+    const float l = row_sum<32>(w.l);
     const uint32_t row = mine + j, token = r.first + row / a.group, head = kh * a.group + row % a.group;
     if (splits == 1) {
         typename C::TQ* out = static_cast<typename C::TQ*>(a.out) + (size_t)token * a.out_stride + (size_t)head * C::HD;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int d = 0; d < C::DT; ++d)
+        for (int d = 0; d < w.DT; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (32 * d + 8 * i < C::HD) store4(out + 32 * d + 8 * i + 4 * h, (f32x4){w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]} * inv);
+                if (32 * d + 8 * i < C::HD) store4(out + 32 * d + 8 * i + 4 * h, w.quad(d, i) * inv);
     } else {
         const uint64_t at = (uint64_t)split * part.rows + (uint64_t)token * a.heads + head;
         if (h == 0) {
-            part.ml[2 * at] = w.m == -INF ? -INF : w.m * w.c;
+            part.ml[2 * at] = w.exponent();
             part.ml[2 * at + 1] = l;
         }
         if (from >= to) return;  // (the joining kernel does not look at sums whose l is 0)
 #pragma unroll
-        for (int d = 0; d < C::DT; ++d)
+        for (int d = 0; d < w.DT; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (32 * d + 8 * i < C::HD)
-                    store4(part.o + at * C::HD + 32 * d + 8 * i + 4 * h, (f32x4){w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]});
+                if (32 * d + 8 * i < C::HD) store4(part.o + at * C::HD + 32 * d + 8 * i + 4 * h, w.quad(d, i));
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Few rows (a single new token, mostly): a workgroup takes 32 rows of a sequence and key head at a time; its four waves take the tiles of 32 keys in
+// Few rows (a single new token, mostly): a workgroup takes 16 rows of a sequence and key head at a time; its four waves take the tiles of 32 keys in
 // turn, each through LDS of its own, without barriers, and are joined at the end.
 // ------------------------------------------------------------------------------------------------------------
-constexpr uint32_t NARROW_ROWS = 32;
+constexpr uint32_t NARROW_ROWS = 16;
 
 template <typename C>
 struct Narrow {
     typedef Stage<C, 32, 64> S;
-    static constexpr int JOIN = 32 * (C::DT * 32 + 1) * 4;  // a wave's sums, rows padded against bank conflicts
+    static constexpr int PITCH = C::HD + 1, JOIN = 16 * PITCH * 4;  // a wave's sums, rows padded against bank conflicts
     static constexpr int WAVE = S::BYTES > JOIN ? (S::BYTES + 15) / 16 * 16 : (JOIN + 15) / 16 * 16;
     static constexpr int LDS = 4 * WAVE;
 };
@@ -610,12 +644,13 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 64 ? 1 : 2) void attenti
 {
     typedef Narrow<C> W;
     __shared__ __attribute__((aligned(1024))) char lds[W::LDS];
-    __shared__ float ml[4][32][2];
+    __shared__ float ml[4][16][2];
+    __shared__ uint8_t marks[4][32 * C::PARTS];
     const uint32_t split = blockIdx.x % splits, rest = blockIdx.x / splits, kh = rest % a.kv_heads, b = rest / a.kv_heads;
     const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, C::PAGED, b);
     const uint32_t rows = r.n * a.group;
     if (rows > most_rows) return;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 31, h = lane >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15;
     char* const mine = lds + wave * W::WAVE;
     for (uint32_t row0 = 0; row0 < rows; row0 += NARROW_ROWS) {
         const uint32_t end = row0 + NARROW_ROWS < rows ? row0 + NARROW_ROWS : rows;
@@ -631,43 +666,44 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 64 ? 1 : 2) void attenti
             }
             continue;
         }
-        Rows<C> w;
+        Rows<C, 16> w;
         w.begin(a, r, kh, row0, rows);
         int32_t t = from + (int32_t)wave;
         if (t < to) {
             typename W::S sk, sv;
-            Place<C, 32> p = place<C, 32>(a, r, kh, span.at(t) * 32);
+            Place p = place<C, 32>(a, r, kh, span.at(t) * 32);
             sk.fetch(a.k, a, r, p, span.at(t) * 32, lane);
             sv.fetch(a.v, a, r, p, span.at(t) * 32, lane);
             for (; t < to; t += 4) {
                 const int32_t key0 = span.at(t) * 32;
                 const uint32_t there = p.there;
                 const bool mixed = !w.all(key0, 32) || there != ~0u;
-                sk.template store<false>(mine, lane);
+                sk.template store<false>(mine, marks[wave], lane);
                 const bool more = t + 4 < to;
                 if (more) {
                     p = place<C, 32>(a, r, kh, span.at(t + 4) * 32);
                     sk.fetch(a.k, a, r, p, span.at(t + 4) * 32, lane);
                 }
                 wave_sync();
-                f32x16 s = w.template scores<W::S::PIECE>(mine);
+                float s[8];
+                w.template scores<W::S::PIECE>(mine, s);
                 wave_sync();
                 if (mixed) w.hide(s, key0, there);
-                const bool bad = mixed && __any(sv.any_not_finite(lane));
-                if (mixed) sv.template store<true>(mine, lane);
-                else sv.template store<false>(mine, lane);
+                bool bad = false;
+                if (mixed) bad = __any(sv.template store<true>(mine, marks[wave], lane));
+                else sv.template store<false>(mine, marks[wave], lane);
                 if (more) sv.fetch(a.v, a, r, p, span.at(t + 4) * 32, lane);
-                w.template softmax<1>(&s);
+                w.template softmax<8>(s);
                 wave_sync();
-                if (bad) w.template values<W::S::PIECE, true>(mine, s, key0, there);
-                else w.template values<W::S::PIECE, false>(mine, s, key0, there);
+                w.template values<W::S::PIECE>(mine, s);
+                if (bad) w.poison(marks[wave], key0, 32, there);
                 wave_sync();
             }
         }
         // join the waves: all relative to the largest exponent
-        const float l = w.l + other_half(w.l);
-        if (h == 0) {
-            ml[wave][j][0] = w.m == -INF ? -INF : w.m * w.c;
+        const float l = row_sum<16>(w.l);
+        if (lane < 16) {
+            ml[wave][j][0] = w.exponent();
             ml[wave][j][1] = l;
         }
         __syncthreads();
@@ -675,13 +711,12 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 64 ? 1 : 2) void attenti
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i][j][0]);
         const float base = top == -INF ? 0.0f : top;
-        const float f = __builtin_amdgcn_exp2f((w.m == -INF ? -INF : w.m * w.c) - base);
+        const float f = __builtin_amdgcn_exp2f(w.exponent() - base);
         float* const sums = reinterpret_cast<float*>(mine);
-        constexpr int PITCH = C::DT * 32 + 1;
 #pragma unroll
-        for (int d = 0; d < C::DT; ++d)
+        for (int d = 0; d < w.DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sums[j * PITCH + 32 * d + w.key_of(i)] = w.o[d][i] * f;
+            for (int i = 0; i < 4; ++i) sums[j * W::PITCH + 16 * d + w.place_of(i)] = w.o[d][i] * f;
         __syncthreads();
         // the row's sums, HD consecutive columns of a row by consecutive threads
         for (uint32_t x = tid; x < (end - row0) * (C::HD / 4); x += 256) {
@@ -689,7 +724,7 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 64 ? 1 : 2) void attenti
             f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float* from_wave = reinterpret_cast<const float*>(lds + i * W::WAVE) + row * PITCH + col;
+                const float* from_wave = reinterpret_cast<const float*>(lds + i * W::WAVE) + row * W::PITCH + col;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] += from_wave[e];
             }
