@@ -514,10 +514,22 @@ struct Wide {
     static constexpr int LDS = 2 * S::BYTES;
 };
 
-// Tiles of rows of all sequences, without knowing their lengths: those of row b begin at slot first_row(b) * group / 128 + b.
-__device__ __forceinline__ uint32_t first_slot(const AttnArgs& a, uint32_t b, uint32_t tokens_before)
+// Blocks of `size` rows of all sequences are numbered without a sum over their lengths: those of row b of the batch, which begins at token
+// `before`, start at number before * group / size + b, which leaves each row as many as it can need.
+__device__ __forceinline__ uint32_t first_slot(const AttnArgs& a, uint32_t b, uint32_t before, uint32_t size)
 {
-    return (uint32_t)((uint64_t)tokens_before * a.group / WIDE_ROWS) + b;
+    return (uint32_t)((uint64_t)before * a.group / size) + b;
+}
+// the row of the batch that has block `slot`, if any has
+__device__ __forceinline__ uint32_t row_of_slot(const AttnArgs& a, uint32_t slot, uint32_t size)
+{
+    uint32_t lo = 0, up = a.batch;
+    while (up - lo > 1) {
+        const uint32_t mid = (lo + up) / 2;
+        if (first_slot(a, mid, clamped_start(a.starts, mid, a.tokens), size) <= slot) lo = mid;
+        else up = mid;
+    }
+    return lo;
 }
 
 template <typename C>
@@ -530,16 +542,10 @@ __global__ __launch_bounds__(256, (C::NK == 3 || C::NQ > 1) && C::HD > 96 ? 1 : 
     __shared__ uint8_t marks[TILE * C::PARTS];
     char *const lk = lds, *const lv = lds + W::S::BYTES;
     const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;  // late rows, which see most keys, first
-    uint32_t lo = 0, up = a.batch;
-    while (up - lo > 1) {
-        const uint32_t mid = (lo + up) / 2;
-        if (first_slot(a, mid, clamped_start(a.starts, mid, a.tokens)) <= slot) lo = mid;
-        else up = mid;
-    }
-    const uint32_t b = __builtin_amdgcn_readfirstlane(lo);
+    const uint32_t b = __builtin_amdgcn_readfirstlane(row_of_slot(a, slot, WIDE_ROWS));
     const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, C::PAGED, b);
-    const uint32_t rows = r.n * a.group, row0 = (slot - first_slot(a, b, r.first)) * WIDE_ROWS;
-    if (slot < first_slot(a, b, r.first) || row0 >= rows || rows <= narrow_rows) return;
+    const uint32_t rows = r.n * a.group, before = first_slot(a, b, r.first, WIDE_ROWS), row0 = (slot - before) * WIDE_ROWS;
+    if (slot < before || row0 >= rows || rows <= narrow_rows) return;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = tid & 31, h = tid >> 5 & 1;
     const uint32_t end = row0 + WIDE_ROWS < rows ? row0 + WIDE_ROWS : rows, mine = row0 + 32 * wave;
     const Span span = span_of(a, r, row0, end - 1, TILE);
@@ -561,6 +567,7 @@ __global__ __launch_bounds__(256, (C::NK == 3 || C::NQ > 1) && C::HD > 96 ? 1 : 
         Place p = place<C, TILE>(a, r, kh, span.at(from) * TILE);
         sk.fetch(a.k, a, r, p, span.at(from) * TILE, tid);
         sv.fetch(a.v, a, r, p, span.at(from) * TILE, tid);
+        Place ahead = place<C, TILE>(a, r, kh, span.at(from + 1) * TILE);  // (the table's entries are asked for a tile before the keys)
         for (int32_t t = from; t < to; ++t) {
             const int32_t key0 = span.at(t) * TILE;
             const bool mixed = !(key0 + TILE <= all_hi && (key0 >= all_lo || key0 + TILE <= w.sinks)) || p.there != ~0u;
@@ -574,9 +581,10 @@ __global__ __launch_bounds__(256, (C::NK == 3 || C::NQ > 1) && C::HD > 96 ? 1 : 
             }
             const uint32_t there = p.there;
             if (t + 1 < to) {
-                p = place<C, TILE>(a, r, kh, span.at(t + 1) * TILE);
+                p = ahead;
                 sk.fetch(a.k, a, r, p, span.at(t + 1) * TILE, tid);
                 sv.fetch(a.v, a, r, p, span.at(t + 1) * TILE, tid);
+                ahead = place<C, TILE>(a, r, kh, span.at(t + 2) * TILE);
             }
             __syncthreads();
             if (!works || !w.some(key0, TILE)) continue;
@@ -620,7 +628,7 @@ __global__ __launch_bounds__(256, (C::NK == 3 || C::NQ > 1) && C::HD > 96 ? 1 : 
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Few rows (a single new token, mostly): a workgroup takes 16 rows of a sequence and key head at a time; its four waves take the tiles of 32 keys in
+// Few rows (a single new token, mostly): a workgroup takes 16 rows of a sequence and key head at a time; its waves take the tiles of 32 keys in
 // turn, each through LDS of its own, without barriers, and are joined at the end.
 // ------------------------------------------------------------------------------------------------------------
 constexpr uint32_t NARROW_ROWS = 16;
@@ -628,9 +636,10 @@ constexpr uint32_t NARROW_ROWS = 16;
 template <typename C>
 struct Narrow {
     typedef Stage<C, 32, 64> S;
+    static constexpr int WAVES = C::NK == 3 && C::HD > 64 ? 4 : 8;
     static constexpr int PITCH = C::HD + 1, JOIN = 16 * PITCH * 4;  // a wave's sums, rows padded against bank conflicts
-    static constexpr int WAVE = S::BYTES > JOIN ? (S::BYTES + 15) / 16 * 16 : (JOIN + 15) / 16 * 16;
-    static constexpr int LDS = 4 * WAVE;
+    static constexpr int WAVE = ((S::BYTES > JOIN ? S::BYTES : JOIN) + 15) / 16 * 16;
+    static constexpr int LDS = WAVES * WAVE;
 };
 
 __device__ __forceinline__ void wave_sync()
@@ -639,66 +648,81 @@ __device__ __forceinline__ void wave_sync()
     __builtin_amdgcn_wave_barrier();
 }
 
+// by_slot: a workgroup per block of 16 rows (first_slot); otherwise one per row of the batch, which takes its blocks one after the other
 template <typename C>
-__global__ __launch_bounds__(256, C::NK == 3 && C::HD > 64 ? 1 : 2) void attention_narrow_kernel(AttnArgs a, uint32_t splits, uint32_t most_rows, Partial part)
+__global__ __launch_bounds__(Narrow<C>::WAVES * 64, Narrow<C>::WAVES / 4) void attention_narrow_kernel(AttnArgs a, uint32_t by_slot, uint32_t splits, uint32_t most_rows, Partial part)
 {
     typedef Narrow<C> W;
+    constexpr int WAVES = W::WAVES;
     __shared__ __attribute__((aligned(1024))) char lds[W::LDS];
-    __shared__ float ml[4][16][2];
-    __shared__ uint8_t marks[4][32 * C::PARTS];
-    const uint32_t split = blockIdx.x % splits, rest = blockIdx.x / splits, kh = rest % a.kv_heads, b = rest / a.kv_heads;
+    __shared__ float ml[WAVES][16][2];
+    __shared__ uint8_t marks[WAVES][32 * C::PARTS];
+    const uint32_t split = blockIdx.x % splits, rest = blockIdx.x / splits, kh = rest % a.kv_heads, slot = rest / a.kv_heads;
+    const uint32_t b = by_slot ? __builtin_amdgcn_readfirstlane(row_of_slot(a, slot, NARROW_ROWS)) : slot;
     const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, C::PAGED, b);
     const uint32_t rows = r.n * a.group;
     if (rows > most_rows) return;
+    uint32_t block = 0, blocks = (rows + NARROW_ROWS - 1) / NARROW_ROWS;
+    if (by_slot) {
+        const uint32_t before = first_slot(a, b, r.first, NARROW_ROWS);
+        if (slot < before || slot - before >= blocks) return;
+        block = slot - before;
+        blocks = block + 1;
+    }
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15;
     char* const mine = lds + wave * W::WAVE;
-    for (uint32_t row0 = 0; row0 < rows; row0 += NARROW_ROWS) {
-        const uint32_t end = row0 + NARROW_ROWS < rows ? row0 + NARROW_ROWS : rows;
+    for (; block < blocks; ++block) {
+        const uint32_t row0 = block * NARROW_ROWS, end = row0 + NARROW_ROWS < rows ? row0 + NARROW_ROWS : rows;
         const Span span = span_of(a, r, row0, end - 1, 32);
         int32_t per = (span.total + (int32_t)splits - 1) / (int32_t)splits;
-        if (per < 4) per = 4;  // a tile for each wave
+        if (per < WAVES) per = WAVES;  // a tile for each wave
         const int32_t from = per * (int32_t)split, to = from + per < span.total ? from + per : span.total;
         if (splits > 1 && from >= to) {  // nothing left for this split
-            for (uint32_t row = row0 + tid; row < end; row += 256) {
+            if (tid < end - row0) {
+                const uint32_t row = row0 + tid;
                 const uint64_t at = (uint64_t)split * part.rows + (uint64_t)(r.first + row / a.group) * a.heads + kh * a.group + row % a.group;
                 part.ml[2 * at] = -INF;
                 part.ml[2 * at + 1] = 0.0f;
             }
             continue;
         }
+        int32_t t = from + (int32_t)wave;
+        typename W::S sk, sv;
+        Place now, next;
+        if (t < to) {  // (before the rows' q: the first keys take longest)
+            now = place<C, 32>(a, r, kh, span.at(t) * 32);
+            sk.fetch(a.k, a, r, now, span.at(t) * 32, lane);
+            sv.fetch(a.v, a, r, now, span.at(t) * 32, lane);
+            next = place<C, 32>(a, r, kh, span.at(t + WAVES) * 32);  // (the table's entries are asked for a tile before the keys)
+        }
         Rows<C, 16> w;
         w.begin(a, r, kh, row0, rows);
-        int32_t t = from + (int32_t)wave;
-        if (t < to) {
-            typename W::S sk, sv;
-            Place p = place<C, 32>(a, r, kh, span.at(t) * 32);
-            sk.fetch(a.k, a, r, p, span.at(t) * 32, lane);
-            sv.fetch(a.v, a, r, p, span.at(t) * 32, lane);
-            for (; t < to; t += 4) {
-                const int32_t key0 = span.at(t) * 32;
-                const uint32_t there = p.there;
-                const bool mixed = !w.all(key0, 32) || there != ~0u;
-                sk.template store<false>(mine, marks[wave], lane);
-                const bool more = t + 4 < to;
-                if (more) {
-                    p = place<C, 32>(a, r, kh, span.at(t + 4) * 32);
-                    sk.fetch(a.k, a, r, p, span.at(t + 4) * 32, lane);
-                }
-                wave_sync();
-                float s[8];
-                w.template scores<W::S::PIECE>(mine, s);
-                wave_sync();
-                if (mixed) w.hide(s, key0, there);
-                bool bad = false;
-                if (mixed) bad = __any(sv.template store<true>(mine, marks[wave], lane));
-                else sv.template store<false>(mine, marks[wave], lane);
-                if (more) sv.fetch(a.v, a, r, p, span.at(t + 4) * 32, lane);
-                w.template softmax<8>(s);
-                wave_sync();
-                w.template values<W::S::PIECE>(mine, s);
-                if (bad) w.poison(marks[wave], key0, 32, there);
-                wave_sync();
+        for (; t < to; t += WAVES) {
+            const int32_t key0 = span.at(t) * 32;
+            const uint32_t there = now.there;
+            const bool mixed = !w.all(key0, 32) || there != ~0u, more = t + WAVES < to;
+            sk.template store<false>(mine, marks[wave], lane);
+            if (more) {
+                now = next;
+                sk.fetch(a.k, a, r, now, span.at(t + WAVES) * 32, lane);
             }
+            wave_sync();
+            float s[8];
+            w.template scores<W::S::PIECE>(mine, s);
+            wave_sync();
+            if (mixed) w.hide(s, key0, there);
+            bool bad = false;
+            if (mixed) bad = __any(sv.template store<true>(mine, marks[wave], lane));
+            else sv.template store<false>(mine, marks[wave], lane);
+            if (more) {
+                sv.fetch(a.v, a, r, now, span.at(t + WAVES) * 32, lane);
+                next = place<C, 32>(a, r, kh, span.at(t + 2 * WAVES) * 32);
+            }
+            w.template softmax<8>(s);
+            wave_sync();
+            w.template values<W::S::PIECE>(mine, s);
+            if (bad) w.poison(marks[wave], key0, 32, there);
+            wave_sync();
         }
         // join the waves: all relative to the largest exponent
         const float l = row_sum<16>(w.l);
@@ -709,31 +733,29 @@ __global__ __launch_bounds__(256, C::NK == 3 && C::HD > 64 ? 1 : 2) void attenti
         __syncthreads();
         float top = -INF;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i][j][0]);
-        const float base = top == -INF ? 0.0f : top;
-        const float f = __builtin_amdgcn_exp2f(w.exponent() - base);
+        for (int i = 0; i < WAVES; ++i) top = fmaxf(top, ml[i][j][0]);
+        const float f = __builtin_amdgcn_exp2f(w.exponent() - (top == -INF ? 0.0f : top));
         float* const sums = reinterpret_cast<float*>(mine);
 #pragma unroll
         for (int d = 0; d < w.DT; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sums[j * W::PITCH + 16 * d + w.place_of(i)] = w.o[d][i] * f;
         __syncthreads();
-        // the row's sums, HD consecutive columns of a row by consecutive threads
-        for (uint32_t x = tid; x < (end - row0) * (C::HD / 4); x += 256) {
+        // HD consecutive columns of a row by consecutive threads
+        for (uint32_t x = tid; x < (end - row0) * (C::HD / 4); x += WAVES * 64) {
             const uint32_t row = x / (C::HD / 4), col = x % (C::HD / 4) * 4;
             f32x4 y = {0.f, 0.f, 0.f, 0.f};
+            float mx = -INF, sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < WAVES; ++i) {
                 const float* from_wave = reinterpret_cast<const float*>(lds + i * W::WAVE) + row * W::PITCH + col;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] += from_wave[e];
+                mx = fmaxf(mx, ml[i][row][0]);
             }
-            float mx = -INF, sum = 0.0f;
+            const float base = mx == -INF ? 0.0f : mx;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, ml[i][row][0]);
-            const float bs = mx == -INF ? 0.0f : mx;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum += ml[i][row][1] * __builtin_amdgcn_exp2f(ml[i][row][0] - bs);
+            for (int i = 0; i < WAVES; ++i) sum += ml[i][row][1] * __builtin_amdgcn_exp2f(ml[i][row][0] - base);
             const uint32_t token = r.first + (row0 + row) / a.group, head = kh * a.group + (row0 + row) % a.group;
             if (splits == 1) {
                 store4(static_cast<typename C::TQ*>(a.out) + (size_t)token * a.out_stride + (size_t)head * C::HD + col, sum == 0.0f ? (f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / sum));
@@ -756,6 +778,7 @@ struct Plan {
     uint32_t slots;                       // of the wide kernel
     uint32_t wide_splits, narrow_splits;
     uint32_t narrow_rows;                 // rows of a sequence and key head up to which the narrow kernel takes them
+    bool by_slot;                         // ... in workgroups of 16 rows each
     Partial part;
 };
 
@@ -768,12 +791,11 @@ int launch(Ctx* ctx, const AttnArgs& a, const Plan& p)
                            p.narrow ? p.narrow_rows : 0, p.part);
         rc = hip_check(ctx, hipGetLastError(), "attention_wide_kernel launch");
     }
-    if constexpr (C::PAGED) {
-        if (!rc && p.narrow) {
-            hipLaunchKernelGGL((attention_narrow_kernel<C>), dim3(a.batch * a.kv_heads * p.narrow_splits), dim3(256), 0, ctx->stream, a, p.narrow_splits,
-                               p.narrow_rows, p.part);
-            rc = hip_check(ctx, hipGetLastError(), "attention_narrow_kernel launch");
-        }
+    if (!rc && p.narrow) {
+        const uint32_t slots = p.by_slot ? (uint32_t)((uint64_t)a.tokens * a.group / NARROW_ROWS) + a.batch : a.batch;
+        hipLaunchKernelGGL((attention_narrow_kernel<C>), dim3(slots * a.kv_heads * p.narrow_splits), dim3(Narrow<C>::WAVES * 64), 0, ctx->stream, a,
+                           (uint32_t)p.by_slot, p.narrow_splits, p.narrow_rows, p.part);
+        rc = hip_check(ctx, hipGetLastError(), "attention_narrow_kernel launch");
     }
     return rc;
 }

@@ -111,55 +111,90 @@ int launch_plain(Ctx* ctx, const AttnArgs& a)
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins what the splits of a row have: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).  A workgroup per token and head; GROUPS
-// of threads take the splits in turn.
+// Joins what the splits of a row have: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).  A workgroup takes `rows` rows of up to 16 of a
+// sequence and key head (blocks of 16 are numbered as first_slot does); of a row's threads head_dim / 4 take four columns each, and `groups` sets of
+// them every groups-th split.
 // ---------------------------------------------------------------------------------------------
+constexpr uint32_t JOIN_ROWS = 16;
+
 template <typename TQ>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::Partial part, uint32_t wide_splits, uint32_t narrow_splits, uint32_t narrow_rows)
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::Partial part, uint32_t rows, uint32_t groups, uint32_t wide_splits,
+                                                             uint32_t narrow_splits, uint32_t narrow_rows)
 {
     __shared__ float sums[256][4];
-    __shared__ float red[8];
-    const uint32_t t = blockIdx.x / a.heads, head = blockIdx.x % a.heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t b = row_of_token(a.starts, a.batch, a.tokens, t);
-    const uint32_t first = clamped_start(a.starts, b, a.tokens), end = clamped_start(a.starts, b + 1, a.tokens);
-    if (t < first || t >= end) return;
-    const uint32_t splits = (end - first) * a.group <= narrow_rows ? narrow_splits : wide_splits;
-    if (splits == 1) return;
+    __shared__ float mls[256][2];
+    const uint32_t parts = (JOIN_ROWS + rows - 1) / rows, tid = threadIdx.x, lanes = a.head_dim / 4;
+    const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, slot = rest / parts;
+    const uint32_t b = attn::row_of_slot(a, slot, JOIN_ROWS);
+    const uint32_t first = clamped_start(a.starts, b, a.tokens), end = clamped_start(a.starts, b + 1, a.tokens), before = attn::first_slot(a, b, first, JOIN_ROWS);
+    if (slot < before || end <= first) return;
+    const uint32_t count = (end - first) * a.group, row0 = (slot - before) * JOIN_ROWS + rest % parts * rows;
+    const uint32_t splits = count <= narrow_rows ? narrow_splits : wide_splits;
+    if (row0 >= count || splits == 1) return;
+    const uint32_t set = tid / lanes, mine = set / groups, g = set % groups, col = tid % lanes * 4, row = row0 + mine;
+    const bool works = mine < rows && row < count && row < (slot - before + 1) * JOIN_ROWS;
+    const uint32_t t = first + row / a.group, head = kh * a.group + row % a.group;
     const uint64_t at = (uint64_t)t * a.heads + head;
-    float top = -__builtin_inff();
-    for (uint32_t s = tid; s < splits; s += 256) top = fmaxf(top, part.ml[2 * (s * part.rows + at)]);
-    top = wave_max(top);
-    if (lane == 0) red[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    float l = 0.0f;
-    for (uint32_t s = tid; s < splits; s += 256) {
-        const float* ml = part.ml + 2 * (s * part.rows + at);
-        l += ml[1] == 0.0f ? 0.0f : ml[1] * __builtin_amdgcn_exp2f(ml[0] - base);
-    }
-    l = wave_sum(l);
-    if (lane == 0) red[4 + wave] = l;
-    __syncthreads();
-    l = (red[4] + red[5]) + (red[6] + red[7]);
-    const uint32_t lanes = a.head_dim / 4, groups = 256 / lanes, g = tid / lanes, col = tid % lanes * 4;
+    float top = -__builtin_inff(), l = 0.0f;
     attn::f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    if (g < groups)
-        for (uint32_t s = g; s < splits; s += groups) {
-            const float* ml = part.ml + 2 * (s * part.rows + at);
-            if (ml[1] != 0.0f) y += *reinterpret_cast<const attn::f32x4*>(part.o + (s * part.rows + at) * a.head_dim + col) * __builtin_amdgcn_exp2f(ml[0] - base);
+    if (works) {
+        constexpr uint32_t AHEAD = 8;  // splits whose results are asked for together
+        for (uint32_t s0 = g; s0 < splits; s0 += AHEAD * groups) {
+            float m[AHEAD], lm[AHEAD];
+            attn::f32x4 x[AHEAD];
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; ++i) {
+                const uint32_t s = s0 + i * groups < splits ? s0 + i * groups : splits - 1;
+                const uint64_t where = s * part.rows + at;
+                m[i] = part.ml[2 * where];
+                lm[i] = s0 + i * groups < splits ? part.ml[2 * where + 1] : 0.0f;
+                x[i] = *reinterpret_cast<const attn::f32x4*>(part.o + where * a.head_dim + col);  // (anything where l is 0)
+            }
+            float up = top;
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; ++i) up = fmaxf(up, m[i]);
+            const float base = up == -__builtin_inff() ? 0.0f : up, alpha = __builtin_amdgcn_exp2f(top - base);
+            top = up;
+            l *= alpha;
+            y *= alpha;
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; ++i) {
+                const float f = __builtin_amdgcn_exp2f(m[i] - base);
+                l += lm[i] == 0.0f ? 0.0f : lm[i] * f;  // (NaN is not)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] += lm[i] == 0.0f ? 0.0f : x[i][e] * f;
+            }
         }
+    }
     *reinterpret_cast<attn::f32x4*>(sums[tid]) = y;
+    mls[tid][0] = top;
+    mls[tid][1] = l;
     __syncthreads();
-    if (tid >= lanes) return;
-    for (uint32_t i = 1; i < groups; ++i) y += *reinterpret_cast<const attn::f32x4*>(sums[tid + i * lanes]);
+    if (!works || g != 0) return;
+    for (uint32_t i = 1; i < groups; ++i) top = fmaxf(top, mls[tid + i * lanes][0]);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    l = 0.0f;
+    y = (attn::f32x4){0.f, 0.f, 0.f, 0.f};
+    for (uint32_t i = 0; i < groups; ++i) {
+        const float lm = mls[tid + i * lanes][1];
+        if (lm == 0.0f) continue;
+        const float f = __builtin_amdgcn_exp2f(mls[tid + i * lanes][0] - base);
+        l += lm * f;
+        y += *reinterpret_cast<const attn::f32x4*>(sums[tid + i * lanes]) * f;
+    }
     attn::store4(static_cast<TQ*>(a.out) + (size_t)t * a.out_stride + (size_t)head * a.head_dim + col, l == 0.0f ? (attn::f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / l));
 }
 
 template <typename TQ>
 int launch_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
 {
-    hipLaunchKernelGGL((attention_join_kernel<TQ>), dim3(a.tokens * a.heads), dim3(256), 0, ctx->stream, a, p.part, p.wide ? p.wide_splits : 1,
+    const uint32_t lanes = a.head_dim / 4, splits = std::max(p.wide_splits, p.narrow_splits);
+    uint32_t groups = 1;
+    while (groups < 16 && groups * 4 < splits && 2 * groups * lanes <= 256) groups *= 2;
+    const uint32_t rows = std::min(JOIN_ROWS, 256 / (lanes * groups)), parts = (JOIN_ROWS + rows - 1) / rows;
+    const uint64_t slots = (uint64_t)a.tokens * a.group / JOIN_ROWS + a.batch, grid = slots * parts * a.kv_heads;
+    if (grid > 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
+    hipLaunchKernelGGL((attention_join_kernel<TQ>), dim3((uint32_t)grid), dim3(256), 0, ctx->stream, a, p.part, rows, groups, p.wide ? p.wide_splits : 1,
                        p.narrow ? p.narrow_splits : 1, p.narrow ? p.narrow_rows : 0);
     return hip_check(ctx, hipGetLastError(), "attention_join_kernel launch");
 }
@@ -182,25 +217,27 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     // keys that a row may see at most
     uint64_t keys = a.paged ? (uint64_t)a.table_width << a.page_shift : a.tokens;
     keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + 1 + a.sinks + attn::WIDE_ROWS);
-    p->narrow = a.paged;
-    p->wide = !a.paged || (a.tokens > a.batch && rows > attn::NARROW_ROWS);
+    const uint64_t wide_items = (rows + attn::WIDE_ROWS - 1) / attn::WIDE_ROWS * a.kv_heads;
+    const bool few = wide_items <= cus / 8;  // so few blocks of 128 rows that most of the device would idle: blocks of 16
+    p->narrow = a.paged || few;
+    p->wide = !few && !(a.paged && a.tokens <= a.batch);
+    p->by_slot = few && a.tokens > a.batch;
     p->narrow_rows = p->wide ? attn::NARROW_ROWS : 0xffffffffu;
     p->wide_splits = p->narrow_splits = 1;
     p->slots = (uint32_t)(rows / attn::WIDE_ROWS) + a.batch;
     if (p->narrow) {
-        const uint64_t items = (uint64_t)a.batch * a.kv_heads;
-        p->narrow_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(8 * cus + items - 1) / items, keys / 512, 256}));
+        const uint64_t items = (p->by_slot ? (rows + attn::NARROW_ROWS - 1) / attn::NARROW_ROWS : a.batch) * a.kv_heads;
+        // every CU its eight waves, of at least 256 keys to a workgroup; where lengths may differ, shares of 1024 keys that can be dealt out evenly
+        const uint64_t full = std::min((cus + items - 1) / items, keys / 256), even = std::min((8 * cus + items - 1) / items, keys / 1024);
+        p->narrow_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::max(keys <= 1024 ? 1 : full, even), 256));
     }
-    if (p->wide) {
-        const uint64_t items = (rows + attn::WIDE_ROWS - 1) / attn::WIDE_ROWS * a.kv_heads;
-        p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + items - 1) / items, keys / 512, 16}));
-    }
+    if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(4 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
     // what the splits hand over is kept below 128 MiB
     const uint64_t row_bytes = (uint64_t)(a.head_dim + 2) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
     p->narrow_splits = (uint32_t)std::min<uint64_t>(p->narrow_splits, most);
     p->wide_splits = (uint32_t)std::min<uint64_t>(p->wide_splits, most);
     const uint32_t splits = std::max(p->narrow_splits, p->wide_splits);
-    if ((uint64_t)p->slots * a.kv_heads * p->wide_splits > 1u << 30 || (uint64_t)a.batch * a.kv_heads * p->narrow_splits > 1u << 30 || (uint64_t)a.tokens * a.heads > 1u << 30)
+    if ((uint64_t)p->slots * a.kv_heads * p->wide_splits > 1u << 30 || (rows / attn::NARROW_ROWS + a.batch) * a.kv_heads * p->narrow_splits > 1u << 30 || (uint64_t)a.tokens * a.heads > 1u << 30)
         return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
     if (splits > 1) {
         int rc = ensure_scratch(ctx, &ctx->d_attn, &ctx->attn_bytes, row_bytes * splits, "attention's partial results");
