@@ -8,12 +8,12 @@
 //   O^T[dim][row] += V^T P^T: the B operand of 16 keys is 8 of those very registers, rounded; the A operand has to hold the same keys in the
 //                            same places, which are two groups of 4 consecutive keys for each half: two transposing reads of LDS
 //                            (ds_read_b64_tr_b16: 16 lanes take 4 rows of 16 columns and get a column of 4 each).
-// Streaming softmax: m is the running maximum of a row's raw scores, p = 2^(c s - c m) with c = scale log2(e), l the sum of p; o and l are
-// multiplied by 2^(c (m - m')) when the maximum rises.
+// Streaming softmax: m is a running maximum of a row's raw scores (RISE below), p = 2^(c s - c m) with c = scale log2(e), l the sum of p; o and l
+// are multiplied by 2^(c (m - m')) when m rises.
 //
 // fp32 operands are taken apart into 16-bit pieces, so that the products run at the 16-bit rate and keep 24 bits: three bf16
 // pieces by truncation (exact: 8 + 8 + 8 bits), of whose nine products the six that reach 2^-24 are taken; over a cache in halves
-// q (brought to 2^11 .. 2^12 by a power of two of its row) and p (times 2^15) are two halves, 22 bits and nothing subnormal that counts.
+// q (brought to 2^11 .. 2^12 by a power of two of its row) and p (times 2^7) are two halves, 22 bits and nothing subnormal that counts.
 // Against v_mfma_f32_32x32x2_f32, 1 / 16 of the 16-bit rate, that is 6 / 16, 3 / 16 and 2 / 16 of the time.
 #pragma once
 #include <type_traits>
@@ -36,6 +36,9 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float INF = __builtin_inff();
+// The maximum that p is relative to follows the scores only when they pass it by a factor of 2^RISE: until then p and l just grow beyond 1, which
+// rounds no differently, and o, 16 to 64 registers, is left alone.
+constexpr float RISE = 8.0f;
 
 // TQ: q and out; TK: keys and values
 template <typename TQ_, typename TK_, int HD_, bool PAGED_>
@@ -48,8 +51,9 @@ struct Config {
     static constexpr int NK = std::is_same<TK, float>::value ? 3 : 1;
     static constexpr int NQ = std::is_same<TQ, float>::value ? (HALF ? 2 : 3) : 1;
     static constexpr int LB = HD * 2;           // bytes of a row of one piece in LDS
+    static constexpr int RB = HD * (int)sizeof(TK);  // ... in memory
     static constexpr int PARTS = HD * (int)sizeof(TK) / 16;  // 16-byte parts of a row in memory
-    static constexpr int P_SHIFT = HALF ? 15 : 0;            // p is carried times 2^15 in halves
+    static constexpr int P_SHIFT = HALF ? 7 : 0;             // p, up to 2^8 (RISE), is carried times 2^7 in halves
 };
 
 // Order of a row's 16-byte parts in LDS: part ^ order(row).  Rows of the first product's reads are 32 consecutive ones at one part; the
@@ -129,18 +133,10 @@ __device__ __forceinline__ float row_sum(float v)
     return v;
 }
 
-// 0xffff where a 16-bit element is infinite or NaN
-template <bool HALF>
-__device__ __forceinline__ uint32_t not_finite(uint32_t two)
-{
-    constexpr uint32_t e = HALF ? 0x7c00u : 0x7f80u;
-    return ((two & e) == e ? 0xffffu : 0u) | (((two >> 16) & e) == e ? 0xffff0000u : 0u);
-}
-
 // Where the keys of a tile lie.  A tile begins at a multiple of 16, pages hold multiples of 16: a group of 16 keys has one base address.
 // Keys behind the sequence or on no page are read from an address that exists; `there` has a bit for each group that is.
 struct Place {
-    int64_t base, step1, step2, step3;  // elements from k or v: of group 0 (not paged: of the sequence), from each group to the next
+    int64_t base0, base1, base2, base3;  // bytes from k or v, of each group (not paged: base0, of the sequence)
     uint32_t there;
 };
 
@@ -149,7 +145,7 @@ __device__ __forceinline__ Place place(const AttnArgs& a, const Row& r, uint32_t
 {
     Place p;
     p.there = ~0u;
-    p.base = p.step1 = p.step2 = p.step3 = 0;
+    p.base0 = p.base1 = p.base2 = p.base3 = 0;
     if constexpr (C::PAGED) {
         auto group = [&](int g) -> int64_t {
             const int32_t key = key0 + 16 * g;
@@ -158,81 +154,118 @@ __device__ __forceinline__ Place place(const AttnArgs& a, const Row& r, uint32_t
                 page = 0;
                 p.there &= ~(1u << g);
             }
-            return ((((int64_t)page * a.kv_heads + kh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * C::HD;
+            return ((((int64_t)page * a.kv_heads + kh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * C::RB;
         };
-        const int64_t g0 = group(0), g1 = group(1);
-        p.base = g0;
-        p.step1 = g1 - g0;
+        p.base0 = group(0);
+        p.base1 = group(1);
         if constexpr (TILE == 64) {
-            const int64_t g2 = group(2), g3 = group(3);
-            p.step2 = g2 - g1;
-            p.step3 = g3 - g2;
+            p.base2 = group(2);
+            p.base3 = group(3);
         }
     } else {
-        p.base = (int64_t)r.first * a.kv_stride + (int64_t)kh * C::HD;
+        p.base0 = ((int64_t)r.first * a.kv_stride + (int64_t)kh * C::HD) * (int64_t)sizeof(typename C::TK);
     }
     return p;
 }
 
-// Copies a tile of keys or values by THREADS threads through registers: fetch() asks for it, store() puts it into LDS, piece by piece.
+// Copies a tile of keys or values by THREADS threads (of `wave`, where there are several) through registers: fetch() asks for it, store() puts it into
+// LDS, piece by piece.
 template <typename C, int TILE, int THREADS>
 struct Stage {
     static constexpr int TOTAL = TILE * C::PARTS, LOADS = (TOTAL + THREADS - 1) / THREADS;
     static constexpr int PIECE = TILE * C::LB;                   // bytes of a piece in LDS
     static constexpr int BYTES = PIECE * C::NK + (C::HD % 32 ? 64 : 0);  // (a half tile of dims reads past the last row)
     u32x4 x[LOADS];
+    bool marked = false;  // this thread has left marks
 
-    __device__ __forceinline__ void fetch(const void* src, const AttnArgs& a, const Row& r, const Place& p, int32_t key0, uint32_t tid)
+    __device__ __forceinline__ void fetch(const void* src, const AttnArgs& a, const Row& r, const Place& p, int32_t key0, uint32_t wave, uint32_t tid)
     {
-        const typename C::TK* s = static_cast<const typename C::TK*>(src);
+        const char* const s = static_cast<const char*>(src);
+        if constexpr (C::PAGED && 64 % C::PARTS == 0) {  // a wave's load is whole rows of one group: 1 KiB on end
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const uint32_t flat = u * THREADS + tid;
-            uint32_t row = flat / C::PARTS;
-            const uint32_t part = flat % C::PARTS;
-            if (TOTAL % THREADS && row >= TILE) row = TILE - 1;  // (not stored)
-            int64_t at;
-            if constexpr (C::PAGED) {
-                at = p.base + (row & 15) * C::HD;
-                at += row < 16 ? 0 : p.step1;
-                if constexpr (TILE == 64) {
-                    at += row < 32 ? 0 : p.step2;
-                    at += row < 48 ? 0 : p.step3;
-                }
-            } else {
-                const int32_t key = key0 + (int32_t)row, k = key < r.length ? key : r.length - 1;
-                at = p.base + (int64_t)k * a.kv_stride;
+            for (int u = 0; u < LOADS; ++u) {
+                const uint32_t row = (u * THREADS + wave * 64) / C::PARTS, g = row >> 4;
+                const int64_t base = g == 0 ? p.base0 : g == 1 ? p.base1 : g == 2 ? p.base2 : p.base3;
+                x[u] = *reinterpret_cast<const u32x4*>(s + base + (row & 15) * C::RB + (tid & 63) * 16);
             }
-            x[u] = *reinterpret_cast<const u32x4*>(s + at + part * (16 / sizeof(typename C::TK)));
+        } else if constexpr (C::PAGED) {
+            const int64_t step1 = p.base1 - p.base0, step2 = p.base2 - p.base1, step3 = p.base3 - p.base2;
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) {
+                const uint32_t flat = u * THREADS + tid, part = flat % C::PARTS;
+                uint32_t row = flat / C::PARTS;
+                if (TOTAL % THREADS && row >= TILE) row = TILE - 1;  // (not stored)
+                int64_t at = p.base0 + (row & 15) * C::RB + part * 16;
+                at += row < 16 ? 0 : step1;
+                if constexpr (TILE == 64) {
+                    at += row < 32 ? 0 : step2;
+                    at += row < 48 ? 0 : step3;
+                }
+                x[u] = *reinterpret_cast<const u32x4*>(s + at);
+            }
+        } else {
+            const uint32_t pitch = a.kv_stride * (uint32_t)sizeof(typename C::TK);  // (a tile is less than 4 GiB of rows)
+            const char* const base = s + p.base0 + (int64_t)key0 * pitch;
+            auto load = [&](int u, uint32_t last) {
+                const uint32_t flat = u * THREADS + tid, row = flat / C::PARTS;
+                x[u] = *reinterpret_cast<const u32x4*>(base + ((row < last ? row : last) * pitch + flat % C::PARTS * 16));
+            };
+            if (key0 + TILE <= r.length) {
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u) load(u, TILE - 1);
+            } else {
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u) load(u, (uint32_t)(r.length - 1 - key0));
+            }
         }
     }
-    // MIXED: elements that are not finite become zeros and get a bit in `marks`, a byte per part of a row; whether there is one
-    template <bool MIXED>
-    __device__ __forceinline__ bool store(char* lds, uint8_t* marks, uint32_t tid)
+    __device__ __forceinline__ void no_marks(uint8_t* marks, uint32_t tid)
     {
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u)
+            if (TOTAL % THREADS == 0 || u * THREADS + tid < TOTAL) marks[u * THREADS + tid] = 0;
+        marked = false;
+    }
+    // Before store() of values that some rows see and others do not: elements that are not finite become zeros and get a bit in `marks`, a
+    // byte per part of a row; whether there is one
+    __device__ __forceinline__ bool clear(uint8_t* marks, uint32_t tid)
+    {
+        // an exponent of all ones carries into the bit above it
+        constexpr uint32_t ones = C::NK == 3 ? 0x7f800000u : C::HALF ? 0x7c007c00u : 0x7f807f80u;
+        constexpr uint32_t carry = C::NK == 3 ? 0x00800000u : C::HALF ? 0x04000400u : 0x00800080u, sign = C::NK == 3 ? 0x80000000u : 0x80008000u;
         uint32_t any = 0;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= (x[u][i] & ones) + carry;
+        if (marked) no_marks(marks, tid);
+        if (!(any & sign)) return false;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            uint32_t found = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t bad = ((x[u][i] & ones) + carry) & sign;
+                if constexpr (C::NK == 3) {
+                    found |= (bad >> 31) << i;
+                    if (bad) x[u][i] = 0;
+                } else {
+                    found |= (bad >> 15 & 1) << 2 * i | (bad >> 31) << (2 * i + 1);
+                    if (bad & 0x8000u) x[u][i] &= 0xffff0000u;
+                    if (bad & 0x80000000u) x[u][i] &= 0xffffu;
+                }
+            }
+            if (TOTAL % THREADS == 0 || u * THREADS + tid < TOTAL) marks[u * THREADS + tid] = (uint8_t)found;
+        }
+        marked = true;
+        return true;
+    }
+    __device__ __forceinline__ void store(char* lds, uint32_t tid) const
+    {
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
             const uint32_t flat = u * THREADS + tid, row = flat / C::PARTS, part = flat % C::PARTS;
             if (TOTAL % THREADS && row >= TILE) continue;
-            if constexpr (MIXED) {
-                uint32_t found = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (C::NK == 3) {
-                        if ((x[u][i] & 0x7f800000u) == 0x7f800000u) {
-                            found |= 1u << i;
-                            x[u][i] = 0;
-                        }
-                    } else {
-                        const uint32_t bad = not_finite<C::HALF>(x[u][i]);
-                        found |= (bad & 1) << 2 * i | (bad >> 31) << (2 * i + 1);
-                        x[u][i] &= ~bad;
-                    }
-                }
-                marks[flat] = (uint8_t)found;
-                any |= found;
-            }
             if constexpr (C::NK == 1) {
                 *reinterpret_cast<u32x4*>(lds + row * C::LB + ((part ^ order<C::HD>(row)) << 4)) = x[u];
             } else {
@@ -244,7 +277,6 @@ struct Stage {
                 for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(to + n * PIECE) = (u32x2){lo[n], hi[n]};
             }
         }
-        return any != 0;
     }
 };
 
@@ -376,9 +408,29 @@ struct Rows {
     // Hides what the row does not see among 32 keys from key0 on; `there`: bits of the two groups of 16 that exist.
     __device__ __forceinline__ void hide(float* s, int32_t key0, uint32_t there) const
     {
+        const int32_t k0 = key0 + 4 * (int32_t)group();
+        auto at = [](int i) { return 4 * GROUPS * (i >> 2) + (i & 3); };  // (place_of without the group)
+        if (key0 + 32 > min_hi) {
+            const int32_t h = hi - k0;
 #pragma unroll
-        for (int i = 0; i < REGS; ++i)
-            if (!sees(key0 + place_of(i)) || !(there >> (i / (REGS / 2)) & 1)) s[i] = -INF;
+            for (int i = 0; i < REGS; ++i) s[i] = at(i) < h ? s[i] : -INF;
+        }
+        if (key0 < max_lo) {
+            const int32_t f = lo - k0;
+            if (key0 >= sinks) {
+#pragma unroll
+                for (int i = 0; i < REGS; ++i) s[i] = at(i) >= f ? s[i] : -INF;
+            } else {
+                const int32_t e = sinks - k0;
+#pragma unroll
+                for (int i = 0; i < REGS; ++i) s[i] = at(i) >= f || at(i) < e ? s[i] : -INF;
+            }
+        }
+        if (C::PAGED && (there & 3) != 3) {
+#pragma unroll
+            for (int i = 0; i < REGS; ++i)
+                if (!(there >> (i / (REGS / 2)) & 1)) s[i] = -INF;
+        }
     }
 
     // The N scores that a lane holds become probabilities; o and l follow the maximum.
@@ -389,7 +441,7 @@ struct Rows {
 #pragma unroll
         for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
         mx = row_max<M>(mx);
-        if (__any(mx > m)) {
+        if (__any(mx * c > m * c + RISE)) {
             const float up = fmaxf(m, mx), base = up == -INF ? 0.0f : up * c;
             const float alpha = __builtin_amdgcn_exp2f(m * c - base);  // 0 at the first keys
             m = up;
@@ -398,13 +450,14 @@ struct Rows {
             for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
         const float base = (m == -INF ? 0.0f : m * c) - (float)C::P_SHIFT;
-        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base));
-            sum += s[i];
+        for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base));
+        if constexpr (C::NQ > 1) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum += s[i];
+            l += sum;
         }
-        l += sum;
     }
 
     // o += V^T p for 32 keys, which lie in LDS from `v` on
@@ -417,6 +470,13 @@ struct Rows {
             uint32_t w[4][C::NQ];
 #pragma unroll
             for (int e = 0; e < 4; ++e) pieces<C::HALF, C::NQ>(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], w[e]);
+            if constexpr (C::NQ == 1) {  // l is the sum of what the products get
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (C::HALF) l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w[e][0]), (f16x2){(_Float16)1.0f, (_Float16)1.0f}, l, false);
+                    else l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[e][0]), (bf16x2){(__bf16)1.0f, (__bf16)1.0f}, l, false);
+                }
+            }
             u32x4 b[C::NQ];
 #pragma unroll
             for (int n = 0; n < C::NQ; ++n) b[n] = (u32x4){w[0][n], w[1][n], w[2][n], w[3][n]};
@@ -564,26 +624,24 @@ __global__ __launch_bounds__(256, (C::NK == 3 || C::NQ > 1) && C::HD > 96 ? 1 : 
     if (tid < 2) bad[tid] = 0;
     if (from < to) {
         typename W::S sk, sv;
+        sv.no_marks(marks, tid);
         Place p = place<C, TILE>(a, r, kh, span.at(from) * TILE);
-        sk.fetch(a.k, a, r, p, span.at(from) * TILE, tid);
-        sv.fetch(a.v, a, r, p, span.at(from) * TILE, tid);
+        sk.fetch(a.k, a, r, p, span.at(from) * TILE, wave, tid);
+        sv.fetch(a.v, a, r, p, span.at(from) * TILE, wave, tid);
         Place ahead = place<C, TILE>(a, r, kh, span.at(from + 1) * TILE);  // (the table's entries are asked for a tile before the keys)
         for (int32_t t = from; t < to; ++t) {
             const int32_t key0 = span.at(t) * TILE;
             const bool mixed = !(key0 + TILE <= all_hi && (key0 >= all_lo || key0 + TILE <= w.sinks)) || p.there != ~0u;
             __syncthreads();  // everybody is done with the tile before
             if (tid == 0) bad[(t + 1) & 1] = 0;
-            sk.template store<false>(lk, marks, tid);
-            if (mixed) {
-                if (sv.template store<true>(lv, marks, tid)) bad[t & 1] = 1;
-            } else {
-                sv.template store<false>(lv, marks, tid);
-            }
+            sk.store(lk, tid);
+            if (mixed && sv.clear(marks, tid)) bad[t & 1] = 1;
+            sv.store(lv, tid);
             const uint32_t there = p.there;
             if (t + 1 < to) {
                 p = ahead;
-                sk.fetch(a.k, a, r, p, span.at(t + 1) * TILE, tid);
-                sv.fetch(a.v, a, r, p, span.at(t + 1) * TILE, tid);
+                sk.fetch(a.k, a, r, p, span.at(t + 1) * TILE, wave, tid);
+                sv.fetch(a.v, a, r, p, span.at(t + 1) * TILE, wave, tid);
                 ahead = place<C, TILE>(a, r, kh, span.at(t + 2) * TILE);
             }
             __syncthreads();
@@ -688,11 +746,12 @@ __global__ __launch_bounds__(Narrow<C>::WAVES * 64, Narrow<C>::WAVES / 4) void a
         }
         int32_t t = from + (int32_t)wave;
         typename W::S sk, sv;
+        sv.no_marks(marks[wave], lane);
         Place now, next;
         if (t < to) {  // (before the rows' q: the first keys take longest)
             now = place<C, 32>(a, r, kh, span.at(t) * 32);
-            sk.fetch(a.k, a, r, now, span.at(t) * 32, lane);
-            sv.fetch(a.v, a, r, now, span.at(t) * 32, lane);
+            sk.fetch(a.k, a, r, now, span.at(t) * 32, 0, lane);
+            sv.fetch(a.v, a, r, now, span.at(t) * 32, 0, lane);
             next = place<C, 32>(a, r, kh, span.at(t + WAVES) * 32);  // (the table's entries are asked for a tile before the keys)
         }
         Rows<C, 16> w;
@@ -701,10 +760,10 @@ __global__ __launch_bounds__(Narrow<C>::WAVES * 64, Narrow<C>::WAVES / 4) void a
             const int32_t key0 = span.at(t) * 32;
             const uint32_t there = now.there;
             const bool mixed = !w.all(key0, 32) || there != ~0u, more = t + WAVES < to;
-            sk.template store<false>(mine, marks[wave], lane);
+            sk.store(mine, lane);
             if (more) {
                 now = next;
-                sk.fetch(a.k, a, r, now, span.at(t + WAVES) * 32, lane);
+                sk.fetch(a.k, a, r, now, span.at(t + WAVES) * 32, 0, lane);
             }
             wave_sync();
             float s[8];
@@ -712,10 +771,10 @@ __global__ __launch_bounds__(Narrow<C>::WAVES * 64, Narrow<C>::WAVES / 4) void a
             wave_sync();
             if (mixed) w.hide(s, key0, there);
             bool bad = false;
-            if (mixed) bad = __any(sv.template store<true>(mine, marks[wave], lane));
-            else sv.template store<false>(mine, marks[wave], lane);
+            if (mixed) bad = __any(sv.clear(marks[wave], lane));
+            sv.store(mine, lane);
             if (more) {
-                sv.fetch(a.v, a, r, now, span.at(t + WAVES) * 32, lane);
+                sv.fetch(a.v, a, r, now, span.at(t + WAVES) * 32, 0, lane);
                 next = place<C, 32>(a, r, kh, span.at(t + 2 * WAVES) * 32);
             }
             w.template softmax<8>(s);

@@ -206,7 +206,7 @@ bool matrix_form(const AttnArgs& a)
     const uint64_t qe = a.dtype == PIMDL_F32 ? 4 : 2, ke = a.cache_dtype == PIMDL_F32 ? 4 : 2;
     uint64_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
     all |= a.q_stride * qe | a.out_stride * qe | (a.paged ? 0 : a.kv_stride * ke);
-    return all % 16 == 0 && (uint64_t)a.tokens * a.group < 1u << 30;
+    return all % 16 == 0 && (uint64_t)a.tokens * a.group < 1u << 30 && a.kv_stride < 1u << 22;
 }
 
 // Which kernels run, and over how many workgroups the keys of a row are split.
