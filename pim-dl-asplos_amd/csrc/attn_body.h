@@ -571,7 +571,12 @@ template <typename C>
 struct Wide {
     static constexpr int TILE = C::NK == 1 ? 64 : 32;
     typedef Stage<C, TILE, 256> S;
-    static constexpr int LDS = 2 * S::BYTES;
+    struct Shared {
+        alignas(16) char k[S::BYTES];
+        alignas(16) char v[S::BYTES];
+        uint32_t bad[2];                 // some value of the tile, or of the one before, is not finite
+        uint8_t marks[TILE * C::PARTS];  // ... which
+    };
 };
 
 // Blocks of `size` rows of all sequences are numbered without a sum over their lengths: those of row b of the batch, which begins at token
@@ -593,15 +598,15 @@ __device__ __forceinline__ uint32_t row_of_slot(const AttnArgs& a, uint32_t slot
 }
 
 template <typename C>
-__global__ __launch_bounds__(256, (C::NK == 3 || C::NQ > 1) && C::HD > 96 ? 1 : 2) void attention_wide_kernel(AttnArgs a, uint32_t slots, uint32_t splits, uint32_t narrow_rows, Partial part)
+__device__ __forceinline__ void wide_rows(const AttnArgs& a, uint32_t block, uint32_t slots, uint32_t splits, uint32_t narrow_rows, const Partial& part, char* shared)
 {
     typedef Wide<C> W;
     constexpr int TILE = W::TILE, KT = TILE / 32;
-    __shared__ __attribute__((aligned(1024))) char lds[W::LDS];
-    __shared__ uint32_t bad[2];
-    __shared__ uint8_t marks[TILE * C::PARTS];
-    char *const lk = lds, *const lv = lds + W::S::BYTES;
-    const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;  // late rows, which see most keys, first
+    typename W::Shared& sh = *reinterpret_cast<typename W::Shared*>(shared);
+    char *const lk = sh.k, *const lv = sh.v;
+    uint32_t* const bad = sh.bad;
+    uint8_t* const marks = sh.marks;
+    const uint32_t kh = block % a.kv_heads, rest = block / a.kv_heads, split = rest % splits, slot = slots - 1 - rest / splits;  // late rows, which see most keys, first
     const uint32_t b = __builtin_amdgcn_readfirstlane(row_of_slot(a, slot, WIDE_ROWS));
     const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, C::PAGED, b);
     const uint32_t rows = r.n * a.group, before = first_slot(a, b, r.first, WIDE_ROWS), row0 = (slot - before) * WIDE_ROWS;
@@ -691,13 +696,16 @@ __global__ __launch_bounds__(256, (C::NK == 3 || C::NQ > 1) && C::HD > 96 ? 1 : 
 // ------------------------------------------------------------------------------------------------------------
 constexpr uint32_t NARROW_ROWS = 16;
 
-template <typename C>
+template <typename C, int WAVES>
 struct Narrow {
     typedef Stage<C, 32, 64> S;
-    static constexpr int WAVES = C::NK == 3 && C::HD > 64 ? 4 : 8;
     static constexpr int PITCH = C::HD + 1, JOIN = 16 * PITCH * 4;  // a wave's sums, rows padded against bank conflicts
     static constexpr int WAVE = ((S::BYTES > JOIN ? S::BYTES : JOIN) + 15) / 16 * 16;
-    static constexpr int LDS = WAVES * WAVE;
+    struct Shared {
+        alignas(16) char lds[WAVES * WAVE];
+        float ml[WAVES][16][2];
+        uint8_t marks[WAVES][32 * C::PARTS];
+    };
 };
 
 __device__ __forceinline__ void wave_sync()
@@ -707,15 +715,15 @@ __device__ __forceinline__ void wave_sync()
 }
 
 // by_slot: a workgroup per block of 16 rows (first_slot); otherwise one per row of the batch, which takes its blocks one after the other
-template <typename C>
-__global__ __launch_bounds__(Narrow<C>::WAVES * 64, Narrow<C>::WAVES / 4) void attention_narrow_kernel(AttnArgs a, uint32_t by_slot, uint32_t splits, uint32_t most_rows, Partial part)
+template <typename C, int WAVES>
+__device__ __forceinline__ void narrow_rows_of(const AttnArgs& a, uint32_t number, uint32_t by_slot, uint32_t splits, uint32_t most_rows, const Partial& part, char* shared)
 {
-    typedef Narrow<C> W;
-    constexpr int WAVES = W::WAVES;
-    __shared__ __attribute__((aligned(1024))) char lds[W::LDS];
-    __shared__ float ml[WAVES][16][2];
-    __shared__ uint8_t marks[WAVES][32 * C::PARTS];
-    const uint32_t split = blockIdx.x % splits, rest = blockIdx.x / splits, kh = rest % a.kv_heads, slot = rest / a.kv_heads;
+    typedef Narrow<C, WAVES> W;
+    typename W::Shared& sh = *reinterpret_cast<typename W::Shared*>(shared);
+    char* const lds = sh.lds;
+    auto& ml = sh.ml;
+    auto& marks = sh.marks;
+    const uint32_t split = number % splits, rest = number / splits, kh = rest % a.kv_heads, slot = rest / a.kv_heads;
     const uint32_t b = by_slot ? __builtin_amdgcn_readfirstlane(row_of_slot(a, slot, NARROW_ROWS)) : slot;
     const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, C::PAGED, b);
     const uint32_t rows = r.n * a.group;
@@ -834,29 +842,54 @@ __global__ __launch_bounds__(Narrow<C>::WAVES * 64, Narrow<C>::WAVES / 4) void a
 // What one call launches, decided by launch_attention.
 struct Plan {
     bool wide, narrow;
-    uint32_t slots;                       // of the wide kernel
+    uint32_t slots;                       // blocks of 128 rows
     uint32_t wide_splits, narrow_splits;
-    uint32_t narrow_rows;                 // rows of a sequence and key head up to which the narrow kernel takes them
+    uint32_t narrow_rows;                 // rows of a sequence and key head up to which they are taken 16 at a time
     bool by_slot;                         // ... in workgroups of 16 rows each
     Partial part;
 };
 
+// Waves of a workgroup that takes 16 rows, alone in its launch: eight, where their LDS fits.
+template <typename C>
+constexpr int NARROW_WAVES = C::NK == 3 && C::HD > 64 ? 4 : 8;
+
+template <typename C>
+__global__ __launch_bounds__(NARROW_WAVES<C> * 64, NARROW_WAVES<C> / 4) void attention_narrow_kernel(AttnArgs a, uint32_t by_slot, uint32_t splits, uint32_t most_rows,
+                                                                                                     Partial part)
+{
+    __shared__ __attribute__((aligned(1024))) char shared[sizeof(typename Narrow<C, NARROW_WAVES<C>>::Shared)];
+    narrow_rows_of<C, NARROW_WAVES<C>>(a, blockIdx.x, by_slot, splits, most_rows, part, shared);
+}
+
+// Blocks of 128 rows, and behind them, for those sequences of the batch that have few, blocks of 16: these wait for memory most of the time, those for
+// the matrix cores, so they share the device better than one launch after the other (16 sequences, half of them with one token: 245 us in two
+// launches, 214 in one).
+template <typename C>
+__global__ __launch_bounds__(256, (C::NK == 3 && C::HD > 80) || (C::NQ > 1 && C::HD > 96) ? 1 : 2) void attention_wide_kernel(AttnArgs a, uint32_t wide_blocks, uint32_t slots, uint32_t splits,
+                                                                                                         uint32_t narrow_splits, uint32_t narrow_rows, Partial part)
+{
+    constexpr size_t WIDE = sizeof(typename Wide<C>::Shared), NARROW = C::PAGED ? sizeof(typename Narrow<C, 4>::Shared) : 0;
+    __shared__ __attribute__((aligned(1024))) char shared[WIDE > NARROW ? WIDE : NARROW];
+    if (!C::PAGED || blockIdx.x < wide_blocks) {
+        wide_rows<C>(a, blockIdx.x, slots, splits, narrow_rows, part, shared);
+    } else {
+        if constexpr (C::PAGED) narrow_rows_of<C, 4>(a, blockIdx.x - wide_blocks, 0, narrow_splits, narrow_rows, part, shared);
+    }
+}
+
 template <typename C>
 int launch(Ctx* ctx, const AttnArgs& a, const Plan& p)
 {
-    int rc = PIMDL_OK;
     if (p.wide) {
-        hipLaunchKernelGGL((attention_wide_kernel<C>), dim3(p.slots * a.kv_heads * p.wide_splits), dim3(256), 0, ctx->stream, a, p.slots, p.wide_splits,
+        const uint32_t wide = p.slots * a.kv_heads * p.wide_splits, narrow = p.narrow ? a.batch * a.kv_heads * p.narrow_splits : 0;
+        hipLaunchKernelGGL((attention_wide_kernel<C>), dim3(wide + narrow), dim3(256), 0, ctx->stream, a, wide, p.slots, p.wide_splits, p.narrow_splits,
                            p.narrow ? p.narrow_rows : 0, p.part);
-        rc = hip_check(ctx, hipGetLastError(), "attention_wide_kernel launch");
+        return hip_check(ctx, hipGetLastError(), "attention_wide_kernel launch");
     }
-    if (!rc && p.narrow) {
-        const uint32_t slots = p.by_slot ? (uint32_t)((uint64_t)a.tokens * a.group / NARROW_ROWS) + a.batch : a.batch;
-        hipLaunchKernelGGL((attention_narrow_kernel<C>), dim3(slots * a.kv_heads * p.narrow_splits), dim3(Narrow<C>::WAVES * 64), 0, ctx->stream, a,
-                           (uint32_t)p.by_slot, p.narrow_splits, p.narrow_rows, p.part);
-        rc = hip_check(ctx, hipGetLastError(), "attention_narrow_kernel launch");
-    }
-    return rc;
+    const uint32_t slots = p.by_slot ? (uint32_t)((uint64_t)a.tokens * a.group / NARROW_ROWS) + a.batch : a.batch;
+    hipLaunchKernelGGL((attention_narrow_kernel<C>), dim3(slots * a.kv_heads * p.narrow_splits), dim3(NARROW_WAVES<C> * 64), 0, ctx->stream, a,
+                       (uint32_t)p.by_slot, p.narrow_splits, p.narrow_rows, p.part);
+    return hip_check(ctx, hipGetLastError(), "attention_narrow_kernel launch");
 }
 
 template <typename TQ, typename TK, bool PAGED>

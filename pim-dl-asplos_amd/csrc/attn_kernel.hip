@@ -231,13 +231,13 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
         const uint64_t full = std::min((cus + items - 1) / items, keys / 256), even = std::min((8 * cus + items - 1) / items, keys / 1024);
         p->narrow_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::max(keys <= 1024 ? 1 : full, even), 256));
     }
-    if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(4 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
+    if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
     // what the splits hand over is kept below 128 MiB
     const uint64_t row_bytes = (uint64_t)(a.head_dim + 2) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
     p->narrow_splits = (uint32_t)std::min<uint64_t>(p->narrow_splits, most);
     p->wide_splits = (uint32_t)std::min<uint64_t>(p->wide_splits, most);
     const uint32_t splits = std::max(p->narrow_splits, p->wide_splits);
-    if ((uint64_t)p->slots * a.kv_heads * p->wide_splits > 1u << 30 || (rows / attn::NARROW_ROWS + a.batch) * a.kv_heads * p->narrow_splits > 1u << 30 || (uint64_t)a.tokens * a.heads > 1u << 30)
+    if ((uint64_t)p->slots * a.kv_heads * p->wide_splits > 1u << 29 || (rows / attn::NARROW_ROWS + a.batch) * a.kv_heads * p->narrow_splits > 1u << 29 || (uint64_t)a.tokens * a.heads > 1u << 30)
         return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
     if (splits > 1) {
         int rc = ensure_scratch(ctx, &ctx->d_attn, &ctx->attn_bytes, row_bytes * splits, "attention's partial results");
