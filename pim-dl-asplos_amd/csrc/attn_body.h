@@ -854,7 +854,7 @@ template <typename C>
 constexpr int NARROW_WAVES = C::NK == 3 && C::HD > 64 ? 4 : 8;
 
 template <typename C>
-__global__ __launch_bounds__(NARROW_WAVES<C> * 64, NARROW_WAVES<C> / 4) void attention_narrow_kernel(AttnArgs a, uint32_t by_slot, uint32_t splits, uint32_t most_rows,
+__global__ __launch_bounds__(NARROW_WAVES<C> * 64, C::NK == 1 && C::HD <= 64 ? 4 : NARROW_WAVES<C> / 4) void attention_narrow_kernel(AttnArgs a, uint32_t by_slot, uint32_t splits, uint32_t most_rows,
                                                                                                      Partial part)
 {
     __shared__ __attribute__((aligned(1024))) char shared[sizeof(typename Narrow<C, NARROW_WAVES<C>>::Shared)];

@@ -227,9 +227,11 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     p->slots = (uint32_t)(rows / attn::WIDE_ROWS) + a.batch;
     if (p->narrow) {
         const uint64_t items = (p->by_slot ? (rows + attn::NARROW_ROWS - 1) / attn::NARROW_ROWS : a.batch) * a.kv_heads;
-        // every CU its eight waves, of at least 256 keys to a workgroup; where lengths may differ, shares of 1024 keys that can be dealt out evenly
-        const uint64_t full = std::min((cus + items - 1) / items, keys / 256), even = std::min((8 * cus + items - 1) / items, keys / 1024);
-        p->narrow_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::max(keys <= 1024 ? 1 : full, even), 256));
+        // Fewer items than CUs: every CU one workgroup, of at least 256 keys.  More: shares of at least 1024 keys, so that long sequences are dealt
+        // out too.  us with shares of 512 / 1024 / 2048 keys for more items: 64 sequences of up to 8191 231 / 203 / 203, 32 of up to 4000, 12 heads,
+        // fp32 116 / 96 / 118; for fewer: two of 100 000 67 / 55 / 50 (one workgroup per CU), 32 of up to 16000 with one key head 52 / 44 / 41.
+        p->narrow_splits = (uint32_t)std::max<uint64_t>(1, 2 * items <= cus ? std::min<uint64_t>({(cus + items - 1) / items, keys / 256, 256})
+                                                                        : std::min<uint64_t>((8 * cus + items - 1) / items, keys / 1024));
     }
     if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
     // what the splits hand over is kept below 128 MiB
