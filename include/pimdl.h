@@ -398,6 +398,8 @@ typedef struct pimdl_paged_cache {
     void *k, *v;             /* [pages][kv_heads][page_tokens][head_dim] each, 16-byte aligned */
     const int32_t* tables;   /* [seqs][table_width] */
     const int32_t* lengths;  /* [seqs]: positions in the cache, those of the call's own tokens included */
+    const int32_t* lacking;  /* [1] or NULL: the book's.  While it is not 0 the room for new tokens has not been made, and
+                              * pimdl_cache_append writes nothing (it would write over older tokens) */
     uint32_t pages, page_tokens; /* page_tokens: a power of two, 16 .. 1024 */
     uint32_t kv_heads, head_dim;
     uint32_t seqs, table_width;

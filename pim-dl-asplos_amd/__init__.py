@@ -106,7 +106,7 @@ class AttentionWindowDesc(ctypes.Structure):
 
 class PagedCacheDesc(ctypes.Structure):
     """pimdl_paged_cache: one layer's share of a paged cache"""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "tables", "lengths")] +
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "tables", "lengths", "lacking")] +
                 [(n, ctypes.c_uint32) for n in ("pages", "page_tokens", "kv_heads", "head_dim", "seqs", "table_width", "dtype")])
 
 

@@ -230,7 +230,7 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
         // Fewer items than CUs: every CU one workgroup, of at least 256 keys.  More: shares of at least 1024 keys, so that long sequences are dealt
         // out too.  us with shares of 512 / 1024 / 2048 keys for more items: 64 sequences of up to 8191 231 / 203 / 203, 32 of up to 4000, 12 heads,
         // fp32 116 / 96 / 118; for fewer: two of 100 000 67 / 55 / 50 (one workgroup per CU), 32 of up to 16000 with one key head 52 / 44 / 41.
-        p->narrow_splits = (uint32_t)std::max<uint64_t>(1, 2 * items <= cus ? std::min<uint64_t>({(cus + items - 1) / items, keys / 256, 256})
+        p->narrow_splits = (uint32_t)std::max<uint64_t>(1, keys <= 1024 ? 1 : 2 * items <= cus ? std::min<uint64_t>({(cus + items - 1) / items, keys / 256, 256})
                                                                         : std::min<uint64_t>((8 * cus + items - 1) / items, keys / 1024));
     }
     if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));

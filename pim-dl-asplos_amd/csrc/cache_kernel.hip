@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const TI* __restrict_
     const uint32_t row = c.kv_heads * c.head_dim / N;  // packs of a token's row
     const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     const uint32_t t = (uint32_t)(item / row), part = (uint32_t)(item % row);
-    if (t >= tokens) return;
+    if (t >= tokens || (c.lacking && *c.lacking != 0)) return;
     const Row r = load_row(starts, seqs, c.tables, c.lengths, tokens, c.seqs, c.table_width, page_shift, true, row_of_token(starts, batch, tokens, t));
     if (t < r.first || t - r.first >= r.n) return;
     const int32_t pos = r.pos0 + (int32_t)(t - r.first);
@@ -256,9 +256,10 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(Pools pl, const int32_t
     copy_pages(pl, src, dst, n, pages, blockIdx.x, gridDim.x);
 }
 
-// ---- fork.  take[i]: the page that entry i's partly filled last page is copied to, -1 where there is none, -2 where the entry is left out
+// ---- fork.  take[i]: the page that entry i's partly filled last page is copied to, -1 where there is none, -2 where the entry is left out; length[i]: of
+// its parent before the call (which may be another entry's child: then 0)
 struct ForkLists {
-    int32_t *fresh, *take, *src, *dst, *count;
+    int32_t *fresh, *take, *length, *src, *dst, *count;
 };
 
 __global__ __launch_bounds__(SCAN) void pages_fork_kernel(Book b, const int32_t* __restrict__ parents, const int32_t* __restrict__ children, uint32_t n,
@@ -283,7 +284,10 @@ __global__ __launch_bounds__(SCAN) void pages_fork_kernel(Book b, const int32_t*
         uint32_t total;
         const uint32_t at = want + block_scan<uint32_t>(page >= 0, tmp, &total);
         if (page >= 0) f.src[at] = page;
-        if (i < n) f.take[i] = page >= 0 ? (int32_t)at : page;
+        if (i < n) {
+            f.take[i] = page >= 0 ? (int32_t)at : page;
+            f.length[i] = page == -2 ? 0 : held_length(b, parents[i]);
+        }
         want += total;
     }
     const uint32_t asked = want < b.pages ? want : b.pages, found = lowest_free(b.refs, b.pages, asked, f.fresh, tmp);
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(256) void pages_fork_apply_kernel(Book b, Pools pl,
     const uint32_t i = blockIdx.x / row_blocks, j0 = blockIdx.x % row_blocks * 1024;
     const int32_t take = f.take[i];
     if (take == -2) return;
-    const int32_t p = parents[i], c = children[i], len = held_length(b, p);
+    const int32_t p = parents[i], c = children[i], len = f.length[i];
     const uint32_t whole = (uint32_t)len / b.page_tokens;
     const int32_t* from = b.tables + (size_t)p * b.width;
     int32_t* to = b.tables + (size_t)c * b.width;
@@ -456,10 +460,10 @@ int launch_pages_reserve(Ctx* ctx, const pimdl_page_book& b, const int32_t* seqs
 int launch_pages_fork(Ctx* ctx, const pimdl_page_book& b, const int32_t* parents, const int32_t* children, uint32_t n)
 {
     int32_t* s;
-    int rc = book_scratch(ctx, 4 * (size_t)n + 1, &s);
+    int rc = book_scratch(ctx, 5 * (size_t)n + 1, &s);
     if (!rc) rc = allow_dynamic_lds(ctx, reinterpret_cast<const void*>(pages_fork_kernel), 16384 * 4, "pages_fork_kernel LDS");
     if (rc) return rc;
-    const ForkLists f = {s + 1, s + 1 + n, s + 1 + 2 * (size_t)n, s + 1 + 3 * (size_t)n, s};
+    const ForkLists f = {s + 1, s + 1 + n, s + 1 + 2 * (size_t)n, s + 1 + 3 * (size_t)n, s + 1 + 4 * (size_t)n, s};
     const Book book = book_of(b);
     hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(SCAN), b.seqs * 4, ctx->stream, book, parents, children, n, f);
     if ((rc = hip_check(ctx, hipGetLastError(), "pages_fork_kernel launch")) || n == 0) return rc;

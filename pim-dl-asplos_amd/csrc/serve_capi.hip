@@ -61,6 +61,7 @@ int check_cache(Ctx* ctx, const char* fn, const pimdl_paged_cache* c, uint32_t d
     if (!rc) rc = check_device(ctx, fn, "cache v", c->v, 16);
     if (!rc) rc = check_device(ctx, fn, "cache tables", c->tables, 4);
     if (!rc) rc = check_device(ctx, fn, "cache lengths", c->lengths, 4);
+    if (!rc && c->lacking) rc = check_device(ctx, fn, "cache lacking", c->lacking, 4);
     return rc;
 }
 

@@ -22,7 +22,8 @@ _CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 class PagedCache:
     """k, v: [layers][pages][kv_heads][page_tokens][head_dim]; tables int32 [seqs][width], lengths int32 [seqs], refs int32 [pages]
     (see pimdl_page_book).  `lacking` (int32 [1], on the device) tells how many pages the last reserve or fork was short of: 0 means done,
-    -1 that a sequence would outgrow its row of the table; nothing else has changed then."""
+    -1 that a sequence would outgrow its row of the table; nothing else has changed then, and append writes nothing until a later reserve or
+    fork has had enough."""
 
     def __init__(self, ctx, pimdl, layers, pages, kv_heads, head_dim, page_tokens=16, dtype="f16", seqs=64, max_len=4096):
         dev = torch.device("cuda", torch.cuda.current_device())
@@ -54,8 +55,8 @@ class PagedCache:
         self._lib = pimdl.lib()
         self._unlimited = pimdl.UNLIMITED
         layer_bytes = k[0].numel() * k.element_size() if layers else 0
-        self._layer = [pimdl.PagedCacheDesc(k.data_ptr() + i * layer_bytes, v.data_ptr() + i * layer_bytes, tables.data_ptr(), lengths.data_ptr(), pages,
-                                            page_tokens, kv_heads, head_dim, tables.shape[0], tables.shape[1], _CODES[k.dtype]) for i in range(layers)]
+        self._layer = [pimdl.PagedCacheDesc(k.data_ptr() + i * layer_bytes, v.data_ptr() + i * layer_bytes, tables.data_ptr(), lengths.data_ptr(),
+                                            self.lacking.data_ptr(), pages, page_tokens, kv_heads, head_dim, tables.shape[0], tables.shape[1], _CODES[k.dtype]) for i in range(layers)]
         self._pools = (ctypes.c_void_p * 2)(k.data_ptr(), v.data_ptr())
         self._book = pimdl.PageBook(tables.data_ptr(), lengths.data_ptr(), refs.data_ptr(), self.lacking.data_ptr(), tables.shape[0], tables.shape[1], pages,
                                     page_tokens, ctypes.cast(self._pools, ctypes.POINTER(ctypes.c_void_p)), 2, layers, layer_bytes // max(pages, 1))
@@ -84,13 +85,11 @@ class PagedCache:
 
     def append(self, layer, k, v, starts, seqs=None):
         """New tokens' keys and values [tokens][kv_heads * head_dim] into the last positions of their sequences (whose room `reserve` has made)."""
-        columns = self.kv_heads * self.head_dim
-        ka, ks, kt = self._rows(k, columns, "k")
-        va, vs, vt = self._rows(v, columns, "v")
-        if (ks, kt, k.shape[0]) != (vs, vt, v.shape[0]):
+        if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
             raise ValueError("k and v must have one shape, stride and type")
+        ka, ks, kt = self._rows(k, self.kv_heads * self.head_dim, "k")
         to, at, batch = self._batch(starts, seqs)
-        self.ctx._check(self._lib.pimdl_cache_append(self.ctx._h, ctypes.byref(self._layer[layer]), to, at, batch, k.shape[0], ka, va, ks, kt))
+        self.ctx._check(self._lib.pimdl_cache_append(self.ctx._h, self._layer[layer], to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt))
 
     def attend(self, layer, q, out, starts, heads, seqs=None, left=None, sinks=0, scale=None):
         """Causal attention of the new tokens (q, out: [tokens][heads * head_dim]) over everything that their sequences have in the cache, or, with
@@ -101,7 +100,7 @@ class PagedCache:
         if qt != ot or q.shape[0] != out.shape[0]:
             raise ValueError("q and out must have one shape and type")
         to, at, batch = self._batch(starts, seqs)
-        self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, ctypes.byref(self._layer[layer]), to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt,
+        self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, self._layer[layer], to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt,
                                                         self._unlimited if left is None else left, sinks,
                                                         1.0 / math.sqrt(self.head_dim) if scale is None else scale))
 
@@ -111,7 +110,7 @@ class PagedCache:
         c, m = self._list(counts, "counts")
         if n != m:
             raise ValueError("seqs and counts must have one length")
-        self.ctx._check(self._lib.pimdl_pages_reserve(self.ctx._h, ctypes.byref(self._book), a, c, n))
+        self.ctx._check(self._lib.pimdl_pages_reserve(self.ctx._h, self._book, a, c, n))
 
     def fork(self, parents, children):
         """Gives each empty sequence children[i] what parents[i] has: whole pages are shared, a partly filled last one is copied."""
@@ -119,16 +118,16 @@ class PagedCache:
         c, m = self._list(children, "children")
         if n != m:
             raise ValueError("parents and children must have one length")
-        self.ctx._check(self._lib.pimdl_pages_fork(self.ctx._h, ctypes.byref(self._book), a, c, n))
+        self.ctx._check(self._lib.pimdl_pages_fork(self.ctx._h, self._book, a, c, n))
 
     def free(self, seqs):
         """Empties the sequences and gives their pages back."""
         a, n = self._list(seqs, "seqs")
-        self.ctx._check(self._lib.pimdl_pages_free(self.ctx._h, ctypes.byref(self._book), a, n))
+        self.ctx._check(self._lib.pimdl_pages_free(self.ctx._h, self._book, a, n))
 
     def compact(self):
         """Moves all pages in use to the front of the cache."""
-        self.ctx._check(self._lib.pimdl_pages_compact(self.ctx._h, ctypes.byref(self._book)))
+        self.ctx._check(self._lib.pimdl_pages_compact(self.ctx._h, self._book))
 
     def copy(self, src, dst):
         """Copies page src[i] to page dst[i] in every layer."""
@@ -136,4 +135,4 @@ class PagedCache:
         c, m = self._list(dst, "dst")
         if n != m:
             raise ValueError("src and dst must have one length")
-        self.ctx._check(self._lib.pimdl_pages_copy(self.ctx._h, ctypes.byref(self._book), a, c, n))
+        self.ctx._check(self._lib.pimdl_pages_copy(self.ctx._h, self._book, a, c, n))

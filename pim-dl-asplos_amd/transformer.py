@@ -61,6 +61,9 @@ class TransformerParams:
     ffn_hidden_dim: int
     layer_num: int
     shapes: dict = field(default_factory=dict)   # "qkv" | "q","k","v" | "o" | "ffn1" | "ffn2" -> AmmShape
+    # (left, right, sinks): a token sees `left` tokens before it, `right` behind it and the first `sinks` of its sequence (pimdl_attention_window);
+    # left or right None: all of them.  None: every token sees every other, as in the reference
+    window: tuple = None
 
     @property
     def n(self):
@@ -74,6 +77,9 @@ class TransformerParams:
         net, ker = cfg["network_params"], cfg["kernel_params"]
         p = cls(int(net["seq_len"]), int(net["batch_size"]), int(net["head_num"]), int(net["head_dim"]),
                 int(net["token_dim"]), int(net["ffn_hidden_dim"]), int(net["layer_num"]))
+        if "attention_window" in net:  # [left, right, sinks]; null: no border on that side
+            left, right, sinks = net["attention_window"]
+            p.window = (None if left is None else int(left), None if right is None else int(right), int(sinks))
         if p.head_num * p.head_dim != p.token_dim:
             raise ValueError("head_num * head_dim != token_dim")
         dims = {"qkv": (p.token_dim, 3 * p.token_dim), "o": (p.token_dim, p.token_dim),
@@ -161,6 +167,8 @@ class TransformerLayer:
         self.fused_qkv = fused_qkv
         self.fused_gelu = fused_gelu
         self.own_attention = True  # head_dim 64: pimdl_attention; other head sizes use PyTorch's fused attention
+        self._unlimited = pimdl.UNLIMITED
+        self._starts = {}  # sequences per batch -> first row of each, for pimdl_attention_window
         self.side = None if fused_qkv else side
         n = params.n
         self.amm = {}
@@ -218,13 +226,27 @@ class TransformerLayer:
                             residual.data_ptr(), y.data_ptr(), 1e-6)
         return y
 
-    def forward(self, x, keep=None):
+    def _attend_window(self, q, k, v, a, B):
+        """Attention in params.window within each of the B sequences of the batch."""
+        p = self.params
+        if B not in self._starts:
+            self._starts[B] = self.torch.arange(0, (B + 1) * p.seq_len, p.seq_len, device=q.device, dtype=self.torch.int32)
+        left, right = (self._unlimited if w is None else w for w in p.window[:2])
+        self.ctx.attention_window_ptr(q.data_ptr(), k.data_ptr(), v.data_ptr(), a.data_ptr(), self._starts[B].data_ptr(), B, B * p.seq_len, p.head_num,
+                                      p.head_num, p.head_dim, q.stride(0), k.stride(0), p.token_dim, left, right, p.window[2],
+                                      1.0 / math.sqrt(p.head_dim))
+
+    def forward(self, x, keep=None, cached=None):
         """x: float32 CUDA tensor [batch*seq][token_dim], row t = (batch t // seq_len, position t % seq_len).
-        `keep`: optional dict that receives every intermediate (for stage-by-stage checks)."""
+        `keep`: optional dict that receives every intermediate (for stage-by-stage checks).
+        `cached`: (PagedCache, layer, starts, seqs): x holds the newest tokens of those sequences instead (row b owns starts[b] ..
+        starts[b + 1] - 1, see kvcache.py); their keys and values go into the cache and they attend to what it holds, causally."""
         torch, p = self.torch, self.params
         n = x.shape[0]
-        if n % p.seq_len:
+        if cached is None and n % p.seq_len:
             raise ValueError("token count is not a multiple of seq_len")
+        if cached is not None and p.window is not None and p.window[1] != 0:
+            raise ValueError("a cache holds no later tokens: the window must have right = 0")
         B, S, H, hd = n // p.seq_len, p.seq_len, p.head_num, p.head_dim
         x = x.contiguous()
         if self.fused_qkv:
@@ -250,7 +272,16 @@ class TransformerLayer:
         else:
             q, k, v = self._run("q", x, n), self._run("k", x, n), self._run("v", x, n)
         att_scale = 1.0 / math.sqrt(p.token_dim / p.head_num)
-        if hd == 64 and self.own_attention:
+        if cached is not None:
+            cache, layer, starts, seqs = cached
+            a = torch.empty((n, p.token_dim), device=x.device, dtype=torch.float32)
+            left, _, sinks = p.window or (None, 0, 0)
+            cache.append(layer, k, v, starts, seqs)
+            cache.attend(layer, q, a, starts, H, seqs, left=left, sinks=sinks)
+        elif p.window is not None:
+            a = torch.empty((n, p.token_dim), device=x.device, dtype=torch.float32)
+            self._attend_window(q, k, v, a, B)
+        elif hd == 64 and self.own_attention:
             # the library's attention kernel reads q, k, v where they are (also as column ranges of the fused
             # projection's output) and writes [n][token_dim] directly
             a = torch.empty((n, p.token_dim), device=x.device, dtype=torch.float32)
@@ -309,6 +340,17 @@ class Transformer:
     def forward(self, x):
         for layer in self.layers:
             x = layer.forward(x)
+        return x
+
+    def extend(self, x, cache, starts, seqs, counts):
+        """The newest tokens of some sequences through the model (a chunk of a prompt, a single token, or both in one batch): x [tokens][token_dim]
+        packed, row b of the batch is the counts[b] tokens starts[b] .. starts[b + 1] - 1 of sequence seqs[b] (int32 device tensors; seqs
+        without repetitions).  Makes room for them in the PagedCache, fills it layer by layer, and every token sees its sequence up to itself
+        (params.window: with right = 0).  cache.lacking tells afterwards whether there were pages enough; if not, the outputs are those of the
+        tokens that the cache had before."""
+        cache.reserve(seqs, counts)
+        for i, layer in enumerate(self.layers):
+            x = layer.forward(x, cached=(cache, i, starts, seqs))
         return x
 
     def capture(self, x):

@@ -352,6 +352,23 @@ def test_append_skips_what_has_no_page(ctx):
     assert torch.equal(f.cache.k.view(torch.int16), before.view(torch.int16))
 
 
+def test_append_without_room_writes_nothing(ctx):
+    """A reserve that lacks pages leaves the lengths as they were: the new tokens' places would be those of older ones."""
+    cache = small_cache(ctx, 5, pages=3, seqs=2, width=8)
+    cache.reserve(ints(0), ints(40))
+    before = cache.k.clone()
+    x, starts = randn(gen_of(1), 20, 32), starts_of([20])
+    cache.reserve(ints(0), ints(20))
+    assert int(cache.lacking) == 1
+    cache.append(0, x, x, starts, ints(0))
+    torch.cuda.synchronize()
+    assert torch.equal(cache.k, before)
+    cache.reserve(ints(0), ints(8))
+    cache.append(0, x[:8], x[:8], starts_of([8]), ints(0))
+    torch.cuda.synchronize()
+    assert int(cache.lacking) == 0 and not torch.equal(cache.k, before)
+
+
 # ---------------------------------------------------------------------------------------------- pages
 
 class Model:
@@ -490,6 +507,26 @@ def test_fork_without_enough_pages_changes_nothing(ctx):
     model.fork([0, 1], [2, 3])
     assert model.lacking == 2
     model.same(cache)
+
+
+def test_forks_of_empty_sequences_that_are_children_themselves(ctx):
+    """Every parent is taken as it was before the call: chains of empty sequences stay empty, in any order of the list and however many there are."""
+    cache = small_cache(ctx, 6, pages=600, seqs=400, width=8)
+    model = Model(cache)
+    cache.reserve(ints(0), ints(100))
+    model.reserve([0], [100])
+    parents, children = [i if i % 2 else 0 for i in range(1, 200)], list(range(2, 201))
+    cache.fork(ints(*parents), ints(*children))
+    model.fork(parents, children)
+    model.same(cache)
+    for _ in range(20):
+        order = np.random.default_rng(_).permutation(199)
+        a, b = [parents[i] for i in order], [children[i] for i in order]
+        cache.free(ints(*children))
+        model.free(children)
+        cache.fork(ints(*a), ints(*b))
+        model.fork(a, b)
+        model.same(cache)
 
 
 def test_book_of_many_pages_and_sequences(ctx):
@@ -705,3 +742,81 @@ def test_wrong_calls_are_refused(ctx):
     # an empty batch is no error
     c.attend(0, q[:0], out[:0], starts_of([]), 4)
     c.free(ints())
+
+
+# ---------------------------------------------------------------------------------------------- the transformer
+
+def _model(ctx, hd, heads, layers, seq_len, batch, window=None, fused=False):
+    from pim_dl_asplos_amd import transformer as T
+    d = heads * hd
+    p = T.TransformerParams(seq_len, batch, heads, hd, d, 2 * d, layers)
+    for op, (k_in, m_out) in {"q": (d, d), "k": (d, d), "v": (d, d), "o": (d, d), "ffn1": (d, 2 * d), "ffn2": (2 * d, d)}.items():
+        p.shapes[op] = T.AmmShape(k_in // 4, 16, k_in, m_out)
+    p.shapes["qkv"] = T.AmmShape(d // 4, 16, d, 3 * d)
+    p.window = window
+    weights = T.synth_layers(p, ctx, pimdl, seed=3, shared_qkv_centroids=fused)
+    if fused:  # one scale for the three tables
+        for w in weights:
+            for name in ("k", "v"):
+                w[name]["scale"] = w["q"]["scale"]
+    return T.Transformer(ctx, pimdl, weights, p, fused_qkv=fused), p
+
+
+@pytest.mark.parametrize("hd,heads,window,fused", [(64, 4, (20, 5, 1), False), (64, 4, (None, 0, 0), True), (80, 2, (9, None, 2), False), (24, 4, (3, 3, 0), False)])
+def test_layer_with_a_window(ctx, hd, heads, window, fused):
+    model, p = _model(ctx, hd, heads, 1, 70, 3, window, fused)
+    x, keep = randn(gen_of(1), p.n, p.token_dim), {}
+    model.layers[0].forward(x, keep)
+    torch.cuda.synchronize()
+    left, right = (1 << 40 if w is None else w for w in window[:2])
+    for b in range(3):
+        rows = slice(70 * b, 70 * b + 70)
+        q, k, v = (keep[n][rows].reshape(70, heads, hd) for n in "qkv")
+        want, off, mass = reference(q, k, v, 0, left, right, window[2], 1 / math.sqrt(hd))
+        check(keep["attn"][rows].reshape(70, heads, hd), want, off, mass, "f32")
+    graph, static_x, static_y = model.capture(x)
+    for i in range(3):
+        static_x.copy_(x * (i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(static_y, model.forward(static_x))
+    model.close()
+
+
+@pytest.mark.parametrize("hd,heads,dtype,window,fused", [(64, 4, "f32", None, False), (64, 4, "f16", (30, 0, 2), True), (80, 2, "bf16", None, False)])
+def test_model_over_a_cache(ctx, hd, heads, dtype, window, fused):
+    """A prompt in two chunks beside single tokens of another sequence, then single tokens: q, k and v of every layer are those of its input rows (the
+    linear layers do not look at the batch), attention is checked against float64 over all that the layer has seen of the sequence."""
+    model, p = _model(ctx, hd, heads, 2, 32, 4, window, fused)
+    cache = K.PagedCache(ctx, pimdl, 2, 40, heads, hd, 16, dtype, 3, 200)
+    seen = {}
+    gen = gen_of(5)
+    left, sinks = (UNL, 0) if window is None else (window[0], window[2])
+    for seqs, counts in (([0, 2], [50, 1]), ([2, 0], [1, 33]), ([0, 2], [1, 1]), ([1, 0, 2], [17, 1, 1])):
+        n = sum(counts)
+        x = randn(gen, n, p.token_dim)
+        starts, lst = starts_of(counts), ints(*seqs)
+        y = model.extend(x, cache, starts, lst, ints(*counts))
+        torch.cuda.synchronize()
+        assert int(cache.lacking) == 0
+        # the same layers once more, with what is in the cache now, stage by stage
+        h = x
+        for i, layer in enumerate(model.layers):
+            keep = {}
+            h = layer.forward(h, keep, cached=(cache, i, starts, lst))
+            torch.cuda.synchronize()
+            at = 0
+            for s, c in zip(seqs, counts):
+                rows = slice(at, at + c)
+                q, k, v = (keep[nm][rows].reshape(c, heads, hd) for nm in "qkv")
+                old = seen.get((i, s), (k[:0].to(TYPES[dtype]), v[:0].to(TYPES[dtype])))
+                kk, vv = (torch.cat([o, t.to(TYPES[dtype])]) for o, t in zip(old, (k, v)))
+                seen[i, s] = (kk, vv)
+                want, off, mass = reference(q, kk, vv, kk.shape[0] - c, left, 0, sinks, 1 / math.sqrt(hd))
+                check(keep["attn"][rows].reshape(c, heads, hd), want, off, mass, "f32")
+                at += c
+        assert torch.equal(h, y)
+    with pytest.raises(ValueError):
+        model.layers[0].params.window = (4, 4, 0)
+        model.extend(x, cache, starts, lst, ints(*counts))
+    model.close()
