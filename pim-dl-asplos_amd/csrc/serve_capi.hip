@@ -57,6 +57,11 @@ int check_cache(Ctx* ctx, const char* fn, const pimdl_paged_cache* c, uint32_t d
     if (c->head_dim > 256 || c->kv_heads > 65535) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "%s: head_dim up to 256, kv_heads below 65536", fn);
     if (c->pages > 0x7fffffffu || (uint64_t)c->table_width * c->page_tokens > 0x7fffffffu - 4096)
         return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "%s: pages and table_width * page_tokens must be below 2^31 - 4096", fn);
+    return PIMDL_OK;
+}
+
+int check_cache_memory(Ctx* ctx, const char* fn, const pimdl_paged_cache* c)
+{
     int rc = check_device(ctx, fn, "cache k", c->k, 16);
     if (!rc) rc = check_device(ctx, fn, "cache v", c->v, 16);
     if (!rc) rc = check_device(ctx, fn, "cache tables", c->tables, 4);
@@ -140,7 +145,7 @@ int pimdl_attention_paged(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const 
     if (!seqs && batch > cache->seqs) return set_error(ctx, PIMDL_ERR_INVALID, "%s: batch=%u exceeds the cache's %u sequences", fn, batch, cache->seqs);
     if (tokens == 0 || batch == 0) return PIMDL_OK;
     const uint32_t e = dtype_bytes(dtype);
-    if ((rc = check_batch(ctx, fn, starts, batch, tokens)) || (seqs && (rc = check_device(ctx, fn, "seqs", seqs, 4))) ||
+    if ((rc = check_cache_memory(ctx, fn, cache)) || (rc = check_batch(ctx, fn, starts, batch, tokens)) || (seqs && (rc = check_device(ctx, fn, "seqs", seqs, 4))) ||
         (rc = check_device(ctx, fn, "q", q, e)) || (rc = check_device(ctx, fn, "out", out, e)))
         return rc;
     if ((rc = activate(ctx))) return rc;
@@ -166,7 +171,7 @@ int pimdl_cache_append(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const int
     if (!seqs && batch > cache->seqs) return set_error(ctx, PIMDL_ERR_INVALID, "%s: batch=%u exceeds the cache's %u sequences", fn, batch, cache->seqs);
     if (tokens == 0 || batch == 0) return PIMDL_OK;
     const uint32_t e = dtype_bytes(dtype);
-    if ((rc = check_batch(ctx, fn, starts, batch, tokens)) || (seqs && (rc = check_device(ctx, fn, "seqs", seqs, 4))) ||
+    if ((rc = check_cache_memory(ctx, fn, cache)) || (rc = check_batch(ctx, fn, starts, batch, tokens)) || (seqs && (rc = check_device(ctx, fn, "seqs", seqs, 4))) ||
         (rc = check_device(ctx, fn, "k", k, e)) || (rc = check_device(ctx, fn, "v", v, e)))
         return rc;
     if ((rc = activate(ctx))) return rc;

@@ -95,10 +95,12 @@ class PagedCache:
         """Causal attention of the new tokens (q, out: [tokens][heads * head_dim]) over everything that their sequences have in the cache, or, with
         `left`, over the `left` positions before each of them and the first `sinks`."""
         columns = heads * self.head_dim
-        qa, qs, qt = self._rows(q, columns, "q")
-        oa, os_, ot = self._rows(out, columns, "out")
-        if qt != ot or q.shape[0] != out.shape[0]:
+        if q.shape != out.shape or q.dtype != out.dtype:
             raise ValueError("q and out must have one shape and type")
+        qa, qs, qt = self._rows(q, columns, "q")
+        oa, os_, _ = self._rows(out, columns, "out")
+        if sinks < 0 or (left is not None and left < 0):
+            raise ValueError("left and sinks count positions")
         to, at, batch = self._batch(starts, seqs)
         self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, self._layer[layer], to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt,
                                                         self._unlimited if left is None else left, sinks,

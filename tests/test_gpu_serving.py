@@ -713,6 +713,9 @@ def test_wrong_calls_are_refused(ctx):
         c.attend(0, q, out, starts, 4, seqs=ints(0))
     with pytest.raises(pimdl.PimdlError):
         c.attend(0, q.bfloat16(), out.bfloat16(), starts, 4)  # over a cache in halves
+    for bad in (dict(left=-1), dict(sinks=-2)):
+        with pytest.raises(ValueError):
+            c.attend(0, q, out, starts, 4, **bad)
     with pytest.raises(pimdl.PimdlError):
         c.attend(0, q, out, starts.cpu(), 4)
     with pytest.raises(pimdl.PimdlError):
