@@ -112,21 +112,22 @@ int launch_plain(Ctx* ctx, const AttnArgs& a)
 
 // ---------------------------------------------------------------------------------------------
 // Joins what the splits of a row have: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).  A workgroup takes `rows` rows of up to 16 of a
-// sequence and key head (blocks of 16 are numbered as first_slot does); of a row's threads head_dim / 4 take four columns each, and `groups` sets of
+// sequence and key head (blocks of 16 are numbered as first_slot does, or, by_row, the first of each row of the batch: where only those of few rows are
+// split, the others would be 20 us of workgroups with nothing to do in a batch of 2300 tokens, 32 heads); of a row's threads head_dim / 4 take four columns each, and `groups` sets of
 // them every groups-th split.
 // ---------------------------------------------------------------------------------------------
 constexpr uint32_t JOIN_ROWS = 16;
 
 template <typename TQ>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::Partial part, uint32_t rows, uint32_t groups, uint32_t wide_splits,
-                                                             uint32_t narrow_splits, uint32_t narrow_rows)
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::Partial part, uint32_t by_row, uint32_t rows, uint32_t groups,
+                                                             uint32_t wide_splits, uint32_t narrow_splits, uint32_t narrow_rows)
 {
     __shared__ float sums[256][4];
     __shared__ float mls[256][2];
     const uint32_t parts = (JOIN_ROWS + rows - 1) / rows, tid = threadIdx.x, lanes = a.head_dim / 4;
     const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, slot = rest / parts;
-    const uint32_t b = attn::row_of_slot(a, slot, JOIN_ROWS);
-    const uint32_t first = clamped_start(a.starts, b, a.tokens), end = clamped_start(a.starts, b + 1, a.tokens), before = attn::first_slot(a, b, first, JOIN_ROWS);
+    const uint32_t b = by_row ? slot : attn::row_of_slot(a, slot, JOIN_ROWS);
+    const uint32_t first = clamped_start(a.starts, b, a.tokens), end = clamped_start(a.starts, b + 1, a.tokens), before = by_row ? slot : attn::first_slot(a, b, first, JOIN_ROWS);
     if (slot < before || end <= first) return;
     const uint32_t count = (end - first) * a.group, row0 = (slot - before) * JOIN_ROWS + rest % parts * rows;
     const uint32_t splits = count <= narrow_rows ? narrow_splits : wide_splits;
@@ -192,9 +193,11 @@ int launch_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
     uint32_t groups = 1;
     while (groups < 16 && groups * 4 < splits && 2 * groups * lanes <= 256) groups *= 2;
     const uint32_t rows = std::min(JOIN_ROWS, 256 / (lanes * groups)), parts = (JOIN_ROWS + rows - 1) / rows;
-    const uint64_t slots = (uint64_t)a.tokens * a.group / JOIN_ROWS + a.batch, grid = slots * parts * a.kv_heads;
+    const bool by_row = p.wide && p.wide_splits == 1;  // (those that are split have up to NARROW_ROWS rows)
+    static_assert(attn::NARROW_ROWS <= JOIN_ROWS, "a block holds all rows of a sequence of few");
+    const uint64_t slots = (by_row ? 0 : (uint64_t)a.tokens * a.group / JOIN_ROWS) + a.batch, grid = slots * parts * a.kv_heads;
     if (grid > 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
-    hipLaunchKernelGGL((attention_join_kernel<TQ>), dim3((uint32_t)grid), dim3(256), 0, ctx->stream, a, p.part, rows, groups, p.wide ? p.wide_splits : 1,
+    hipLaunchKernelGGL((attention_join_kernel<TQ>), dim3((uint32_t)grid), dim3(256), 0, ctx->stream, a, p.part, (uint32_t)by_row, rows, groups, p.wide ? p.wide_splits : 1,
                        p.narrow ? p.narrow_splits : 1, p.narrow ? p.narrow_rows : 0);
     return hip_check(ctx, hipGetLastError(), "attention_join_kernel launch");
 }

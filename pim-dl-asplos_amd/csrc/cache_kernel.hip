@@ -116,22 +116,28 @@ __device__ __forceinline__ T block_scan(T v, T* tmp, T* total)
     return tmp[wave] + x - v;
 }
 
-// The `want` lowest free pages into fresh[0 ..]; returns how many of them there are.
-__device__ uint32_t lowest_free(const int32_t* refs, uint32_t pages, uint32_t want, int32_t* fresh, uint32_t* tmp)
+// Which of a thread's pages in the SCAN_EACH * SCAN from p0 on are free.  Asked for before anything that it does not wait for.
+constexpr uint32_t SCAN_EACH = 8;
+__device__ __forceinline__ uint32_t free_mask(const int32_t* refs, uint32_t pages, uint32_t p0)
 {
-    constexpr uint32_t EACH = 8;
-    uint32_t found = 0;
-    for (uint32_t p0 = 0; p0 < pages && found < want; p0 += SCAN * EACH) {
-        const uint32_t p = p0 + threadIdx.x * EACH;
-        uint32_t mask = 0;
+    const uint32_t p = p0 + threadIdx.x * SCAN_EACH;
+    uint32_t mask = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i)
-            if (p + i < pages && refs[p + i] == 0) mask |= 1u << i;
+    for (uint32_t i = 0; i < SCAN_EACH; ++i)
+        if (p + i < pages && refs[p + i] == 0) mask |= 1u << i;
+    return mask;
+}
+// The `want` lowest free pages into fresh[0 ..] (device memory or LDS); returns how many of them there are.  `mask`: free_mask of page 0.
+__device__ __forceinline__ uint32_t lowest_free(const int32_t* refs, uint32_t pages, uint32_t want, uint32_t mask, int32_t* fresh, uint32_t* tmp)
+{
+    uint32_t found = 0;
+    for (uint32_t p0 = 0; p0 < pages && found < want; p0 += SCAN * SCAN_EACH) {
+        if (p0) mask = free_mask(refs, pages, p0);
         uint32_t total, at = found + block_scan<uint32_t>(__popc(mask), tmp, &total);
 #pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i)
+        for (uint32_t i = 0; i < SCAN_EACH; ++i)
             if (mask >> i & 1) {
-                if (at < want) fresh[at] = (int32_t)(p + i);
+                if (at < want) fresh[at] = (int32_t)(p0 + threadIdx.x * SCAN_EACH + i);
                 ++at;
             }
         found += total;
@@ -165,12 +171,14 @@ __device__ __forceinline__ int32_t short_of(uint64_t want, uint32_t found)
 }
 
 __global__ __launch_bounds__(SCAN) void pages_reserve_kernel(Book b, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, uint32_t n,
-                                                             int32_t* __restrict__ fresh)
+                                                             int32_t* fresh)
 {
     extern __shared__ int32_t lds[];  // mark[seqs], base[n]
     __shared__ uint64_t tmp64[SCAN / 64 + 1];
     __shared__ uint32_t tmp32[SCAN / 64 + 1], too_long;
+    __shared__ int32_t few[SCAN];  // the new pages, where they fit
     int32_t *mark = lds, *base = lds + b.seqs;
+    const uint32_t mask = free_mask(b.refs, b.pages, 0);
     if (threadIdx.x == 0) too_long = 0;
     first_places(seqs, n, mark, b.seqs);
     auto grown = [&](uint32_t i, int32_t* s, int32_t* have) -> int64_t {  // the new length of entry i's sequence, or -1
@@ -198,7 +206,9 @@ __global__ __launch_bounds__(SCAN) void pages_reserve_kernel(Book b, const int32
         if (threadIdx.x == 0) *b.lacking = -1;
         return;
     }
-    const uint32_t asked = (uint32_t)(want < b.pages ? want : b.pages), found = lowest_free(b.refs, b.pages, asked, fresh, tmp32);
+    const uint32_t asked = (uint32_t)(want < b.pages ? want : b.pages);
+    if (asked <= SCAN) fresh = few;
+    const uint32_t found = lowest_free(b.refs, b.pages, asked, mask, fresh, tmp32);
     if (found < want) {
         if (threadIdx.x == 0) *b.lacking = short_of(want, found);
         return;
@@ -267,40 +277,59 @@ __global__ __launch_bounds__(SCAN) void pages_fork_kernel(Book b, const int32_t*
 {
     extern __shared__ int32_t lds[];  // mark[seqs]
     __shared__ uint32_t tmp[SCAN / 64 + 1];
+    __shared__ int32_t few[SCAN];  // the new pages, where they fit
     int32_t* mark = lds;
+    const uint32_t mask = free_mask(b.refs, b.pages, 0);
     first_places(children, n, mark, b.seqs);
-    auto last_page = [&](uint32_t i) -> int32_t {  // of entry i's parent if partly filled, -1: none, -2: the entry is left out
+    // the last page of entry i's parent if partly filled, -1: none, -2: the entry is left out
+    auto last_page = [&](uint32_t i, int32_t* len) -> int32_t {
         const int32_t p = parents[i], c = children[i];
+        *len = 0;
         if (p < 0 || (uint32_t)p >= b.seqs || c < 0 || (uint32_t)c >= b.seqs || mark[c] != (int32_t)i || b.lengths[c] != 0) return -2;
-        const int32_t len = held_length(b, p);
-        if (len % b.page_tokens == 0) return -1;
-        const int32_t page = b.tables[(size_t)p * b.width + len / b.page_tokens];
+        *len = held_length(b, p);
+        if (*len % b.page_tokens == 0) return -1;
+        const int32_t page = b.tables[(size_t)p * b.width + *len / b.page_tokens];
         return page >= 0 && (uint32_t)page < b.pages ? page : -1;
     };
-    uint32_t want = 0;
+    uint32_t want = 0, at = 0, total;
+    int32_t page = -2, len = 0;
     for (uint32_t i0 = 0; i0 < n; i0 += SCAN) {
         const uint32_t i = i0 + threadIdx.x;
-        const int32_t page = i < n ? last_page(i) : -2;
-        uint32_t total;
-        const uint32_t at = want + block_scan<uint32_t>(page >= 0, tmp, &total);
-        if (page >= 0) f.src[at] = page;
-        if (i < n) {
+        page = i < n ? last_page(i, &len) : -2;
+        at = want + block_scan<uint32_t>(page >= 0, tmp, &total);
+        if (n > SCAN && i < n) {  // (else they stay in registers)
+            if (page >= 0) f.src[at] = page;
             f.take[i] = page >= 0 ? (int32_t)at : page;
-            f.length[i] = page == -2 ? 0 : held_length(b, parents[i]);
+            f.length[i] = len;
         }
         want += total;
     }
-    const uint32_t asked = want < b.pages ? want : b.pages, found = lowest_free(b.refs, b.pages, asked, f.fresh, tmp);
+    const uint32_t asked = want < b.pages ? want : b.pages;
+    int32_t* const fresh = asked <= SCAN ? few : f.fresh;
+    const uint32_t found = lowest_free(b.refs, b.pages, asked, mask, fresh, tmp);
     const bool done = found == want;
-    for (uint32_t i = threadIdx.x; i < n; i += SCAN) {
-        if (!done) f.take[i] = -2;
-        else if (f.take[i] >= 0) f.take[i] = f.fresh[f.take[i]];
-    }
-    if (done)
-        for (uint32_t t = threadIdx.x; t < want; t += SCAN) {
-            f.dst[t] = f.fresh[t];
-            b.refs[f.fresh[t]] = 1;
+    if (n <= SCAN) {
+        if (threadIdx.x < n) {
+            const int32_t take = !done ? -2 : page >= 0 ? fresh[at] : page;
+            f.take[threadIdx.x] = take;
+            f.length[threadIdx.x] = len;
+            if (take >= 0) {
+                f.src[at] = page;
+                f.dst[at] = take;
+                b.refs[take] = 1;
+            }
         }
+    } else {
+        for (uint32_t i = threadIdx.x; i < n; i += SCAN) {
+            if (!done) f.take[i] = -2;
+            else if (f.take[i] >= 0) f.take[i] = fresh[f.take[i]];
+        }
+        if (done)
+            for (uint32_t t = threadIdx.x; t < want; t += SCAN) {
+                f.dst[t] = fresh[t];
+                b.refs[fresh[t]] = 1;
+            }
+    }
     if (threadIdx.x == 0) {
         *f.count = done ? (int32_t)want : 0;
         *b.lacking = short_of(want, found);
