@@ -368,9 +368,9 @@ PIMDL_API int pimdl_attention(pimdl_ctx* ctx, const float* q, const float* k, co
  * h / (heads / kv_heads), heads a multiple of kv_heads.  head_dim 1 .. 256; 32, 64, 80, 96 and 128 run on the matrix
  * cores (given 16-byte aligned rows), other sizes on a plain kernel.  Strides are in elements.
  *
- * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max_j), over the keys that a query sees.  Scores, maxima,
+ * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max_j), over the keys that a query sees; |scale| up to 2^96.  Scores, maxima,
  * sums and accumulators are fp32.  With fp32 operands products keep fp32 accuracy (factors of 24 bits; 22 of q and p over a
- * cache in halves); with 16-bit operands p_j is rounded to that type once, before it meets v_j.  A query that sees no key gives
+ * cache in halves); with 16-bit operands p_j is rounded to that type at most once, before it meets v_j.  A query that sees no key gives
  * zeros.  Rows of K and V that a query does not see -- hidden by the window, behind a length, of other sequences, on pages of
  * nobody -- do not change its result whatever they hold, infinities and NaN included; an element of its own q or of a row that it
  * sees which is not finite makes the results it enters infinite or NaN. */
@@ -415,7 +415,8 @@ PIMDL_API int pimdl_attention_paged(pimdl_ctx* ctx, const pimdl_paged_cache* cac
                                     uint32_t heads, uint32_t q_stride, uint32_t out_stride, uint32_t dtype,
                                     uint32_t left, uint32_t sinks, float scale);
 /* Writes the new tokens' keys and values ([tokens][kv_stride], rounded to nearest even to the cache's type) at those
- * positions.  dtype: PIMDL_F32, or the cache's own 16-bit type. */
+ * positions, whoever else holds the page (a fork never shares one that is not full).  A sequence stands in `seqs` once: two rows of the
+ * batch with the same sequence would write the same places.  dtype: PIMDL_F32, or the cache's own 16-bit type. */
 PIMDL_API int pimdl_cache_append(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const int32_t* seqs,
                                  const int32_t* starts, uint32_t batch, uint32_t tokens, const void* k, const void* v,
                                  uint32_t kv_stride, uint32_t dtype);

@@ -98,6 +98,10 @@ __device__ __forceinline__ void pieces(float x, float y, uint32_t* out)
     } else if constexpr (N == 1) {
         bf16x2 a = {(__bf16)x, (__bf16)y};
         out[0] = __builtin_bit_cast(uint32_t, a);
+    } else if constexpr (N == 2) {
+        bf16x2 a = {(__bf16)x, (__bf16)y}, b = {(__bf16)(x - (float)a[0]), (__bf16)(y - (float)a[1])};
+        out[0] = __builtin_bit_cast(uint32_t, a);
+        out[1] = __builtin_bit_cast(uint32_t, b);
     } else {
         out[0] = high_halves(bits(x), bits(y));
         x -= number(bits(x) & 0xffff0000u);
@@ -303,6 +307,8 @@ struct Rows {
     static constexpr bool REST = C::HD % STEP != 0;                          // M == 16, groups 2 and 3 repeat the dims of 0 and 1 against zeros of q
     static constexpr int DT = (C::HD + M - 1) / M;             // tiles of the second (80 dims, M == 32: of the last one only half counts)
     static constexpr int QUADS = REGS / 4, OREGS = M * M / 64, OQUADS = OREGS / 4;
+    // pieces of p: in 16 bits it is rounded to one for many rows, where that is a third of the matrix instructions; few rows wait for memory
+    static constexpr int NP = C::NQ == 1 && M == 16 ? 2 : C::NQ;
     typedef typename std::conditional<M == 32, f32x16, f32x4>::type Acc;
     static constexpr int KT = M == 32 ? 1 : 2;  // accumulators of 32 keys
 
@@ -327,7 +333,7 @@ struct Rows {
         const uint32_t g = group(), mine = row0 + row() < rows ? row0 + row() : rows - 1;  // rows past the last repeat it; they are never stored
         const uint32_t token = mine / a.group, head = kh * a.group + mine % a.group;
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;  // c is positive, so that the largest score has the largest exponent
-        c = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * LOG2E;
+        c = fminf((a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale), 1.2e-38f)) * LOG2E, 3e38f);
         const typename C::TQ* const base = static_cast<const typename C::TQ*>(a.q) + (size_t)(r.first + token) * a.q_stride + (size_t)head * C::HD;
         if constexpr (C::NQ == 1) {
             const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u, keep = sign == 0.0f ? 0u : ~0u;
@@ -354,6 +360,7 @@ struct Rows {
                 factor *= number((uint32_t)(127 + e) << 23);
                 c *= number((uint32_t)(127 - e) << 23);
             }
+            c = fminf(fmaxf(c, 1.2e-38f), 3e38f);  // (0 or infinity times a hidden score would be NaN)
 #pragma unroll
             for (int s = 0; s < 2 * KS; ++s) {
                 uint32_t w[2][C::NQ];
@@ -387,14 +394,15 @@ struct Rows {
     __device__ __forceinline__ bool all(int32_t key0, int32_t n) const { return key0 + n <= min_hi && (key0 >= max_lo || key0 + n <= sinks); }
     __device__ __forceinline__ bool sees(int32_t key) const { return key < hi && (key >= lo || key < sinks); }
 
-    // of a product of NQ and NK pieces those that reach the last bit of the larger count, small ones first
+    // of a product of N and NK pieces those that reach the last bit of the larger count, small ones first
+    template <int N>
     static __device__ __forceinline__ void product(const u32x4* x, const u32x4* y, Acc& sum)
     {
 #pragma unroll
-        for (int w = C::NK == 1 ? C::NQ - 1 : 2; w >= 0; --w)
+        for (int w = C::NK == 1 ? N - 1 : 2; w >= 0; --w)
 #pragma unroll
             for (int n = 0; n < C::NK; ++n)
-                if (w - n >= 0 && w - n < C::NQ) sum = mfma<C::HALF>(x[n], y[w - n], sum);
+                if (w - n >= 0 && w - n < N) sum = mfma<C::HALF>(x[n], y[w - n], sum);
     }
 
     // scores of 32 keys, which lie in LDS from `k` on, pieces PIECE bytes apart
@@ -413,7 +421,7 @@ struct Rows {
                 for (int n = 0; n < C::NK; ++n) x[n] = *reinterpret_cast<const u32x4*>(at + n * PIECE + (((dims(st) / 8) ^ order<C::HD>(t * M + j)) << 4));
 #pragma unroll
                 for (int n = 0; n < C::NQ; ++n) y[n] = q[n][st];
-                product(x, y, acc);
+                product<C::NQ>(x, y, acc);
             }
 #pragma unroll
             for (int i = 0; i < OREGS; ++i) s[t * OREGS + i] = acc[i];
@@ -456,18 +464,25 @@ struct Rows {
 #pragma unroll
         for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
         mx = row_max<M>(mx);
-        if (__any(mx * c > m * c + RISE)) {
-            const float up = fmaxf(m, mx), base = up == -INF ? 0.0f : up * c;
-            const float alpha = __builtin_amdgcn_exp2f(m * c - base);  // 0 at the first keys
+        if (__any((mx - m) * c > RISE)) {
+            const float up = fmaxf(m, mx);
+            const float alpha = __builtin_amdgcn_exp2f((m - (up == -INF ? 0.0f : up)) * c);  // 0 at the first keys
             m = up;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
-        const float base = (m == -INF ? 0.0f : m * c) - (float)C::P_SHIFT;
+        float base = m == -INF ? 0.0f : m * c;
+        if (__any(fabsf(base) > 0x1p20f)) {  // (rare) the rounding of m c would be a factor of its own
+            const float most = m == -INF ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] -= most;
+            base = 0.0f;
+        }
+        base -= (float)C::P_SHIFT;
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base));
-        if constexpr (C::NQ > 1) {
+        if constexpr (NP > 1) {
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < N; ++i) sum += s[i];
@@ -482,19 +497,19 @@ struct Rows {
         const uint32_t i = threadIdx.x & 15, side = row() / 16, g = group();
 #pragma unroll
         for (int st = 0; st < REGS / 8; ++st) {
-            uint32_t w[4][C::NQ];
+            uint32_t w[4][NP];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pieces<C::HALF, C::NQ>(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], w[e]);
-            if constexpr (C::NQ == 1) {  // l is the sum of what the products get
+            for (int e = 0; e < 4; ++e) pieces<C::HALF, NP>(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], w[e]);
+            if constexpr (NP == 1) {  // l is the sum of what the products get
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (C::HALF) l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w[e][0]), (f16x2){(_Float16)1.0f, (_Float16)1.0f}, l, false);
                     else l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[e][0]), (bf16x2){(__bf16)1.0f, (__bf16)1.0f}, l, false);
                 }
             }
-            u32x4 b[C::NQ];
+            u32x4 b[NP];
 #pragma unroll
-            for (int n = 0; n < C::NQ; ++n) b[n] = (u32x4){w[0][n], w[1][n], w[2][n], w[3][n]};
+            for (int n = 0; n < NP; ++n) b[n] = (u32x4){w[0][n], w[1][n], w[2][n], w[3][n]};
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 u32x4 x[C::NK];
@@ -509,7 +524,7 @@ struct Rows {
                     }
                     x[n] = (u32x4){half[0][0], half[0][1], half[1][0], half[1][1]};
                 }
-                product(x, b, o[d]);
+                product<NP>(x, b, o[d]);
             }
         }
     }

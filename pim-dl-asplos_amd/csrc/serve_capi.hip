@@ -40,7 +40,7 @@ int check_heads(Ctx* ctx, const char* fn, uint32_t heads, uint32_t kv_heads, uin
     if (heads > 65535) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "%s: heads must be below 65536", fn);
     if ((uint64_t)heads * head_dim > q_stride || (uint64_t)heads * head_dim > out_stride)
         return set_error(ctx, PIMDL_ERR_INVALID, "%s: q_stride and out_stride must hold heads * head_dim elements", fn);
-    if (!(scale - scale == 0.0f)) return set_error(ctx, PIMDL_ERR_INVALID, "%s: scale is not finite", fn);
+    if (!(scale >= -0x1p96f && scale <= 0x1p96f)) return set_error(ctx, PIMDL_ERR_INVALID, "%s: scale must be finite, of a magnitude up to 2^96", fn);
     return PIMDL_OK;
 }
 

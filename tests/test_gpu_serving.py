@@ -567,6 +567,82 @@ def test_pages_copy(ctx):
     assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v)
 
 
+# ---------------------------------------------------------------------------------------------- beyond 32 bits
+
+def test_pages_beyond_four_gigabytes(ctx):
+    """A cache of 4.9 GB for keys and as much for values, whose sequences lie at its end: append, attention, fork and compaction."""
+    pages, kv, hd, heads = 150000, 8, 128, 16
+    k, v = (torch.empty(1, pages, kv, 16, hd, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    tables = torch.full((4, 8), -1, dtype=torch.int32)
+    tables[0, :5] = torch.arange(pages - 1, pages - 6, -1)
+    refs = torch.zeros(pages, dtype=torch.int32)
+    refs[-5:] = 1
+    cache = K.PagedCache.over(ctx, pimdl, k, v, tables.cuda(), ints(70, 0, 0, 0), refs.cuda())
+    gen = gen_of(2)
+    kk, vv = (randn(gen, 70, kv * hd, dtype="bf16") for _ in range(2))
+    cache.append(0, kk, vv, starts_of([70]), ints(0))
+    kk, vv = (x.reshape(70, kv, hd) for x in (kk, vv))
+
+    def attend(s, n):
+        q = randn(gen, n, heads * hd, dtype="bf16")
+        out = torch.zeros_like(q)
+        cache.attend(0, q, out, starts_of([n]), heads, ints(s))
+        torch.cuda.synchronize()
+        want, off, mass = reference(q.reshape(n, heads, hd), kk, vv, 70 - n, UNL, 0, 0, 1 / math.sqrt(hd))
+        check(out.reshape(n, heads, hd), want, off, mass, "bf16")
+
+    attend(0, 1)
+    attend(0, 40)
+    cache.fork(ints(0), ints(3))
+    attend(3, 1)
+    cache.free(ints(0))
+    cache.compact()
+    torch.cuda.synchronize()
+    assert cache.tables[3, :5].tolist() == [4, 3, 2, 1, 0] and cache.refs[:6].tolist() == [1, 1, 1, 1, 1, 0] and int(cache.refs.sum()) == 5
+    attend(3, 1)
+    attend(3, 40)
+
+
+@pytest.mark.parametrize("hd", [64, 20])
+def test_window_rows_beyond_four_gigabytes(ctx, hd):
+    n, stride = 70000, 32768
+    buf = torch.empty(n, stride, device="cuda", dtype=torch.bfloat16)
+    for c in range(3):
+        buf[:, c * 64:c * 64 + hd] = randn(gen_of(c), n, hd, dtype="bf16")
+    out = buf[:, 192:192 + hd]
+    window(ctx, buf[:, :hd], buf[:, 64:64 + hd], buf[:, 128:128 + hd], out, [n - 300, 300], 1, 1, hd, 0, 0, 0, "bf16")
+    torch.cuda.synchronize()
+    assert torch.equal(out, buf[:, 128:128 + hd])  # each token sees itself alone
+    window(ctx, buf[:, :hd], buf[:, 64:64 + hd], buf[:, 128:128 + hd], out, [n - 300, 300], 1, 1, hd, 5, 0, 1, "bf16")
+    torch.cuda.synchronize()
+    q, k, v = (buf[-300:, c * 64:c * 64 + hd, None].transpose(1, 2) for c in range(3))
+    want, off, mass = reference(q, k, v, 0, 5, 0, 1, 1 / math.sqrt(hd))
+    check(out[-300:, None], want, off, mass, "bf16")
+
+
+@pytest.mark.parametrize("scale", [1e-38, 3e38, -2e38, 7e28, -7e28])
+def test_scales_at_the_ends_of_their_range(ctx, scale):
+    """Nearly uniform shares, and the largest score takes all, with rows of keys that are hidden in the same tile."""
+    for dtype, cache in (("f32", "f16"), ("f32", "f32"), ("bf16", "bf16")):
+        f = Filled(ctx, 60, [50], 1, 64, 16, cache)
+        q = randn(gen_of(4), 20, 64, dtype=dtype)
+        q[:] = q[0]
+        out = torch.zeros_like(q)
+        if abs(scale) > 2.0 ** 96:  # scores of ordinary sizes would not be fp32 numbers
+            with pytest.raises(pimdl.PimdlError):
+                f.cache.attend(0, q, out, starts_of([20]), 1, scale=scale)
+            continue
+        f.cache.attend(0, q, out, starts_of([20]), 1, scale=scale)
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all()
+        k, v = (x[0, :, 0].double() for x in f.rows[0])
+        for i in range(20):
+            seen = 31 + i
+            s = (q[i].double() @ k[:seen].T) * math.copysign(1, scale)
+            want = v[:seen].mean(0) if abs(scale) < 1 else v[int(s.argmax())]
+            torch.testing.assert_close(out[i].double(), want, rtol=2 * HALF[dtype] + 1e-5, atol=HALF[dtype] + 1e-5)
+
+
 # ---------------------------------------------------------------------------------------------- together
 
 def test_forked_sequences_go_on_from_one_prompt(ctx):
