@@ -165,21 +165,20 @@ __device__ __forceinline__ Place place(const AttnArgs& a, const Row& r, uint32_t
     p.there = ~0u;
     p.base0 = p.base1 = p.base2 = p.base3 = 0;
     if constexpr (C::PAGED) {
-        const uint64_t page_bytes = (uint64_t)(a.kv_heads << a.page_shift) * C::RB;
-        auto group = [&](int g) -> int64_t {
-            uint32_t page = (uint32_t)__builtin_amdgcn_readlane(ahead.entry, g);
-            if (page >= a.pages) {  // (-1, too)
-                page = 0;
-                p.there &= ~(1u << g);
-            }
-            const uint32_t row = (kh << a.page_shift) + (uint32_t)((key0 + 16 * g) & ((1 << a.page_shift) - 1));
-            return (int64_t)(page * page_bytes + (uint64_t)row * C::RB);
+        // every lane for its own group, on the vector unit: a wave gets a scalar instruction through in four times the time
+        const uint32_t page_bytes = (a.kv_heads << a.page_shift) * (uint32_t)C::RB, lane_group = threadIdx.x % (TILE / 16);
+        const bool there = (uint32_t)ahead.entry < a.pages;  // (not -1)
+        const uint32_t row = (kh << a.page_shift) + ((uint32_t)(key0 + 16 * (int32_t)lane_group) & ((1u << a.page_shift) - 1));
+        const uint64_t base = (uint64_t)(there ? (uint32_t)ahead.entry : 0u) * page_bytes + row * (uint32_t)C::RB;
+        p.there = (uint32_t)__ballot(there) | ~((1u << TILE / 16) - 1);
+        auto of_group = [&](int g) {
+            return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(base >> 32), g) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)base, g));
         };
-        p.base0 = group(0);
-        p.base1 = group(1);
+        p.base0 = of_group(0);
+        p.base1 = of_group(1);
         if constexpr (TILE == 64) {
-            p.base2 = group(2);
-            p.base3 = group(3);
+            p.base2 = of_group(2);
+            p.base3 = of_group(3);
         }
     } else {
         p.base0 = ((int64_t)r.first * a.kv_stride + (int64_t)kh * C::HD) * (int64_t)sizeof(typename C::TK);

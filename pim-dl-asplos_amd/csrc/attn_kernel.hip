@@ -209,6 +209,8 @@ bool matrix_form(const AttnArgs& a)
     const uint64_t qe = a.dtype == PIMDL_F32 ? 4 : 2, ke = a.cache_dtype == PIMDL_F32 ? 4 : 2;
     uint64_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
     all |= a.q_stride * qe | a.out_stride * qe | (a.paged ? 0 : a.kv_stride * ke);
+    // (offsets within a page, or within a tile of rows, are 32-bit numbers)
+    if (a.paged && ((uint64_t)a.kv_heads << a.page_shift) * a.head_dim * ke >= 1ull << 32) return false;
     return all % 16 == 0 && (uint64_t)a.tokens * a.group < 1u << 30 && a.kv_stride < 1u << 22;
 }
 
