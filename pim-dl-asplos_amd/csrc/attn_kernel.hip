@@ -119,71 +119,81 @@ int launch_plain(Ctx* ctx, const AttnArgs& a)
 constexpr uint32_t JOIN_ROWS = 16;
 
 template <typename TQ>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::Partial part, uint32_t by_row, uint32_t rows, uint32_t groups,
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::Partial part, uint32_t by_row, uint32_t parts, uint32_t rows, uint32_t groups,
                                                              uint32_t wide_splits, uint32_t narrow_splits, uint32_t narrow_rows)
 {
     __shared__ float sums[256][4];
     __shared__ float mls[256][2];
-    const uint32_t parts = (JOIN_ROWS + rows - 1) / rows, tid = threadIdx.x, lanes = a.head_dim / 4;
+    const uint32_t tid = threadIdx.x, lanes = a.head_dim / 4;
     const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, slot = rest / parts;
     const uint32_t b = by_row ? slot : attn::row_of_slot(a, slot, JOIN_ROWS);
     const uint32_t first = clamped_start(a.starts, b, a.tokens), end = clamped_start(a.starts, b + 1, a.tokens), before = by_row ? slot : attn::first_slot(a, b, first, JOIN_ROWS);
     if (slot < before || end <= first) return;
-    const uint32_t count = (end - first) * a.group, row0 = (slot - before) * JOIN_ROWS + rest % parts * rows;
+    const uint32_t count = (end - first) * a.group, row0 = (slot - before) * JOIN_ROWS, stop = row0 + JOIN_ROWS < count ? row0 + JOIN_ROWS : count;
     const uint32_t splits = count <= narrow_rows ? narrow_splits : wide_splits;
     if (row0 >= count || splits == 1) return;
-    const uint32_t set = tid / lanes, mine = set / groups, g = set % groups, col = tid % lanes * 4, row = row0 + mine;
-    const bool works = mine < rows && row < count && row < (slot - before + 1) * JOIN_ROWS;
-    const uint32_t t = first + row / a.group, head = kh * a.group + row % a.group;
-    const uint64_t at = (uint64_t)t * a.heads + head;
-    float top = -__builtin_inff(), l = 0.0f;
-    attn::f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    if (works) {
-        constexpr uint32_t AHEAD = 8;  // splits whose results are asked for together
-        for (uint32_t s0 = g; s0 < splits; s0 += AHEAD * groups) {
-            float m[AHEAD], lm[AHEAD];
-            attn::f32x4 x[AHEAD];
+    const uint32_t set = tid / lanes, mine = set / groups, g = set % groups, col = tid % lanes * 4;
+    for (uint32_t from = row0 + rest % parts * rows; from < stop; from += parts * rows) {
+        const uint32_t row = from + mine;
+        const bool works = mine < rows && row < stop;
+        const uint32_t t = first + row / a.group, head = kh * a.group + row % a.group;
+        const uint64_t at = (uint64_t)t * a.heads + head;
+        float top = -__builtin_inff(), l = 0.0f;
+        attn::f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        auto take = [&](auto count) __attribute__((always_inline)) {
+            constexpr uint32_t AHEAD = decltype(count)::value;  // splits whose results are asked for together
+            for (uint32_t s0 = g; s0 < splits; s0 += AHEAD * groups) {
+                float m[AHEAD], lm[AHEAD];
+                attn::f32x4 x[AHEAD];
 #pragma unroll
-            for (uint32_t i = 0; i < AHEAD; ++i) {
-                const uint32_t s = s0 + i * groups < splits ? s0 + i * groups : splits - 1;
-                const uint64_t where = s * part.rows + at;
-                m[i] = part.ml[2 * where];
-                lm[i] = s0 + i * groups < splits ? part.ml[2 * where + 1] : 0.0f;
-                x[i] = *reinterpret_cast<const attn::f32x4*>(part.o + where * a.head_dim + col);  // (anything where l is 0)
+                for (uint32_t i = 0; i < AHEAD; ++i) {
+                    const uint32_t s = s0 + i * groups < splits ? s0 + i * groups : splits - 1;
+                    const uint64_t where = s * part.rows + at;
+                    m[i] = part.ml[2 * where];
+                    lm[i] = s0 + i * groups < splits ? part.ml[2 * where + 1] : 0.0f;
+                    x[i] = *reinterpret_cast<const attn::f32x4*>(part.o + where * a.head_dim + col);  // (anything where l is 0)
+                }
+                float up = top;
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) up = fmaxf(up, m[i]);
+                const float base = up == -__builtin_inff() ? 0.0f : up, alpha = __builtin_amdgcn_exp2f(top - base);
+                top = up;
+                l *= alpha;
+                y *= alpha;
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) {
+                    const float f = __builtin_amdgcn_exp2f(m[i] - base);
+                    l += lm[i] == 0.0f ? 0.0f : lm[i] * f;  // (NaN is not)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] += lm[i] == 0.0f ? 0.0f : x[i][e] * f;
+                }
             }
-            float up = top;
-#pragma unroll
-            for (uint32_t i = 0; i < AHEAD; ++i) up = fmaxf(up, m[i]);
-            const float base = up == -__builtin_inff() ? 0.0f : up, alpha = __builtin_amdgcn_exp2f(top - base);
-            top = up;
-            l *= alpha;
-            y *= alpha;
-#pragma unroll
-            for (uint32_t i = 0; i < AHEAD; ++i) {
-                const float f = __builtin_amdgcn_exp2f(m[i] - base);
-                l += lm[i] == 0.0f ? 0.0f : lm[i] * f;  // (NaN is not)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] += lm[i] == 0.0f ? 0.0f : x[i][e] * f;
-            }
+        };
+        if (works) {
+            if (splits <= 2 * groups) take(std::integral_constant<uint32_t, 2>{});
+            else if (splits <= 4 * groups) take(std::integral_constant<uint32_t, 4>{});
+            else take(std::integral_constant<uint32_t, 8>{});
         }
+        *reinterpret_cast<attn::f32x4*>(sums[tid]) = y;
+        mls[tid][0] = top;
+        mls[tid][1] = l;
+        __syncthreads();
+        if (works && g == 0) {
+            for (uint32_t i = 1; i < groups; ++i) top = fmaxf(top, mls[tid + i * lanes][0]);
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+            l = 0.0f;
+            y = (attn::f32x4){0.f, 0.f, 0.f, 0.f};
+            for (uint32_t i = 0; i < groups; ++i) {
+                const float lm = mls[tid + i * lanes][1];
+                if (lm == 0.0f) continue;
+                const float f = __builtin_amdgcn_exp2f(mls[tid + i * lanes][0] - base);
+                l += lm * f;
+                y += *reinterpret_cast<const attn::f32x4*>(sums[tid + i * lanes]) * f;
+            }
+            attn::store4(static_cast<TQ*>(a.out) + (size_t)t * a.out_stride + (size_t)head * a.head_dim + col, l == 0.0f ? (attn::f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / l));
+        }
+        __syncthreads();
     }
-    *reinterpret_cast<attn::f32x4*>(sums[tid]) = y;
-    mls[tid][0] = top;
-    mls[tid][1] = l;
-    __syncthreads();
-    if (!works || g != 0) return;
-    for (uint32_t i = 1; i < groups; ++i) top = fmaxf(top, mls[tid + i * lanes][0]);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    l = 0.0f;
-    y = (attn::f32x4){0.f, 0.f, 0.f, 0.f};
-    for (uint32_t i = 0; i < groups; ++i) {
-        const float lm = mls[tid + i * lanes][1];
-        if (lm == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f(mls[tid + i * lanes][0] - base);
-        l += lm * f;
-        y += *reinterpret_cast<const attn::f32x4*>(sums[tid + i * lanes]) * f;
-    }
-    attn::store4(static_cast<TQ*>(a.out) + (size_t)t * a.out_stride + (size_t)head * a.head_dim + col, l == 0.0f ? (attn::f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / l));
 }
 
 template <typename TQ>
@@ -192,12 +202,15 @@ int launch_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
     const uint32_t lanes = a.head_dim / 4, splits = std::max(p.wide_splits, p.narrow_splits);
     uint32_t groups = 1;
     while (groups < 16 && groups * 4 < splits && 2 * groups * lanes <= 256) groups *= 2;
-    const uint32_t rows = std::min(JOIN_ROWS, 256 / (lanes * groups)), parts = (JOIN_ROWS + rows - 1) / rows;
+    const uint32_t rows = std::min(JOIN_ROWS, 256 / (lanes * groups));
     const bool by_row = p.wide && p.wide_splits == 1;  // (those that are split have up to NARROW_ROWS rows)
     static_assert(attn::NARROW_ROWS <= JOIN_ROWS, "a block holds all rows of a sequence of few");
-    const uint64_t slots = (by_row ? 0 : (uint64_t)a.tokens * a.group / JOIN_ROWS) + a.batch, grid = slots * parts * a.kv_heads;
+    const uint64_t slots = (by_row ? 0 : (uint64_t)a.tokens * a.group / JOIN_ROWS) + a.batch;
+    // workgroups that share a block, where there are few blocks
+    const uint32_t parts = slots * a.kv_heads >= 4 * (uint64_t)ctx->prop.multiProcessorCount ? 1 : (JOIN_ROWS + rows - 1) / rows;
+    const uint64_t grid = slots * parts * a.kv_heads;
     if (grid > 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
-    hipLaunchKernelGGL((attention_join_kernel<TQ>), dim3((uint32_t)grid), dim3(256), 0, ctx->stream, a, p.part, (uint32_t)by_row, rows, groups, p.wide ? p.wide_splits : 1,
+    hipLaunchKernelGGL((attention_join_kernel<TQ>), dim3((uint32_t)grid), dim3(256), 0, ctx->stream, a, p.part, (uint32_t)by_row, parts, rows, groups, p.wide ? p.wide_splits : 1,
                        p.narrow ? p.narrow_splits : 1, p.narrow ? p.narrow_rows : 0);
     return hip_check(ctx, hipGetLastError(), "attention_join_kernel launch");
 }
