@@ -236,7 +236,13 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     uint64_t keys = a.paged ? (uint64_t)a.table_width << a.page_shift : a.tokens;
     keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + 1 + a.sinks + attn::WIDE_ROWS);
     const uint64_t wide_items = (rows + attn::WIDE_ROWS - 1) / attn::WIDE_ROWS * a.kv_heads;
-    const bool few = wide_items <= cus / 8;  // so few blocks of 128 rows that most of the device would idle: blocks of 16
+    // So few blocks of 128 rows that most of the device would idle take blocks of 16, unless there are so many keys that every one of those fills
+    // its CU anyway: 2^15 scores a CU.  us in blocks of 16 / 128: windows over 128 to 512 tokens, 12 heads, fp32 (12 / 24 / 36 / 48 blocks of 128)
+    // 6.7 / 12.1, 7.7 / 18.4, 16.1 / 25.2, 19.4 / 32.0, over 1024 (96) 44.9 / 37.6; 32 heads over 8, bf16, 256 and 512 tokens (64, 128) 12.8 / 11.7,
+    // 27.7 / 17.7.  New tokens of a paged cache, 32 heads over 8, at 2^13 scores a CU: 15.9 / 25.1 (16 over 4000 keys); 2^14: 18.4 / 26.9 (32),
+    // 14.3 / 24.4 (8 x 16 over 1000); 2^15: 23.8 / 28.9 (64), 34.8 / 37.7 (8 x 8); 2^16: 50.5 / 31.2 (128), 57.8 / 41.0 (8 x 16), 34.4 / 40.6 (32 over
+    // 16000); 2^17: 56.6 / 45.4 (64 over 16000), 95.3 / 50.9 (8 x 32).
+    const bool few = 16 * wide_items <= 3 * cus && (uint64_t)a.tokens * a.heads * keys <= cus << 15;
     p->narrow = a.paged || few;
     p->wide = !few && !(a.paged && a.tokens <= a.batch);
     p->by_slot = few && a.tokens > a.batch;
@@ -245,12 +251,16 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     p->slots = (uint32_t)(rows / attn::WIDE_ROWS) + a.batch;
     if (p->narrow) {
         const uint64_t items = (p->by_slot ? (rows + attn::NARROW_ROWS - 1) / attn::NARROW_ROWS : a.batch) * a.kv_heads;
-        // Fewer items than CUs: every CU one workgroup, of at least 256 keys.  More: shares of at least 1024 keys, so that long sequences are dealt
+        // Up to 1024 keys: no split, whose join costs more than it saves (32 heads over 8, bf16, one sequence of 777: 8.8 us, in three 11.3; of 1500
+        // 12.3 and 11.3, of 2000 14.7 and 11.2).  Fewer items than half the CUs: every CU one workgroup, of at least 256 keys.  More: shares of at least 1024 keys, so that long sequences are dealt
         // out too.  us with shares of 512 / 1024 / 2048 keys for more items: 64 sequences of up to 8191 231 / 203 / 203, 32 of up to 4000, 12 heads,
         // fp32 116 / 96 / 118; for fewer: two of 100 000 67 / 55 / 50 (one workgroup per CU), 32 of up to 16000 with one key head 52 / 44 / 41.
         p->narrow_splits = (uint32_t)std::max<uint64_t>(1, keys <= 1024 ? 1 : 2 * items <= cus ? std::min<uint64_t>({(cus + items - 1) / items, keys / 256, 256})
                                                                         : std::min<uint64_t>((8 * cus + items - 1) / items, keys / 1024));
     }
+    // Two workgroups a CU, which is what registers leave room for.  us at 2 / 3 / 4: 10 chunks of 200 to 400 tokens over up to 4000 keys, 16 heads over
+    // 8, bf16, 145 / 137 / 137, of 300 to 600 187 / 189 / 189; one of 256 over 16000, 32 heads over 8, 108 / 128 / 117; two of 500 to 700 over 5000, 12
+    // heads, fp32 over fp16, 68 / 64 / 68; 64 sequences with 1 to 40 new tokens over up to 5000 174 / 192 / 199.
     if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
     // what the splits hand over is kept below 128 MiB
     const uint64_t row_bytes = (uint64_t)(a.head_dim + 2) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
