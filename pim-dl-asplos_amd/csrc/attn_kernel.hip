@@ -24,26 +24,47 @@ __device__ __forceinline__ float wave_sum(float v)
 }
 
 // ---------------------------------------------------------------------------------------------
-// Any head size up to 256, any stride and alignment: a wave takes one query of one head, a lane a key at a time for the scores and up to
-// four columns of the output, with the running maximum m and sum l of a streaming softmax in between: a block of 64 keys
-// with maximum m' gives o = o 2^(m - m') + sum p v, l = l 2^(m - m') + sum p, p = 2^(s - m').
+// Any head size up to 256, any stride and alignment: a workgroup takes one query of one head, its four waves blocks of 64 keys in turn, each with the
+// running maximum m and sum l of a streaming softmax: a block with maximum m' gives o = o 2^(m - m') + sum p v, l = l 2^(m - m') + sum p,
+// p = 2^(s - m').  Eight lanes share a key and read its row N elements each, 8 keys at once, so that a load takes whole lines; lane (key j, eighth e) has columns
+// (8 c + e) N + i of q, and of the sums over its keys, which are added up over lanes and waves at the end.  Bound by the loads' latency, so eight of them are asked
+// for before the first is used: 32 sequences of up to 4000, 16 heads over 4, bf16, of 256 dims 141 us (210 where the compiler waits for each; 327 MB of keys and values, 4 times from
+// L2), of 72 73 us, 48 37 us, 70 (elements of 2 bytes) 170 us; a window of 257 of 4 x 750 tokens, 12 heads of 72, fp32, 611 us, where matrix instructions
+// take 68 for 80.
 // ---------------------------------------------------------------------------------------------
-template <typename TQ, typename TK, bool PAGED>
-__global__ __launch_bounds__(256) void attention_plain_kernel(AttnArgs a)
+template <typename TQ, typename TK, bool PAGED, int N, int DIMS>
+__global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kernel(AttnArgs a)
 {
-    __shared__ float qs[4][256];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t item = (uint64_t)blockIdx.x * 4 + wave;
-    const uint32_t t = (uint32_t)(item / a.heads), h = (uint32_t)(item % a.heads);
+    constexpr int CHUNKS = DIMS / (8 * N), BATCH = CHUNKS < 8 ? CHUNKS : 8, AHEAD = 8 / BATCH;  // loads of a row, and rows, under way together
+    // a load, taken as bits: what is not there is cleared by a mask, for which the compiler does not take the load apart or put it behind a branch
+    typedef typename std::conditional<N * sizeof(TK) == 16, attn::u32x4, typename std::conditional<sizeof(TK) == 4, uint32_t, uint16_t>::type>::type Bits;
+    struct Pack {
+        TK x[N];
+    };
+    static_assert(sizeof(Bits) == sizeof(Pack), "a load holds N elements");
+    __shared__ float sums[4][DIMS];
+    __shared__ float mls[4][2];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e8 = lane & 7, j8 = lane >> 3;
+    // heads that share a key head on one XCD (workgroups are dealt out to 8 in turn)
+    const uint32_t item = blockIdx.x / (8 * a.group) * 8 + blockIdx.x % 8;
+    const uint32_t t = item / a.kv_heads, kh = item % a.kv_heads, h = kh * a.group + blockIdx.x / 8 % a.group;
     if (t >= a.tokens) return;
     const uint32_t b = row_of_token(a.starts, a.batch, a.tokens, t);
     const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, PAGED, b);
     if (t < r.first || t - r.first >= r.n) return;  // a row of no sequence
-    const uint32_t hd = a.head_dim, kh = h / a.group;
+    const uint32_t hd = a.head_dim;
     const TQ* q = static_cast<const TQ*>(a.q) + (size_t)t * a.q_stride + (size_t)h * hd;
-    for (uint32_t d = lane; d < hd; d += 64) qs[wave][d] = to_float(q[d]);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    float qs[CHUNKS][N], o[CHUNKS][N];
+    auto offset = [&](int c) { return (8 * c + e8) * N < hd ? (8 * c + e8) * N : 0; };  // of the lane's columns, 0 behind the last
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const uint32_t col = (8 * c + e8) * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            qs[c][i] = col < hd ? to_float(q[col + i]) : 0.0f;
+            o[c][i] = 0.0f;
+        }
+    }
 
     const int64_t pos = r.pos0 + (int64_t)(t - r.first);
     const int64_t hi64 = pos + (int64_t)a.right + 1;
@@ -63,16 +84,50 @@ __global__ __launch_bounds__(256) void attention_plain_kernel(AttnArgs a)
     };
     const TK* k = static_cast<const TK*>(a.k);
     const TK* v = static_cast<const TK*>(a.v);
-    float m = -__builtin_inff(), l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    float m = -__builtin_inff(), l = 0.0f;
     auto keys = [&](int32_t from, int32_t to) {
-        for (int32_t j0 = from; j0 < to; j0 += 64) {
-            const int32_t j = j0 + (int32_t)lane;
+        for (int32_t j0 = from + 64 * (int32_t)wave; j0 < to; j0 += 256) {
+            const int32_t j = j0 + (int32_t)(8 * e8 + j8);  // the lane's own key, whose place, score and p it holds
+            int64_t at = j < to ? row_at(j) : -1;
+            auto row = [&](int g) { return (int64_t)__shfl((int)(at >> 32), (int)(8 * j8) + g) << 32 | (uint32_t)__shfl((int)at, (int)(8 * j8) + g); };
+            // chunks c0 .. c0 + BATCH - 1 of rows g0 .. g0 + AHEAD - 1, all asked for before the first is needed
+            Bits x[AHEAD][BATCH];
+            bool there[AHEAD];
+            auto fetch = [&](const TK* src, int g0, int c0) {
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int64_t from = row(g0 + u);
+                    there[u] = from >= 0;
+                    const TK* const start = src + (from < 0 ? 0 : from);
+#pragma unroll
+                    for (int c = 0; c < BATCH; ++c) x[u][c] = *reinterpret_cast<const Bits*>(start + offset(c0 + c));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
             float s = -__builtin_inff();
-            int64_t at = -1;
-            if (j < to && (at = row_at(j)) >= 0) {
-                float dot = 0.0f;
-                for (uint32_t d = 0; d < hd; ++d) dot = fmaf(qs[wave][d], to_float(k[at + d]), dot);
-                s = dot * a.scale * LOG2E;
+#pragma unroll 1
+            for (int g0 = 0; g0 < 8; g0 += AHEAD) {
+                float dot[AHEAD] = {};
+#pragma unroll
+                for (int c0 = 0; c0 < CHUNKS; c0 += BATCH) {
+                    fetch(k, g0, c0);
+#pragma unroll
+                    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                        for (int c = 0; c < BATCH; ++c) {
+                            // (an infinite element must not meet the 0 behind q's last)
+                            const Pack y = __builtin_bit_cast(Pack, (Bits)(x[u][c] & ((8 * (c0 + c) + e8) * N < hd ? ~0u : 0u)));
+#pragma unroll
+                            for (int i = 0; i < N; ++i) dot[u] = fmaf(qs[c0 + c][i], to_float(y.x[i]), dot[u]);
+                        }
+                }
+#pragma unroll
+                for (int w = 1; w < 8; w <<= 1)
+#pragma unroll
+                    for (int u = 0; u < AHEAD; ++u) dot[u] += __shfl_xor(dot[u], w);
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+                    if (e8 == (uint32_t)(g0 + u) && at >= 0) s = dot[u] * a.scale * LOG2E;
             }
             const float mx = fmaxf(m, wave_max(s));
             const float base = mx == -__builtin_inff() ? 0.0f : mx;  // (nothing yet but scores of -infinity)
@@ -80,34 +135,79 @@ __global__ __launch_bounds__(256) void attention_plain_kernel(AttnArgs a)
             m = mx;
             l = l * alpha + wave_sum(p);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] *= alpha;
-            const int32_t count = to - j0 < 64 ? to - j0 : 64;
-            for (int32_t jj = 0; jj < count; ++jj) {
-                const float pj = __shfl(p, jj);
-                const int64_t row = ((int64_t)__shfl((int)(at >> 32), jj) << 32) | (uint32_t)__shfl((int)at, jj);
-                if (row < 0) continue;
+            for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (lane + 64 * i < hd) o[i] = fmaf(pj, to_float(v[row + lane + 64 * i]), o[i]);
+                for (int i = 0; i < N; ++i) o[c][i] *= alpha;
+#pragma unroll 1
+            for (int g0 = 0; g0 < 8; g0 += AHEAD) {
+                float pj[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) pj[u] = __shfl(p, (int)(8 * j8) + g0 + u);
+#pragma unroll
+                for (int c0 = 0; c0 < CHUNKS; c0 += BATCH) {
+                    fetch(v, g0, c0);
+#pragma unroll
+                    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                        for (int c = 0; c < BATCH; ++c) {
+                            const Pack y = __builtin_bit_cast(Pack, (Bits)(x[u][c] & (there[u] ? ~0u : 0u)));
+#pragma unroll
+                            for (int i = 0; i < N; ++i) o[c0 + c][i] = fmaf(pj[u], to_float(y.x[i]), o[c0 + c][i]);
+                        }
+                }
             }
         }
     };
     keys(0, sinks);
     keys(lo, hi);
-    TQ* out = static_cast<TQ*>(a.out) + (size_t)t * a.out_stride + (size_t)h * hd;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < hd) out[lane + 64 * i] = (TQ)(l == 0.0f ? 0.0f : o[i] * inv);
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int w = 8; w < 64; w <<= 1) o[c][i] += __shfl_xor(o[c][i], w);
+            if (j8 == 0) sums[wave][(8 * c + e8) * N + i] = o[c][i];
+        }
+    if (lane == 0) {
+        mls[wave][0] = m;
+        mls[wave][1] = l;
+    }
+    __syncthreads();
+    const float top = fmaxf(fmaxf(mls[0][0], mls[1][0]), fmaxf(mls[2][0], mls[3][0])), base = top == -__builtin_inff() ? 0.0f : top;
+    float f[4];
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = exp2f(mls[w][0] - base);
+        l += mls[w][1] * f[w];
+    }
+    if (threadIdx.x < hd) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum += sums[w][threadIdx.x] * f[w];
+        static_cast<TQ*>(a.out)[(size_t)t * a.out_stride + (size_t)h * hd + threadIdx.x] = (TQ)(l == 0.0f ? 0.0f : sum * (1.0f / l));
+    }
+}
+
+template <typename TQ, typename TK, bool PAGED, int N>
+int launch_plain_of(Ctx* ctx, const AttnArgs& a)
+{
+    const uint64_t items = ((uint64_t)a.tokens * a.kv_heads + 7) / 8 * 8 * a.group;
+    if (items > 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
+    const dim3 grid((uint32_t)items);
+    if (a.head_dim <= 64) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 64>), grid, dim3(256), 0, ctx->stream, a);
+    else if (a.head_dim <= 128) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 128>), grid, dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 256>), grid, dim3(256), 0, ctx->stream, a);
+    return hip_check(ctx, hipGetLastError(), "attention_plain_kernel launch");
 }
 
 template <typename TQ, typename TK>
 int launch_plain(Ctx* ctx, const AttnArgs& a)
 {
-    const uint32_t grid = (uint32_t)(((uint64_t)a.tokens * a.heads + 3) / 4);
-    if (a.paged) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, true>), dim3(grid), dim3(256), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, false>), dim3(grid), dim3(256), 0, ctx->stream, a);
-    return hip_check(ctx, hipGetLastError(), "attention_plain_kernel launch");
+    constexpr int N = 16 / sizeof(TK);
+    const bool packs = a.head_dim % N == 0 && ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15) == 0 && (a.paged || a.kv_stride % N == 0);
+    if (a.paged) return packs ? launch_plain_of<TQ, TK, true, N>(ctx, a) : launch_plain_of<TQ, TK, true, 1>(ctx, a);
+    return packs ? launch_plain_of<TQ, TK, false, N>(ctx, a) : launch_plain_of<TQ, TK, false, 1>(ctx, a);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -285,7 +385,6 @@ int launch_attention(Ctx* ctx, const AttnArgs& a)
 {
     if (a.tokens == 0 || a.batch == 0) return PIMDL_OK;
     if (!matrix_form(a)) {
-        if ((uint64_t)a.tokens * a.heads / 4 >= 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
         if (a.dtype == PIMDL_BF16) return launch_plain<__bf16, __bf16>(ctx, a);
         if (a.dtype == PIMDL_F16) return launch_plain<_Float16, _Float16>(ctx, a);
         if (a.cache_dtype == PIMDL_BF16) return launch_plain<float, __bf16>(ctx, a);

@@ -11,7 +11,9 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------------------------------------------------
-// append: token t's columns, N at a time, rounded to nearest even and stored where its position lies.
+// append: token t's columns, N at a time, rounded to nearest even and stored where its position lies.  One pass, bound by HBM: 8 prompts of up to 4000 tokens, 16 heads
+// of 128, fp32 to bf16, 91 us, 5.4 TB/s; 64 single tokens 3.6 us, the launch.  us by 8 elements / by one: 16 heads of 128 91, of 31, an eighth of whose
+// lanes' bytes each load takes, 92 for a quarter as much.
 // ------------------------------------------------------------------------------------------------------------
 template <typename T, int N>
 struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
@@ -233,7 +235,7 @@ __global__ __launch_bounds__(SCAN) void pages_reserve_kernel(Book b, const int32
     if (threadIdx.x == 0) *b.lacking = 0;
 }
 
-// ---- copies of pages: `count` pairs, a workgroup 16 KiB of one pair in one layer of one buffer at a time
+// ---- copies of pages: `count` pairs, a workgroup 16 KiB of one pair in one layer of one buffer at a time: its loads all asked for before the first store
 constexpr uint32_t COPY_BYTES = 16384;
 
 __device__ __forceinline__ void copy_pages(const Pools& pl, const int32_t* src, const int32_t* dst, uint32_t count, uint32_t pages, uint32_t block,
@@ -266,7 +268,9 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(Pools pl, const int32_t
     copy_pages(pl, src, dst, n, pages, blockIdx.x, gridDim.x);
 }
 
-// ---- fork.  take[i]: the page that entry i's partly filled last page is copied to, -1 where there is none, -2 where the entry is left out; length[i]: of
+// ---- fork: one workgroup decides (6.5 us for 32 entries, a chain of loads: the list, the parent's length, its last page, the counts), the device copies (7.6 us for
+// 19 MB in 12 layers); each waits for the launch before more than for memory.
+// take[i]: the page that entry i's partly filled last page is copied to, -1 where there is none, -2 where the entry is left out; length[i]: of
 // its parent before the call (which may be another entry's child: then 0)
 struct ForkLists {
     int32_t *fresh, *take, *length, *src, *dst, *count;
@@ -377,7 +381,8 @@ __global__ __launch_bounds__(256) void pages_free_kernel(Book b, const int32_t* 
 }
 
 // ---- compaction.  rank(p): pages in use before p; L: pages in use.  The page at p >= L is the (rank(p) - rank(L))-th to move, the free
-// place p < L the (p - rank(p))-th to be filled.
+// place p < L the (p - rank(p))-th to be filled.  Ranks take two launches of 4.5 us; moving a third of 4096 pages in 12 layers 288 us, read and
+// written at 5.0 TB/s.
 constexpr uint32_t COMPACT_PAGES = 1024;  // that a workgroup looks at
 struct CompactLists {
     int32_t *counts, *holes, *mover, *rank, *meta;  // in use per workgroup; places by order; pages by rank; rank by page; L and rank(L)

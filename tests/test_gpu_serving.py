@@ -899,3 +899,29 @@ def test_model_over_a_cache(ctx, hd, heads, dtype, window, fused):
         model.layers[0].params.window = (4, 4, 0)
         model.extend(x, cache, starts, lst, ints(*counts))
     model.close()
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("hd", [1, 7, 8, 36, 63, 72, 112, 129, 136, 200, 255, 256])
+def test_head_sizes_of_the_plain_kernel(ctx, dtype, cache, hd):
+    """Rows of whole 16 bytes and others, heads whose number is no multiple of 8, blocks of 64 keys that waves take in turn, sinks that end inside one."""
+    paged_case(ctx, hd, [1, 3, 0, 2], [64, 65, 3, 700], 6, 3, hd, 16, dtype, cache)
+    paged_case(ctx, hd + 1, [2, 1], [321, 257], 5, 1, hd, 32, dtype, cache, left=130, sinks=67)
+    if dtype == cache:
+        window_case(ctx, hd, [66, 1, 130], 6, 2, hd, 70, 3, 5, dtype)
+        window_case(ctx, hd, [300], 3, 3, hd, UNL, UNL, 0, dtype)
+
+
+@pytest.mark.parametrize("hd", [20, 72, 200])
+def test_infinite_keys_in_the_plain_kernel(ctx, hd):
+    """A key of +infinity in its last column meets nothing behind a head's columns: q of the opposite sign gives it no share, by a score of -infinity."""
+    gen = gen_of(hd)
+    q, k, v = (randn(gen, 90, hd) for _ in range(3))
+    q[:, hd - 1] = -q[:, hd - 1].abs() - 0.1
+    out = torch.zeros(90, hd, device="cuda")
+    k[:, hd - 1][[0, 33, 70]] = float("inf")
+    window(ctx, q, k, v, out, [90], 1, 1, hd, UNL, UNL, 0, "f32")
+    torch.cuda.synchronize()
+    others = [i for i in range(90) if i not in (0, 33, 70)]
+    want, off, mass = reference(q[:, None], k[others][:, None], v[others][:, None], 0, UNL, UNL, 0, 1 / math.sqrt(hd))
+    check(out[:, None], want, off, mass, "f32")
