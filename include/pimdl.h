@@ -360,7 +360,8 @@ PIMDL_API int pimdl_attention(pimdl_ctx* ctx, const float* q, const float* k, co
  * mask (src/host/transformer_layer.cpp:211-230), has none of it.  Everything here takes DEVICE pointers, is queued
  * on the context's stream and may be captured into a HIP graph (after one call outside the capture, which sizes the
  * context's scratch); `starts`, `lengths`, tables and lists are read on the device when the kernels run, so a
- * captured step follows them from replay to replay.
+ * captured step follows them from replay to replay.  Calls of one context share its scratch, recorded ones too: replay its
+ * graphs one after the other, or give each stream a context of its own.
  *
  * A batch is PACKED: sequence b owns rows starts[b] .. starts[b + 1] - 1 of the token buffers ([batch + 1] ascending
  * numbers; what lies beyond `tokens` is taken for `tokens`).  Rows of no sequence are neither read nor written.

@@ -229,10 +229,13 @@ class TransformerLayer:
     def _attend_window(self, q, k, v, a, B):
         """Attention in params.window within each of the B sequences of the batch."""
         p = self.params
-        if B not in self._starts:
-            self._starts[B] = self.torch.arange(0, (B + 1) * p.seq_len, p.seq_len, device=q.device, dtype=self.torch.int32)
+        starts = self._starts.get(B)
+        if starts is None and self.torch.cuda.is_current_stream_capturing():
+            starts = self.torch.arange(0, (B + 1) * p.seq_len, p.seq_len, device=q.device, dtype=self.torch.int32)  # (there from the replay on only)
+        elif starts is None:  # copied from the host: there, on any stream, when the call returns
+            starts = self._starts[B] = self.torch.tensor(range(0, (B + 1) * p.seq_len, p.seq_len), device=q.device, dtype=self.torch.int32)
         left, right = (self._unlimited if w is None else w for w in p.window[:2])
-        self.ctx.attention_window_ptr(q.data_ptr(), k.data_ptr(), v.data_ptr(), a.data_ptr(), self._starts[B].data_ptr(), B, B * p.seq_len, p.head_num,
+        self.ctx.attention_window_ptr(q.data_ptr(), k.data_ptr(), v.data_ptr(), a.data_ptr(), starts.data_ptr(), B, B * p.seq_len, p.head_num,
                                       p.head_num, p.head_dim, q.stride(0), k.stride(0), p.token_dim, left, right, p.window[2],
                                       1.0 / math.sqrt(p.head_dim))
 
@@ -347,7 +350,7 @@ class Transformer:
         packed, row b of the batch is the counts[b] tokens starts[b] .. starts[b + 1] - 1 of sequence seqs[b] (int32 device tensors; seqs
         without repetitions).  Makes room for them in the PagedCache, fills it layer by layer, and every token sees its sequence up to itself
         (params.window: with right = 0).  cache.lacking tells afterwards whether there were pages enough; if not, the outputs are those of the
-        tokens that the cache had before."""
+        tokens that the cache had before.  Rows of x behind the last sequence (a batch padded for a recorded step) come out undefined."""
         cache.reserve(seqs, counts)
         for i, layer in enumerate(self.layers):
             x = layer.forward(x, cached=(cache, i, starts, seqs))

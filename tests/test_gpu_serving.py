@@ -925,3 +925,27 @@ def test_infinite_keys_in_the_plain_kernel(ctx, hd):
     others = [i for i in range(90) if i not in (0, 33, 70)]
     want, off, mass = reference(q[:, None], k[others][:, None], v[others][:, None], 0, UNL, UNL, 0, 1 / math.sqrt(hd))
     check(out[:, None], want, off, mass, "f32")
+
+
+def test_windowed_layer_first_called_under_a_capture(ctx):
+    """What a call that is only recorded makes is there from the replay on: an eager call before it must not use that."""
+    model, p = _model(ctx, 64, 4, 1, 70, 3, (20, 5, 1), False)
+    x = randn(gen_of(2), p.n, p.token_dim)
+    want = model.layers[0].forward(x)[:140].clone()  # (three sequences: sizes the scratch)
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    ctx.set_stream(side.cuda_stream)
+    try:
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+            recorded = model.layers[0].forward(x[:140])  # two: for the first time
+    finally:
+        ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    eager = model.layers[0].forward(x[:140])
+    torch.cuda.synchronize()
+    assert torch.equal(eager, want)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(recorded, want)
+        assert torch.equal(model.layers[0].forward(x[:140]), want)
+    model.close()
