@@ -80,7 +80,7 @@ int allow_dynamic_lds(Ctx* ctx, const void* kernel, int lds_bytes, const char* w
     return rc;
 }
 
-bool is_device_ptr(const void* p)
+static bool is_device_ptr(const void* p)
 {
     hipPointerAttribute_t attr;
     memset(&attr, 0, sizeof(attr));

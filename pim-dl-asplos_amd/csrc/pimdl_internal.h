@@ -165,7 +165,6 @@ int hip_check(Ctx* ctx, hipError_t e, const char* what);
 // Raises a kernel's dynamic LDS limit to `lds_bytes`, once per (device of ctx, kernel); safe from several threads.
 int allow_dynamic_lds(Ctx* ctx, const void* kernel, int lds_bytes, const char* what);
 
-bool is_device_ptr(const void* p);
 int activate(Ctx* ctx);  // makes the context's device the current one
 // grow-only scratch of the context; refused while its stream is being captured
 int ensure_scratch(Ctx* ctx, char** buf, size_t* have, size_t need, const char* what);
