@@ -5,7 +5,7 @@
 // Both products run on v_mfma_f32_32x32x16, transposed, so that a lane keeps to one row and nothing changes lanes in between:
 //   S^T[key][row] = K Q^T:   A = K (32 keys x 16 dims), B = the rows' q.  Lane (row j, half h) gets keys 8 (i / 4) + 4 h + i % 4,
 //                            i = 0 .. 15: a row's maximum and sum are 16 registers and one exchange between halves.
-//   O^T[dim][row] += V^T P^T: the B operand of 16 keys is 8 of those very registers, rounded; the A operand has to hold the same keys in the
+//   O^T[dim][row] += V^T P^T: the B operand of 16 keys is 8 of those very registers, in 16-bit pieces; the A operand has to hold the same keys in the
 //                            same places, which are two groups of 4 consecutive keys for each half: two transposing reads of LDS
 //                            (ds_read_b64_tr_b16: 16 lanes take 4 rows of 16 columns and get a column of 4 each).
 // Streaming softmax: m is a running maximum of a row's raw scores (RISE below), p = 2^(c s - c m) with c = scale log2(e), l the sum of p; o and l
@@ -306,8 +306,10 @@ struct Rows {
     static constexpr bool REST = C::HD % STEP != 0;                          // M == 16, groups 2 and 3 repeat the dims of 0 and 1 against zeros of q
     static constexpr int DT = (C::HD + M - 1) / M;             // tiles of the second (80 dims, M == 32: of the last one only half counts)
     static constexpr int QUADS = REGS / 4, OREGS = M * M / 64, OQUADS = OREGS / 4;
-    // pieces of p: in 16 bits it is rounded to one for many rows, where that is a third of the matrix instructions; few rows wait for memory
-    static constexpr int NP = C::NQ == 1 && M == 16 ? 2 : C::NQ;
+    // pieces of p: two in 16 bits, 16 or 22 bits of it, so that the output alone is rounded to 16 and a token's result does not depend on how many others
+    // share its call.  One piece would save many rows a third of their matrix instructions (6 prompts, window 1024, bf16: 318 us against 408) and put
+    // 2.06e-3 between them and 64 bits where rounding the output takes 1.58e-3; few rows wait for memory.
+    static constexpr int NP = C::NQ == 1 ? 2 : C::NQ;
     typedef typename std::conditional<M == 32, f32x16, f32x4>::type Acc;
     static constexpr int KT = M == 32 ? 1 : 2;  // accumulators of 32 keys
 
@@ -481,12 +483,10 @@ struct Rows {
         base -= (float)C::P_SHIFT;
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base));
-        if constexpr (NP > 1) {
-            float sum = 0.0f;
+        float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum += s[i];
-            l += sum;
-        }
+        for (int i = 0; i < N; ++i) sum += s[i];
+        l += sum;
     }
 
     // o += V^T p for 32 keys, which lie in LDS from `v` on
@@ -499,13 +499,6 @@ struct Rows {
             uint32_t w[4][NP];
 #pragma unroll
             for (int e = 0; e < 4; ++e) pieces<C::HALF, NP>(p[8 * st + 2 * e], p[8 * st + 2 * e + 1], w[e]);
-            if constexpr (NP == 1) {  // l is the sum of what the products get
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (C::HALF) l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w[e][0]), (f16x2){(_Float16)1.0f, (_Float16)1.0f}, l, false);
-                    else l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[e][0]), (bf16x2){(__bf16)1.0f, (__bf16)1.0f}, l, false);
-                }
-            }
             u32x4 b[NP];
 #pragma unroll
             for (int n = 0; n < NP; ++n) b[n] = (u32x4){w[0][n], w[1][n], w[2][n], w[3][n]};

@@ -949,3 +949,53 @@ def test_windowed_layer_first_called_under_a_capture(ctx):
         assert torch.equal(recorded, want)
         assert torch.equal(model.layers[0].forward(x[:140]), want)
     model.close()
+
+
+# ---------------------------------------------------------------------------------------------- shares in two pieces
+
+# What the two 16-bit numbers that stand for a share leave out, relative to it: each is off by at most half a step, the second of what the first left
+# (bf16 2^-8 twice, halves 2^-11 twice).  Halves: what lies below their smallest step, 2^-24, of a share that is carried times 2^7, at most 2^-32 a key.
+PIECES = {"f16": 2.0 ** -22, "bf16": 2.0 ** -16}
+
+
+def check_pieces(got, want, off, mass, dtype, keys, most):
+    """As check(), but the output alone is rounded to 16 bits."""
+    tol = off + PIECES[dtype] * mass + (keys * 2.0 ** -32 * most if dtype == "f16" else 0.0) + HALF[dtype] * want.abs() + 2.0 ** -126
+    bad = (got.double() - want).abs() > tol
+    assert not torch.isnan(got).any()
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}, worst {float(((got.double() - want).abs() / tol).max()):.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("counts,hd", [([900, 1200, 40], 64), ([700, 1100, 300], 128), ([40, 1], 64)])
+def test_window_rounds_its_output_alone(ctx, dtype, counts, hd):
+    """Many tokens (blocks of 128 rows) and few: shares keep 16 bits or more."""
+    heads, kv, n = 8, 2, sum(counts)
+    buf = randn(gen_of(hd), n, (heads + 2 * kv) * hd, dtype=dtype)
+    q, k, v = buf[:, :heads * hd], buf[:, heads * hd:(heads + kv) * hd], buf[:, (heads + kv) * hd:]
+    out = torch.zeros(n, heads * hd, device="cuda", dtype=TYPES[dtype])
+    window(ctx, q, k, v, out, counts, heads, kv, hd, 500, 0, 2, dtype)
+    torch.cuda.synchronize()
+    at = 0
+    for c in counts:
+        rows = slice(at, at + c)
+        want, off, mass = reference(q[rows].reshape(c, heads, hd), k[rows].reshape(c, kv, hd), v[rows].reshape(c, kv, hd), 0, 500, 0, 2, 1 / math.sqrt(hd))
+        check_pieces(out[rows].reshape(c, heads, hd), want, off, mass, dtype, 503, float(v.abs().max()))
+        at += c
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("counts,lengths,hd", [([600, 600], [4000, 3000], 64), ([600, 1, 600], [3000, 900, 2000], 128), ([1, 3], [700, 900], 128)])
+def test_pages_round_their_output_alone(ctx, dtype, counts, lengths, hd):
+    heads, kv = 8, 2
+    f = Filled(ctx, hd, lengths, kv, hd, 16, dtype)
+    q = randn(gen_of(hd + 1), sum(counts), heads * hd, dtype=dtype)
+    out = torch.zeros_like(q)
+    f.cache.attend(0, q, out, starts_of(counts), heads)
+    torch.cuda.synchronize()
+    at = 0
+    for s, c in enumerate(counts):
+        k, v = (x[0] for x in f.rows[s])
+        want, off, mass = reference(q[at:at + c].reshape(c, heads, hd), k, v, lengths[s] - c, UNL, 0, 0, 1 / math.sqrt(hd))
+        check_pieces(out[at:at + c].reshape(c, heads, hd), want, off, mass, dtype, lengths[s], float(v.abs().max()))
+        at += c
