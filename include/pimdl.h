@@ -370,7 +370,7 @@ PIMDL_API int pimdl_attention(pimdl_ctx* ctx, const float* q, const float* k, co
  * cores (given 16-byte aligned rows), other sizes on a plain kernel.  Strides are in elements.
  *
  * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max_j), over the keys that a query sees; |scale| up to 2^96.  Scores, maxima,
- * sums and accumulators are fp32.  With fp32 operands products keep fp32 accuracy (factors of 24 bits; 22 of q and p over a
+ * sums and accumulators are fp32.  Both sums are what the formula says, p_j at most 1: where sum_j p_j v_j passes the range of fp32 the result is infinite.  With fp32 operands products keep fp32 accuracy (factors of 24 bits; 22 of q and p over a
  * cache in halves); with 16-bit operands p_j meets v_j as the sum of two numbers of that type (16 bits in bf16, 22 in halves).  A query that sees no key gives
  * zeros.  Rows of K and V that a query does not see -- hidden by the window, behind a length, of other sequences, on pages of
  * nobody -- do not change its result whatever they hold, infinities and NaN included; an element of its own q or of a row that it

@@ -53,7 +53,9 @@ struct Config {
     static constexpr int LB = HD * 2;           // bytes of a row of one piece in LDS
     static constexpr int RB = HD * (int)sizeof(TK);  // ... in memory
     static constexpr int PARTS = HD * (int)sizeof(TK) / 16;  // 16-byte parts of a row in memory
-    static constexpr int P_SHIFT = HALF ? 7 : 0;             // p, up to 2^8 (RISE), is carried times 2^7 in halves
+    // p, up to 2^8 (RISE), is carried times 2^7 in halves, whose values leave room for that, and times 2^-8 otherwise: at most 1, so that a value near
+    // the type's largest stays finite
+    static constexpr int P_SHIFT = HALF ? 7 : -8;
 };
 
 // Order of a row's 16-byte parts in LDS: part ^ order(row).  Rows of the first product's reads are 32 consecutive ones at one part; the

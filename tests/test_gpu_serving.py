@@ -999,3 +999,45 @@ def test_pages_round_their_output_alone(ctx, dtype, counts, lengths, hd):
         want, off, mass = reference(q[at:at + c].reshape(c, heads, hd), k, v, lengths[s] - c, UNL, 0, 0, 1 / math.sqrt(hd))
         check_pieces(out[at:at + c].reshape(c, heads, hd), want, off, mass, dtype, lengths[s], float(v.abs().max()))
         at += c
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("at", [0, 31, 40, 130, 330, 599])
+def test_values_near_the_largest_number_stay_finite(ctx, dtype, cache, at):
+    """One key, with a share of up to 2^7.5 times the others', has a value of 3.3e38, the others zeros: share x value is finite."""
+    big = 3.3e38
+
+    def fill(k, v, key):
+        k.zero_(), v.zero_()
+        k[key, ..., 0] = 7.5 * math.log(2)
+        v[key, ..., 3], v[key, ..., 5] = big, -big
+
+    # single tokens, and chunks, over pages
+    for counts in ([1], [600]):
+        f = Filled(ctx, 1, [600], 8, 64, 16, cache)
+        k, v = (torch.zeros(600, 8, 64, device="cuda", dtype=TYPES[cache]) for _ in range(2))
+        fill(k, v, at)
+        place = torch.arange(600, device="cuda")
+        page = f.cache.tables[0].long()[place // 16]
+        for pool, x in ((f.cache.k, k), (f.cache.v, v)):
+            pool[0, page, :, place % 16] = x
+        q = torch.zeros(counts[0], 8 * 64, device="cuda", dtype=TYPES[dtype])
+        q[:, ::64] = 1.0
+        out = torch.zeros_like(q)
+        f.cache.attend(0, q, out, starts_of(counts), 8, scale=1.0)
+        torch.cuda.synchronize()
+        want, off, mass = reference(q.reshape(-1, 8, 64), k, v, 600 - counts[0], UNL, 0, 0, 1.0)
+        check(out.reshape(-1, 8, 64), want, off, mass, dtype)
+    if dtype != cache:
+        return
+    for n, hd in ((900, 64), (600, 64), (600, 72)):  # blocks of 128 rows; fewer; the plain kernel
+        heads = 8 if n > 600 else 1
+        k, v = (torch.zeros(n, heads, hd, device="cuda", dtype=TYPES[dtype]) for _ in range(2))
+        fill(k, v, at)
+        q = torch.zeros(n, heads * hd, device="cuda", dtype=TYPES[dtype])
+        q[:, ::hd] = 1.0
+        out = torch.zeros_like(q)
+        window(ctx, q, k.reshape(n, -1), v.reshape(n, -1), out, [n], heads, heads, hd, UNL, UNL, 0, dtype, scale=1.0)
+        torch.cuda.synchronize()
+        want, off, mass = reference(q.reshape(n, heads, hd), k, v, 0, UNL, UNL, 0, 1.0)
+        check(out.reshape(n, heads, hd), want, off, mass, dtype)
