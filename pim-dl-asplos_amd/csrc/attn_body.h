@@ -476,7 +476,7 @@ struct Rows {
             for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
         float base = m == -INF ? 0.0f : m * c;
-        if (__any(fabsf(base) > 0x1p20f)) {  // (rare) the rounding of m c would be a factor of its own
+        if (__any(fabsf(base) > 0x1p10f)) {  // (rare) the rounding of m c, a factor of up to 2^(2^-15) below, would be one that counts
             const float most = m == -INF ? 0.0f : m;
 #pragma unroll
             for (int i = 0; i < N; ++i) s[i] -= most;
@@ -543,15 +543,21 @@ struct Rows {
     }
 
     __device__ __forceinline__ f32x4 quad(int d, int i) const { return (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}; }
-    __device__ __forceinline__ float exponent() const { return m == -INF ? -INF : m * c; }
 };
 
-// Results of keys that are split over workgroups: per split and row of the output (token, head) the sums, the exponent c m that they are
-// relative to, and l.
+// Results of keys that are split over workgroups: per split and row of the output (token, head) the sums, and the maximum m that they are relative
+// to, l, and c (1 where l is 0).  Joins take 2^(c (m - m')): of c m itself the rounding would be a factor of its own between large scores.
 struct Partial {
-    float* o;    // [splits][rows][head_dim]
-    float* ml;   // [splits][rows][2]
+    static constexpr uint32_t STATS = 3;
+    float* o;      // [splits][rows][head_dim]
+    float* stats;  // [splits][rows][STATS]
     uint64_t rows;
+    __device__ __forceinline__ void put(uint64_t at, float m, float l, float c) const
+    {
+        stats[STATS * at] = m;
+        stats[STATS * at + 1] = l;
+        stats[STATS * at + 2] = c;
+    }
 };
 
 template <typename TQ>
@@ -708,10 +714,7 @@ __device__ __forceinline__ void wide_rows(const AttnArgs& a, uint32_t block, uin
                 if (32 * d + 8 * i < C::HD) store4(out + 32 * d + 8 * i + 4 * h, w.quad(d, i) * inv);
     } else {
         const uint64_t at = (uint64_t)split * part.rows + (uint64_t)token * a.heads + head;
-        if (h == 0) {
-            part.ml[2 * at] = w.exponent();
-            part.ml[2 * at + 1] = l;
-        }
+        if (h == 0) part.put(at, w.m, l, w.c);
         if (from >= to) return;  // (the joining kernel does not look at sums whose l is 0)
 #pragma unroll
         for (int d = 0; d < w.DT; ++d)
@@ -735,7 +738,8 @@ struct Narrow {
     static constexpr int WAVE = ((S::BYTES > JOIN ? S::BYTES : JOIN) + 15) / 16 * 16;
     struct Shared {
         alignas(16) char lds[WAVES * WAVE];
-        float ml[WAVES][16][2];
+        float ml[WAVES][16][2];  // m, and l relative to the waves' largest m
+        float c[16];
         uint8_t marks[WAVES][32 * C::PARTS];
     };
 };
@@ -779,8 +783,7 @@ __device__ __forceinline__ void narrow_rows_of(const AttnArgs& a, uint32_t numbe
             if (tid < end - row0) {
                 const uint32_t row = row0 + tid;
                 const uint64_t at = (uint64_t)split * part.rows + (uint64_t)(r.first + row / a.group) * a.heads + kh * a.group + row % a.group;
-                part.ml[2 * at] = -INF;
-                part.ml[2 * at + 1] = 0.0f;
+                part.put(at, -INF, 0.0f, 1.0f);
             }
             continue;
         }
@@ -825,17 +828,16 @@ __device__ __forceinline__ void narrow_rows_of(const AttnArgs& a, uint32_t numbe
             if (bad) w.poison(marks[wave], key0, 32, there);
             wave_sync();
         }
-        // join the waves: all relative to the largest exponent
+        // join the waves: all relative to the largest maximum
         const float l = row_sum<16>(w.l);
-        if (lane < 16) {
-            ml[wave][j][0] = w.exponent();
-            ml[wave][j][1] = l;
-        }
+        if (lane < 16) ml[wave][j][0] = w.m;
         __syncthreads();
         float top = -INF;
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) top = fmaxf(top, ml[i][j][0]);
-        const float f = __builtin_amdgcn_exp2f(w.exponent() - (top == -INF ? 0.0f : top));
+        const float f = __builtin_amdgcn_exp2f((w.m - (top == -INF ? 0.0f : top)) * w.c);
+        if (lane < 16) ml[wave][j][1] = l * f;
+        if (tid < 16) sh.c[j] = w.c;
         float* const sums = reinterpret_cast<float*>(mine);
 #pragma unroll
         for (int d = 0; d < w.DT; ++d)
@@ -853,19 +855,14 @@ __device__ __forceinline__ void narrow_rows_of(const AttnArgs& a, uint32_t numbe
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] += from_wave[e];
                 mx = fmaxf(mx, ml[i][row][0]);
+                sum += ml[i][row][1];
             }
-            const float base = mx == -INF ? 0.0f : mx;
-#pragma unroll
-            for (int i = 0; i < WAVES; ++i) sum += ml[i][row][1] * __builtin_amdgcn_exp2f(ml[i][row][0] - base);
             const uint32_t token = r.first + (row0 + row) / a.group, head = kh * a.group + (row0 + row) % a.group;
             if (splits == 1) {
                 store4(static_cast<typename C::TQ*>(a.out) + (size_t)token * a.out_stride + (size_t)head * C::HD + col, sum == 0.0f ? (f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / sum));
             } else {
                 const uint64_t at = (uint64_t)split * part.rows + (uint64_t)token * a.heads + head;
-                if (col == 0) {
-                    part.ml[2 * at] = mx;
-                    part.ml[2 * at + 1] = sum;
-                }
+                if (col == 0) part.put(at, mx, sum, sh.c[row]);
                 store4(part.o + at * C::HD + col, y);
             }
         }

@@ -25,8 +25,8 @@ __device__ __forceinline__ float wave_sum(float v)
 
 // ---------------------------------------------------------------------------------------------
 // Any head size up to 256, any stride and alignment: a workgroup takes one query of one head, its four waves blocks of 64 keys in turn, each with the
-// running maximum m and sum l of a streaming softmax: a block with maximum m' gives o = o 2^(m - m') + sum p v, l = l 2^(m - m') + sum p,
-// p = 2^(s - m').  Eight lanes share a key and read its row N elements each, 8 keys at once, so that a load takes whole lines; lane (key j, eighth e) has columns
+// running maximum m and sum l of a streaming softmax: a block with maximum m' gives o = o 2^(c (m - m')) + sum p v, l = l 2^(c (m - m')) + sum p,
+// p = 2^(c (s - m')), s being raw products (times the scale's sign) and c = |scale| log2(e).  Eight lanes share a key and read its row N elements each, 8 keys at once, so that a load takes whole lines; lane (key j, eighth e) has columns
 // (8 c + e) N + i of q, and of the sums over its keys, which are added up over lanes and waves at the end.  Bound by the loads' latency, so eight of them are asked
 // for before the first is used: 32 sequences of up to 4000, 16 heads over 4, bf16, of 256 dims 141 us (210 where the compiler waits for each; 327 MB of keys and values, 4 times from
 // L2), of 72 73 us, 48 37 us, 70 (elements of 2 bytes) 170 us; a window of 257 of 4 x 750 tokens, 12 heads of 72, fp32, 611 us, where matrix instructions
@@ -84,6 +84,7 @@ __global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kern
     };
     const TK* k = static_cast<const TK*>(a.k);
     const TK* v = static_cast<const TK*>(a.v);
+    const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f, scale = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * LOG2E;
     float m = -__builtin_inff(), l = 0.0f;
     auto keys = [&](int32_t from, int32_t to) {
         for (int32_t j0 = from + 64 * (int32_t)wave; j0 < to; j0 += 256) {
@@ -127,11 +128,11 @@ __global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kern
                     for (int u = 0; u < AHEAD; ++u) dot[u] += __shfl_xor(dot[u], w);
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u)
-                    if (e8 == (uint32_t)(g0 + u) && at >= 0) s = dot[u] * a.scale * LOG2E;
+                    if (e8 == (uint32_t)(g0 + u) && at >= 0) s = dot[u] * sign;
             }
             const float mx = fmaxf(m, wave_max(s));
             const float base = mx == -__builtin_inff() ? 0.0f : mx;  // (nothing yet but scores of -infinity)
-            const float p = exp2f(s - base), alpha = exp2f(m - base);
+            const float p = exp2f((s - base) * scale), alpha = exp2f((m - base) * scale);
             m = mx;
             l = l * alpha + wave_sum(p);
 #pragma unroll
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kern
     l = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        f[w] = exp2f(mls[w][0] - base);
+        f[w] = exp2f((mls[w][0] - base) * scale);
         l += mls[w][1] * f[w];
     }
     if (threadIdx.x < hd) {
@@ -211,7 +212,7 @@ int launch_plain(Ctx* ctx, const AttnArgs& a)
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins what the splits of a row have: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).  A workgroup takes `rows` rows of up to 16 of a
+// Joins what the splits of a row have: out = sum_s o_s 2^(c (m_s - m)) / sum_s l_s 2^(c (m_s - m)).  A workgroup takes `rows` rows of up to 16 of a
 // sequence and key head (blocks of 16 are numbered as first_slot does, or, by_row, the first of each row of the batch: where only those of few rows are
 // split, the others would be 20 us of workgroups with nothing to do in a batch of 2300 tokens, 32 heads); of a row's threads head_dim / 4 take four columns each, and `groups` sets of
 // them every groups-th split.
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
                                                              uint32_t wide_splits, uint32_t narrow_splits, uint32_t narrow_rows)
 {
     __shared__ float sums[256][4];
-    __shared__ float mls[256][2];
+    __shared__ float mls[256][attn::Partial::STATS];
     const uint32_t tid = threadIdx.x, lanes = a.head_dim / 4;
     const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, slot = rest / parts;
     const uint32_t b = by_row ? slot : attn::row_of_slot(a, slot, JOIN_ROWS);
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
         const bool works = mine < rows && row < stop;
         const uint32_t t = first + row / a.group, head = kh * a.group + row % a.group;
         const uint64_t at = (uint64_t)t * a.heads + head;
-        float top = -__builtin_inff(), l = 0.0f;
+        float top = -__builtin_inff(), l = 0.0f, c = 1.0f;  // c: of a split that has seen keys, the same in all of them
         attn::f32x4 y = {0.f, 0.f, 0.f, 0.f};
         auto take = [&](auto count) __attribute__((always_inline)) {
             constexpr uint32_t AHEAD = decltype(count)::value;  // splits whose results are asked for together
@@ -249,20 +250,22 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
                 for (uint32_t i = 0; i < AHEAD; ++i) {
                     const uint32_t s = s0 + i * groups < splits ? s0 + i * groups : splits - 1;
                     const uint64_t where = s * part.rows + at;
-                    m[i] = part.ml[2 * where];
-                    lm[i] = s0 + i * groups < splits ? part.ml[2 * where + 1] : 0.0f;
+                    const float* const stats = part.stats + attn::Partial::STATS * where;
+                    m[i] = stats[0];
+                    lm[i] = s0 + i * groups < splits ? stats[1] : 0.0f;
+                    c = lm[i] == 0.0f ? c : stats[2];
                     x[i] = *reinterpret_cast<const attn::f32x4*>(part.o + where * a.head_dim + col);  // (anything where l is 0)
                 }
                 float up = top;
 #pragma unroll
                 for (uint32_t i = 0; i < AHEAD; ++i) up = fmaxf(up, m[i]);
-                const float base = up == -__builtin_inff() ? 0.0f : up, alpha = __builtin_amdgcn_exp2f(top - base);
+                const float base = up == -__builtin_inff() ? 0.0f : up, alpha = __builtin_amdgcn_exp2f((top - base) * c);
                 top = up;
                 l *= alpha;
                 y *= alpha;
 #pragma unroll
                 for (uint32_t i = 0; i < AHEAD; ++i) {
-                    const float f = __builtin_amdgcn_exp2f(m[i] - base);
+                    const float f = __builtin_amdgcn_exp2f((m[i] - base) * c);
                     l += lm[i] == 0.0f ? 0.0f : lm[i] * f;  // (NaN is not)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y[e] += lm[i] == 0.0f ? 0.0f : x[i][e] * f;
@@ -277,6 +280,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
         *reinterpret_cast<attn::f32x4*>(sums[tid]) = y;
         mls[tid][0] = top;
         mls[tid][1] = l;
+        mls[tid][2] = c;
         __syncthreads();
         if (works && g == 0) {
             for (uint32_t i = 1; i < groups; ++i) top = fmaxf(top, mls[tid + i * lanes][0]);
@@ -286,7 +290,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
             for (uint32_t i = 0; i < groups; ++i) {
                 const float lm = mls[tid + i * lanes][1];
                 if (lm == 0.0f) continue;
-                const float f = __builtin_amdgcn_exp2f(mls[tid + i * lanes][0] - base);
+                const float f = __builtin_amdgcn_exp2f((mls[tid + i * lanes][0] - base) * mls[tid + i * lanes][2]);
                 l += lm * f;
                 y += *reinterpret_cast<const attn::f32x4*>(sums[tid + i * lanes]) * f;
             }
@@ -363,7 +367,7 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     // heads, fp32 over fp16, 68 / 64 / 68; 64 sequences with 1 to 40 new tokens over up to 5000 174 / 192 / 199.
     if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
     // what the splits hand over is kept below 128 MiB
-    const uint64_t row_bytes = (uint64_t)(a.head_dim + 2) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
+    const uint64_t row_bytes = (uint64_t)(a.head_dim + attn::Partial::STATS) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
     p->narrow_splits = (uint32_t)std::min<uint64_t>(p->narrow_splits, most);
     p->wide_splits = (uint32_t)std::min<uint64_t>(p->wide_splits, most);
     const uint32_t splits = std::max(p->narrow_splits, p->wide_splits);
@@ -374,7 +378,7 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
         if (rc) return rc;
         p->part.rows = (uint64_t)a.tokens * a.heads;
         p->part.o = reinterpret_cast<float*>(ctx->d_attn);
-        p->part.ml = p->part.o + p->part.rows * splits * a.head_dim;
+        p->part.stats = p->part.o + p->part.rows * splits * a.head_dim;
     }
     return PIMDL_OK;
 }

@@ -1041,3 +1041,58 @@ def test_values_near_the_largest_number_stay_finite(ctx, dtype, cache, at):
         torch.cuda.synchronize()
         want, off, mass = reference(q.reshape(n, heads, hd), k, v, 0, UNL, UNL, 0, 1.0)
         check(out.reshape(n, heads, hd), want, off, mass, dtype)
+
+
+# ---------------------------------------------------------------------------------------------- large scores
+
+def check_shares(got, want, mass, dtype, keys, product, most):
+    """Scores that are integers, exact in fp32, 5 apart at most: shares depend on their differences alone, whatever their size.  An exponent is off by
+    2 U of up to 5 log2(e), 10 U in the share, its power by 4 U, and sums by keys / 16 + 64 additions, numerator and denominator; up to 2^10 the
+    running maximum times the scale is rounded, by 2^-15 in the exponent, twice."""
+    tol = (2 * (keys / 16 + 64) + 64) * U + (2.0 ** -14 if product * math.log2(math.e) <= 2 ** 10 else 0.0)
+    check_pieces(got, want, tol * mass, mass, dtype, keys, most) if dtype != "f32" else check(got, want, tol * mass, mass, dtype)
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("hd", [64, 72])
+@pytest.mark.parametrize("log", [0, 9, 15, 19, 21, 23])
+def test_shares_of_large_scores(ctx, dtype, cache, hd, log):
+    """The same differences of scores on top of 2^log: single tokens (waves, then splits, are joined), chunks of both block sizes, windows, other head
+    sizes, a negative scale."""
+    first, second = 2.0 ** (log // 2), 2.0 ** (log - log // 2)
+    rng = np.random.default_rng(log)
+
+    def rows(n, heads, sign, t):
+        x = torch.zeros(n, heads, hd, device="cuda", dtype=TYPES[t])
+        x[..., 0] = second * sign
+        x[..., 1] = torch.from_numpy(rng.integers(0, 6, (n, heads))).cuda() * sign
+        return x
+
+    for counts, lengths, heads, kv in (([1], [700], 4, 2), ([1, 1], [6000, 300], 4, 2), ([30], [500], 4, 2), ([600, 600], [4000, 3000], 8, 2)):
+        f = Filled(ctx, log, lengths, kv, hd, 16, cache)
+        q = torch.zeros(sum(counts), heads * hd, device="cuda", dtype=TYPES[dtype])
+        q[:, ::hd], q[:, 1::hd] = first, 1.0
+        out = torch.zeros_like(q)
+        sign = -1 if len(counts) == 2 and counts[0] == 1 else 1
+        given = []
+        for s, n in enumerate(lengths):
+            k, place = rows(n, kv, sign, cache), torch.arange(n, device="cuda")
+            f.cache.k[0, f.cache.tables[s].long()[place // 16], :, place % 16] = k
+            given.append((k, f.rows[s][1][0]))
+        f.cache.attend(0, q, out, starts_of(counts), heads, scale=float(sign))
+        torch.cuda.synchronize()
+        at = 0
+        for s, c in enumerate(counts):
+            want, _, mass = reference(q[at:at + c].reshape(c, heads, hd), *given[s], lengths[s] - c, UNL, 0, 0, float(sign))
+            check_shares(out[at:at + c].reshape(c, heads, hd), want, mass, dtype, lengths[s], 2 ** log, float(given[s][1].abs().max()))
+            at += c
+    if dtype != cache:
+        return
+    for n, heads in ((300, 1), (900, 8)):
+        q, k, v = torch.zeros(n, heads * hd, device="cuda", dtype=TYPES[dtype]), rows(n, heads, 1, dtype), randn(gen_of(1), n, heads, hd, dtype=dtype)
+        q[:, ::hd], q[:, 1::hd] = first, 1.0
+        out = torch.zeros_like(q)
+        window(ctx, q, k.reshape(n, -1), v.reshape(n, -1), out, [n], heads, heads, hd, 400, 70, 3, dtype, scale=1.0)
+        torch.cuda.synchronize()
+        want, _, mass = reference(q.reshape(n, heads, hd), k, v, 0, 400, 70, 3, 1.0)
+        check_shares(out.reshape(n, heads, hd), want, mass, dtype, n, 2 ** log, float(v.abs().max()))
