@@ -468,7 +468,7 @@ struct Rows {
         for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
         mx = row_max<M>(mx);
         if (__any((mx - m) * c > RISE)) {
-            const float up = fmaxf(m, mx);
+            const float up = (mx - m) * c > RISE ? mx : m;  // each row by its own scores: what others see must not round it differently
             const float alpha = __builtin_amdgcn_exp2f((m - (up == -INF ? 0.0f : up)) * c);  // 0 at the first keys
             m = up;
             l *= alpha;
@@ -476,11 +476,12 @@ struct Rows {
             for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
         float base = m == -INF ? 0.0f : m * c;
-        if (__any(fabsf(base) > 0x1p10f)) {  // (rare) the rounding of m c, a factor of up to 2^(2^-15) below, would be one that counts
-            const float most = m == -INF ? 0.0f : m;
+        const bool far = fabsf(base) > 0x1p10f;
+        if (__any(far)) {  // (rare) the rounding of m c, a factor of up to 2^(2^-15) below, would be one that counts
+            const float most = far ? m : 0.0f;
 #pragma unroll
             for (int i = 0; i < N; ++i) s[i] -= most;
-            base = 0.0f;
+            base = far ? 0.0f : base;
         }
         base -= (float)C::P_SHIFT;
 #pragma unroll

@@ -1096,3 +1096,35 @@ def test_shares_of_large_scores(ctx, dtype, cache, hd, log):
         torch.cuda.synchronize()
         want, _, mass = reference(q.reshape(n, heads, hd), k, v, 0, 400, 70, 3, 1.0)
         check_shares(out.reshape(n, heads, hd), want, mass, dtype, n, 2 ** log, float(v.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,heads,hd", [(300, 1, 64), (900, 8, 64), (700, 8, 128), (120, 2, 72)])
+def test_rows_do_not_depend_on_each_other(ctx, dtype, n, heads, hd):
+    """Bit for bit: a large key changes the rows that see it and no others, a large query its own row and head alone (few tokens, blocks of 128 rows, other
+    head sizes)."""
+    gen = gen_of(n)
+    q, k, v = (randn(gen, n, heads * hd, dtype=dtype) for _ in range(3))
+    out = torch.zeros_like(q)
+
+    def run():
+        window(ctx, q, k, v, out, [100, n - 100], heads, heads, hd, 7, 0, 0, dtype)
+        torch.cuda.synchronize()
+        return out.clone()
+
+    plain = run()
+    seen = torch.zeros(n, dtype=torch.bool, device="cuda")
+    for at, factor in ((40, 20.0), (41, 1000.0), (110, -1000.0)):
+        k[at] = q[at + 2] * factor
+        seen[at:at + 8] = True
+        got = run()
+        assert torch.isfinite(got).all() and not torch.equal(got[seen], plain[seen])
+        assert torch.equal(got[~seen], plain[~seen]), at
+    plain = run()
+    for at, factor in ((12, 30.0), (13, 1000.0), (115, 1000.0)):
+        q[at, :hd] *= factor
+        got = run()
+        got[at, :hd] = plain[at, :hd]
+        assert torch.equal(got, plain), at
+        q[at, :hd] /= factor
+        plain = run()
