@@ -336,7 +336,7 @@ struct Rows {
         const uint32_t g = group(), mine = row0 + row() < rows ? row0 + row() : rows - 1;  // rows past the last repeat it; they are never stored
         const uint32_t token = mine / a.group, head = kh * a.group + mine % a.group;
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;  // c is positive, so that the largest score has the largest exponent
-        c = fminf((a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale), 1.2e-38f)) * LOG2E, 3e38f);
+        c = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * LOG2E;
         const typename C::TQ* const base = static_cast<const typename C::TQ*>(a.q) + (size_t)(r.first + token) * a.q_stride + (size_t)head * C::HD;
         if constexpr (C::NQ == 1) {
             const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u, keep = sign == 0.0f ? 0u : ~0u;
@@ -359,11 +359,11 @@ struct Rows {
                 for (int s = 0; s < 2 * KS; ++s) big = fmaxf(fmaxf(big, fmaxf(fabsf(x[s][0]), fabsf(x[s][1]))), fmaxf(fabsf(x[s][2]), fabsf(x[s][3])));
                 big = row_max<M>(big);
                 int e = 11 - ((int)(bits(big) >> 23 & 255) - 127);
-                e = e < -100 ? -100 : e > 100 ? 100 : e;
+                e = e > 126 ? 126 : e;  // (-117 at least)
                 factor *= number((uint32_t)(127 + e) << 23);
                 c *= number((uint32_t)(127 - e) << 23);
             }
-            c = fminf(fmaxf(c, 1.2e-38f), 3e38f);  // (0 or infinity times a hidden score would be NaN)
+            c = fminf(fmaxf(c, 1.4e-45f), 3e38f);  // (0 or infinity times a hidden score would be NaN)
 #pragma unroll
             for (int s = 0; s < 2 * KS; ++s) {
                 uint32_t w[2][C::NQ];

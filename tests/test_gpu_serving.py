@@ -1128,3 +1128,22 @@ def test_rows_do_not_depend_on_each_other(ctx, dtype, n, heads, hd):
         assert torch.equal(got, plain), at
         q[at, :hd] /= factor
         plain = run()
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("hd", [64, 72])
+@pytest.mark.parametrize("size,scale", [(3e36, 1e-38), (3e36, 2e-39), (3e36, 4e-37), (1e-33, 2.0 ** 96), (1e-36, 2.0 ** 96)])
+def test_queries_at_the_ends_of_fp32(ctx, dtype, cache, hd, size, scale):
+    """Products near the largest fp32 number under scales below the smallest normal one, and queries near that under the largest scale."""
+    for counts, lengths, heads, kv in (([1, 2], [300, 50], 4, 2), ([600, 600], [700, 900], 8, 8)):
+        f = Filled(ctx, hd, lengths, kv, hd, 16, cache)
+        q = randn(gen_of(2), sum(counts), heads * hd, scale=size)
+        out = torch.zeros_like(q)
+        f.cache.attend(0, q, out, starts_of(counts), heads, scale=scale)
+        torch.cuda.synchronize()
+        at = 0
+        for s, c in enumerate(counts):
+            k, v = (x[0] for x in f.rows[s])
+            want, off, mass = reference(q[at:at + c].reshape(c, heads, hd), k, v, lengths[s] - c, UNL, 0, 0, float(np.float32(scale)))
+            check(out[at:at + c].reshape(c, heads, hd), want, off, mass, dtype)
+            at += c
