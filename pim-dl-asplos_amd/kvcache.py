@@ -83,6 +83,12 @@ class PagedCache:
             raise ValueError("starts must hold one number more than seqs")
         return to, at, m
 
+    def check_batch(self, starts, seqs=None):
+        """Refuses tensors that append and attend would not take for a batch."""
+        _, _, batch = self._batch(starts, seqs)
+        if seqs is None and batch > self.tables.shape[0]:
+            raise ValueError(f"{batch} rows: the cache has {self.tables.shape[0]} sequences")
+
     def append(self, layer, k, v, starts, seqs=None):
         """New tokens' keys and values [tokens][kv_heads * head_dim] into the last positions of their sequences (whose room `reserve` has made)."""
         if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:

@@ -171,6 +171,7 @@ class TransformerLayer:
         self._starts = {}  # sequences per batch -> first row of each, for pimdl_attention_window
         self.side = None if fused_qkv else side
         n = params.n
+        self._max_tokens = n
         self.amm = {}
         lin = dict(weights)
         if fused_qkv:  # one operator producing [q | k | v]: LUT columns and biases concatenated
@@ -239,6 +240,25 @@ class TransformerLayer:
                                       p.head_num, p.head_dim, q.stride(0), k.stride(0), p.token_dim, left, right, p.window[2],
                                       1.0 / math.sqrt(p.head_dim))
 
+    def check_cached(self, x, cache, layer, starts, seqs):
+        """Refuses what forward(x, cached=(cache, layer, starts, seqs)) could not do, before anything is written."""
+        p = self.params
+        if p.window is not None and p.window[1] != 0:
+            raise ValueError("a cache holds no later tokens: the window must have right = 0")
+        if not 0 <= layer < cache.layers:
+            raise ValueError(f"a cache of {cache.layers} layers has no layer {layer}")
+        if (cache.kv_heads, cache.head_dim) != (p.head_num, p.head_dim):
+            raise ValueError(f"a cache of {cache.kv_heads} heads of {cache.head_dim} under a layer of {p.head_num} of {p.head_dim}")
+        if p.head_dim > 256 or cache.page_tokens not in (16, 32, 64, 128, 256, 512, 1024):
+            raise ValueError("attention over pages takes heads of up to 256, pages of a power of two from 16 to 1024 tokens")
+        if x.dim() != 2 or x.shape[1] != p.token_dim or x.dtype != self.torch.float32:
+            raise ValueError(f"x must be float32 [tokens][{p.token_dim}]")
+        if x.shape[0] > self._max_tokens:
+            raise ValueError(f"{x.shape[0]} tokens: the layer is built for {self._max_tokens}")
+        cache.check_batch(starts, seqs)
+        if any(t.device != cache.k.device for t in (x, starts, seqs) if t is not None):
+            raise ValueError("x, starts and seqs must be on the cache's GPU")
+
     def forward(self, x, keep=None, cached=None):
         """x: float32 CUDA tensor [batch*seq][token_dim], row t = (batch t // seq_len, position t % seq_len).
         `keep`: optional dict that receives every intermediate (for stage-by-stage checks).
@@ -248,8 +268,8 @@ class TransformerLayer:
         n = x.shape[0]
         if cached is None and n % p.seq_len:
             raise ValueError("token count is not a multiple of seq_len")
-        if cached is not None and p.window is not None and p.window[1] != 0:
-            raise ValueError("a cache holds no later tokens: the window must have right = 0")
+        if cached is not None:
+            self.check_cached(x, *cached)
         B, S, H, hd = n // p.seq_len, p.seq_len, p.head_num, p.head_dim
         x = x.contiguous()
         if self.fused_qkv:
@@ -348,10 +368,14 @@ class Transformer:
     def extend(self, x, cache, starts, seqs, counts):
         """The newest tokens of some sequences through the model (a chunk of a prompt, a single token, or both in one batch): x [tokens][token_dim]
         packed, row b of the batch is the counts[b] tokens starts[b] .. starts[b + 1] - 1 of sequence seqs[b] (int32 device tensors; seqs
-        without repetitions).  Makes room for them in the PagedCache, fills it layer by layer, and every token sees its sequence up to itself
+        without repetitions).  A call that cannot be done raises before the cache changes.  Makes room for them in the PagedCache, fills it layer by layer, and every token sees its sequence up to itself
         (params.window: with right = 0).  cache.lacking tells afterwards whether there were pages enough; if not, the outputs are those of the
         tokens that the cache had before.  Rows of x behind the last sequence (a batch padded for a recorded step) come out undefined."""
-        cache.reserve(seqs, counts)
+        for i, layer in enumerate(self.layers):
+            layer.check_cached(x, cache, i, starts, seqs)
+        cache.reserve(seqs, counts)  # (which refuses lists that do not fit)
+        if x.shape[0] == 0:
+            return x
         for i, layer in enumerate(self.layers):
             x = layer.forward(x, cached=(cache, i, starts, seqs))
         return x

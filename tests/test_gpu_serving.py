@@ -1147,3 +1147,27 @@ def test_queries_at_the_ends_of_fp32(ctx, dtype, cache, hd, size, scale):
             want, off, mass = reference(q[at:at + c].reshape(c, heads, hd), k, v, lengths[s] - c, UNL, 0, 0, float(np.float32(scale)))
             check(out[at:at + c].reshape(c, heads, hd), want, off, mass, dtype)
             at += c
+
+
+def test_a_refused_extend_leaves_the_cache_as_it_was(ctx):
+    model, p = _model(ctx, 64, 4, 2, 32, 4)
+    shapes = {"layers": dict(layers=1), "heads": dict(kv_heads=2), "dims": dict(head_dim=32), "window": {}, "tokens": {}, "columns": {}}
+    for name, change in shapes.items():
+        a = dict(layers=2, pages=40, kv_heads=4, head_dim=64) | change
+        cache = K.PagedCache(ctx, pimdl, a["layers"], a["pages"], a["kv_heads"], a["head_dim"], 16, "f16", 3, 200)
+        cache.reserve(ints(1), ints(20))
+        torch.cuda.synchronize()
+        before = [t.clone() for t in (cache.tables, cache.lengths, cache.refs, cache.lacking)]
+        n = 129 if name == "tokens" else 5
+        p.window = (4, 4, 0) if name == "window" else None
+        with pytest.raises(ValueError):
+            model.extend(randn(gen_of(1), n, 255 if name == "columns" else 256), cache, starts_of([n]), ints(1), ints(n))
+        torch.cuda.synchronize()
+        for was, now in zip(before, (cache.tables, cache.lengths, cache.refs, cache.lacking)):
+            assert torch.equal(was, now), name
+    p.window = None
+    cache = K.PagedCache(ctx, pimdl, 2, 40, 4, 64, 16, "f16", 3, 200)
+    empty = model.extend(randn(gen_of(1), 0, 256), cache, starts_of([0, 0]), ints(0, 1), ints(0, 0))
+    torch.cuda.synchronize()
+    assert empty.shape == (0, 256) and int(cache.lacking) == 0 and int(cache.lengths.sum()) == 0
+    model.close()

@@ -1,0 +1,122 @@
+"""Host logic of serving that needs no GPU: what Transformer.extend and PagedCache refuse, and that a refused call has changed nothing.  Stand-ins
+record what would have been launched."""
+import types
+
+import pytest
+import torch
+
+from __graft_entry__ import load_package
+
+pimdl = load_package()
+from pim_dl_asplos_amd import kvcache as K  # noqa: E402
+from pim_dl_asplos_amd import transformer as T  # noqa: E402
+
+
+class Recorder:
+    """Takes any call of the library's binding and says that it went well."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append(name) or 0
+
+
+def params(window=None, heads=4, hd=64):
+    p = T.TransformerParams(8, 2, heads, hd, heads * hd, 2 * heads * hd, 2)
+    p.window = window
+    return p
+
+
+def context():
+    return types.SimpleNamespace(_h=None, _check=lambda rc: None)
+
+
+def cache_of(ctx, layers=2, heads=4, hd=64, page_tokens=16, seqs=3):
+    c = K.PagedCache.__new__(K.PagedCache)
+    c.ctx, c._lib, c._unlimited, c._book = ctx, Recorder(), pimdl.UNLIMITED, None
+    c.layers, c.kv_heads, c.head_dim, c.page_tokens = layers, heads, hd, page_tokens
+    c.k = torch.zeros(layers, 2, heads, page_tokens, hd)
+    c.tables = torch.full((seqs, 4), -1, dtype=torch.int32)
+    c._layer = [None] * layers
+    return c
+
+
+def model_of(ctx, p, layers=2):
+    made = []
+    for _ in range(layers):
+        layer = T.TransformerLayer.__new__(T.TransformerLayer)
+        layer.ctx, layer.params, layer.torch, layer._max_tokens, layer._unlimited = ctx, p, torch, p.n, pimdl.UNLIMITED
+        made.append(layer)
+    return T.Transformer.from_layers(made, p)
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+class Reached(Exception):
+    pass
+
+
+def extend(monkeypatch, model, cache, x=None, starts=None, seqs=None, counts=None):
+    """extend() up to the first layer's kernels."""
+    def run(self, *a):
+        raise Reached
+
+    monkeypatch.setattr(T.TransformerLayer, "_run", run)
+    for layer in model.layers:
+        layer.side, layer.fused_qkv, layer.qkv_group = None, True, None
+    return model.extend(torch.zeros(3, 256) if x is None else x, cache, ints(0, 2, 3) if starts is None else starts, ints(0, 2) if seqs is None else seqs,
+                        ints(2, 1) if counts is None else counts)
+
+
+def test_extend_reserves_and_runs(monkeypatch):
+    ctx = context()
+    for window in (None, (5, 0, 1), (None, 0, 0)):
+        cache = cache_of(ctx, layers=3)  # (a layer more than the model)
+        with pytest.raises(Reached):
+            extend(monkeypatch, model_of(ctx, params(window)), cache)
+        assert cache._lib.calls == ["pimdl_pages_reserve"]
+
+
+def test_extend_without_tokens_reserves_and_returns(monkeypatch):
+    ctx = context()
+    cache, x = cache_of(ctx), torch.zeros(0, 256)
+    assert extend(monkeypatch, model_of(ctx, params()), cache, x=x, starts=ints(0, 0, 0), counts=ints(0, 0)) is x
+    assert cache._lib.calls == ["pimdl_pages_reserve"]
+
+
+@pytest.mark.parametrize("window,cache,call,text", [
+    ((4, 4, 0), {}, {}, "right = 0"),
+    ((4, None, 0), {}, {}, "right = 0"),
+    (None, dict(layers=1), {}, "no layer 1"),
+    (None, dict(heads=2), {}, "2 heads of 64"),
+    (None, dict(hd=32), {}, "4 heads of 32"),
+    (None, dict(page_tokens=24), {}, "power of two"),
+    (None, {}, dict(x=torch.zeros(3, 255)), r"\[tokens\]\[256\]"),
+    (None, {}, dict(x=torch.zeros(3, 256, dtype=torch.float16)), "float32"),
+    (None, {}, dict(x=torch.zeros(768)), "float32"),
+    (None, {}, dict(x=torch.zeros(17, 256)), "built for 16"),
+    (None, {}, dict(x=torch.zeros(3, 256, device="meta")), "the cache's GPU"),
+    (None, {}, dict(starts=ints(0, 3)), "one number more"),
+    (None, {}, dict(starts=torch.tensor([0, 2, 3])), "int32"),
+    (None, {}, dict(starts=ints(0, 2, 3).to("meta")), "the cache's GPU"),
+    (None, {}, dict(seqs=ints(0, 1, 2)), "one number more"),
+    (None, {}, dict(counts=ints(3)), "one length"),
+    (None, {}, dict(counts=torch.tensor([2, 1])), "int32"),
+])
+def test_a_refused_extend_leaves_the_book_alone(monkeypatch, window, cache, call, text):
+    ctx = context()
+    c = cache_of(ctx, **cache)
+    with pytest.raises(ValueError, match=text):
+        extend(monkeypatch, model_of(ctx, params(window)), c, **call)
+    assert c._lib.calls == []
+
+
+def test_heads_beyond_the_kernels_are_refused_first(monkeypatch):
+    ctx = context()
+    c = cache_of(ctx, heads=1, hd=260)
+    with pytest.raises(ValueError, match="up to 256"):
+        extend(monkeypatch, model_of(ctx, params(heads=1, hd=260)), c, x=torch.zeros(3, 260))
+    assert c._lib.calls == []
