@@ -215,6 +215,8 @@ def _ptr(a):
 
 
 class Context:
+    stream = None  # what set_stream was given, None: the context's own
+
     def __init__(self, device=0):
         self._h = ctypes.c_void_p()
         rc = lib().pimdl_init(device, ctypes.byref(self._h))
@@ -239,6 +241,11 @@ class Context:
 
     def set_stream(self, hip_stream):
         self._check(lib().pimdl_set_stream(self._h, ctypes.c_void_p(hip_stream) if hip_stream else None))
+        self.stream = hip_stream or None
+
+    def in_order_with(self, other):
+        """Whether calls of both contexts run one after the other: they are one, or on one stream."""
+        return self is other or (self.stream is not None and self.stream == other.stream)
 
     def synchronize(self):
         self._check(lib().pimdl_synchronize(self._h))

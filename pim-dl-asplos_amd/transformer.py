@@ -243,6 +243,8 @@ class TransformerLayer:
     def check_cached(self, x, cache, layer, starts, seqs):
         """Refuses what forward(x, cached=(cache, layer, starts, seqs)) could not do, before anything is written."""
         p = self.params
+        if not self.ctx.in_order_with(cache.ctx):
+            raise ValueError("the cache's context runs on another stream than the layer's: nothing orders their calls")
         if p.window is not None and p.window[1] != 0:
             raise ValueError("a cache holds no later tokens: the window must have right = 0")
         if not 0 <= layer < cache.layers:
@@ -368,7 +370,8 @@ class Transformer:
     def extend(self, x, cache, starts, seqs, counts):
         """The newest tokens of some sequences through the model (a chunk of a prompt, a single token, or both in one batch): x [tokens][token_dim]
         packed, row b of the batch is the counts[b] tokens starts[b] .. starts[b + 1] - 1 of sequence seqs[b] (int32 device tensors; seqs
-        without repetitions).  A call that cannot be done raises before the cache changes.  Makes room for them in the PagedCache, fills it layer by layer, and every token sees its sequence up to itself
+        without repetitions).  The cache is one of the layers' context, or of one on its stream.  A call that
+        cannot be done raises before the cache changes.  Makes room for them in the PagedCache, fills it layer by layer, and every token sees its sequence up to itself
         (params.window: with right = 0).  cache.lacking tells afterwards whether there were pages enough; if not, the outputs are those of the
         tokens that the cache had before.  Rows of x behind the last sequence (a batch padded for a recorded step) come out undefined."""
         for i, layer in enumerate(self.layers):

@@ -1171,3 +1171,27 @@ def test_a_refused_extend_leaves_the_cache_as_it_was(ctx):
     torch.cuda.synchronize()
     assert empty.shape == (0, 256) and int(cache.lacking) == 0 and int(cache.lengths.sum()) == 0
     model.close()
+
+
+def test_a_cache_of_another_context_needs_the_same_stream(ctx):
+    model, p = _model(ctx, 64, 4, 2, 32, 4)
+    other, side = pimdl.Context(0), torch.cuda.Stream()
+    cache = K.PagedCache(other, pimdl, 2, 40, 4, 64, 16, "f16", 3, 200)
+    torch.cuda.synchronize()
+    x, starts, seqs, counts = randn(gen_of(1), 5, 256), starts_of([5]), ints(1), ints(5)
+    assert other.stream is None
+    with pytest.raises(ValueError, match="another stream"):
+        model.extend(x, cache, starts, seqs, counts)
+    torch.cuda.synchronize()
+    assert int(cache.lengths.sum()) == 0
+    try:
+        for c in (ctx, other):
+            c.set_stream(side.cuda_stream)
+        with torch.cuda.stream(side):
+            model.extend(x, cache, starts, seqs, counts)
+        torch.cuda.synchronize()
+        assert int(cache.lengths[1]) == 5 and int(cache.lacking) == 0
+    finally:
+        ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    model.close()
+    other.close()

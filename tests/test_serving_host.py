@@ -1,7 +1,5 @@
 """Host logic of serving that needs no GPU: what Transformer.extend and PagedCache refuse, and that a refused call has changed nothing.  Stand-ins
 record what would have been launched."""
-import types
-
 import pytest
 import torch
 
@@ -28,8 +26,10 @@ def params(window=None, heads=4, hd=64):
     return p
 
 
-def context():
-    return types.SimpleNamespace(_h=None, _check=lambda rc: None)
+def context(stream=None):
+    c = pimdl.Context.__new__(pimdl.Context)
+    c._h, c.stream = None, stream
+    return c
 
 
 def cache_of(ctx, layers=2, heads=4, hd=64, page_tokens=16, seqs=3):
@@ -120,3 +120,12 @@ def test_heads_beyond_the_kernels_are_refused_first(monkeypatch):
     with pytest.raises(ValueError, match="up to 256"):
         extend(monkeypatch, model_of(ctx, params(heads=1, hd=260)), c, x=torch.zeros(3, 260))
     assert c._lib.calls == []
+
+
+def test_a_cache_on_another_stream_is_refused(monkeypatch):
+    """Two contexts: their calls are in order only where both were given the same stream."""
+    for own, other, fine in ((None, None, False), (7, None, False), (None, 7, False), (7, 8, False), (7, 7, True)):
+        cache = cache_of(context(other))
+        with pytest.raises(Reached if fine else ValueError, match=None if fine else "another stream"):
+            extend(monkeypatch, model_of(context(own), params()), cache)
+        assert cache._lib.calls == (["pimdl_pages_reserve"] if fine else [])
