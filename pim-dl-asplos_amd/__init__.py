@@ -341,6 +341,10 @@ class Context:
                              left, right, sinks, scale, dtype=F32):
         """Device addresses; attention within each sequence of a packed batch (sequence b owns rows starts[b] .. starts[b + 1] - 1)
         where position p sees key j if j <= p + right and (j + left >= p or j < sinks); UNLIMITED opens a side.  Strides in elements."""
+        numbers = (batch, tokens, heads, kv_heads, head_dim, q_stride, kv_stride, out_stride, left, right, sinks, dtype)
+        if min(numbers) < 0 or max(numbers) > 0xFFFFFFFF:  # a 32-bit field would take it for another number
+            names = ("batch", "tokens", "heads", "kv_heads", "head_dim", "q_stride", "kv_stride", "out_stride", "left", "right", "sinks", "dtype")
+            raise ValueError(", ".join(f"{name}={n}" for name, n in zip(names, numbers) if not 0 <= n <= 0xFFFFFFFF) + " must be 0 .. 2^32 - 1")
         d = AttentionWindowDesc(q, k, v, out, starts, batch, tokens, heads, kv_heads, head_dim, q_stride, kv_stride, out_stride, left, right,
                                 sinks, dtype, scale)
         self._check(lib().pimdl_attention_window(self._h, ctypes.byref(d)))

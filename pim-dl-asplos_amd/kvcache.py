@@ -70,7 +70,10 @@ class PagedCache:
         """Address, row stride and type of a packed tensor; a column range of a wider one is fine."""
         if t.dim() != 2 or t.shape[1] != columns or (t.shape[1] > 1 and t.stride(1) != 1) or t.dtype not in _CODES:
             raise ValueError(f"{name} must be [tokens][{columns}] with unit column stride")
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), columns), _CODES[t.dtype]
+        stride = t.stride(0) if t.shape[0] > 1 else columns  # (of a single row it says nothing)
+        if stride > self._unlimited:
+            raise ValueError(f"{name}: a row stride of {stride} (up to 2^32 - 1)")
+        return t.data_ptr(), stride, _CODES[t.dtype]
 
     def _batch(self, starts, seqs):
         at, n = self._list(starts, "starts")
@@ -105,11 +108,12 @@ class PagedCache:
             raise ValueError("q and out must have one shape and type")
         qa, qs, qt = self._rows(q, columns, "q")
         oa, os_, _ = self._rows(out, columns, "out")
-        if sinks < 0 or (left is not None and left < 0):
-            raise ValueError("left and sinks count positions")
+        left = self._unlimited if left is None else left
+        if not (0 <= left <= self._unlimited and 0 <= sinks <= self._unlimited):
+            raise ValueError(f"left={left} and sinks={sinks} must be counts of positions, below 2^32")
         to, at, batch = self._batch(starts, seqs)
         self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, self._layer[layer], to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt,
-                                                        self._unlimited if left is None else left, sinks,
+                                                        left, sinks,
                                                         1.0 / math.sqrt(self.head_dim) if scale is None else scale))
 
     def reserve(self, seqs, counts):

@@ -25,6 +25,7 @@ Op order of one layer (transformer_layer.cpp, "step" comments):
     y       = h + norm(f; output LayerNorm)          (:599-611)
 """
 import math
+import operator
 import os
 import sys
 import time
@@ -69,6 +70,15 @@ class TransformerParams:
     def n(self):
         return self.seq_len * self.batch_size
 
+    def borders(self, unlimited=0xFFFFFFFF):
+        """window as numbers of 32 bits, `unlimited` for a side without a border"""
+        left, right, sinks = self.window
+        left, right = (unlimited if w is None else operator.index(w) for w in (left, right))
+        sinks = operator.index(sinks)
+        if not all(0 <= w <= unlimited for w in (left, right, sinks)):
+            raise ValueError(f"window={self.window}: counts of positions, or None")
+        return left, right, sinks
+
     @classmethod
     def from_yaml(cls, path):
         import yaml
@@ -80,6 +90,7 @@ class TransformerParams:
         if "attention_window" in net:  # [left, right, sinks]; null: no border on that side
             left, right, sinks = net["attention_window"]
             p.window = (None if left is None else int(left), None if right is None else int(right), int(sinks))
+            p.borders()
         if p.head_num * p.head_dim != p.token_dim:
             raise ValueError("head_num * head_dim != token_dim")
         dims = {"qkv": (p.token_dim, 3 * p.token_dim), "o": (p.token_dim, p.token_dim),
@@ -235,9 +246,9 @@ class TransformerLayer:
             starts = self.torch.arange(0, (B + 1) * p.seq_len, p.seq_len, device=q.device, dtype=self.torch.int32)  # (there from the replay on only)
         elif starts is None:  # copied from the host: there, on any stream, when the call returns
             starts = self._starts[B] = self.torch.tensor(range(0, (B + 1) * p.seq_len, p.seq_len), device=q.device, dtype=self.torch.int32)
-        left, right = (self._unlimited if w is None else w for w in p.window[:2])
+        left, right, sinks = p.borders(self._unlimited)
         self.ctx.attention_window_ptr(q.data_ptr(), k.data_ptr(), v.data_ptr(), a.data_ptr(), starts.data_ptr(), B, B * p.seq_len, p.head_num,
-                                      p.head_num, p.head_dim, q.stride(0), k.stride(0), p.token_dim, left, right, p.window[2],
+                                      p.head_num, p.head_dim, q.stride(0), k.stride(0), p.token_dim, left, right, sinks,
                                       1.0 / math.sqrt(p.head_dim))
 
     def check_cached(self, x, cache, layer, starts, seqs):
@@ -245,7 +256,7 @@ class TransformerLayer:
         p = self.params
         if not self.ctx.in_order_with(cache.ctx):
             raise ValueError("the cache's context runs on another stream than the layer's: nothing orders their calls")
-        if p.window is not None and p.window[1] != 0:
+        if p.window is not None and p.borders(self._unlimited)[1] != 0:
             raise ValueError("a cache holds no later tokens: the window must have right = 0")
         if not 0 <= layer < cache.layers:
             raise ValueError(f"a cache of {cache.layers} layers has no layer {layer}")

@@ -1,7 +1,10 @@
 """Host logic of serving that needs no GPU: what Transformer.extend and PagedCache refuse, and that a refused call has changed nothing.  Stand-ins
 record what would have been launched."""
+import os
+
 import pytest
 import torch
+import yaml
 
 from __graft_entry__ import load_package
 
@@ -129,3 +132,57 @@ def test_a_cache_on_another_stream_is_refused(monkeypatch):
         with pytest.raises(Reached if fine else ValueError, match=None if fine else "another stream"):
             extend(monkeypatch, model_of(context(own), params()), cache)
         assert cache._lib.calls == (["pimdl_pages_reserve"] if fine else [])
+
+
+WINDOW = dict(q=1, k=1, v=1, out=1, starts=1, batch=1, tokens=4, heads=2, kv_heads=1, head_dim=64, q_stride=128, kv_stride=64, out_stride=128, left=5, right=0,
+              sinks=1, scale=1.0)
+
+
+@pytest.mark.parametrize("name", ["left", "right", "sinks", "batch", "tokens", "heads", "kv_heads", "head_dim", "q_stride", "kv_stride", "out_stride", "dtype"])
+def test_numbers_that_32_bits_do_not_hold_are_refused(monkeypatch, name):
+    """-1 would become no border, 2^32 none at all."""
+    monkeypatch.setattr(pimdl, "lib", lambda: pytest.fail("the library was called"))
+    for bad in (-1, -2 ** 31, 2 ** 32, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match=name):
+            context().attention_window_ptr(**(WINDOW | {name: bad}))
+
+
+def test_attend_refuses_numbers_that_32_bits_do_not_hold():
+    c, q = cache_of(context()), torch.zeros(2, 256)
+    for bad in (dict(left=-1), dict(left=2 ** 32), dict(sinks=-1), dict(sinks=2 ** 32 + 1)):
+        with pytest.raises(ValueError, match=list(bad)[0]):
+            c.attend(0, q, torch.zeros(2, 256), ints(0, 1, 2), 4, **bad)
+    far = torch.empty_strided((2, 256), (2 ** 32 + 256, 1), device="meta")
+    with pytest.raises(ValueError, match="stride"):
+        c.attend(0, far, far, ints(0, 1, 2), 4)
+    assert c._lib.calls == []
+    c.attend(0, q, torch.zeros(2, 256), ints(0, 1, 2), 4, left=0xFFFFFFFF, sinks=3)
+    c.attend(0, q[:1], torch.zeros(1, 256), ints(0, 1), 4, left=0)
+    assert c._lib.calls == ["pimdl_attention_paged"] * 2
+
+
+@pytest.mark.parametrize("window", [(-1, 0, 0), (3, -2, 0), (3, 0, -1), (2 ** 32, 0, 0), (None, 2 ** 32, 0), (None, None, 2 ** 40)])
+def test_windows_out_of_range_are_refused(monkeypatch, window):
+    ctx = context()
+    cache = cache_of(ctx)
+    with pytest.raises(ValueError, match="window"):
+        params(window).borders()
+    with pytest.raises(ValueError, match="window"):
+        extend(monkeypatch, model_of(ctx, params(window)), cache)
+    assert cache._lib.calls == []
+    with pytest.raises(TypeError):
+        params((1.5, 0, 0)).borders()
+    assert params((None, 7, 2)).borders() == (pimdl.UNLIMITED, 7, 2)
+
+
+def test_a_configuration_with_a_window_out_of_range_is_refused(tmp_path):
+    cfg = yaml.safe_load(open(os.path.join(os.path.dirname(__file__), "golden", "transformer_small.yaml")))
+    for window, fine in (([5, None, 1], True), ([-5, 0, 1], False), ([5, 0, 1 << 32], False)):
+        cfg["network_params"]["attention_window"] = window
+        path = tmp_path / "w.yaml"
+        path.write_text(yaml.safe_dump(cfg))
+        if fine:
+            assert T.TransformerParams.from_yaml(path).window == (5, None, 1)
+        else:
+            with pytest.raises(ValueError, match="window"):
+                T.TransformerParams.from_yaml(path)
