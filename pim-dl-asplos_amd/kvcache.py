@@ -86,6 +86,11 @@ class PagedCache:
             raise ValueError("starts must hold one number more than seqs")
         return to, at, m
 
+    def _of(self, layer):
+        if not 0 <= layer < self.layers:
+            raise IndexError(f"a cache of {self.layers} layers has no layer {layer}")
+        return self._layer[layer]
+
     def check_batch(self, starts, seqs=None):
         """Refuses tensors that append and attend would not take for a batch."""
         _, _, batch = self._batch(starts, seqs)
@@ -98,7 +103,7 @@ class PagedCache:
             raise ValueError("k and v must have one shape, stride and type")
         ka, ks, kt = self._rows(k, self.kv_heads * self.head_dim, "k")
         to, at, batch = self._batch(starts, seqs)
-        self.ctx._check(self._lib.pimdl_cache_append(self.ctx._h, self._layer[layer], to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt))
+        self.ctx._check(self._lib.pimdl_cache_append(self.ctx._h, self._of(layer), to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt))
 
     def attend(self, layer, q, out, starts, heads, seqs=None, left=None, sinks=0, scale=None):
         """Causal attention of the new tokens (q, out: [tokens][heads * head_dim]) over everything that their sequences have in the cache, or, with
@@ -112,7 +117,7 @@ class PagedCache:
         if not (0 <= left <= self._unlimited and 0 <= sinks <= self._unlimited):
             raise ValueError(f"left={left} and sinks={sinks} must be counts of positions, below 2^32")
         to, at, batch = self._batch(starts, seqs)
-        self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, self._layer[layer], to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt,
+        self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, self._of(layer), to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt,
                                                         left, sinks,
                                                         1.0 / math.sqrt(self.head_dim) if scale is None else scale))
 

@@ -186,3 +186,15 @@ def test_a_configuration_with_a_window_out_of_range_is_refused(tmp_path):
         else:
             with pytest.raises(ValueError, match="window"):
                 T.TransformerParams.from_yaml(path)
+
+
+@pytest.mark.parametrize("layer", [-1, -2, 2, 7])
+def test_layers_that_are_not_there_are_refused(layer):
+    c, x = cache_of(context()), torch.zeros(2, 256)
+    with pytest.raises(IndexError, match="layer"):
+        c.append(layer, x, x, ints(0, 1, 2))
+    with pytest.raises(IndexError, match="layer"):
+        c.attend(layer, x, torch.zeros(2, 256), ints(0, 1, 2), 4)
+    assert c._lib.calls == []
+    c.append(1, x, x, ints(0, 1, 2))
+    assert c._lib.calls == ["pimdl_cache_append"]
