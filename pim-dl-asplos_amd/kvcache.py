@@ -1,8 +1,8 @@
 """A paged cache of keys and values over torch tensors, for serving a causal LUT-NN transformer on one MI355X.
 
 The reference recomputes whole sequences in every forward (inference-engine/src/host/transformer_layer.cpp:211-230) and has no
-cache; this is what a caller needs to feed a model its new tokens only.  Everything stays on the device, the bookkeeping included: no call
-here waits for the GPU, and a step (reserve, then per layer append and attend) can be recorded into a HIP graph.
+cache; this is what a caller needs to feed a model its new tokens only.  Everything stays on the device, the bookkeeping included: once a cache is made no
+call here waits for the GPU, and a step (reserve, then per layer append and attend) can be recorded into a HIP graph.
 
     cache = PagedCache(ctx, pimdl, layers=12, pages=4096, kv_heads=12, head_dim=64, page_tokens=16, dtype="f16", seqs=64, max_len=2048)
     cache.reserve(seqs, counts)                      # room for counts[i] more positions of sequence seqs[i]
@@ -51,6 +51,9 @@ class PagedCache:
             raise ValueError("a cache's tensors must be contiguous and on one GPU")
         self.ctx, self.k, self.v, self.tables, self.lengths, self.refs = ctx, k, v, tables, lengths, refs
         self.lacking = torch.zeros(1, device=k.device, dtype=torch.int32)
+        # torch has queued zeros on its own stream, the context may have another: they are there when this returns (under a capture, from the replay on)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(k.device).synchronize()
         self.layers, self.kv_heads, self.head_dim, self.page_tokens = layers, kv_heads, head_dim, page_tokens
         self._lib = pimdl.lib()
         self._unlimited = pimdl.UNLIMITED

@@ -1195,3 +1195,30 @@ def test_a_cache_of_another_context_needs_the_same_stream(ctx):
         ctx.set_stream(torch.cuda.current_stream().cuda_stream)
     model.close()
     other.close()
+
+
+@pytest.mark.parametrize("over", [False, True])
+def test_a_cache_made_on_a_busy_stream_is_ready_for_another(ctx, over):
+    """torch's current stream has work queued when the cache's tensors are made on it; the context has a stream of its own and uses them at once."""
+    own, side = pimdl.Context(0), torch.cuda.Stream()
+    a = torch.zeros(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    dirt = torch.full((1 << 20,), 77, device="cuda", dtype=torch.int32)  # what freed memory holds
+    lists = [(ints(s), ints(n)) for s, n in ((2, 40), (0, 16))]
+    torch.cuda.synchronize()
+    del dirt
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            a = a @ a
+        if over:
+            k, v = (torch.zeros(1, 30, 1, 16, 64, device="cuda", dtype=torch.float16) for _ in range(2))
+            cache = K.PagedCache.over(own, pimdl, k, v, torch.full((4, 8), -1, device="cuda", dtype=torch.int32), torch.zeros(4, device="cuda", dtype=torch.int32),
+                                      torch.zeros(30, device="cuda", dtype=torch.int32))
+        else:
+            cache = K.PagedCache(own, pimdl, 1, 30, 1, 64, 16, "f16", 4, 128)
+        for seqs, counts in lists:
+            cache.reserve(seqs, counts)
+    torch.cuda.synchronize()
+    assert cache.lengths.tolist() == [16, 0, 40, 0] and int(cache.lacking) == 0
+    assert cache.tables[2].tolist() == [0, 1, 2] + [-1] * 5 and cache.tables[0].tolist() == [3] + [-1] * 7
+    assert cache.refs.tolist() == [1] * 4 + [0] * 26
+    own.close()
