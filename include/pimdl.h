@@ -422,6 +422,17 @@ PIMDL_API int pimdl_cache_append(pimdl_ctx* ctx, const pimdl_paged_cache* cache,
                                  const int32_t* starts, uint32_t batch, uint32_t tokens, const void* k, const void* v,
                                  uint32_t kv_stride, uint32_t dtype);
 
+/* How the last pimdl_attention_window or pimdl_attention_paged of the context was launched, for tests and profiles: the choice goes by sizes alone, never
+ * by what is in device memory. */
+typedef struct pimdl_attention_plan {
+    uint32_t plain;          /* 1: the kernel of other head sizes; all else is 0 */
+    uint32_t wide, narrow;   /* 1: blocks of 128 rows; blocks of 16 rows (both: one launch for sequences of many and of few rows) */
+    uint32_t wide_splits, narrow_splits; /* workgroups that the keys of a block are split over */
+    uint32_t by_slot;        /* narrow: a workgroup per block of 16 rows, not per row of the batch */
+    uint32_t join;           /* 0: no splits to be joined; 1: of all blocks; 2: of the rows of the batch that have few rows */
+} pimdl_attention_plan;
+PIMDL_API int pimdl_attention_last_plan(const pimdl_ctx* ctx, pimdl_attention_plan* out);
+
 /* The pages' bookkeeping lives on the device, so that a step never waits for the host.  Page p is free where refs[p] == 0;
  * otherwise refs[p] is the number of sequences that hold it.  A sequence holds the first ceil(length / page_tokens) entries of
  * its table row; the others are -1.  Lists may name a sequence twice: only its first place counts; what is out of range is left

@@ -39,7 +39,7 @@ EXPORTS = ["pimdl_init", "pimdl_destroy", "pimdl_last_error", "pimdl_set_stream"
            "pimdl_amm_create_with", "pimdl_amm_set_tuning", "pimdl_amm_get_tuning", "pimdl_lutgen_mode",
            "pimdl_diag_mfma_error_crafted", "pimdl_amm_last_gather_kernel", "pimdl_amm_run_breakdown", "pimdl_diag_host_copy",
            "pimdl_attention_window", "pimdl_attention_paged", "pimdl_cache_append", "pimdl_pages_reserve", "pimdl_pages_fork",
-           "pimdl_pages_free", "pimdl_pages_compact", "pimdl_pages_copy"]
+           "pimdl_pages_free", "pimdl_pages_compact", "pimdl_pages_copy", "pimdl_attention_last_plan"]
 NOALLOC_SCRATCH_BYTES = 8 << 20
 
 
@@ -118,6 +118,11 @@ class PageBook(ctypes.Structure):
                  ("page_bytes", ctypes.c_uint64)])
 
 
+class AttentionPlan(ctypes.Structure):
+    """pimdl_attention_plan"""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("plain", "wide", "narrow", "wide_splits", "narrow_splits", "by_slot", "join")]
+
+
 _lib = None
 
 
@@ -190,6 +195,7 @@ def lib():
     L.pimdl_pages_free.argtypes = [vp, book, vp, u32]
     L.pimdl_pages_compact.argtypes = [vp, book]
     L.pimdl_pages_copy.argtypes = [vp, book, vp, vp, u32]
+    L.pimdl_attention_last_plan.argtypes = [vp, ctypes.POINTER(AttentionPlan)]
     for name in EXPORTS:
         if name != "pimdl_last_error":
             getattr(L, name).restype = ctypes.c_int
@@ -348,6 +354,12 @@ class Context:
         d = AttentionWindowDesc(q, k, v, out, starts, batch, tokens, heads, kv_heads, head_dim, q_stride, kv_stride, out_stride, left, right,
                                 sinks, dtype, scale)
         self._check(lib().pimdl_attention_window(self._h, ctypes.byref(d)))
+
+    def last_attention(self):
+        """How the last windowed or paged attention call was launched (pimdl_attention_plan)."""
+        plan = AttentionPlan()
+        self._check(lib().pimdl_attention_last_plan(self._h, ctypes.byref(plan)))
+        return {name: getattr(plan, name) for name, _ in plan._fields_}
 
     def amm_group(self, amms):
         return AmmGroup(self, amms)

@@ -308,6 +308,7 @@ int launch_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
     while (groups < 16 && groups * 4 < splits && 2 * groups * lanes <= 256) groups *= 2;
     const uint32_t rows = std::min(JOIN_ROWS, 256 / (lanes * groups));
     const bool by_row = p.wide && p.wide_splits == 1;  // (those that are split have up to NARROW_ROWS rows)
+    ctx->attn_plan.join = by_row ? 2 : 1;
     static_assert(attn::NARROW_ROWS <= JOIN_ROWS, "a block holds all rows of a sequence of few");
     const uint64_t slots = (by_row ? 0 : (uint64_t)a.tokens * a.group / JOIN_ROWS) + a.batch;
     // workgroups that share a block, where there are few blocks
@@ -387,8 +388,10 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
 
 int launch_attention(Ctx* ctx, const AttnArgs& a)
 {
+    ctx->attn_plan = {};
     if (a.tokens == 0 || a.batch == 0) return PIMDL_OK;
     if (!matrix_form(a)) {
+        ctx->attn_plan.plain = 1;
         if (a.dtype == PIMDL_BF16) return launch_plain<__bf16, __bf16>(ctx, a);
         if (a.dtype == PIMDL_F16) return launch_plain<_Float16, _Float16>(ctx, a);
         if (a.cache_dtype == PIMDL_BF16) return launch_plain<float, __bf16>(ctx, a);
@@ -398,6 +401,7 @@ int launch_attention(Ctx* ctx, const AttnArgs& a)
     attn::Plan p;
     int rc = make_plan(ctx, a, &p);
     if (rc) return rc;
+    ctx->attn_plan = {0, p.wide, p.narrow, p.wide ? p.wide_splits : 0, p.narrow ? p.narrow_splits : 0, p.by_slot, 0};
     if (a.dtype == PIMDL_BF16) rc = attn::launch_bf16(ctx, a, p);
     else if (a.dtype == PIMDL_F16) rc = attn::launch_f16(ctx, a, p);
     else if (a.cache_dtype == PIMDL_BF16) rc = attn::launch_f32_bf16(ctx, a, p);

@@ -703,6 +703,7 @@ int pimdl_init(int device, pimdl_ctx** out)
     ctx->d_cent = nullptr; ctx->cent_bytes = 0;
     ctx->d_attn = nullptr; ctx->attn_bytes = 0;
     ctx->d_book = nullptr; ctx->book_bytes = 0;
+    ctx->attn_plan = {};
     ctx->d_static_scratch = nullptr;
     ctx->pipe = nullptr;
     for (auto& ev : ctx->ev) ev = nullptr;

@@ -155,6 +155,7 @@ struct Ctx {
     size_t attn_bytes;
     char* d_book;        // lists of pages that the page book's kernels hand to each other
     size_t book_bytes;
+    pimdl_attention_plan attn_plan;  // of the last attention call
     hipEvent_t ev[4];
     HostPipe* pipe;      // created by the first call that hands over a host buffer
     std::mutex host_mutex;  // held by a call while it uses `pipe` or d_lutgen: table construction may run beside another thread's calls

@@ -159,6 +159,13 @@ int pimdl_attention_paged(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const 
     return launch_attention(ctx, a);
 }
 
+int pimdl_attention_last_plan(const pimdl_ctx* ctx, pimdl_attention_plan* out)
+{
+    if (!ctx || !out) return PIMDL_ERR_INVALID;
+    *out = ctx->attn_plan;
+    return PIMDL_OK;
+}
+
 int pimdl_cache_append(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const int32_t* seqs, const int32_t* starts, uint32_t batch,
                        uint32_t tokens, const void* k, const void* v, uint32_t kv_stride, uint32_t dtype)
 {

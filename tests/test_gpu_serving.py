@@ -976,6 +976,7 @@ def test_window_rounds_its_output_alone(ctx, dtype, counts, hd):
     out = torch.zeros(n, heads * hd, device="cuda", dtype=TYPES[dtype])
     window(ctx, q, k, v, out, counts, heads, kv, hd, 500, 0, 2, dtype)
     torch.cuda.synchronize()
+    plan_is(ctx, wide=int(n > 100), narrow=int(n <= 100))
     at = 0
     for c in counts:
         rows = slice(at, at + c)
@@ -993,6 +994,7 @@ def test_pages_round_their_output_alone(ctx, dtype, counts, lengths, hd):
     out = torch.zeros_like(q)
     f.cache.attend(0, q, out, starts_of(counts), heads)
     torch.cuda.synchronize()
+    plan_is(ctx, wide=int(sum(counts) > 100), narrow=1)
     at = 0
     for s, c in enumerate(counts):
         k, v = (x[0] for x in f.rows[s])
@@ -1221,4 +1223,195 @@ def test_a_cache_made_on_a_busy_stream_is_ready_for_another(ctx, over):
     assert cache.lengths.tolist() == [16, 0, 40, 0] and int(cache.lacking) == 0
     assert cache.tables[2].tolist() == [0, 1, 2] + [-1] * 5 and cache.tables[0].tolist() == [3] + [-1] * 7
     assert cache.refs.tolist() == [1] * 4 + [0] * 26
+    own.close()
+
+
+# ---------------------------------------------------------------------------------------------- blocks of 128 rows
+
+# The plans that the sizes below have on 256 CUs; a rule that moves gets other sizes here, so that every kernel and join stays tested.
+
+def plan_is(ctx, **want):
+    got = ctx.last_attention()
+    assert {k: got[k] for k in want} == want, got
+
+
+def blocks_case(ctx, seed, counts, lengths, heads, kv, hd, page_tokens, dtype, cache, left=None, sinks=0):
+    paged_case(ctx, seed, counts, lengths, heads, kv, hd, page_tokens, dtype, cache, left, sinks)
+    return ctx.last_attention()
+
+
+PAIRS = [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [32, 64, 80, 96, 128])
+def test_many_rows_in_a_window(ctx, dtype, hd):
+    """Ragged, shared key heads, sinks: without splits, and with splits that are joined."""
+    counts = [700, 1, 129, 0, 900, 128, 127]
+    window_case(ctx, hd, counts, 8, 2, hd, 300, 40, 5, dtype)
+    plan_is(ctx, plain=0, wide=1, narrow=0, wide_splits=1, join=0)
+    window_case(ctx, hd + 1, counts, 8, 2, hd, UNL, 0, 0, dtype)
+    plan_is(ctx, wide=1, narrow=0, wide_splits=3, join=1)
+    window_case(ctx, hd + 2, counts, 8, 2, hd, UNL, UNL, 0, dtype, scale=-0.3 / math.sqrt(hd))
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("hd", [32, 64, 80, 96, 128])
+def test_many_rows_over_pages_in_splits_beside_few(ctx, dtype, cache, hd):
+    """Chunks in blocks of 128 rows and single tokens in blocks of 16, one launch, both split, one join; with and without a window."""
+    counts, lengths = [600, 513, 1, 0, 40], [4000, 1200, 900, 30, 41]
+    plan = blocks_case(ctx, hd, counts, lengths, 8, 2, hd, 16, dtype, cache)
+    assert plan == dict(plain=0, wide=1, narrow=1, wide_splits=7, narrow_splits=15, by_slot=0, join=1), plan
+    plan = blocks_case(ctx, hd + 1, counts, lengths, 8, 2, hd, 64, dtype, cache, left=333, sinks=70)
+    assert plan["wide"] and plan["narrow"] and plan["wide_splits"] == 1 and plan["join"] == 0, plan
+
+
+@pytest.mark.parametrize("dtype,cache,hd", [("bf16", "bf16", 128), ("f32", "f16", 64), ("f32", "f32", 80)])
+def test_joins_of_the_rows_with_few(ctx, dtype, cache, hd):
+    """Blocks of 128 rows enough to fill the device, unsplit; the keys of single tokens beside them are split, and only those are joined."""
+    plan = blocks_case(ctx, hd, [2100, 1, 2100, 3, 1], [2100, 3000, 2500, 1100, 17], 16, 2, hd, 32, dtype, cache)
+    assert plan["wide"] and plan["narrow"] and plan["wide_splits"] == 1 and plan["narrow_splits"] > 1 and plan["join"] == 2, plan
+
+
+@pytest.mark.parametrize("n", [1, 15, 16, 31, 32, 33, 63, 64, 65, 96, 127, 128, 129, 255, 257])
+@pytest.mark.parametrize("left,right,sinks", [(UNL, UNL, 0), (UNL, 0, 0), (33, 0, 5), (31, 31, 0), (64, 1, 33)])
+def test_many_rows_at_the_edges_of_blocks(ctx, n, left, right, sinks):
+    for dtype in ("bf16", "f32"):
+        window_case(ctx, n, [n, 3, 1500, n], 8, 2, 64, left, right, sinks, dtype)
+        plan_is(ctx, wide=1, narrow=0)
+
+
+@pytest.mark.parametrize("left,sinks", [(None, 0), (100, 4)])
+@pytest.mark.parametrize("n", [5, 33, 64, 127, 129])
+def test_many_rows_at_the_edges_of_pages(ctx, n, left, sinks):
+    """Chunks that end inside pages and tiles, one that is longer than what its sequence holds."""
+    for dtype, cache in (("bf16", "bf16"), ("f32", "f16"), ("f32", "f32")):
+        plan = blocks_case(ctx, n, [n, 900, 40], [n + 60, 900 + n, 30], 8, 2, 64, 16, dtype, cache, left, sinks)
+        assert plan["wide"] and plan["narrow"], plan
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_what_the_window_hides_changes_nothing_in_many_rows(ctx, dtype, hd):
+    """Keys and values that are not finite, at the borders of waves (32 rows), tiles (32 or 64 keys) and blocks (128 rows): rows that see them are not finite, in
+    all columns for a key, in its column for a value; all others are bit for bit what they were."""
+    heads, n = 8, 1500
+    gen = gen_of(hd)
+    q, k, v = (randn(gen, n, heads * hd, dtype=dtype) for _ in range(3))
+    out = torch.zeros_like(q)
+    places = [60, 125, 700 + 63, 700 + 64, 1499]
+
+    def run():
+        out.fill_(7.0)
+        window(ctx, q, k, v, out, [700, n - 700], heads, heads, hd, 7, 0, 0, dtype)
+        torch.cuda.synchronize()
+        plan_is(ctx, wide=1, wide_splits=1)
+        return out.clone()
+
+    plain = run()
+    assert torch.isfinite(plain).all()
+    seen = torch.zeros(n, dtype=torch.bool, device="cuda")
+    kept = k.clone()
+    for at in places:
+        k[at, 3 * hd:4 * hd] = float("inf")  # head 3's
+        seen[at:at + 8] = True
+    got = run()
+    assert torch.equal(got[~seen], plain[~seen])
+    assert torch.equal(got[:, :3 * hd], plain[:, :3 * hd]) and torch.equal(got[:, 4 * hd:], plain[:, 4 * hd:])
+    assert not torch.isfinite(got[seen, 3 * hd:4 * hd]).any()
+    k.copy_(kept)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        hit = torch.zeros_like(q, dtype=torch.bool)
+        kept = v.clone()
+        for i, at in enumerate(places):
+            col = (i + 2) * hd + (7 * i + hd - 1) % hd
+            v[at, col] = bad
+            hit[at:min(at + 8, 700 if at < 700 else n), col] = True
+        got = run()
+        assert not torch.isfinite(got[hit]).any()
+        # (the value's column of rows that see it aside) nothing has changed
+        assert torch.equal(got[~hit], plain[~hit])
+        v.copy_(kept)
+
+
+def reference_where(q, k, v, seen, scale):
+    """As reference(), for keys that `seen` [n][keys] names."""
+    n, h, hd = q.shape
+    kv, keys = k.shape[1], k.shape[0]
+    out, off, mass = (torch.zeros((n, h, hd), dtype=torch.float64, device=q.device) for _ in range(3))
+    for i in range(h):
+        qh, kh, vh = q[:, i].double(), k[:, i // (h // kv)].double(), v[:, i // (h // kv)].double()
+        s = torch.where(seen, (qh @ kh.t().contiguous()) * scale, -math.inf)
+        ds = torch.where(seen, (hd + 8) * U * abs(scale) * (qh.abs() @ kh.abs().t().contiguous()), 0.0)
+        p = torch.softmax(s, -1)
+        out[:, i], mass[:, i] = p @ vh, p @ vh.abs()
+        off[:, i] = (2 * torch.expm1(2 * ds.amax(-1, keepdim=True)) + 16 * U + 2 * (keys / 16 + 64) * U) * mass[:, i]
+    return out, off, mass
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_many_rows_over_pages_that_are_not_there(ctx, dtype, cache, hd):
+    n, c, heads = 1700, 800, 8
+    f = Filled(ctx, 12, [n], 8, hd, 16, cache, width=110)
+    gone = [1, 4, 50, 51, 90]
+    for page, entry in zip(gone, (-1, 1 << 30, f.cache.k.shape[1], -7, -1)):
+        f.cache.tables[0, page] = entry
+    q = randn(gen_of(13), c, heads * hd, dtype=dtype)
+    out = torch.zeros_like(q)
+    f.cache.attend(0, q, out, starts_of([c]), heads)
+    torch.cuda.synchronize()
+    plan_is(ctx, wide=1)
+    j, p = torch.arange(n, device="cuda"), torch.arange(n - c, n, device="cuda")
+    there = ~torch.isin(j // 16, torch.tensor(gone, device="cuda"))
+    k, v = (x[0] for x in f.rows[0])
+    want, off, mass = reference_where(q.reshape(c, heads, hd), k, v, (j[None] <= p[:, None]) & there[None], 1 / math.sqrt(hd))
+    check(out.reshape(c, heads, hd), want, off, mass, dtype)
+
+
+def test_captured_chunks_beside_single_tokens(ctx):
+    """A mixed step recorded once and replayed as chunks and single tokens change places, against eager calls of another context."""
+    heads, kv, hd = 8, 2, 64
+    own, side = pimdl.Context(0), torch.cuda.Stream()
+    caches = []
+    for c in (ctx, own):
+        f = Filled(c, 3, [2500, 1300, 900], kv, hd, 16, "bf16", spare=200, width=200)
+        caches.append(f.cache)
+    torch.cuda.synchronize()
+    total = 1300
+    seqs, counts, starts = ints(0, 1, 2), ints(700, 1, 599), starts_of([700, 1, 599])
+    qkv = randn(gen_of(3), total, (heads + 2 * kv) * hd, dtype="bf16")
+    outs = [torch.zeros(total, heads * hd, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+
+    def step(cache, out):
+        cache.append(0, qkv[:, heads * hd:(heads + kv) * hd], qkv[:, (heads + kv) * hd:], starts, seqs)
+        cache.attend(0, qkv[:, :heads * hd], out, starts, heads, seqs)
+
+    torch.cuda.synchronize()
+    own.set_stream(side.cuda_stream)
+    with torch.cuda.stream(side):
+        step(caches[1], outs[1])
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+        step(caches[1], outs[1])
+    assert own.last_attention()["wide"] and own.last_attention()["narrow"] and own.last_attention()["join"]
+    for i, now in enumerate(([700, 1, 599], [1, 1298, 1], [600, 0, 700], [3, 2, 1], [1300, 0, 0])):
+        torch.cuda.synchronize()
+        starts.copy_(starts_of(now))
+        qkv.copy_(randn(gen_of(10 + i), *qkv.shape, dtype="bf16"))
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        step(caches[0], outs[0])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1]), i
+        at, n = starts_of(now).tolist(), [2500, 1300, 900]
+        for s, c in enumerate(now):  # and against float64 over what the cache holds
+            pages = caches[0].tables[s].long()[:-(-n[s] // 16)]
+            k, v = (x[0, pages].transpose(1, 2).reshape(-1, kv, hd)[:n[s]] for x in (caches[0].k, caches[0].v))
+            want, off, mass = reference(qkv[at[s]:at[s + 1], :heads * hd].reshape(c, heads, hd), k, v, n[s] - c, UNL, 0, 0, 0.125)
+            check(outs[0][at[s]:at[s + 1]].reshape(c, heads, hd), want, off, mass, "bf16")
     own.close()
