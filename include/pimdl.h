@@ -366,7 +366,8 @@ PIMDL_API int pimdl_attention(pimdl_ctx* ctx, const float* q, const float* k, co
  * A batch is PACKED: sequence b owns rows starts[b] .. starts[b + 1] - 1 of the token buffers ([batch + 1] ascending
  * numbers; what lies beyond `tokens` is taken for `tokens`).  Rows of no sequence are neither read nor written.
  * Heads: a row holds head h in columns h * head_dim .. + head_dim - 1, and query head h reads key head
- * h / (heads / kv_heads), heads a multiple of kv_heads.  head_dim 1 .. 256; 32, 64, 80, 96 and 128 run on the matrix
+ * h / (heads / kv_heads), heads a multiple of kv_heads.  batch below 2^24, tokens below 2^30, tokens * heads up to 2^30; a call
+ * for which a launch would need 2^32 threads (millions of sequences) is refused as PIMDL_ERR_UNSUPPORTED.  head_dim 1 .. 256; 32, 64, 80, 96 and 128 run on the matrix
  * cores (given 16-byte aligned rows), other sizes on a plain kernel.  Strides are in elements.
  *
  * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max_j), over the keys that a query sees; |scale| up to 2^96.  Scores, maxima,

@@ -46,8 +46,8 @@ __global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kern
     __shared__ float mls[4][2];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e8 = lane & 7, j8 = lane >> 3;
     // heads that share a key head on one XCD (workgroups are dealt out to 8 in turn)
-    const uint32_t item = blockIdx.x / (8 * a.group) * 8 + blockIdx.x % 8;
-    const uint32_t t = item / a.kv_heads, kh = item % a.kv_heads, h = kh * a.group + blockIdx.x / 8 % a.group;
+    const uint32_t block = blockIdx.y * gridDim.x + blockIdx.x, item = block / (8 * a.group) * 8 + block % 8;
+    const uint32_t t = item / a.kv_heads, kh = item % a.kv_heads, h = kh * a.group + block / 8 % a.group;
     if (t >= a.tokens) return;
     const uint32_t b = row_of_token(a.starts, a.batch, a.tokens, t);
     const Row r = load_row(a.starts, a.seqs, a.tables, a.lengths, a.tokens, a.seq_count, a.table_width, a.page_shift, PAGED, b);
@@ -195,7 +195,7 @@ int launch_plain_of(Ctx* ctx, const AttnArgs& a)
 {
     const uint64_t items = ((uint64_t)a.tokens * a.kv_heads + 7) / 8 * 8 * a.group;
     if (items > 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
-    const dim3 grid((uint32_t)items);
+    const dim3 grid = grid_of(items);
     if (a.head_dim <= 64) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 64>), grid, dim3(256), 0, ctx->stream, a);
     else if (a.head_dim <= 128) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 128>), grid, dim3(256), 0, ctx->stream, a);
     else hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 256>), grid, dim3(256), 0, ctx->stream, a);
@@ -300,6 +300,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
     }
 }
 
+// Whether only rows of the batch with up to NARROW_ROWS rows are split.
+bool joins_by_row(const attn::Plan& p) { return p.wide && p.wide_splits == 1; }
+
 template <typename TQ>
 int launch_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
 {
@@ -307,14 +310,13 @@ int launch_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
     uint32_t groups = 1;
     while (groups < 16 && groups * 4 < splits && 2 * groups * lanes <= 256) groups *= 2;
     const uint32_t rows = std::min(JOIN_ROWS, 256 / (lanes * groups));
-    const bool by_row = p.wide && p.wide_splits == 1;  // (those that are split have up to NARROW_ROWS rows)
+    const bool by_row = joins_by_row(p);
     ctx->attn_plan.join = by_row ? 2 : 1;
     static_assert(attn::NARROW_ROWS <= JOIN_ROWS, "a block holds all rows of a sequence of few");
     const uint64_t slots = (by_row ? 0 : (uint64_t)a.tokens * a.group / JOIN_ROWS) + a.batch;
     // workgroups that share a block, where there are few blocks
     const uint32_t parts = slots * a.kv_heads >= 4 * (uint64_t)ctx->prop.multiProcessorCount ? 1 : (JOIN_ROWS + rows - 1) / rows;
     const uint64_t grid = slots * parts * a.kv_heads;
-    if (grid > 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
     hipLaunchKernelGGL((attention_join_kernel<TQ>), dim3((uint32_t)grid), dim3(256), 0, ctx->stream, a, p.part, (uint32_t)by_row, parts, rows, groups, p.wide ? p.wide_splits : 1,
                        p.narrow ? p.narrow_splits : 1, p.narrow ? p.narrow_rows : 0);
     return hip_check(ctx, hipGetLastError(), "attention_join_kernel launch");
@@ -372,7 +374,11 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     p->narrow_splits = (uint32_t)std::min<uint64_t>(p->narrow_splits, most);
     p->wide_splits = (uint32_t)std::min<uint64_t>(p->wide_splits, most);
     const uint32_t splits = std::max(p->narrow_splits, p->wide_splits);
-    if ((uint64_t)p->slots * a.kv_heads * p->wide_splits > 1u << 29 || (rows / attn::NARROW_ROWS + a.batch) * a.kv_heads * p->narrow_splits > 1u << 29 || (uint64_t)a.tokens * a.heads > 1u << 30)
+    const uint64_t batch_rows = (uint64_t)a.batch * a.kv_heads, blocks16 = rows / attn::NARROW_ROWS * a.kv_heads + batch_rows;
+    const bool fits = p->wide ? fits_launch((uint64_t)p->slots * a.kv_heads * p->wide_splits + (p->narrow ? batch_rows * p->narrow_splits : 0), 256)
+                              : fits_launch((p->by_slot ? blocks16 : batch_rows) * p->narrow_splits, 512);
+    const bool join_fits = splits == 1 || fits_launch(joins_by_row(*p) ? batch_rows : blocks16, 256);
+    if ((uint64_t)a.tokens * a.heads > 1u << 30 || !fits || !join_fits)
         return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
     if (splits > 1) {
         int rc = ensure_scratch(ctx, &ctx->d_attn, &ctx->attn_bytes, row_bytes * splits, "attention's partial results");

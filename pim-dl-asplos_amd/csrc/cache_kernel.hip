@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const TI* __restrict_
                                                            uint32_t tokens, uint32_t kv_stride, uint32_t page_shift)
 {
     const uint32_t row = c.kv_heads * c.head_dim / N;  // packs of a token's row
-    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t item = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
     const uint32_t t = (uint32_t)(item / row), part = (uint32_t)(item % row);
     if (t >= tokens || (c.lacking && *c.lacking != 0)) return;
     const Row r = load_row(starts, seqs, c.tables, c.lengths, tokens, c.seqs, c.table_width, page_shift, true, row_of_token(starts, batch, tokens, t));
@@ -55,8 +55,8 @@ int launch_append(Ctx* ctx, const pimdl_paged_cache& c, const int32_t* seqs, con
 {
     const bool packs = c.head_dim % 8 == 0 && kv_stride * sizeof(TI) % 16 == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
     const uint64_t items = (uint64_t)tokens * c.kv_heads * c.head_dim / (packs ? 8 : 1);
-    if (items / 256 >= 0x7fffffffu) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "pimdl_cache_append: too many elements for one launch");
-    const dim3 grid((uint32_t)((items + 255) / 256));
+    if (items > 65535ull * GRID_X * 256) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "pimdl_cache_append: too many elements for one launch");
+    const dim3 grid = grid_of((items + 255) / 256);
     const uint32_t shift = (uint32_t)__builtin_ctz(c.page_tokens);
     const TI *ki = static_cast<const TI*>(k), *vi = static_cast<const TI*>(v);
     if (packs) hipLaunchKernelGGL((cache_append_kernel<TI, TC, 8>), grid, dim3(256), 0, ctx->stream, ki, vi, c, seqs, starts, batch, tokens, kv_stride, shift);
@@ -499,13 +499,13 @@ int launch_pages_fork(Ctx* ctx, const pimdl_page_book& b, const int32_t* parents
     if (rc) return rc;
     const ForkLists f = {s + 1, s + 1 + n, s + 1 + 2 * (size_t)n, s + 1 + 3 * (size_t)n, s + 1 + 4 * (size_t)n, s};
     const Book book = book_of(b);
-    hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(SCAN), b.seqs * 4, ctx->stream, book, parents, children, n, f);
-    if ((rc = hip_check(ctx, hipGetLastError(), "pages_fork_kernel launch")) || n == 0) return rc;
     const Pools p = pools_of(b);
     const uint32_t row_blocks = (b.table_width + 1023) / 1024;
-    const uint64_t blocks = (uint64_t)n * row_blocks;
-    if (blocks > 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "pimdl_pages_fork: rows of %u pages, %u of them", b.table_width, n);
-    hipLaunchKernelGGL(pages_fork_apply_kernel, dim3((uint32_t)blocks + copy_blocks(ctx, p, n)), dim3(256), 0, ctx->stream, book, p, parents, children, n, row_blocks, f);
+    const uint64_t blocks = (uint64_t)n * row_blocks + copy_blocks(ctx, p, n);
+    if (!fits_launch(blocks, 256)) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "pimdl_pages_fork: rows of %u pages, %u of them", b.table_width, n);
+    hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(SCAN), b.seqs * 4, ctx->stream, book, parents, children, n, f);
+    if ((rc = hip_check(ctx, hipGetLastError(), "pages_fork_kernel launch")) || n == 0) return rc;
+    hipLaunchKernelGGL(pages_fork_apply_kernel, dim3((uint32_t)blocks), dim3(256), 0, ctx->stream, book, p, parents, children, n, row_blocks, f);
     return hip_check(ctx, hipGetLastError(), "pages_fork_apply_kernel launch");
 }
 

@@ -17,6 +17,11 @@ struct AttnArgs {
     float scale;
 };
 
+// A launch has fewer than 2^32 threads along x, so workgroups beyond GRID_X lie in rows of that many (a multiple of the XCDs that they are dealt out to).
+constexpr uint32_t GRID_X = 1u << 20;
+inline bool fits_launch(uint64_t blocks, uint32_t threads) { return blocks * threads < 1ull << 32; }
+inline dim3 grid_of(uint64_t blocks) { return blocks <= GRID_X ? dim3((uint32_t)blocks) : dim3(GRID_X, (uint32_t)((blocks + GRID_X - 1) / GRID_X)); }
+
 int launch_attention(Ctx* ctx, const AttnArgs& a);
 int launch_cache_append(Ctx* ctx, const pimdl_paged_cache& c, const int32_t* seqs, const int32_t* starts, uint32_t batch, uint32_t tokens,
                         const void* k, const void* v, uint32_t kv_stride, uint32_t dtype);

@@ -1415,3 +1415,57 @@ def test_captured_chunks_beside_single_tokens(ctx):
             want, off, mass = reference(qkv[at[s]:at[s + 1], :heads * hd].reshape(c, heads, hd), k, v, n[s] - c, UNL, 0, 0, 0.125)
             check(outs[0][at[s]:at[s + 1]].reshape(c, heads, hd), want, off, mass, "bf16")
     own.close()
+
+
+# ---------------------------------------------------------------------------------------------- launches of 2^32 threads
+
+def test_plain_kernel_beyond_one_row_of_workgroups(ctx):
+    """2^20 tokens of 16 heads, a workgroup each: every token sees itself alone, then two."""
+    n, heads, hd = 1 << 20, 16, 16
+    k = torch.zeros(n, heads * hd, device="cuda", dtype=torch.float16)
+    v = randn(gen_of(1), n, heads * hd, dtype="f16")
+    out = torch.zeros_like(v)
+    window(ctx, k, k, v, out, [n - 1000, 1000], heads, heads, hd, 0, 0, 0, "f16")
+    torch.cuda.synchronize()
+    plan_is(ctx, plain=1)
+    assert torch.equal(out, v)
+    window(ctx, k, k, v, out, [n - 1000, 1000], heads, heads, hd, 1, 0, 0, "f16")
+    torch.cuda.synchronize()
+    assert torch.equal(out[1:n - 1000], ((v[:n - 1001].float() + v[1:n - 1000].float()) / 2).half())
+    assert torch.equal(out[-999:], ((v[-1000:-1].float() + v[-999:].float()) / 2).half()) and torch.equal(out[[0, n - 1000]], v[[0, n - 1000]])
+
+
+def test_append_beyond_one_row_of_workgroups(ctx):
+    """More than 2^32 elements, one at a time: the last five tokens alone are a sequence's."""
+    kv, hd, n = 64, 250, 268436
+    x = torch.empty(n, kv * hd, device="cuda", dtype=torch.float16)
+    x[-5:] = randn(gen_of(2), 5, kv * hd, dtype="f16")
+    k, v = (torch.zeros(1, 2, kv, 16, hd, device="cuda", dtype=torch.float16) for _ in range(2))
+    cache = K.PagedCache.over(ctx, pimdl, k, v, ints(1, 0)[None].contiguous(), ints(18), torch.ones(2, dtype=torch.int32, device="cuda"))
+    cache.append(0, x, x, ints(n - 5, n))
+    torch.cuda.synchronize()
+    for pool in (k, v):
+        got = torch.cat([pool[0, 1], pool[0, 0]], 1).transpose(0, 1).reshape(32, -1)
+        assert torch.equal(got[13:18], x[-5:]) and (got[:13] == 0).all() and (got[18:] == 0).all()
+
+
+def test_more_sequences_than_a_launch_takes_are_refused(ctx):
+    """Two million sequences of one token, 8 heads: just below 2^32 threads each token has its own value, above the call is refused and nothing written."""
+    heads, hd = 8, 32
+    n = 1 << 21
+    k = torch.zeros(n, heads * hd, device="cuda", dtype=torch.bfloat16)
+    v = randn(gen_of(3), n, heads * hd, dtype="bf16")
+    out = torch.zeros_like(v)
+    starts = torch.arange(n + 1, device="cuda", dtype=torch.int32)
+
+    def run(count):
+        ctx.attention_window_ptr(k.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), starts.data_ptr(), count, count, heads, heads, hd, heads * hd, heads * hd,
+                                 heads * hd, UNL, UNL, 0, 1.0, pimdl.BF16)
+        torch.cuda.synchronize()
+
+    with pytest.raises(pimdl.PimdlError) as e:
+        run(n)
+    assert e.value.code == pimdl.ERR_UNSUPPORTED and (out == 0).all()
+    count = n - (1 << 15)
+    run(count)
+    assert torch.equal(out[:count], v[:count]) and (out[count:] == 0).all()
