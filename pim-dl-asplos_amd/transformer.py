@@ -179,7 +179,7 @@ class TransformerLayer:
         self.fused_gelu = fused_gelu
         self.own_attention = True  # head_dim 64: pimdl_attention; other head sizes use PyTorch's fused attention
         self._unlimited = pimdl.UNLIMITED
-        self._starts = {}  # sequences per batch -> first row of each, for pimdl_attention_window
+        self._starts = {}  # (sequences per batch, their length) -> first row of each, for pimdl_attention_window
         self.side = None if fused_qkv else side
         n = params.n
         self._max_tokens = n
@@ -241,11 +241,11 @@ class TransformerLayer:
     def _attend_window(self, q, k, v, a, B):
         """Attention in params.window within each of the B sequences of the batch."""
         p = self.params
-        starts = self._starts.get(B)
+        starts = self._starts.get((B, p.seq_len))
         if starts is None and self.torch.cuda.is_current_stream_capturing():
             starts = self.torch.arange(0, (B + 1) * p.seq_len, p.seq_len, device=q.device, dtype=self.torch.int32)  # (there from the replay on only)
         elif starts is None:  # copied from the host: there, on any stream, when the call returns
-            starts = self._starts[B] = self.torch.tensor(range(0, (B + 1) * p.seq_len, p.seq_len), device=q.device, dtype=self.torch.int32)
+            starts = self._starts[B, p.seq_len] = self.torch.tensor(range(0, (B + 1) * p.seq_len, p.seq_len), device=q.device, dtype=self.torch.int32)
         left, right, sinks = p.borders(self._unlimited)
         self.ctx.attention_window_ptr(q.data_ptr(), k.data_ptr(), v.data_ptr(), a.data_ptr(), starts.data_ptr(), B, B * p.seq_len, p.head_num,
                                       p.head_num, p.head_dim, q.stride(0), k.stride(0), p.token_dim, left, right, sinks,

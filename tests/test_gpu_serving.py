@@ -1469,3 +1469,19 @@ def test_more_sequences_than_a_launch_takes_are_refused(ctx):
     count = n - (1 << 15)
     run(count)
     assert torch.equal(out[:count], v[:count]) and (out[count:] == 0).all()
+
+
+def test_windowed_layer_after_another_sequence_length(ctx):
+    """As many sequences of another length: their first rows are others."""
+    model, p = _model(ctx, 64, 4, 1, 70, 3, (20, 5, 1), False)
+    for length in (70, 35, 70, 50):
+        p.seq_len = length
+        x, keep = randn(gen_of(length), 2 * length, p.token_dim), {}
+        model.layers[0].forward(x, keep)
+        torch.cuda.synchronize()
+        for b in range(2):
+            rows = slice(length * b, length * (b + 1))
+            q, k, v = (keep[n][rows].reshape(length, 4, 64) for n in "qkv")
+            want, off, mass = reference(q, k, v, 0, 20, 5, 1, 0.125)
+            check(keep["attn"][rows].reshape(length, 4, 64), want, off, mass, "f32")
+    model.close()
