@@ -549,15 +549,13 @@ struct Rows {
 // Results of keys that are split over workgroups: per split and row of the output (token, head) the sums, and the maximum m that they are relative
 // to, l, and c (1 where l is 0).  Joins take 2^(c (m - m')): of c m itself the rounding would be a factor of its own between large scores.
 struct Partial {
-    static constexpr uint32_t STATS = 3;
+    static constexpr uint32_t STATS = 4;  // (one load; the fourth is not used)
     float* o;      // [splits][rows][head_dim]
     float* stats;  // [splits][rows][STATS]
     uint64_t rows;
     __device__ __forceinline__ void put(uint64_t at, float m, float l, float c) const
     {
-        stats[STATS * at] = m;
-        stats[STATS * at + 1] = l;
-        stats[STATS * at + 2] = c;
+        *reinterpret_cast<f32x4*>(stats + STATS * at) = (f32x4){m, l, c, 0.0f};
     }
 };
 

@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
                                                              uint32_t wide_splits, uint32_t narrow_splits, uint32_t narrow_rows)
 {
     __shared__ float sums[256][4];
-    __shared__ float mls[256][attn::Partial::STATS];
+    __shared__ float mls[256][3];
     const uint32_t tid = threadIdx.x, lanes = a.head_dim / 4;
     const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, slot = rest / parts;
     const uint32_t b = by_row ? slot : attn::row_of_slot(a, slot, JOIN_ROWS);
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
                 for (uint32_t i = 0; i < AHEAD; ++i) {
                     const uint32_t s = s0 + i * groups < splits ? s0 + i * groups : splits - 1;
                     const uint64_t where = s * part.rows + at;
-                    const float* const stats = part.stats + attn::Partial::STATS * where;
+                    const attn::f32x4 stats = *reinterpret_cast<const attn::f32x4*>(part.stats + attn::Partial::STATS * where);
                     m[i] = stats[0];
                     lm[i] = s0 + i * groups < splits ? stats[1] : 0.0f;
                     c = lm[i] == 0.0f ? c : stats[2];
