@@ -546,16 +546,20 @@ struct Rows {
     __device__ __forceinline__ f32x4 quad(int d, int i) const { return (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}; }
 };
 
-// Results of keys that are split over workgroups: per split and row of the output (token, head) the sums, and the maximum m that they are relative
-// to, l, and c (1 where l is 0).  Joins take 2^(c (m - m')): of c m itself the rounding would be a factor of its own between large scores.
+// Results of keys that are split over workgroups: per split and row of the output (token, head) the sums, the maximum m that they are relative
+// to, and l; per row c, which the first split leaves.  Joins take 2^(c (m - m')): of c m itself the rounding would be a factor of its own between large
+// scores.
 struct Partial {
-    static constexpr uint32_t STATS = 4;  // (one load; the fourth is not used)
-    float* o;      // [splits][rows][head_dim]
-    float* stats;  // [splits][rows][STATS]
+    float* o;    // [splits][rows][head_dim]
+    float* ml;   // [splits][rows][2]
+    float* c;    // [rows]
     uint64_t rows;
-    __device__ __forceinline__ void put(uint64_t at, float m, float l, float c) const
+    __device__ __forceinline__ void put(uint32_t split, uint64_t row, float m, float l, float scale) const
     {
-        *reinterpret_cast<f32x4*>(stats + STATS * at) = (f32x4){m, l, c, 0.0f};
+        const uint64_t at = split * rows + row;
+        ml[2 * at] = m;
+        ml[2 * at + 1] = l;
+        if (split == 0) c[row] = scale;
     }
 };
 
@@ -712,8 +716,8 @@ __device__ __forceinline__ void wide_rows(const AttnArgs& a, uint32_t block, uin
             for (int i = 0; i < 4; ++i)
                 if (32 * d + 8 * i < C::HD) store4(out + 32 * d + 8 * i + 4 * h, w.quad(d, i) * inv);
     } else {
-        const uint64_t at = (uint64_t)split * part.rows + (uint64_t)token * a.heads + head;
-        if (h == 0) part.put(at, w.m, l, w.c);
+        const uint64_t to_row = (uint64_t)token * a.heads + head, at = split * part.rows + to_row;
+        if (h == 0) part.put(split, to_row, w.m, l, w.c);
         if (from >= to) return;  // (the joining kernel does not look at sums whose l is 0)
 #pragma unroll
         for (int d = 0; d < w.DT; ++d)
@@ -781,8 +785,7 @@ __device__ __forceinline__ void narrow_rows_of(const AttnArgs& a, uint32_t numbe
         if (splits > 1 && from >= to) {  // nothing left for this split
             if (tid < end - row0) {
                 const uint32_t row = row0 + tid;
-                const uint64_t at = (uint64_t)split * part.rows + (uint64_t)(r.first + row / a.group) * a.heads + kh * a.group + row % a.group;
-                part.put(at, -INF, 0.0f, 1.0f);
+                part.put(split, (uint64_t)(r.first + row / a.group) * a.heads + kh * a.group + row % a.group, -INF, 0.0f, 1.0f);
             }
             continue;
         }
@@ -860,9 +863,9 @@ __device__ __forceinline__ void narrow_rows_of(const AttnArgs& a, uint32_t numbe
             if (splits == 1) {
                 store4(static_cast<typename C::TQ*>(a.out) + (size_t)token * a.out_stride + (size_t)head * C::HD + col, sum == 0.0f ? (f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / sum));
             } else {
-                const uint64_t at = (uint64_t)split * part.rows + (uint64_t)token * a.heads + head;
-                if (col == 0) part.put(at, mx, sum, sh.c[row]);
-                store4(part.o + at * C::HD + col, y);
+                const uint64_t to_row = (uint64_t)token * a.heads + head;
+                if (col == 0) part.put(split, to_row, mx, sum, sh.c[row]);
+                store4(part.o + (split * part.rows + to_row) * C::HD + col, y);
             }
         }
         __syncthreads();

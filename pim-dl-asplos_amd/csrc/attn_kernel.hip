@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
                                                              uint32_t wide_splits, uint32_t narrow_splits, uint32_t narrow_rows)
 {
     __shared__ float sums[256][4];
-    __shared__ float mls[256][3];
+    __shared__ float mls[256][2];
     const uint32_t tid = threadIdx.x, lanes = a.head_dim / 4;
     const uint32_t kh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, slot = rest / parts;
     const uint32_t b = by_row ? slot : attn::row_of_slot(a, slot, JOIN_ROWS);
@@ -239,7 +239,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
         const bool works = mine < rows && row < stop;
         const uint32_t t = first + row / a.group, head = kh * a.group + row % a.group;
         const uint64_t at = (uint64_t)t * a.heads + head;
-        float top = -__builtin_inff(), l = 0.0f, c = 1.0f;  // c: of a split that has seen keys, the same in all of them
+        float top = -__builtin_inff(), l = 0.0f;
+        const float c = works ? part.c[at] : 1.0f;
         attn::f32x4 y = {0.f, 0.f, 0.f, 0.f};
         auto take = [&](auto count) __attribute__((always_inline)) {
             constexpr uint32_t AHEAD = decltype(count)::value;  // splits whose results are asked for together
@@ -250,10 +251,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
                 for (uint32_t i = 0; i < AHEAD; ++i) {
                     const uint32_t s = s0 + i * groups < splits ? s0 + i * groups : splits - 1;
                     const uint64_t where = s * part.rows + at;
-                    const attn::f32x4 stats = *reinterpret_cast<const attn::f32x4*>(part.stats + attn::Partial::STATS * where);
-                    m[i] = stats[0];
-                    lm[i] = s0 + i * groups < splits ? stats[1] : 0.0f;
-                    c = lm[i] == 0.0f ? c : stats[2];
+                    m[i] = part.ml[2 * where];
+                    lm[i] = s0 + i * groups < splits ? part.ml[2 * where + 1] : 0.0f;
                     x[i] = *reinterpret_cast<const attn::f32x4*>(part.o + where * a.head_dim + col);  // (anything where l is 0)
                 }
                 float up = top;
@@ -280,7 +279,6 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
         *reinterpret_cast<attn::f32x4*>(sums[tid]) = y;
         mls[tid][0] = top;
         mls[tid][1] = l;
-        mls[tid][2] = c;
         __syncthreads();
         if (works && g == 0) {
             for (uint32_t i = 1; i < groups; ++i) top = fmaxf(top, mls[tid + i * lanes][0]);
@@ -290,7 +288,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, attn::P
             for (uint32_t i = 0; i < groups; ++i) {
                 const float lm = mls[tid + i * lanes][1];
                 if (lm == 0.0f) continue;
-                const float f = __builtin_amdgcn_exp2f((mls[tid + i * lanes][0] - base) * mls[tid + i * lanes][2]);
+                const float f = __builtin_amdgcn_exp2f((mls[tid + i * lanes][0] - base) * c);
                 l += lm * f;
                 y += *reinterpret_cast<const attn::f32x4*>(sums[tid + i * lanes]) * f;
             }
@@ -370,7 +368,7 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     // heads, fp32 over fp16, 68 / 64 / 68; 64 sequences with 1 to 40 new tokens over up to 5000 174 / 192 / 199.
     if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
     // what the splits hand over is kept below 128 MiB
-    const uint64_t row_bytes = (uint64_t)(a.head_dim + attn::Partial::STATS) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
+    const uint64_t row_bytes = (uint64_t)(a.head_dim + 2) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
     p->narrow_splits = (uint32_t)std::min<uint64_t>(p->narrow_splits, most);
     p->wide_splits = (uint32_t)std::min<uint64_t>(p->wide_splits, most);
     const uint32_t splits = std::max(p->narrow_splits, p->wide_splits);
@@ -381,11 +379,12 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     if ((uint64_t)a.tokens * a.heads > 1u << 30 || !fits || !join_fits)
         return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
     if (splits > 1) {
-        int rc = ensure_scratch(ctx, &ctx->d_attn, &ctx->attn_bytes, row_bytes * splits, "attention's partial results");
+        int rc = ensure_scratch(ctx, &ctx->d_attn, &ctx->attn_bytes, row_bytes * splits + (uint64_t)a.tokens * a.heads * 4, "attention's partial results");
         if (rc) return rc;
         p->part.rows = (uint64_t)a.tokens * a.heads;
         p->part.o = reinterpret_cast<float*>(ctx->d_attn);
-        p->part.stats = p->part.o + p->part.rows * splits * a.head_dim;
+        p->part.ml = p->part.o + p->part.rows * splits * a.head_dim;
+        p->part.c = p->part.ml + p->part.rows * splits * 2;
     }
     return PIMDL_OK;
 }
