@@ -141,7 +141,7 @@ __device__ __forceinline__ float row_sum(float v)
 
 // Where the keys of a tile lie.  A tile begins at a multiple of 16, pages hold multiples of 16: a group of 16 keys has one base address.  The table's
 // entries are asked for a tile ahead, by a load of the vector memory like the keys', which return in order (a scalar load in flight makes
-// every wait for LDS a wait for all of LDS: 4 prompts of 4096 tokens 772 us with scalar loads, 673): lane i % GROUPS has group i's.
+// every wait for LDS a wait for all of LDS: 4 prompts of 4096 tokens 772 us with scalar loads, 673, shares being in one piece then; 860 in two): lane i % GROUPS has group i's.
 template <typename C, int TILE>
 struct Ahead {
     int32_t entry = 0;
@@ -597,9 +597,10 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Row& r, uint32_
 // ------------------------------------------------------------------------------------------------------------
 // Many rows: a workgroup takes 128 rows of a sequence and key head, its four waves 32 each, and all of them go through the same tiles of keys and
 // values in LDS.  The next tile is on its way in registers while one is worked on.  128 rows read keys and values once where 64 would twice; at 32 rows a
-// wave o, q, the scores and the tile to come are 168 to 256 registers, two waves per SIMD.  Bound by those two waves' latencies between products and exponentials:
-// 6 prompts of up to 4096 tokens, 32 heads over 8, window 1024, bf16, 314 us (matrix instructions 37 % of the SIMDs' cycles, others 39 %); whole sequences of 4096
-// 957 TFLOP/s; fp32, 6 documents, window 257 + 256, 170 us (46 and 47 %).
+// wave o, q, the scores and the tile to come are 168 to 256 registers, two waves per SIMD.  Bound by what those two waves leave uncovered between products and exponentials:
+// whole sequences of 4096 tokens, 32 heads over 8, bf16, 719 TFLOP/s (matrix instructions, a third of them for the second piece of p, 53 % of the SIMDs' cycles,
+// others 50 %); 6 prompts of up to 4096, window 1024, 404 us, 570 TFLOP/s (45 and 49 %): tiles at a window's two borders are taken whole, 1.11 times the keys that
+// are seen, and a block of 14.5 tiles on average waits for its first one; fp32, 6 documents, window 257 + 256, 170 to 176 us (45 and 46 %).
 // ------------------------------------------------------------------------------------------------------------
 constexpr uint32_t WIDE_ROWS = 128;
 
@@ -897,7 +898,7 @@ __global__ __launch_bounds__(NARROW_WAVES<C> * 64, C::NK == 1 && C::HD <= 64 ? 4
 
 // Blocks of 128 rows, and behind them, for those sequences of the batch that have few, blocks of 16: these wait for memory most of the time, those for
 // the matrix cores, so they share the device better than one launch after the other (16 sequences, half of them with one token: 245 us in two
-// launches, 214 in one).
+// launches, 214 in one, shares being in one piece then).
 template <typename C>
 __global__ __launch_bounds__(256, (C::NK == 3 && C::HD > 80) || (C::NQ > 1 && C::HD > 96) ? 1 : 2) void attention_wide_kernel(AttnArgs a, uint32_t wide_blocks, uint32_t slots, uint32_t splits,
                                                                                                          uint32_t narrow_splits, uint32_t narrow_rows, Partial part)

@@ -343,10 +343,11 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     const uint64_t wide_items = (rows + attn::WIDE_ROWS - 1) / attn::WIDE_ROWS * a.kv_heads;
     // So few blocks of 128 rows that most of the device would idle take blocks of 16, unless there are so many keys that every one of those fills
     // its CU anyway: 2^15 scores a CU.  us in blocks of 16 / 128: windows over 128 to 512 tokens, 12 heads, fp32 (12 / 24 / 36 / 48 blocks of 128)
-    // 6.7 / 12.1, 7.7 / 18.4, 16.1 / 25.2, 19.4 / 32.0, over 1024 (96) 44.9 / 37.6; 32 heads over 8, bf16, 256 and 512 tokens (64, 128) 12.8 / 11.7,
-    // 27.7 / 17.7.  New tokens of a paged cache, 32 heads over 8, at 2^13 scores a CU: 15.9 / 25.1 (16 over 4000 keys); 2^14: 18.4 / 26.9 (32),
-    // 14.3 / 24.4 (8 x 16 over 1000); 2^15: 23.8 / 28.9 (64), 34.8 / 37.7 (8 x 8); 2^16: 50.5 / 31.2 (128), 57.8 / 41.0 (8 x 16), 34.4 / 40.6 (32 over
-    // 16000); 2^17: 56.6 / 45.4 (64 over 16000), 95.3 / 50.9 (8 x 32).
+    // 6.6 / 12.2, 7.6 / 18.3, 15.9 / 25.1, 19.2 / 31.8, over 1024 (96) 44.4 / 38.4; 32 heads over 8, bf16, 256 and 512 tokens (64, 128) 12.4 / 13.4,
+    // 26.9 / 21.1.  New tokens of a paged cache, 32 heads over 8, at 2^13 scores a CU: 15.6 / 30.0 (16 over 4000 keys); 2^14: 17.9 / 31.5 (32),
+    // 14.3 / 29.1 (8 x 16 over 1000); 2^15: 22.8 / 34.1 (64), 34.6 / 40.3 (8 x 8); 2^16: 51.4 / 36.6 (128), 58.5 / 46.3 (8 x 16), 34.8 / 48.5 (32 over
+    // 16000); 2^17: 56.5 / 54.0 (64 over 16000), 95.5 / 56.0 (8 x 32).  Keys are counted by what a row of the table can hold, not by what it does: the
+    // lengths are on the device.
     const bool few = 16 * wide_items <= 3 * cus && (uint64_t)a.tokens * a.heads * keys <= cus << 15;
     p->narrow = a.paged || few;
     p->wide = !few && !(a.paged && a.tokens <= a.batch);
@@ -363,9 +364,11 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
         p->narrow_splits = (uint32_t)std::max<uint64_t>(1, keys <= 1024 ? 1 : 2 * items <= cus ? std::min<uint64_t>({(cus + items - 1) / items, keys / 256, 256})
                                                                         : std::min<uint64_t>((8 * cus + items - 1) / items, keys / 1024));
     }
-    // Two workgroups a CU, which is what registers leave room for.  us at 2 / 3 / 4: 10 chunks of 200 to 400 tokens over up to 4000 keys, 16 heads over
-    // 8, bf16, 145 / 137 / 137, of 300 to 600 187 / 189 / 189; one of 256 over 16000, 32 heads over 8, 108 / 128 / 117; two of 500 to 700 over 5000, 12
-    // heads, fp32 over fp16, 68 / 64 / 68; 64 sequences with 1 to 40 new tokens over up to 5000 174 / 192 / 199.
+    // About two workgroups a CU, rounded up: registers leave room for two, or for one in fp32 above 80 dims and fp32 over 16 bits above 96, which the rule
+    // does not look at.  us at 1 / 2 / 3 / 4: 10 chunks of 200 to 400 tokens over up to 4000 keys, 16 heads over 8, bf16, 189 / 180 / 165 / 165, of 300 to
+    // 600 235 / 235 / 231 / 231; one of 256 over 16000, 32 heads over 8, 171 / 137 / 158 / 143; two of 500 to 700 over 5000, 12 heads, fp32 over fp16,
+    // 70 / 70 / 66 / 70; 64 sequences with 1 to 40 new tokens over up to 5000 179 / 191 / 214 / 221; 16 with chunks of up to 512 or a token over up to 6000
+    // 214 / 224 / 225 / 236; three of 300 to 512 over up to 3000, 16 heads of 80, fp32, 144 / 118 / 125 / 124.
     if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
     // what the splits hand over is kept below 128 MiB
     const uint64_t row_bytes = (uint64_t)(a.head_dim + 2) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
