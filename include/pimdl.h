@@ -423,7 +423,62 @@ PIMDL_API int pimdl_cache_append(pimdl_ctx* ctx, const pimdl_paged_cache* cache,
                                  const int32_t* starts, uint32_t batch, uint32_t tokens, const void* k, const void* v,
                                  uint32_t kv_stride, uint32_t dtype);
 
-/* How the last pimdl_attention_window or pimdl_attention_paged of the context was launched, for tests and profiles: the choice goes by sizes alone, never
+/* ---- rotated positions ------------------------------------------------------------------------------
+ * Queries and keys turned by their positions, so that their products depend on distances: at position p the pair (a, b) of a head's columns that belongs to
+ * frequency f becomes (a cos pf - b sin pf, a sin pf + b cos pf).  The angle is a product in 64 bits, brought into a quarter turn there, so far positions
+ * lose nothing; sines, products and sums are fp32, rounded once to the output's type.  The reference's layer has no positions of its own
+ * (src/host/transformer_layer.cpp:263-625 takes features that hold them). */
+typedef enum pimdl_rotary_pairs {
+    PIMDL_PAIRS_HALVES = 0,     /* column i belongs with i + dims / 2 */
+    PIMDL_PAIRS_NEIGHBOURS = 1  /* column 2 i with 2 i + 1 */
+} pimdl_rotary_pairs;
+typedef struct pimdl_rotary {
+    const double* freqs;     /* DEVICE [dims / 2]: radians a position, finite */
+    uint32_t dims;           /* even, 2 .. head_dim: a head's columns from there on are left as they are */
+    uint32_t pairs;          /* pimdl_rotary_pairs */
+} pimdl_rotary;
+
+/* Queries and keys of a packed batch whose sequences start at position 0 (what comes before pimdl_attention or pimdl_attention_window).  Either
+ * may be left out (heads or kv_heads 0).  An output may be its input, with one stride for both, and overlap nothing else.  `depths` ([tokens], or NULL):
+ * position depths[t] for token t instead of its place in its sequence. */
+typedef struct pimdl_rotate_desc {
+    const void *q, *k;       /* [tokens][q_stride], [tokens][k_stride] */
+    void *q_out, *k_out;     /* [tokens][q_out_stride], [tokens][k_out_stride] */
+    const int32_t *starts, *depths;
+    uint32_t batch, tokens, heads, kv_heads, head_dim;
+    uint32_t q_stride, k_stride, q_out_stride, k_out_stride;
+    uint32_t dtype;          /* pimdl_dtype of all four */
+} pimdl_rotate_desc;
+PIMDL_API int pimdl_rotate(pimdl_ctx* ctx, const pimdl_rotary* rotary, const pimdl_rotate_desc* d);
+/* pimdl_cache_append with the keys turned on the way, by lengths[s] - n + i (the place of token i of the row's n), or, with `depths`,
+ * lengths[s] - n + depths[t] (a tree's tokens; they are stored at place i all the same).  Queries ([tokens][q_stride], of the same type) are turned along into q_out,
+ * which may be q with one stride for both; heads 0: none.  Queries are turned, by the numbers above, whether or not their keys have a place in the cache. */
+PIMDL_API int pimdl_cache_append_rotary(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const int32_t* seqs,
+                                        const int32_t* starts, uint32_t batch, uint32_t tokens, const void* k, const void* v,
+                                        uint32_t kv_stride, uint32_t dtype, const pimdl_rotary* rotary, const int32_t* depths,
+                                        const void* q, void* q_out, uint32_t heads, uint32_t q_stride, uint32_t q_out_stride);
+
+/* ---- trees of drafted tokens ------------------------------------------------------------------------
+ * A sequence's newest n tokens may be a tree of candidates instead of one continuation: node i (the row's i-th token, stored in the cache at place
+ * lengths[s] - n + i) follows node parents[i] < i of its row, or, with -1, what the cache held before.  Its position is lengths[s] - n + its depth.
+ * A parent that is neither -1 nor an earlier node counts as -1. */
+typedef struct pimdl_tree {
+    const uint32_t* masks;   /* [tokens][words]: bit j of row t: node j of t's row of the batch is t itself or one of its ancestors */
+    const int32_t* depths;   /* [tokens]: how many ancestors t has */
+    uint32_t words;          /* 1 .. 32: of a row; a row of the batch has up to 32 * words nodes */
+} pimdl_tree;
+/* Fills masks and depths from parents ([tokens]), once for all layers of a step.  A row of more than 32 * words nodes gets zeros: its
+ * tokens see what the cache held before and nothing of each other.  Rows of tokens of no sequence are left as they are. */
+PIMDL_API int pimdl_tree_build(pimdl_ctx* ctx, const int32_t* parents, const int32_t* starts, uint32_t batch, uint32_t tokens,
+                               uint32_t words, uint32_t* masks, int32_t* depths);
+/* pimdl_attention_paged for trees: node t at position p sees key j of those before the tree if j + left >= p or j < sinks, and of the tree
+ * itself and its ancestors those whose positions satisfy the same. */
+PIMDL_API int pimdl_attention_tree(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const int32_t* seqs,
+                                   const int32_t* starts, uint32_t batch, uint32_t tokens, const pimdl_tree* tree, const void* q,
+                                   void* out, uint32_t heads, uint32_t q_stride, uint32_t out_stride, uint32_t dtype,
+                                   uint32_t left, uint32_t sinks, float scale);
+
+/* How the last pimdl_attention_window, pimdl_attention_paged or pimdl_attention_tree of the context was launched, for tests and profiles: the choice goes by sizes alone, never
  * by what is in device memory. */
 typedef struct pimdl_attention_plan {
     uint32_t plain;          /* 1: the kernel of other head sizes; all else is 0 */
@@ -467,6 +522,16 @@ PIMDL_API int pimdl_pages_compact(pimdl_ctx* ctx, const pimdl_page_book* book);
 /* Copies page src[i] to page dst[i] in every pool (pairs out of range are left out); tables, lengths and refs are neither read nor
  * written and may be NULL.  No dst may be another pair's dst or src. */
 PIMDL_API int pimdl_pages_copy(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_t* src, const int32_t* dst, uint32_t n);
+
+/* Ends sequences behind the chosen branch of their trees: row b of the batch has its n nodes at the last n positions of sequence s = seqs[b] (b where
+ * seqs is NULL), and last[b] is the node that the branch ends with (-1: none is kept).  In every layer of every pool the rows of the branch's nodes, root
+ * first, move to the places from lengths[s] - n on, the sequence becomes lengths[s] - n + kept[b] long, and pages that it no longer needs are given back;
+ * kept[b] is the branch's length.  A row is left as it is, with kept[b] = -1, where last[b] is no node of it or lacks its own bit in the masks, where it has more
+ * nodes than the sequence has positions or the masks hold, where s is out of range or stands in the list before, where another sequence holds a page that would
+ * be written or left partly filled (a fork made while the tree was there), and while *lacking is not 0, since the tree is not in the cache then. */
+PIMDL_API int pimdl_pages_accept(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_t* seqs, const int32_t* starts,
+                                 uint32_t batch, uint32_t tokens, const pimdl_tree* tree, const int32_t* last, uint32_t row_bytes,
+                                 int32_t* kept);
 
 /* ---- introspection ---------------------------------------------------------------------------
  * No reference counterpart: figures a benchmark needs to place a kernel on its roofline. */

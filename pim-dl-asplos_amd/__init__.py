@@ -22,6 +22,7 @@ BIAS_ONCE, BIAS_TIMES_CB = 0, 1
 ACT_NONE, ACT_GELU_TANH = 0, 1
 F32, F16, BF16 = 0, 1, 2
 DTYPES = {"f32": F32, "f16": F16, "bf16": BF16}
+PAIRS = {"halves": 0, "neighbours": 1}  # of columns that turn together: i with i + dims / 2, or 2 i with 2 i + 1
 UNLIMITED = 0xFFFFFFFF  # of a window: no border on that side
 
 ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = -1, -2, -3
@@ -39,7 +40,8 @@ EXPORTS = ["pimdl_init", "pimdl_destroy", "pimdl_last_error", "pimdl_set_stream"
            "pimdl_amm_create_with", "pimdl_amm_set_tuning", "pimdl_amm_get_tuning", "pimdl_lutgen_mode",
            "pimdl_diag_mfma_error_crafted", "pimdl_amm_last_gather_kernel", "pimdl_amm_run_breakdown", "pimdl_diag_host_copy",
            "pimdl_attention_window", "pimdl_attention_paged", "pimdl_cache_append", "pimdl_pages_reserve", "pimdl_pages_fork",
-           "pimdl_pages_free", "pimdl_pages_compact", "pimdl_pages_copy", "pimdl_attention_last_plan"]
+           "pimdl_pages_free", "pimdl_pages_compact", "pimdl_pages_copy", "pimdl_attention_last_plan",
+           "pimdl_rotate", "pimdl_cache_append_rotary", "pimdl_tree_build", "pimdl_attention_tree", "pimdl_pages_accept"]
 NOALLOC_SCRATCH_BYTES = 8 << 20
 
 
@@ -116,6 +118,23 @@ class PageBook(ctypes.Structure):
                 [(n, ctypes.c_uint32) for n in ("seqs", "table_width", "pages", "page_tokens")] +
                 [("pools", ctypes.POINTER(ctypes.c_void_p)), ("pool_count", ctypes.c_uint32), ("layers", ctypes.c_uint32),
                  ("page_bytes", ctypes.c_uint64)])
+
+
+class RotaryDesc(ctypes.Structure):
+    """pimdl_rotary: which columns of a head are turned, and how far at each position"""
+    _fields_ = [("freqs", ctypes.c_void_p), ("dims", ctypes.c_uint32), ("pairs", ctypes.c_uint32)]
+
+
+class RotateDesc(ctypes.Structure):
+    """pimdl_rotate_desc"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "starts", "depths")] +
+                [(n, ctypes.c_uint32) for n in ("batch", "tokens", "heads", "kv_heads", "head_dim", "q_stride", "k_stride", "q_out_stride",
+                                                "k_out_stride", "dtype")])
+
+
+class TreeDesc(ctypes.Structure):
+    """pimdl_tree: what the nodes of trees of drafted tokens see of each other, and their depths"""
+    _fields_ = [("masks", ctypes.c_void_p), ("depths", ctypes.c_void_p), ("words", ctypes.c_uint32)]
 
 
 class AttentionPlan(ctypes.Structure):
@@ -195,6 +214,12 @@ def lib():
     L.pimdl_pages_free.argtypes = [vp, book, vp, u32]
     L.pimdl_pages_compact.argtypes = [vp, book]
     L.pimdl_pages_copy.argtypes = [vp, book, vp, vp, u32]
+    tree = ctypes.POINTER(TreeDesc)
+    L.pimdl_rotate.argtypes = [vp, ctypes.POINTER(RotaryDesc), ctypes.POINTER(RotateDesc)]
+    L.pimdl_cache_append_rotary.argtypes = ([vp, ctypes.POINTER(PagedCacheDesc), vp, vp, u32, u32, vp, vp, u32, u32, ctypes.POINTER(RotaryDesc), vp, vp, vp] + [u32] * 3)
+    L.pimdl_tree_build.argtypes = [vp, vp, vp, u32, u32, u32, vp, vp]
+    L.pimdl_attention_tree.argtypes = [vp, ctypes.POINTER(PagedCacheDesc), vp, vp, u32, u32, tree, vp, vp, u32, u32, u32, u32, u32, u32, ctypes.c_float]
+    L.pimdl_pages_accept.argtypes = [vp, book, vp, vp, u32, u32, tree, vp, u32, vp]
     L.pimdl_attention_last_plan.argtypes = [vp, ctypes.POINTER(AttentionPlan)]
     for name in EXPORTS:
         if name != "pimdl_last_error":

@@ -40,13 +40,13 @@ constexpr float INF = __builtin_inff();
 // rounds no differently, and o, 16 to 64 registers, is left alone.
 constexpr float RISE = 8.0f;
 
-// TQ: q and out; TK: keys and values
-template <typename TQ_, typename TK_, int HD_, bool PAGED_>
+// TQ: q and out; TK: keys and values; TREE: the new tokens are trees (pimdl_attention_tree)
+template <typename TQ_, typename TK_, int HD_, bool PAGED_, bool TREE_ = false>
 struct Config {
     typedef TQ_ TQ;
     typedef TK_ TK;
     static constexpr int HD = HD_;
-    static constexpr bool PAGED = PAGED_;
+    static constexpr bool PAGED = PAGED_, TREE = TREE_;
     static constexpr bool HALF = std::is_same<TK, _Float16>::value;  // the products' type: halves, or bf16
     static constexpr int NK = std::is_same<TK, float>::value ? 3 : 1;
     static constexpr int NQ = std::is_same<TQ, float>::value ? (HALF ? 2 : 3) : 1;
@@ -138,6 +138,47 @@ __device__ __forceinline__ float row_sum(float v)
     }
     return v;
 }
+
+// Trees of drafted tokens: which keys one row sees among those of its tree, the keys from r.pos0 on.  What lies before is not this one's to hide.
+struct Kin {
+    const uint32_t* mask;    // of the row's node
+    const int32_t* depths;   // of the tree's nodes
+    int32_t root, depth, words;
+    int64_t left, sinks;
+    bool cut;                // the window ends within the row's branch
+
+    __device__ __forceinline__ void begin(const AttnArgs& a, const Row& r, uint32_t token)
+    {
+        mask = a.masks + (size_t)(r.first + token) * a.words;
+        depths = a.depths + r.first;
+        root = r.pos0;
+        depth = depths[token];
+        words = (int32_t)a.words;
+        left = a.left;
+        sinks = a.sinks;
+        cut = (int64_t)depth > left;
+    }
+    __device__ __forceinline__ bool near(int32_t node) const { return depth - (int64_t)depths[node] <= left || root + (int64_t)depths[node] < sinks; }
+    __device__ __forceinline__ uint32_t word(int32_t i) const { return i < 0 ? ~0u : i < words ? mask[i] : 0u; }
+    // bit i: key0 + i is not hidden; of keys that the row's own is not before
+    __device__ __forceinline__ uint32_t sees32(int32_t key0, int32_t own) const
+    {
+        const int32_t at = key0 - root;
+        uint32_t bits = __builtin_amdgcn_alignbit(word((at >> 5) + 1), word(at >> 5), at & 31);
+        if (__any(cut)) {  // (rare)
+#pragma unroll 1
+            for (int32_t i = 0; i < 32; ++i)
+                if (cut && at + i >= 0 && at + i <= own && (bits >> i & 1) && !near(at + i)) bits &= ~(1u << i);
+        }
+        return bits;
+    }
+    __device__ __forceinline__ bool sees(int32_t key) const
+    {
+        const int32_t at = key - root;
+        return at < 0 || ((word(at >> 5) >> (at & 31) & 1) && (!cut || near(at)));
+    }
+};
+struct NoKin {};
 
 // Where the keys of a tile lie.  A tile begins at a multiple of 16, pages hold multiples of 16: a group of 16 keys has one base address.  The table's
 // entries are asked for a tile ahead, by a load of the vector memory like the keys', which return in order (a scalar load in flight makes
@@ -321,6 +362,7 @@ struct Rows {
     int32_t min_hi, max_hi, min_lo, max_lo;  // over the wave's rows
     float m, l;
     Acc o[DT];
+    typename std::conditional<C::TREE, Kin, NoKin>::type kin;
 
     static __device__ __forceinline__ uint32_t row() { return threadIdx.x % M; }
     static __device__ __forceinline__ uint32_t group() { return (threadIdx.x & 63) / M; }
@@ -377,7 +419,7 @@ struct Rows {
             const int64_t e = (int64_t)r.pos0 + t + a.right + 1;
             return (int32_t)(e < 0 ? 0 : e < r.length ? e : r.length);
         };
-        auto border_lo = [&](uint32_t t) {
+        auto border_lo = [&](int64_t t) {
             const int64_t e = (int64_t)r.pos0 + t - a.left;
             return (int32_t)(e < 0 ? 0 : e < 0x7fffffff ? e : 0x7fffffff);
         };
@@ -386,6 +428,13 @@ struct Rows {
         lo = border_lo(token);
         const uint32_t t0 = row0 / a.group, t1 = (row0 + 32 < rows ? row0 + 31 : rows - 1) / a.group;
         min_hi = border_hi(t0), max_hi = border_hi(t1), min_lo = border_lo(t0), max_lo = border_lo(t1);
+        if constexpr (C::TREE) {  // all of them see, in their windows, what was there before the tree, whose depths are between 0 and the last row's token
+            const int32_t root = r.pos0 > 0 ? r.pos0 : 0;
+            kin.begin(a, r, token);
+            lo = border_lo(kin.depth);
+            lo = lo < root ? lo : root;
+            min_hi = root, min_lo = border_lo(0), max_lo = max_lo < root ? max_lo : root;
+        }
         m = -INF;
         l = 0.0f;
 #pragma unroll
@@ -395,7 +444,13 @@ struct Rows {
     // keys key0 .. key0 + n - 1: whether some row sees some of them, whether every row sees all of them
     __device__ __forceinline__ bool some(int32_t key0, int32_t n) const { return key0 < max_hi && (key0 + n > min_lo || key0 < sinks); }
     __device__ __forceinline__ bool all(int32_t key0, int32_t n) const { return key0 + n <= min_hi && (key0 >= max_lo || key0 + n <= sinks); }
-    __device__ __forceinline__ bool sees(int32_t key) const { return key < hi && (key >= lo || key < sinks); }
+    __device__ __forceinline__ bool sees(int32_t key) const
+    {
+        if constexpr (C::TREE) {
+            if (key < hi && !kin.sees(key)) return false;
+        }
+        return key < hi && (key >= lo || key < sinks);
+    }
 
     // of a product of N and NK pieces those that reach the last bit of the larger count, small ones first
     template <int N>
@@ -440,6 +495,11 @@ struct Rows {
             const int32_t h = hi - k0;
 #pragma unroll
             for (int i = 0; i < REGS; ++i) s[i] = at(i) < h ? s[i] : -INF;
+            if constexpr (C::TREE) {
+                const uint32_t seen = kin.sees32(key0, hi - 1 - kin.root) >> (4 * group());
+#pragma unroll
+                for (int i = 0; i < REGS; ++i) s[i] = seen >> at(i) & 1 ? s[i] : -INF;
+            }
         }
         if (key0 < max_lo) {
             const int32_t f = lo - k0;
@@ -582,9 +642,10 @@ struct Span {
     __device__ __forceinline__ int32_t at(int32_t t) const { return t < sinks ? t : first + (t - sinks); }
 };
 
+template <bool TREE>
 __device__ __forceinline__ Span span_of(const AttnArgs& a, const Row& r, uint32_t row0, uint32_t row1, int32_t tile)
 {
-    const int64_t top = (int64_t)r.pos0 + row1 / a.group + a.right + 1, low = (int64_t)r.pos0 + row0 / a.group - a.left;
+    const int64_t top = (int64_t)r.pos0 + row1 / a.group + a.right + 1, low = (int64_t)r.pos0 + (TREE ? 0 : row0 / a.group) - a.left;
     const int32_t hi = (int32_t)(top < 0 ? 0 : top < r.length ? top : r.length), lo = (int32_t)(low < 0 ? 0 : low < hi ? low : hi);
     Span s;
     s.first = lo / tile;
@@ -650,7 +711,7 @@ __device__ __forceinline__ void wide_rows(const AttnArgs& a, uint32_t block, uin
     if (slot < before || row0 >= rows || rows <= narrow_rows) return;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = tid & 31, h = tid >> 5 & 1;
     const uint32_t end = row0 + WIDE_ROWS < rows ? row0 + WIDE_ROWS : rows, mine = row0 + 32 * wave;
-    const Span span = span_of(a, r, row0, end - 1, TILE);
+    const Span span = span_of<C::TREE>(a, r, row0, end - 1, TILE);
     const int32_t per = (span.total + (int32_t)splits - 1) / (int32_t)splits, from = per * (int32_t)split;
     const int32_t to = from + per < span.total ? from + per : span.total;
     const bool works = mine < end;
@@ -658,7 +719,7 @@ __device__ __forceinline__ void wide_rows(const AttnArgs& a, uint32_t block, uin
     w.begin(a, r, kh, works ? mine : row0, rows);
     // whether every row of the workgroup sees all of a tile
     const int32_t all_hi = [&] {
-        const int64_t e = (int64_t)r.pos0 + row0 / a.group + a.right + 1;
+        const int64_t e = C::TREE ? (int64_t)r.pos0 : (int64_t)r.pos0 + row0 / a.group + a.right + 1;
         return (int32_t)(e < 0 ? 0 : e < r.length ? e : r.length);
     }();
     const int64_t all_lo = (int64_t)r.pos0 + (end - 1) / a.group - a.left;
@@ -779,7 +840,7 @@ __device__ __forceinline__ void narrow_rows_of(const AttnArgs& a, uint32_t numbe
     char* const mine = lds + wave * W::WAVE;
     for (; block < blocks; ++block) {
         const uint32_t row0 = block * NARROW_ROWS, end = row0 + NARROW_ROWS < rows ? row0 + NARROW_ROWS : rows;
-        const Span span = span_of(a, r, row0, end - 1, 32);
+        const Span span = span_of<C::TREE>(a, r, row0, end - 1, 32);
         int32_t per = (span.total + (int32_t)splits - 1) / (int32_t)splits;
         if (per < WAVES) per = WAVES;  // a tile for each wave
         const int32_t from = per * (int32_t)split, to = from + per < span.total ? from + per : span.total;
@@ -927,15 +988,15 @@ int launch(Ctx* ctx, const AttnArgs& a, const Plan& p)
     return hip_check(ctx, hipGetLastError(), "attention_narrow_kernel launch");
 }
 
-template <typename TQ, typename TK, bool PAGED>
+template <typename TQ, typename TK, bool PAGED, bool TREE = false>
 int launch_heads(Ctx* ctx, const AttnArgs& a, const Plan& p)
 {
     switch (a.head_dim) {
-    case 32: return launch<Config<TQ, TK, 32, PAGED>>(ctx, a, p);
-    case 64: return launch<Config<TQ, TK, 64, PAGED>>(ctx, a, p);
-    case 80: return launch<Config<TQ, TK, 80, PAGED>>(ctx, a, p);
-    case 96: return launch<Config<TQ, TK, 96, PAGED>>(ctx, a, p);
-    default: return launch<Config<TQ, TK, 128, PAGED>>(ctx, a, p);
+    case 32: return launch<Config<TQ, TK, 32, PAGED, TREE>>(ctx, a, p);
+    case 64: return launch<Config<TQ, TK, 64, PAGED, TREE>>(ctx, a, p);
+    case 80: return launch<Config<TQ, TK, 80, PAGED, TREE>>(ctx, a, p);
+    case 96: return launch<Config<TQ, TK, 96, PAGED, TREE>>(ctx, a, p);
+    default: return launch<Config<TQ, TK, 128, PAGED, TREE>>(ctx, a, p);
     }
 }
 
@@ -945,6 +1006,11 @@ int launch_f32_f16(Ctx* ctx, const AttnArgs& a, const Plan& p);
 int launch_f32_bf16(Ctx* ctx, const AttnArgs& a, const Plan& p);
 int launch_f16(Ctx* ctx, const AttnArgs& a, const Plan& p);
 int launch_bf16(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_tree_f32(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_tree_f32_f16(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_tree_f32_bf16(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_tree_f16(Ctx* ctx, const AttnArgs& a, const Plan& p);
+int launch_tree_bf16(Ctx* ctx, const AttnArgs& a, const Plan& p);
 
 }  // namespace attn
 }  // namespace pimdl

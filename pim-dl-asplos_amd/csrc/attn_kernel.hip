@@ -32,7 +32,7 @@ __device__ __forceinline__ float wave_sum(float v)
 // L2), of 72 73 us, 48 37 us, 70 (elements of 2 bytes) 170 us; a window of 257 of 4 x 750 tokens, 12 heads of 72, fp32, 611 us, where matrix instructions
 // take 68 for 80.
 // ---------------------------------------------------------------------------------------------
-template <typename TQ, typename TK, bool PAGED, int N, int DIMS>
+template <typename TQ, typename TK, bool PAGED, bool TREE, int N, int DIMS>
 __global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kernel(AttnArgs a)
 {
     constexpr int CHUNKS = DIMS / (8 * N), BATCH = CHUNKS < 8 ? CHUNKS : 8, AHEAD = 8 / BATCH;  // loads of a row, and rows, under way together
@@ -69,7 +69,13 @@ __global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kern
     const int64_t pos = r.pos0 + (int64_t)(t - r.first);
     const int64_t hi64 = pos + (int64_t)a.right + 1;
     const int32_t hi = (int32_t)(hi64 < 0 ? 0 : hi64 < r.length ? hi64 : r.length);
-    const int64_t lo64 = pos - (int64_t)a.left;
+    typename std::conditional<TREE, attn::Kin, attn::NoKin>::type kin;
+    int64_t lo64 = pos - (int64_t)a.left;
+    if constexpr (TREE) {  // the window of what was there before the tree; the tree's own keys go by kin
+        kin.begin(a, r, t - r.first);
+        lo64 = (int64_t)r.pos0 + kin.depth - (int64_t)a.left;
+        lo64 = lo64 < r.pos0 ? lo64 : r.pos0;
+    }
     const int32_t lo = (int32_t)(lo64 < 0 ? 0 : lo64 < hi ? lo64 : hi);
     const int32_t sinks = a.sinks < (uint32_t)lo ? (int32_t)a.sinks : lo;
     // element offset of key j's row of this head, or -1 where its page does not exist
@@ -90,6 +96,9 @@ __global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kern
         for (int32_t j0 = from + 64 * (int32_t)wave; j0 < to; j0 += 256) {
             const int32_t j = j0 + (int32_t)(8 * e8 + j8);  // the lane's own key, whose place, score and p it holds
             int64_t at = j < to ? row_at(j) : -1;
+            if constexpr (TREE) {
+                if (j < to && !kin.sees(j)) at = -1;
+            }
             auto row = [&](int g) { return (int64_t)__shfl((int)(at >> 32), (int)(8 * j8) + g) << 32 | (uint32_t)__shfl((int)at, (int)(8 * j8) + g); };
             // chunks c0 .. c0 + BATCH - 1 of rows g0 .. g0 + AHEAD - 1, all asked for before the first is needed
             Bits x[AHEAD][BATCH];
@@ -190,15 +199,15 @@ __global__ __launch_bounds__(256, DIMS == 256 ? 2 : 3) void attention_plain_kern
     }
 }
 
-template <typename TQ, typename TK, bool PAGED, int N>
+template <typename TQ, typename TK, bool PAGED, bool TREE, int N>
 int launch_plain_of(Ctx* ctx, const AttnArgs& a)
 {
     const uint64_t items = ((uint64_t)a.tokens * a.kv_heads + 7) / 8 * 8 * a.group;
     if (items > 1u << 30) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "attention: too many rows for one launch");
     const dim3 grid = grid_of(items);
-    if (a.head_dim <= 64) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 64>), grid, dim3(256), 0, ctx->stream, a);
-    else if (a.head_dim <= 128) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 128>), grid, dim3(256), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, N, 256>), grid, dim3(256), 0, ctx->stream, a);
+    if (a.head_dim <= 64) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, TREE, N, 64>), grid, dim3(256), 0, ctx->stream, a);
+    else if (a.head_dim <= 128) hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, TREE, N, 128>), grid, dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((attention_plain_kernel<TQ, TK, PAGED, TREE, N, 256>), grid, dim3(256), 0, ctx->stream, a);
     return hip_check(ctx, hipGetLastError(), "attention_plain_kernel launch");
 }
 
@@ -207,8 +216,9 @@ int launch_plain(Ctx* ctx, const AttnArgs& a)
 {
     constexpr int N = 16 / sizeof(TK);
     const bool packs = a.head_dim % N == 0 && ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15) == 0 && (a.paged || a.kv_stride % N == 0);
-    if (a.paged) return packs ? launch_plain_of<TQ, TK, true, N>(ctx, a) : launch_plain_of<TQ, TK, true, 1>(ctx, a);
-    return packs ? launch_plain_of<TQ, TK, false, N>(ctx, a) : launch_plain_of<TQ, TK, false, 1>(ctx, a);
+    if (a.masks) return packs ? launch_plain_of<TQ, TK, true, true, N>(ctx, a) : launch_plain_of<TQ, TK, true, true, 1>(ctx, a);
+    if (a.paged) return packs ? launch_plain_of<TQ, TK, true, false, N>(ctx, a) : launch_plain_of<TQ, TK, true, false, 1>(ctx, a);
+    return packs ? launch_plain_of<TQ, TK, false, false, N>(ctx, a) : launch_plain_of<TQ, TK, false, false, 1>(ctx, a);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -339,7 +349,7 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     const uint64_t rows = (uint64_t)a.tokens * a.group, cus = (uint64_t)ctx->prop.multiProcessorCount;
     // keys that a row may see at most
     uint64_t keys = a.paged ? (uint64_t)a.table_width << a.page_shift : a.tokens;
-    keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + 1 + a.sinks + attn::WIDE_ROWS);
+    keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + 1 + a.sinks + attn::WIDE_ROWS + 32 * (uint64_t)a.words);
     const uint64_t wide_items = (rows + attn::WIDE_ROWS - 1) / attn::WIDE_ROWS * a.kv_heads;
     // So few blocks of 128 rows that most of the device would idle take blocks of 16, unless there are so many keys that every one of those fills
     // its CU anyway: 2^15 scores a CU.  us in blocks of 16 / 128: windows over 128 to 512 tokens, 12 heads, fp32 (12 / 24 / 36 / 48 blocks of 128)
@@ -410,11 +420,12 @@ int launch_attention(Ctx* ctx, const AttnArgs& a)
     int rc = make_plan(ctx, a, &p);
     if (rc) return rc;
     ctx->attn_plan = {0, p.wide, p.narrow, p.wide ? p.wide_splits : 0, p.narrow ? p.narrow_splits : 0, p.by_slot, 0};
-    if (a.dtype == PIMDL_BF16) rc = attn::launch_bf16(ctx, a, p);
-    else if (a.dtype == PIMDL_F16) rc = attn::launch_f16(ctx, a, p);
-    else if (a.cache_dtype == PIMDL_BF16) rc = attn::launch_f32_bf16(ctx, a, p);
-    else if (a.cache_dtype == PIMDL_F16) rc = attn::launch_f32_f16(ctx, a, p);
-    else rc = attn::launch_f32(ctx, a, p);
+    const bool tree = a.masks != nullptr;
+    if (a.dtype == PIMDL_BF16) rc = tree ? attn::launch_tree_bf16(ctx, a, p) : attn::launch_bf16(ctx, a, p);
+    else if (a.dtype == PIMDL_F16) rc = tree ? attn::launch_tree_f16(ctx, a, p) : attn::launch_f16(ctx, a, p);
+    else if (a.cache_dtype == PIMDL_BF16) rc = tree ? attn::launch_tree_f32_bf16(ctx, a, p) : attn::launch_f32_bf16(ctx, a, p);
+    else if (a.cache_dtype == PIMDL_F16) rc = tree ? attn::launch_tree_f32_f16(ctx, a, p) : attn::launch_f32_f16(ctx, a, p);
+    else rc = tree ? attn::launch_tree_f32(ctx, a, p) : attn::launch_f32(ctx, a, p);
     if (rc || (p.wide_splits == 1 && p.narrow_splits == 1)) return rc;
     if (a.dtype == PIMDL_BF16) return launch_join<__bf16>(ctx, a, p);
     if (a.dtype == PIMDL_F16) return launch_join<_Float16>(ctx, a, p);

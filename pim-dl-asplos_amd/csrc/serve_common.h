@@ -15,6 +15,26 @@ struct AttnArgs {
     uint32_t pages, page_shift, table_width, seq_count;  // paged only
     uint32_t dtype, cache_dtype, paged;
     float scale;
+    // of a tree of drafted tokens (masks null: there is none): see pimdl_tree
+    const uint32_t* masks;
+    const int32_t* depths;
+    uint32_t words;
+};
+
+// One call of pimdl_rotate or pimdl_cache_append_rotary, checked by the caller.
+struct RotaryArgs {
+    const double* freqs;
+    uint32_t dims, pairs;
+    const int32_t *starts, *depths;  // depths may be null
+    uint32_t batch, tokens, heads, kv_heads, head_dim;
+    const void *q, *k, *v;
+    void *q_out, *k_out;             // k_out: not paged
+    uint32_t q_stride, k_stride, q_out_stride, k_out_stride;  // k_stride: of v too
+    uint32_t dtype;
+    // paged only
+    const int32_t* seqs;             // may be null
+    pimdl_paged_cache cache;
+    uint32_t page_shift;
 };
 
 // A launch has fewer than 2^32 threads along x, so workgroups beyond GRID_X lie in rows of that many (a multiple of the XCDs that they are dealt out to).
@@ -25,6 +45,11 @@ inline dim3 grid_of(uint64_t blocks) { return blocks <= GRID_X ? dim3((uint32_t)
 int launch_attention(Ctx* ctx, const AttnArgs& a);
 int launch_cache_append(Ctx* ctx, const pimdl_paged_cache& c, const int32_t* seqs, const int32_t* starts, uint32_t batch, uint32_t tokens,
                         const void* k, const void* v, uint32_t kv_stride, uint32_t dtype);
+int launch_rotary(Ctx* ctx, const RotaryArgs& a, bool paged);
+int launch_tree_build(Ctx* ctx, const int32_t* parents, const int32_t* starts, uint32_t batch, uint32_t tokens, uint32_t words, uint32_t* masks,
+                      int32_t* depths);
+int launch_pages_accept(Ctx* ctx, const pimdl_page_book& b, const int32_t* seqs, const int32_t* starts, uint32_t batch, uint32_t tokens,
+                        const pimdl_tree& tree, const int32_t* last, uint32_t row_bytes, int32_t* kept);
 int launch_pages_reserve(Ctx* ctx, const pimdl_page_book& b, const int32_t* seqs, const int32_t* counts, uint32_t n);
 int launch_pages_fork(Ctx* ctx, const pimdl_page_book& b, const int32_t* parents, const int32_t* children, uint32_t n);
 int launch_pages_free(Ctx* ctx, const pimdl_page_book& b, const int32_t* seqs, uint32_t n);

@@ -9,6 +9,19 @@ call here waits for the GPU, and a step (reserve, then per layer append and atte
     for layer in ...:
         cache.append(layer, k, v, starts, seqs)      # the new tokens' keys and values, packed: row b owns starts[b] .. starts[b + 1] - 1
         cache.attend(layer, q, out, starts, heads, seqs)
+
+Rotated positions: a Rotary turns the keys on their way into the cache, and the queries along with them:
+
+    rotary = Rotary(ctx, pimdl, head_dim=64, base=10000.0)
+        cache.append(layer, k, v, starts, seqs, rotary=rotary, q=q, q_out=q)
+
+Drafts: the new tokens of a sequence may be a tree of candidates.  A step over them reserves room for all, and ends with the branch that the model agrees with:
+
+    tree = DraftTree(ctx, pimdl, tokens, most=64)    # room for so many tokens, in trees of up to 64
+    tree.build(parents, starts)                      # parents[t]: the node (of its own sequence's) that token t follows, -1: none
+        cache.append(layer, k, v, starts, seqs, rotary=rotary, q=q, q_out=q, tree=tree)
+        cache.attend(layer, q, out, starts, heads, seqs, tree=tree)
+    cache.accept(tree, last, kept, starts, seqs)     # last[b]: the node that the branch of row b ends with
 """
 import ctypes
 import math
@@ -17,6 +30,127 @@ import torch
 
 _TORCH = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 _CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _int_list(t, name):
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector")
+    return t.data_ptr(), t.shape[0]
+
+
+def _packed(t, columns, name):
+    """Address, row stride and type of a packed tensor; a column range of a wider one is fine."""
+    if t.dim() != 2 or t.shape[1] != columns or (t.shape[1] > 1 and t.stride(1) != 1) or t.dtype not in _CODES:
+        raise ValueError(f"{name} must be [tokens][{columns}] with unit column stride")
+    stride = t.stride(0) if t.shape[0] > 1 else columns  # (of a single row it says nothing)
+    if stride > 0xFFFFFFFF:
+        raise ValueError(f"{name}: a row stride of {stride} (up to 2^32 - 1)")
+    return t.data_ptr(), stride, _CODES[t.dtype]
+
+
+class Rotary:
+    """Turns queries and keys by their positions: at position p the pair (a, b) of a head's columns that belongs to frequency f becomes
+    (a cos pf - b sin pf, a sin pf + b cos pf).  The first `dims` columns of a head turn (all of them by default), column i with i + dims / 2 (pairs="halves") or 2 i with
+    2 i + 1 ("neighbours").  Frequency i is base^(-2 i / dims), or freqs[i] (float64 [dims / 2] on the device, radians a position): scaled ones for
+    longer contexts, say."""
+
+    def __init__(self, ctx, pimdl, head_dim, base=10000.0, dims=None, pairs="halves", freqs=None):
+        if pairs not in pimdl.PAIRS:
+            raise ValueError(f"pairs={pairs!r}: 'halves' or 'neighbours'")
+        if freqs is None:
+            dims = head_dim if dims is None else dims
+            if dims % 2 or not 2 <= dims <= head_dim:
+                raise ValueError(f"dims={dims} must be even, 2 .. head_dim={head_dim}")
+            if not (0 < base < math.inf):
+                raise ValueError(f"base={base} must be positive and finite")
+            freqs = torch.tensor([float(base) ** (-i / dims) for i in range(0, dims, 2)], dtype=torch.float64, device=torch.device("cuda", torch.cuda.current_device()))
+        if freqs.dim() != 1 or freqs.dtype != torch.float64 or not freqs.is_contiguous() or not 2 <= 2 * freqs.shape[0] <= head_dim:
+            raise ValueError(f"freqs must be a contiguous float64 vector of 1 to {head_dim // 2}")
+        if dims is not None and dims != 2 * freqs.shape[0]:
+            raise ValueError(f"{freqs.shape[0]} frequencies turn {2 * freqs.shape[0]} columns, not dims={dims}")
+        self.ctx, self.head_dim, self.dims, self.pairs, self.freqs = ctx, head_dim, 2 * freqs.shape[0], pairs, freqs
+        self._desc, self._rows = pimdl.RotaryDesc(freqs.data_ptr(), self.dims, pimdl.PAIRS[pairs]), pimdl.RotateDesc
+        self._lib = pimdl.lib()
+
+    def _heads(self, t, name):
+        if t.dim() != 2 or t.shape[1] % self.head_dim:
+            raise ValueError(f"{name} must be [tokens][heads * {self.head_dim}]")
+        return t.shape[1] // self.head_dim
+
+    def check_fits(self, cache):
+        """Refuses what PagedCache.append(..., rotary=self) could not do."""
+        if self.head_dim != cache.head_dim:
+            raise ValueError(f"a rotation of heads of {self.head_dim} over a cache of heads of {cache.head_dim}")
+
+    def rotate(self, q, k, q_out, k_out, starts, positions=None):
+        """Turns whole sequences, which begin at position 0: q, q_out [tokens][heads * head_dim] and k, k_out [tokens][kv_heads * head_dim], packed, sequence b
+        at rows starts[b] .. starts[b + 1] - 1.  An output may be its input.  `positions`: an int32 vector of the tokens' own positions instead."""
+        if q.shape != q_out.shape or k.shape != k_out.shape or q.shape[0] != k.shape[0]:
+            raise ValueError("q and q_out, and k and k_out, must have one shape, all four one number of rows")
+        if len({t.dtype for t in (q, k, q_out, k_out)}) != 1:
+            raise ValueError("q, k, q_out and k_out must have one type")
+        heads, kv_heads = self._heads(q, "q"), self._heads(k, "k")
+        qa, qs, dtype = _packed(q, q.shape[1], "q")
+        ka, ks, _ = _packed(k, k.shape[1], "k")
+        qo, qos, _ = _packed(q_out, q.shape[1], "q_out")
+        ko, kos, _ = _packed(k_out, k.shape[1], "k_out")
+        at, n = _int_list(starts, "starts")
+        if n < 1:
+            raise ValueError("starts must hold one number more than there are sequences")
+        pa = None
+        if positions is not None:
+            pa, m = _int_list(positions, "positions")
+            if m != q.shape[0]:
+                raise ValueError("positions must hold a number for each token")
+        d = self._rows(qa, ka, qo, ko, at, pa, n - 1, q.shape[0], heads, kv_heads, self.head_dim, qs, ks, qos, kos, dtype)
+        self.ctx._check(self._lib.pimdl_rotate(self.ctx._h, self._desc, d))
+
+
+class DraftTree:
+    """What the nodes of the trees of a batch see of each other: masks int32 [tokens][words] (bit j of row t: node j of t's sequence is t or one of
+    its ancestors) and depths int32 [tokens] (how many ancestors t has), for up to `tokens` tokens in trees of up to `most` nodes (1024)."""
+
+    def __init__(self, ctx, pimdl, tokens, most=64):
+        if tokens < 0 or not 1 <= most <= 1024:
+            raise ValueError(f"tokens={tokens} and most={most}: trees have 1 to 1024 nodes")
+        dev = torch.device("cuda", torch.cuda.current_device())
+        masks, depths = torch.zeros(tokens, -(-most // 32), device=dev, dtype=torch.int32), torch.zeros(tokens, device=dev, dtype=torch.int32)
+        # (see PagedCache: they are there when this returns)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(dev).synchronize()
+        self._bind(ctx, pimdl, masks, depths)
+
+    @classmethod
+    def over(cls, ctx, pimdl, masks, depths):
+        """Over tensors that exist already; they stay the caller's."""
+        self = cls.__new__(cls)
+        self._bind(ctx, pimdl, masks, depths)
+        return self
+
+    def _bind(self, ctx, pimdl, masks, depths):
+        if masks.dim() != 2 or depths.shape != masks.shape[:1] or masks.dtype != torch.int32 or depths.dtype != torch.int32:
+            raise ValueError("masks must be int32 [tokens][words], depths int32 [tokens]")
+        if not 1 <= masks.shape[1] <= 32:
+            raise ValueError(f"{masks.shape[1]} words: 1 to 32, of 32 nodes each")
+        if not masks.is_contiguous() or not depths.is_contiguous() or masks.device != depths.device:
+            raise ValueError("masks and depths must be contiguous and on one GPU")
+        self.ctx, self.masks, self.depths = ctx, masks, depths
+        self._lib, self._desc = pimdl.lib(), pimdl.TreeDesc(masks.data_ptr(), depths.data_ptr(), masks.shape[1])
+
+    def check_tokens(self, tokens):
+        """Refuses batches of more tokens than there is room for."""
+        if tokens > self.masks.shape[0]:
+            raise ValueError(f"{tokens} tokens: the tree has room for {self.masks.shape[0]}")
+
+    def build(self, parents, starts):
+        """Token t, the (t - starts[b])-th node of row b's tree, follows node parents[t] of that tree, or, with -1, what the sequence has in the cache; a parent stands before
+        its children.  A tree of more nodes than there are bits is left empty: its tokens see nothing of each other, not even themselves."""
+        pa, n = _int_list(parents, "parents")
+        at, m = _int_list(starts, "starts")
+        if m < 1:
+            raise ValueError("starts must hold one number more than there are sequences")
+        self.check_tokens(n)
+        self.ctx._check(self._lib.pimdl_tree_build(self.ctx._h, pa, at, m - 1, n, self._desc.words, self._desc.masks, self._desc.depths))
 
 
 class PagedCache:
@@ -60,31 +194,18 @@ class PagedCache:
         layer_bytes = k[0].numel() * k.element_size() if layers else 0
         self._layer = [pimdl.PagedCacheDesc(k.data_ptr() + i * layer_bytes, v.data_ptr() + i * layer_bytes, tables.data_ptr(), lengths.data_ptr(),
                                             self.lacking.data_ptr(), pages, page_tokens, kv_heads, head_dim, tables.shape[0], tables.shape[1], _CODES[k.dtype]) for i in range(layers)]
+        self._row_bytes = head_dim * k.element_size()
         self._pools = (ctypes.c_void_p * 2)(k.data_ptr(), v.data_ptr())
         self._book = pimdl.PageBook(tables.data_ptr(), lengths.data_ptr(), refs.data_ptr(), self.lacking.data_ptr(), tables.shape[0], tables.shape[1], pages,
                                     page_tokens, ctypes.cast(self._pools, ctypes.POINTER(ctypes.c_void_p)), 2, layers, layer_bytes // max(pages, 1))
 
-    def _list(self, t, name):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 vector")
-        return t.data_ptr(), t.shape[0]
-
-    def _rows(self, t, columns, name):
-        """Address, row stride and type of a packed tensor; a column range of a wider one is fine."""
-        if t.dim() != 2 or t.shape[1] != columns or (t.shape[1] > 1 and t.stride(1) != 1) or t.dtype not in _CODES:
-            raise ValueError(f"{name} must be [tokens][{columns}] with unit column stride")
-        stride = t.stride(0) if t.shape[0] > 1 else columns  # (of a single row it says nothing)
-        if stride > self._unlimited:
-            raise ValueError(f"{name}: a row stride of {stride} (up to 2^32 - 1)")
-        return t.data_ptr(), stride, _CODES[t.dtype]
-
     def _batch(self, starts, seqs):
-        at, n = self._list(starts, "starts")
+        at, n = _int_list(starts, "starts")
         if n < 1:
             raise ValueError("starts must hold one number more than there are sequences")
         if seqs is None:
             return None, at, n - 1
-        to, m = self._list(seqs, "seqs")
+        to, m = _int_list(seqs, "seqs")
         if m != n - 1:
             raise ValueError("starts must hold one number more than seqs")
         return to, at, m
@@ -100,50 +221,85 @@ class PagedCache:
         if seqs is None and batch > self.tables.shape[0]:
             raise ValueError(f"{batch} rows: the cache has {self.tables.shape[0]} sequences")
 
-    def append(self, layer, k, v, starts, seqs=None):
-        """New tokens' keys and values [tokens][kv_heads * head_dim] into the last positions of their sequences (whose room `reserve` has made)."""
+    def append(self, layer, k, v, starts, seqs=None, rotary=None, q=None, q_out=None, tree=None):
+        """New tokens' keys and values [tokens][kv_heads * head_dim] into the last positions of their sequences (whose room `reserve` has made).  With `rotary`
+        the keys are turned by those positions on the way, and queries q [tokens][heads * head_dim], if any, into q_out (which may be q); with `tree` by the
+        positions that their nodes have (the draft's first one, and the node's depth on top)."""
         if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
             raise ValueError("k and v must have one shape, stride and type")
-        ka, ks, kt = self._rows(k, self.kv_heads * self.head_dim, "k")
+        ka, ks, kt = _packed(k, self.kv_heads * self.head_dim, "k")
         to, at, batch = self._batch(starts, seqs)
+        if rotary is not None:
+            rotary.check_fits(self)
+            depths = None
+            if tree is not None:
+                tree.check_tokens(k.shape[0])
+                depths = tree._desc.depths
+            heads = qa = qo = qs = qos = 0
+            if q is not None:
+                if q_out is None or q.shape != q_out.shape or q.dtype != k.dtype or q_out.dtype != k.dtype or q.shape[:1] != k.shape[:1]:
+                    raise ValueError("q and q_out must have one shape, and k's type and number of rows")
+                heads = rotary._heads(q, "q")
+                qa, qs, _ = _packed(q, q.shape[1], "q")
+                qo, qos, _ = _packed(q_out, q.shape[1], "q_out")
+            self.ctx._check(self._lib.pimdl_cache_append_rotary(self.ctx._h, self._of(layer), to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt, rotary._desc, depths,
+                                                                qa, qo, heads, qs, qos))
+            return
+        if q is not None:
+            raise ValueError("queries are turned by a rotary: none is given")
         self.ctx._check(self._lib.pimdl_cache_append(self.ctx._h, self._of(layer), to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt))
 
-    def attend(self, layer, q, out, starts, heads, seqs=None, left=None, sinks=0, scale=None):
+    def attend(self, layer, q, out, starts, heads, seqs=None, left=None, sinks=0, scale=None, tree=None):
         """Causal attention of the new tokens (q, out: [tokens][heads * head_dim]) over everything that their sequences have in the cache, or, with
-        `left`, over the `left` positions before each of them and the first `sinks`."""
+        `left`, over the `left` positions before each of them and the first `sinks`.  With `tree` the new tokens of a sequence see what it had before, themselves and
+        their ancestors."""
         columns = heads * self.head_dim
         if q.shape != out.shape or q.dtype != out.dtype:
             raise ValueError("q and out must have one shape and type")
-        qa, qs, qt = self._rows(q, columns, "q")
-        oa, os_, _ = self._rows(out, columns, "out")
+        qa, qs, qt = _packed(q, columns, "q")
+        oa, os_, _ = _packed(out, columns, "out")
         left = self._unlimited if left is None else left
         if not (0 <= left <= self._unlimited and 0 <= sinks <= self._unlimited):
             raise ValueError(f"left={left} and sinks={sinks} must be counts of positions, below 2^32")
         to, at, batch = self._batch(starts, seqs)
-        self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, self._of(layer), to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt,
-                                                        left, sinks,
-                                                        1.0 / math.sqrt(self.head_dim) if scale is None else scale))
+        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
+        if tree is not None:
+            tree.check_tokens(q.shape[0])
+            self.ctx._check(self._lib.pimdl_attention_tree(self.ctx._h, self._of(layer), to, at, batch, q.shape[0], tree._desc, qa, oa, heads, qs, os_, qt, left, sinks, scale))
+            return
+        self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, self._of(layer), to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt, left, sinks, scale))
 
     def reserve(self, seqs, counts):
         """Makes sequence seqs[i] counts[i] positions longer (pages: the lowest free ones)."""
-        a, n = self._list(seqs, "seqs")
-        c, m = self._list(counts, "counts")
+        a, n = _int_list(seqs, "seqs")
+        c, m = _int_list(counts, "counts")
         if n != m:
             raise ValueError("seqs and counts must have one length")
         self.ctx._check(self._lib.pimdl_pages_reserve(self.ctx._h, self._book, a, c, n))
 
     def fork(self, parents, children):
         """Gives each empty sequence children[i] what parents[i] has: whole pages are shared, a partly filled last one is copied."""
-        a, n = self._list(parents, "parents")
-        c, m = self._list(children, "children")
+        a, n = _int_list(parents, "parents")
+        c, m = _int_list(children, "children")
         if n != m:
             raise ValueError("parents and children must have one length")
         self.ctx._check(self._lib.pimdl_pages_fork(self.ctx._h, self._book, a, c, n))
 
     def free(self, seqs):
         """Empties the sequences and gives their pages back."""
-        a, n = self._list(seqs, "seqs")
+        a, n = _int_list(seqs, "seqs")
         self.ctx._check(self._lib.pimdl_pages_free(self.ctx._h, self._book, a, n))
+
+    def accept(self, tree, last, kept, starts, seqs=None):
+        """Ends the sequences behind a branch of their trees: of row b, whose nodes are the newest starts[b + 1] - starts[b] positions, the nodes from the root to last[b]
+        (-1: none) move to the front of those positions, the others go, and their pages are free again.  kept[b]: how many stayed, -1 where the sequence has been
+        left as it was (last[b] is no node of it; it is listed twice; the last reserve lacked pages; a fork made meanwhile holds the draft's pages too)."""
+        to, at, batch = self._batch(starts, seqs)
+        la, n = _int_list(last, "last")
+        ka, m = _int_list(kept, "kept")
+        if n != batch or m != batch:
+            raise ValueError("last and kept must hold a number for each sequence of the batch")
+        self.ctx._check(self._lib.pimdl_pages_accept(self.ctx._h, self._book, to, at, batch, tree.masks.shape[0], tree._desc, la, self._row_bytes, ka))
 
     def compact(self):
         """Moves all pages in use to the front of the cache."""
@@ -151,8 +307,8 @@ class PagedCache:
 
     def copy(self, src, dst):
         """Copies page src[i] to page dst[i] in every layer."""
-        a, n = self._list(src, "src")
-        c, m = self._list(dst, "dst")
+        a, n = _int_list(src, "src")
+        c, m = _int_list(dst, "dst")
         if n != m:
             raise ValueError("src and dst must have one length")
         self.ctx._check(self._lib.pimdl_pages_copy(self.ctx._h, self._book, a, c, n))

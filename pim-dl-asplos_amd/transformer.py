@@ -65,6 +65,9 @@ class TransformerParams:
     # (left, right, sinks): a token sees `left` tokens before it, `right` behind it and the first `sinks` of its sequence (pimdl_attention_window);
     # left or right None: all of them.  None: every token sees every other, as in the reference
     window: tuple = None
+    # (base, dims, pairs): queries and keys are turned by their positions before they meet (kvcache.Rotary); dims None: all columns of a head.
+    # None: positions are in the features, as in the reference
+    rotary: tuple = None
 
     @property
     def n(self):
@@ -79,6 +82,14 @@ class TransformerParams:
             raise ValueError(f"window={self.window}: counts of positions, or None")
         return left, right, sinks
 
+    def turns(self):
+        """rotary as what kvcache.Rotary takes"""
+        base, dims, pairs = self.rotary
+        base, dims = float(base), self.head_dim if dims is None else operator.index(dims)
+        if not 0 < base < math.inf or dims % 2 or not 2 <= dims <= self.head_dim or pairs not in ("halves", "neighbours"):
+            raise ValueError(f"rotary={self.rotary}: a positive base, an even number of columns up to head_dim={self.head_dim}, and 'halves' or 'neighbours'")
+        return {"base": base, "dims": dims, "pairs": pairs}
+
     @classmethod
     def from_yaml(cls, path):
         import yaml
@@ -91,6 +102,9 @@ class TransformerParams:
             left, right, sinks = net["attention_window"]
             p.window = (None if left is None else int(left), None if right is None else int(right), int(sinks))
             p.borders()
+        if "rotary" in net:  # [base, dims, pairs]; dims null: all of a head
+            p.rotary = tuple(net["rotary"])
+            p.turns()
         if p.head_num * p.head_dim != p.token_dim:
             raise ValueError("head_num * head_dim != token_dim")
         dims = {"qkv": (p.token_dim, 3 * p.token_dim), "o": (p.token_dim, p.token_dim),
@@ -166,6 +180,7 @@ def load_npz(path, params):
 
 class TransformerLayer:
     """One encoder layer resident on the GPU: six LUT-AMM operators and two LayerNorms."""
+    rotary = None  # kvcache.Rotary of params.rotary
 
     def __init__(self, ctx, pimdl, weights, params, fused_qkv=False, side=None, fused_gelu=True):
         """fused_gelu: GELU is applied by the first feed-forward operator's own epilogue instead of a pass of
@@ -181,6 +196,12 @@ class TransformerLayer:
         self._unlimited = pimdl.UNLIMITED
         self._starts = {}  # (sequences per batch, their length) -> first row of each, for pimdl_attention_window
         self.side = None if fused_qkv else side
+        if params.rotary is not None:
+            try:
+                from .kvcache import Rotary
+            except ImportError:  # this file on its own (its command)
+                from pim_dl_asplos_amd.kvcache import Rotary
+            self.rotary = Rotary(ctx, pimdl, params.head_dim, **params.turns())
         n = params.n
         self._max_tokens = n
         self.amm = {}
@@ -238,21 +259,26 @@ class TransformerLayer:
                             residual.data_ptr(), y.data_ptr(), 1e-6)
         return y
 
-    def _attend_window(self, q, k, v, a, B):
-        """Attention in params.window within each of the B sequences of the batch."""
+    def _starts_of(self, q, B):
+        """First row of each of the B sequences of the batch, and the last one's end."""
         p = self.params
         starts = self._starts.get((B, p.seq_len))
         if starts is None and self.torch.cuda.is_current_stream_capturing():
             starts = self.torch.arange(0, (B + 1) * p.seq_len, p.seq_len, device=q.device, dtype=self.torch.int32)  # (there from the replay on only)
         elif starts is None:  # copied from the host: there, on any stream, when the call returns
             starts = self._starts[B, p.seq_len] = self.torch.tensor(range(0, (B + 1) * p.seq_len, p.seq_len), device=q.device, dtype=self.torch.int32)
+        return starts
+
+    def _attend_window(self, q, k, v, a, B):
+        """Attention in params.window within each of the B sequences of the batch."""
+        p, starts = self.params, self._starts_of(q, B)
         left, right, sinks = p.borders(self._unlimited)
         self.ctx.attention_window_ptr(q.data_ptr(), k.data_ptr(), v.data_ptr(), a.data_ptr(), starts.data_ptr(), B, B * p.seq_len, p.head_num,
                                       p.head_num, p.head_dim, q.stride(0), k.stride(0), p.token_dim, left, right, sinks,
                                       1.0 / math.sqrt(p.head_dim))
 
-    def check_cached(self, x, cache, layer, starts, seqs):
-        """Refuses what forward(x, cached=(cache, layer, starts, seqs)) could not do, before anything is written."""
+    def check_cached(self, x, cache, layer, starts, seqs, tree=None):
+        """Refuses what forward(x, cached=(cache, layer, starts, seqs, tree)) could not do, before anything is written."""
         p = self.params
         if not self.ctx.in_order_with(cache.ctx):
             raise ValueError("the cache's context runs on another stream than the layer's: nothing orders their calls")
@@ -269,6 +295,12 @@ class TransformerLayer:
         if x.shape[0] > self._max_tokens:
             raise ValueError(f"{x.shape[0]} tokens: the layer is built for {self._max_tokens}")
         cache.check_batch(starts, seqs)
+        if tree is not None:
+            tree.check_tokens(x.shape[0])
+            if not self.ctx.in_order_with(tree.ctx):
+                raise ValueError("the tree's context runs on another stream than the layer's: nothing orders their calls")
+            if tree.masks.device != cache.k.device:
+                raise ValueError("the tree must be on the cache's GPU")
         if any(t.device != cache.k.device for t in (x, starts, seqs) if t is not None):
             raise ValueError("x, starts and seqs must be on the cache's GPU")
 
@@ -276,7 +308,9 @@ class TransformerLayer:
         """x: float32 CUDA tensor [batch*seq][token_dim], row t = (batch t // seq_len, position t % seq_len).
         `keep`: optional dict that receives every intermediate (for stage-by-stage checks).
         `cached`: (PagedCache, layer, starts, seqs): x holds the newest tokens of those sequences instead (row b owns starts[b] ..
-        starts[b + 1] - 1, see kvcache.py); their keys and values go into the cache and they attend to what it holds, causally."""
+        starts[b + 1] - 1, see kvcache.py); their keys and values go into the cache and they attend to what it holds, causally, or, with a DraftTree as a
+        fifth, as the nodes of their trees.
+        With params.rotary `keep` has q and k as they meet: turned (k of a cached call: as it came, it is turned on its way into the cache)."""
         torch, p = self.torch, self.params
         n = x.shape[0]
         if cached is None and n % p.seq_len:
@@ -308,12 +342,18 @@ class TransformerLayer:
         else:
             q, k, v = self._run("q", x, n), self._run("k", x, n), self._run("v", x, n)
         att_scale = 1.0 / math.sqrt(p.token_dim / p.head_num)
+        if self.rotary is not None and cached is None:
+            self.rotary.rotate(q, k, q, k, self._starts_of(q, B))
         if cached is not None:
-            cache, layer, starts, seqs = cached
+            cache, layer, starts, seqs, *tree = cached
+            tree = tree[0] if tree else None
             a = torch.empty((n, p.token_dim), device=x.device, dtype=torch.float32)
             left, _, sinks = p.window or (None, 0, 0)
-            cache.append(layer, k, v, starts, seqs)
-            cache.attend(layer, q, a, starts, H, seqs, left=left, sinks=sinks)
+            if self.rotary is not None:
+                cache.append(layer, k, v, starts, seqs, rotary=self.rotary, q=q, q_out=q, tree=tree)
+            else:
+                cache.append(layer, k, v, starts, seqs)
+            cache.attend(layer, q, a, starts, H, seqs, left=left, sinks=sinks, tree=tree)
         elif p.window is not None:
             a = torch.empty((n, p.token_dim), device=x.device, dtype=torch.float32)
             self._attend_window(q, k, v, a, B)
@@ -378,20 +418,22 @@ class Transformer:
             x = layer.forward(x)
         return x
 
-    def extend(self, x, cache, starts, seqs, counts):
+    def extend(self, x, cache, starts, seqs, counts, tree=None):
         """The newest tokens of some sequences through the model (a chunk of a prompt, a single token, or both in one batch): x [tokens][token_dim]
         packed, row b of the batch is the counts[b] tokens starts[b] .. starts[b + 1] - 1 of sequence seqs[b] (int32 device tensors; seqs
         without repetitions).  The cache is one of the layers' context, or of one on its stream.  A call that
         cannot be done raises before the cache changes.  Makes room for them in the PagedCache, fills it layer by layer, and every token sees its sequence up to itself
         (params.window: with right = 0).  cache.lacking tells afterwards whether there were pages enough; if not, the outputs are those of the
-        tokens that the cache had before.  Rows of x behind the last sequence (a batch padded for a recorded step) come out undefined."""
+        tokens that the cache had before.  Rows of x behind the last sequence (a batch padded for a recorded step) come out undefined.
+        `tree`: a DraftTree that has been built over `starts`: the new tokens are candidates, each seeing what its sequence had before, its
+        ancestors and itself; cache.accept(tree, last, kept, starts, seqs) then keeps a branch of each."""
         for i, layer in enumerate(self.layers):
-            layer.check_cached(x, cache, i, starts, seqs)
+            layer.check_cached(x, cache, i, starts, seqs, tree)
         cache.reserve(seqs, counts)  # (which refuses lists that do not fit)
         if x.shape[0] == 0:
             return x
         for i, layer in enumerate(self.layers):
-            x = layer.forward(x, cached=(cache, i, starts, seqs))
+            x = layer.forward(x, cached=(cache, i, starts, seqs, tree))
         return x
 
     def capture(self, x):
