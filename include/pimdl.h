@@ -483,7 +483,7 @@ PIMDL_API int pimdl_attention_tree(pimdl_ctx* ctx, const pimdl_paged_cache* cach
 typedef struct pimdl_attention_plan {
     uint32_t plain;          /* 1: the kernel of other head sizes; all else is 0 */
     uint32_t wide, narrow;   /* 1: blocks of 128 rows; blocks of 16 rows (both: one launch for sequences of many and of few rows) */
-    uint32_t wide_splits, narrow_splits; /* workgroups that the keys of a block are split over */
+    uint32_t wide_splits, narrow_splits; /* workgroups that the keys of a block are split over (wide with 0: the blocks are dealt out evenly) */
     uint32_t by_slot;        /* narrow: a workgroup per block of 16 rows, not per row of the batch */
     uint32_t join;           /* 0: no splits to be joined; 1: of all blocks; 2: of the rows of the batch that have few rows */
 } pimdl_attention_plan;

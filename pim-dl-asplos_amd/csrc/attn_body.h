@@ -101,8 +101,11 @@ __device__ __forceinline__ void pieces(float x, float y, uint32_t* out)
         bf16x2 a = {(__bf16)x, (__bf16)y};
         out[0] = __builtin_bit_cast(uint32_t, a);
     } else if constexpr (N == 2) {
-        bf16x2 a = {(__bf16)x, (__bf16)y}, b = {(__bf16)(x - (float)a[0]), (__bf16)(y - (float)a[1])};
-        out[0] = __builtin_bit_cast(uint32_t, a);
+        bf16x2 a = {(__bf16)x, (__bf16)y};
+        uint32_t w = __builtin_bit_cast(uint32_t, a);
+        asm("" : "+v"(w));  // (or each half is converted once more, alone)
+        bf16x2 b = {(__bf16)(x - number(w << 16)), (__bf16)(y - number(w & 0xffff0000u))};
+        out[0] = w;
         out[1] = __builtin_bit_cast(uint32_t, b);
     } else {
         out[0] = high_halves(bits(x), bits(y));
@@ -199,6 +202,7 @@ struct Ahead {
 struct Place {
     int64_t base0, base1, base2, base3;  // bytes from k or v, of each group (not paged: base0, of the sequence)
     uint32_t there;
+    uint64_t of_lane;                    // paged: that of group lane % GROUPS
 };
 
 template <typename C, int TILE>
@@ -207,12 +211,14 @@ __device__ __forceinline__ Place place(const AttnArgs& a, const Row& r, uint32_t
     Place p;
     p.there = ~0u;
     p.base0 = p.base1 = p.base2 = p.base3 = 0;
+    p.of_lane = 0;
     if constexpr (C::PAGED) {
         // every lane for its own group, on the vector unit: a wave gets a scalar instruction through in four times the time
         const uint32_t page_bytes = (a.kv_heads << a.page_shift) * (uint32_t)C::RB, lane_group = threadIdx.x % (TILE / 16);
         const bool there = (uint32_t)ahead.entry < a.pages;  // (not -1)
         const uint32_t row = (kh << a.page_shift) + ((uint32_t)(key0 + 16 * (int32_t)lane_group) & ((1u << a.page_shift) - 1));
         const uint64_t base = (uint64_t)(there ? (uint32_t)ahead.entry : 0u) * page_bytes + row * (uint32_t)C::RB;
+        p.of_lane = base;
         p.there = (uint32_t)__ballot(there) | ~((1u << TILE / 16) - 1);
         auto of_group = [&](int g) {
             return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(base >> 32), g) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)base, g));
@@ -278,6 +284,23 @@ struct Stage {
 #pragma unroll
                 for (int u = 0; u < LOADS; ++u) load(u, (uint32_t)(r.length - 1 - key0));
             }
+        }
+    }
+    // The same for workgroups of any size: a load's group goes by the wave.
+    __device__ __forceinline__ void fetch_by_wave(const void* src, const AttnArgs& a, const Row& r, const Place& p, int32_t key0, uint32_t wave, uint32_t tid)
+    {
+        if constexpr (64 % C::PARTS == 0) {
+            const char* const s = static_cast<const char*>(src);
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) {
+                uint32_t row = (u * THREADS + wave * 64) / C::PARTS;
+                if (TOTAL % THREADS && row >= TILE) row = TILE - 64 / C::PARTS;  // (not stored)
+                const int g = (int)(row >> 4);
+                const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(p.of_lane >> 32), g) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)p.of_lane, g);
+                x[u] = *reinterpret_cast<const u32x4*>(s + base + (row & 15) * C::RB + (tid & 63) * 16);
+            }
+        } else {
+            fetch(src, a, r, p, key0, wave, tid);
         }
     }
     __device__ __forceinline__ void no_marks(uint8_t* marks, uint32_t tid)
@@ -519,13 +542,10 @@ struct Rows {
         }
     }
 
-    // The N scores that a lane holds become probabilities; o and l follow the maximum.
+    // m, o and l follow `mx`, the largest of a lane's N scores: probabilities are 2^(c s - what this returns).
     template <int N>
-    __device__ __forceinline__ void softmax(float* s)
+    __device__ __forceinline__ float follow(float* s, float mx)
     {
-        float mx = s[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
         mx = row_max<M>(mx);
         if (__any((mx - m) * c > RISE)) {
             const float up = (mx - m) * c > RISE ? mx : m;  // each row by its own scores: what others see must not round it differently
@@ -543,7 +563,17 @@ struct Rows {
             for (int i = 0; i < N; ++i) s[i] -= most;
             base = far ? 0.0f : base;
         }
-        base -= (float)C::P_SHIFT;
+        return base - (float)C::P_SHIFT;
+    }
+
+    // The N scores that a lane holds become probabilities; o and l follow the maximum.
+    template <int N>
+    __device__ __forceinline__ void softmax(float* s)
+    {
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
+        const float base = follow<N>(s, mx);
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base));
         float sum = 0.0f;
@@ -934,6 +964,16 @@ __device__ __forceinline__ void narrow_rows_of(const AttnArgs& a, uint32_t numbe
     }
 }
 
+// Workgroups of four waves with 32 rows each that share a CU, by their registers.
+template <typename C>
+constexpr uint32_t PER_CU = (C::NK == 3 && C::HD > 80) || (C::NQ > 1 && C::HD > 96) ? 1 : 2;
+
+}  // namespace attn
+}  // namespace pimdl
+#include "attn_deal.h"
+namespace pimdl {
+namespace attn {
+
 // What one call launches, decided by launch_attention.
 struct Plan {
     bool wide, narrow;
@@ -942,6 +982,9 @@ struct Plan {
     uint32_t narrow_rows;                 // rows of a sequence and key head up to which they are taken 16 at a time
     bool by_slot;                         // ... in workgroups of 16 rows each
     Partial part;
+    uint32_t deal;                        // shares that a tree's blocks are dealt out in (0: none of this)
+    uint32_t deal_rows;                   // rows of such a block
+    DealPart deal_part;
 };
 
 // Waves of a workgroup that takes 16 rows, alone in its launch: eight, where their LDS fits.  us with four / eight: one sequence of 777 keys, 12 heads, fp32 over
@@ -961,7 +1004,7 @@ __global__ __launch_bounds__(NARROW_WAVES<C> * 64, C::NK == 1 && C::HD <= 64 ? 4
 // the matrix cores, so they share the device better than one launch after the other (16 sequences, half of them with one token: 245 us in two
 // launches, 214 in one, shares being in one piece then).
 template <typename C>
-__global__ __launch_bounds__(256, (C::NK == 3 && C::HD > 80) || (C::NQ > 1 && C::HD > 96) ? 1 : 2) void attention_wide_kernel(AttnArgs a, uint32_t wide_blocks, uint32_t slots, uint32_t splits,
+__global__ __launch_bounds__(256, PER_CU<C>) void attention_wide_kernel(AttnArgs a, uint32_t wide_blocks, uint32_t slots, uint32_t splits,
                                                                                                          uint32_t narrow_splits, uint32_t narrow_rows, Partial part)
 {
     constexpr size_t WIDE = sizeof(typename Wide<C>::Shared), NARROW = C::PAGED ? sizeof(typename Narrow<C, 4>::Shared) : 0;
@@ -976,6 +1019,12 @@ __global__ __launch_bounds__(256, (C::NK == 3 && C::HD > 80) || (C::NQ > 1 && C:
 template <typename C>
 int launch(Ctx* ctx, const AttnArgs& a, const Plan& p)
 {
+    if constexpr (C::TREE) {
+        if (p.deal) {
+            hipLaunchKernelGGL((attention_deal_kernel<C>), dim3(p.deal), dim3(Deal<C>::THREADS), 0, ctx->stream, a, p.deal_part);
+            return hip_check(ctx, hipGetLastError(), "attention_deal_kernel launch");
+        }
+    }
     if (p.wide) {
         const uint32_t wide = p.slots * a.kv_heads * p.wide_splits, narrow = p.narrow ? a.batch * a.kv_heads * p.narrow_splits : 0;
         hipLaunchKernelGGL((attention_wide_kernel<C>), dim3(wide + narrow), dim3(256), 0, ctx->stream, a, wide, p.slots, p.wide_splits, p.narrow_splits,

@@ -330,6 +330,58 @@ int launch_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
     return hip_check(ctx, hipGetLastError(), "attention_join_kernel launch");
 }
 
+// ---------------------------------------------------------------------------------------------
+// Joins the shares of the blocks of an even deal (see attn_deal.h): workgroup (chunk, w) some rows of the block that begins in share w and goes on; head_dim / 4 threads of a row
+// take four columns each.
+// ---------------------------------------------------------------------------------------------
+template <typename TQ>
+__global__ __launch_bounds__(256) void attention_deal_join_kernel(AttnArgs a, attn::DealPart part, uint32_t block_rows)
+{
+    constexpr uint32_t AHEAD = 8;
+    const uint32_t tid = threadIdx.x, lanes = a.head_dim / 4, col = tid % lanes * 4, share = blockIdx.y, row = blockIdx.x * (256 / lanes) + tid / lanes;
+    const attn::u32x4 size = part.joins[2 * share], where = part.joins[2 * share + 1];
+    const uint32_t count = size[0];
+    if (row >= size[1] || tid / lanes >= 256 / lanes) return;
+    float top = -__builtin_inff(), l = 0.0f;
+    attn::f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s0 = 0; s0 < count; s0 += AHEAD) {
+        attn::f32x4 mlc[AHEAD], x[AHEAD];
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const uint32_t s = s0 + i < count ? s0 + i : count - 1;
+            const size_t at = (size_t)(s == 0 ? 2 * share + 1 : 2 * (share + s)) * block_rows + row;
+            mlc[i] = part.mlc[at];
+            x[i] = *reinterpret_cast<const attn::f32x4*>(part.o + at * a.head_dim + col);
+            if (s0 + i >= count) mlc[i][1] = 0.0f;
+        }
+        float up = top;
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) up = fmaxf(up, mlc[i][0]);
+        const float base = up == -__builtin_inff() ? 0.0f : up, c = mlc[0][2], alpha = __builtin_amdgcn_exp2f((top - base) * c);
+        top = up;
+        l *= alpha;
+        y *= alpha;
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const float f = __builtin_amdgcn_exp2f((mlc[i][0] - base) * c);
+            l += mlc[i][1] == 0.0f ? 0.0f : mlc[i][1] * f;  // (NaN is not)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] += mlc[i][1] == 0.0f ? 0.0f : x[i][e] * f;
+        }
+    }
+    const uint32_t of_seq = where[1] + row, token = where[0] + of_seq / a.group, head = where[2] * a.group + of_seq % a.group;
+    attn::store4(static_cast<TQ*>(a.out) + (size_t)token * a.out_stride + (size_t)head * a.head_dim + col, l == 0.0f ? (attn::f32x4){0.f, 0.f, 0.f, 0.f} : y * (1.0f / l));
+}
+
+template <typename TQ>
+int launch_deal_join(Ctx* ctx, const AttnArgs& a, const attn::Plan& p)
+{
+    ctx->attn_plan.join = 1;
+    const uint32_t rows = 256 / (a.head_dim / 4);
+    hipLaunchKernelGGL((attention_deal_join_kernel<TQ>), dim3((p.deal_rows + rows - 1) / rows, p.deal), dim3(256), 0, ctx->stream, a, p.deal_part, p.deal_rows);
+    return hip_check(ctx, hipGetLastError(), "attention_deal_join_kernel launch");
+}
+
 // Whether the matrix-core kernels take the call: head sizes that they are built for, rows of whole 16 bytes.
 bool matrix_form(const AttnArgs& a)
 {
@@ -380,6 +432,29 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     // 70 / 70 / 66 / 70; 64 sequences with 1 to 40 new tokens over up to 5000 179 / 191 / 214 / 221; 16 with chunks of up to 512 or a token over up to 6000
     // 214 / 224 / 225 / 236; three of 300 to 512 over up to 3000, 16 heads of 80, fp32, 144 / 118 / 125 / 124.
     if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
+    // Trees of more than 32 rows a sequence, on average, and 16 tiles of 64 keys a CU: an even deal over the device's CUs, where the units of any lengths fit in 32 bits.  us dealt / in
+    // blocks of 128 rows with equal splits, both with their joins: 32 sequences of 16 to 64 nodes over up to 8191 keys, 32 heads over 8, bf16, 251 / 333 (300 in four splits, the best), two of 36
+    // and 42 over 100 000 and 130 000, 16 heads over 2, fp16, 172 / 290; one of 16 over 64 000 66 / 123; four of 100 to 250 in a window of 1024, 16 heads of 80, fp32, whose tiles count
+    // four times, 68 / 81.  At 16 tiles a CU both take the same (8 of 16 or of 32 nodes over 4000 41 / 40, 49 / 49; 16 of 16 over 2000 45 / 45), below it the deal's own 20 us
+    // tell (one of 64 over 16 000 54 / 48; two of 128 over 2000 40 / 37), and few rows wait for memory in blocks of 16 (64 of 4 nodes over 2000 111 / 85; 32 of 8 over 1000 55 / 34).
+    const uint64_t tiles_a_cu = (rows / 256 + a.batch) * a.kv_heads * (keys / 64 + 1) * (a.cache_dtype == PIMDL_F32 ? 4 : 1) / cus;
+    if (a.masks && p->wide && a.batch <= attn::DEAL_BATCH && rows > 32ull * a.batch && tiles_a_cu >= 16) {
+        const bool alone = (a.cache_dtype == PIMDL_F32 && a.head_dim > 80) || (a.dtype == PIMDL_F32 && a.head_dim > 96);  // (as PER_CU)
+        const uint64_t block_rows = attn::deal_rows(alone), groups = rows / 32 + a.batch;  // (of 32 rows, at most)
+        const uint64_t most_units = groups * a.kv_heads * (3 * (((uint64_t)a.table_width << a.page_shift) / attn::deal_tile(a.cache_dtype == PIMDL_F32, a.head_dim) + 1) + attn::DEAL_BLOCK);
+        if (most_units < 1ull << 31) {
+            p->deal = (uint32_t)std::min<uint64_t>(cus, (most_units + attn::DEAL_LEAST - 1) / attn::DEAL_LEAST);
+            p->deal_rows = (uint32_t)block_rows;
+            p->narrow = false;
+            const uint64_t slots = 2ull * p->deal, slot_rows = slots * block_rows;
+            int rc = ensure_scratch(ctx, &ctx->d_attn, &ctx->attn_bytes, slot_rows * (a.head_dim + 4) * 4 + slots * 16, "attention's partial results");
+            if (rc) return rc;
+            p->deal_part.o = reinterpret_cast<float*>(ctx->d_attn);
+            p->deal_part.mlc = reinterpret_cast<attn::f32x4*>(p->deal_part.o + slot_rows * a.head_dim);
+            p->deal_part.joins = reinterpret_cast<attn::u32x4*>(p->deal_part.mlc + slot_rows);
+            return PIMDL_OK;
+        }
+    }
     // what the splits hand over is kept below 128 MiB
     const uint64_t row_bytes = (uint64_t)(a.head_dim + 2) * 4 * a.tokens * a.heads, most = std::max<uint64_t>(1, (128ull << 20) / row_bytes);
     p->narrow_splits = (uint32_t)std::min<uint64_t>(p->narrow_splits, most);
@@ -419,13 +494,18 @@ int launch_attention(Ctx* ctx, const AttnArgs& a)
     attn::Plan p;
     int rc = make_plan(ctx, a, &p);
     if (rc) return rc;
-    ctx->attn_plan = {0, p.wide, p.narrow, p.wide ? p.wide_splits : 0, p.narrow ? p.narrow_splits : 0, p.by_slot, 0};
+    ctx->attn_plan = {0, p.wide, p.narrow, p.wide && !p.deal ? p.wide_splits : 0, p.narrow ? p.narrow_splits : 0, p.by_slot, 0};
     const bool tree = a.masks != nullptr;
     if (a.dtype == PIMDL_BF16) rc = tree ? attn::launch_tree_bf16(ctx, a, p) : attn::launch_bf16(ctx, a, p);
     else if (a.dtype == PIMDL_F16) rc = tree ? attn::launch_tree_f16(ctx, a, p) : attn::launch_f16(ctx, a, p);
     else if (a.cache_dtype == PIMDL_BF16) rc = tree ? attn::launch_tree_f32_bf16(ctx, a, p) : attn::launch_f32_bf16(ctx, a, p);
     else if (a.cache_dtype == PIMDL_F16) rc = tree ? attn::launch_tree_f32_f16(ctx, a, p) : attn::launch_f32_f16(ctx, a, p);
     else rc = tree ? attn::launch_tree_f32(ctx, a, p) : attn::launch_f32(ctx, a, p);
+    if (rc == PIMDL_OK && p.deal) {
+        if (a.dtype == PIMDL_BF16) return launch_deal_join<__bf16>(ctx, a, p);
+        if (a.dtype == PIMDL_F16) return launch_deal_join<_Float16>(ctx, a, p);
+        return launch_deal_join<float>(ctx, a, p);
+    }
     if (rc || (p.wide_splits == 1 && p.narrow_splits == 1)) return rc;
     if (a.dtype == PIMDL_BF16) return launch_join<__bf16>(ctx, a, p);
     if (a.dtype == PIMDL_F16) return launch_join<_Float16>(ctx, a, p);

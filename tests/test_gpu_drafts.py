@@ -437,6 +437,44 @@ def test_large_trees_and_long_contexts(ctx, dtype, cache, hd):
     tree_case(ctx, 3, [16], [9000], 2, 2, hd, 16, dtype, cache, left=5000, sinks=4)
 
 
+# The plans that the sizes below have on 256 CUs; a rule that moves gets other sizes here, so that every way stays tested.
+DEALT = dict(plain=0, wide=1, narrow=0, wide_splits=0, join=1)
+
+
+def dealt(plan):
+    assert {k: plan[k] for k in DEALT} == DEALT, plan
+
+
+@pytest.mark.parametrize("n", [8, 9, 16, 17, 24, 31, 32, 33, 40, 41, 48, 49, 56, 64, 65, 80, 127, 128, 129, 192])
+def test_dealt_blocks_of_any_number_of_rows(ctx, n):
+    """1 to 8 groups of 32 rows, of which waves have whole tiles or halves, and several blocks; contexts that are cut over many shares, over few, and not at all."""
+    dealt(tree_case(ctx, n, [n, 70, n, 40, n], [40000, 9000, n + 1, 300, n], 8, 2, 128, 64, "bf16", "bf16"))
+    tree_case(ctx, n, [n, 3, n], [30000, 500, 8000 + n], 12, 3, 64, 16, "f32", "f16", left=9000, sinks=70, width=3)  # (fewer rows: blocks of 16)
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("hd", [32, 64, 80, 96, 128])
+@pytest.mark.parametrize("left,sinks", [(None, 0), (4000, 4)])
+def test_dealt_blocks_of_every_type_and_head_size(ctx, dtype, cache, hd, left, sinks):
+    dealt(tree_case(ctx, hd, [100, 20, 33, 0, 150, 1], [9000, 900, 5033, 70, 150, 3000], 16, 8, hd, 16, dtype, cache, left, sinks))
+
+
+def test_dealt_blocks_of_many_sequences(ctx):
+    """As many as a deal takes, and one more, whose blocks are split evenly."""
+    for batch in (512, 513):
+        plan = tree_case(ctx, batch, [2, 5] * (batch // 2) + [3] * (batch % 2), [40, 90] * (batch // 2 - 1) + [40, 600] + [60] * (batch % 2), 48, 4, 32, 16, "bf16", "bf16")
+        if batch == 512:
+            dealt(plan)
+        else:
+            assert plan["wide"] and plan["narrow"] and plan["wide_splits"] >= 1, plan
+
+
+def test_dealt_blocks_of_short_sequences(ctx):
+    """More blocks than shares, which are not cut, and rows that see nothing."""
+    dealt(tree_case(ctx, 7, [40, 64] * 30 + [1], [40, 100] * 30 + [3000], 8, 8, 64, 16, "f16", "f16"))
+    dealt(tree_case(ctx, 8, [40, 64] * 30 + [1], [17, 0] * 30 + [3000], 8, 8, 64, 16, "f16", "f16"))
+
+
 def test_more_words_than_nodes_change_nothing(ctx):
     for most in (40, 64, 65, 1024):
         tree_case(ctx, 5, [40, 3], [200, 300], 4, 2, 64, 16, "bf16", "bf16", most=most)
@@ -478,7 +516,7 @@ def test_a_chain_is_a_continuation(ctx, dtype, cache, hd, left, sinks):
 
 
 @pytest.mark.parametrize("dtype,cache", PAIRS)
-@pytest.mark.parametrize("hd,nodes", [(64, 40), (64, 300), (80, 40), (24, 40)])
+@pytest.mark.parametrize("hd,nodes", [(64, 40), (64, 300), (80, 40), (24, 40), (128, 1000)])
 def test_what_a_tree_hides_changes_nothing(ctx, dtype, cache, hd, nodes):
     """Infinities and NaN in the keys and values of a node reach its descendants and itself, and nobody else bit for bit; what lies behind a sequence reaches nobody."""
     lengths, heads = [100 + nodes], 4
