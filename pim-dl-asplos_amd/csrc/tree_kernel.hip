@@ -49,14 +49,18 @@ __global__ __launch_bounds__(WORDS < 2 ? 64 : WORDS * 32) void tree_build_kernel
             next[i] = to;
         }
     }
-    if (i >= n) return;
-    int32_t depth = -1;
+    if (i < n) {
+        int32_t depth = -1;
 #pragma unroll
-    for (int w = 0; w < WORDS; ++w) {
-        if ((uint32_t)w < words) masks[(uint64_t)(first + i) * words + w] = mine[w];
-        depth += __popc(mine[w]);
+        for (int w = 0; w < WORDS; ++w) depth += __popc(mine[w]);
+        depths[first + i] = depth;
     }
-    depths[first + i] = depth;
+    // out of LDS in the order of memory: a word of each lane's own mask would be 64 lines a store (64 trees of 512 nodes 10.4 us, this way 7.3)
+    uint32_t* const out = masks + (uint64_t)first * words;
+    for (uint32_t at = i; at < n * words; at += blockDim.x) {
+        const uint32_t node = words == WORDS ? at / WORDS : at / words;
+        out[at] = seen[node * PITCH + at - node * words];
+    }
 }
 
 template <int WORDS>
@@ -71,6 +75,8 @@ int launch_build(Ctx* ctx, const int32_t* parents, const int32_t* starts, uint32
 // The branch is the set bits of its last node's mask, in order; its j-th node moves to place j, which is never behind its own.  A thread of the first launch owns a
 // part of a row (of one head, layer and pool) and moves that of every node in order, ACCEPT_AHEAD of them asked for before the first is stored: none of them is a place
 // that has been written, as later nodes lie behind all places up to their own.
+// Memory bounds it: the branches of 64 trees in 12 layers, 8 heads of 128, bf16, 158 MB, take 47 us (3.4 TB/s; a plain copy reaches 4.8), 16 rows ahead 48; the book
+// 4 us.  One branch alone waits for memory five times in a row: 6.6 us.
 // ------------------------------------------------------------------------------------------------------------
 struct AcceptArgs {
     const int32_t *seqs, *starts, *last, *lengths, *refs, *lacking, *tables;
@@ -83,6 +89,7 @@ struct AcceptPools {
     uint32_t count, layers, runs, row_bytes;  // runs: of page_tokens rows in a page
     uint64_t page_bytes, layer_bytes;
 };
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));  // (an array of HIP's own uint4 would be in scratch)
 constexpr uint32_t ACCEPT_NODES = 1024, ACCEPT_AHEAD = 8;
 
 template <typename T>
@@ -160,8 +167,8 @@ __global__ __launch_bounds__(256) void pages_accept_kernel(AcceptArgs a, AcceptP
     for (uint32_t j = unmoved + tid; j < count; j += 256) {
         const int64_t f = byte_of(base + path[j]), t = byte_of(base + j);
         // (a row on no page is not there: what would move from it or to it stays)
-        from[j - unmoved] = f < 0 || t < 0 ? ~0ull : (uint64_t)f;
-        to[j - unmoved] = (uint64_t)t;
+        from[j - unmoved] = f < 0 || t < 0 ? 0 : (uint64_t)f;
+        to[j - unmoved] = f < 0 || t < 0 ? ~0ull : (uint64_t)t;
     }
     __syncthreads();
     if (blockIdx.x == 0 && tid == 0) a.kept[b] = wrong ? -1 : (int32_t)count;
@@ -173,13 +180,15 @@ __global__ __launch_bounds__(256) void pages_accept_kernel(AcceptArgs a, AcceptP
         const uint32_t part = (uint32_t)(c % parts), rest = (uint32_t)(c / parts), run = rest % pl.runs, slot = rest / pl.runs;
         char* const at = pl.at[slot / pl.layers] + (size_t)(slot % pl.layers) * pl.layer_bytes + run * run_bytes + (size_t)part * sizeof(T);
         for (uint32_t j0 = 0; j0 < rows; j0 += ACCEPT_AHEAD) {
-            T x[ACCEPT_AHEAD];
+            typename std::conditional<sizeof(T) < 4, uint32_t, T>::type x[ACCEPT_AHEAD];
 #pragma unroll
-            for (uint32_t j = 0; j < ACCEPT_AHEAD; ++j)
-                if (j0 + j < rows && from[j0 + j] != ~0ull) x[j] = *reinterpret_cast<const T*>(at + from[j0 + j]);
+            for (uint32_t j = 0; j < ACCEPT_AHEAD; ++j) x[j] = *reinterpret_cast<const T*>(at + from[j0 + j < rows ? j0 + j : rows - 1]);
 #pragma unroll
-            for (uint32_t j = 0; j < ACCEPT_AHEAD; ++j)
-                if (j0 + j < rows && from[j0 + j] != ~0ull) *reinterpret_cast<T*>(at + to[j0 + j]) = x[j];
+            for (uint32_t j = 0; j < ACCEPT_AHEAD; ++j) {
+                const uint64_t place = to[j0 + j < rows ? j0 + j : rows - 1];
+                asm("" : "+v"(x[j]));  // (or the compiler asks for it in the branch, behind all others)
+                if (j0 + j < rows && place != ~0ull) *reinterpret_cast<T*>(at + place) = (T)x[j];
+            }
         }
     }
 }
@@ -238,7 +247,7 @@ int launch_pages_accept(Ctx* ctx, const pimdl_page_book& b, const int32_t* seqs,
     pl.page_bytes = b.page_bytes, pl.layer_bytes = b.page_bytes * b.pages;
     for (uint32_t i = 0; i < b.pool_count; ++i) pl.at[i] = static_cast<char*>(b.pools[i]);
     int rc;
-    if (row_bytes % 16 == 0) rc = launch_accept<uint4>(ctx, a, pl);
+    if (row_bytes % 16 == 0) rc = launch_accept<u32x4>(ctx, a, pl);
     else if (row_bytes % 4 == 0) rc = launch_accept<uint32_t>(ctx, a, pl);
     else if (row_bytes % 2 == 0) rc = launch_accept<uint16_t>(ctx, a, pl);
     else rc = launch_accept<uint8_t>(ctx, a, pl);

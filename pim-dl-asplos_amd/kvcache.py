@@ -40,12 +40,13 @@ def _int_list(t, name):
 
 def _packed(t, columns, name):
     """Address, row stride and type of a packed tensor; a column range of a wider one is fine."""
-    if t.dim() != 2 or t.shape[1] != columns or (t.shape[1] > 1 and t.stride(1) != 1) or t.dtype not in _CODES:
+    shape, stride, dtype = t.shape, t.stride(), _CODES.get(t.dtype)
+    if len(shape) != 2 or shape[1] != columns or (columns > 1 and stride[1] != 1) or dtype is None:
         raise ValueError(f"{name} must be [tokens][{columns}] with unit column stride")
-    stride = t.stride(0) if t.shape[0] > 1 else columns  # (of a single row it says nothing)
+    stride = stride[0] if shape[0] > 1 else columns  # (of a single row it says nothing)
     if stride > 0xFFFFFFFF:
         raise ValueError(f"{name}: a row stride of {stride} (up to 2^32 - 1)")
-    return t.data_ptr(), stride, _CODES[t.dtype]
+    return t.data_ptr(), stride, dtype
 
 
 class Rotary:
@@ -72,10 +73,10 @@ class Rotary:
         self._desc, self._rows = pimdl.RotaryDesc(freqs.data_ptr(), self.dims, pimdl.PAIRS[pairs]), pimdl.RotateDesc
         self._lib = pimdl.lib()
 
-    def _heads(self, t, name):
-        if t.dim() != 2 or t.shape[1] % self.head_dim:
+    def _heads(self, shape, name):
+        if len(shape) != 2 or shape[1] % self.head_dim:
             raise ValueError(f"{name} must be [tokens][heads * {self.head_dim}]")
-        return t.shape[1] // self.head_dim
+        return shape[1] // self.head_dim
 
     def check_fits(self, cache):
         """Refuses what PagedCache.append(..., rotary=self) could not do."""
@@ -85,24 +86,25 @@ class Rotary:
     def rotate(self, q, k, q_out, k_out, starts, positions=None):
         """Turns whole sequences, which begin at position 0: q, q_out [tokens][heads * head_dim] and k, k_out [tokens][kv_heads * head_dim], packed, sequence b
         at rows starts[b] .. starts[b + 1] - 1.  An output may be its input.  `positions`: an int32 vector of the tokens' own positions instead."""
-        if q.shape != q_out.shape or k.shape != k_out.shape or q.shape[0] != k.shape[0]:
+        q_shape, k_shape = q.shape, k.shape
+        if q_shape != q_out.shape or k_shape != k_out.shape or q_shape[0] != k_shape[0]:
             raise ValueError("q and q_out, and k and k_out, must have one shape, all four one number of rows")
-        if len({t.dtype for t in (q, k, q_out, k_out)}) != 1:
+        if not q.dtype == k.dtype == q_out.dtype == k_out.dtype:
             raise ValueError("q, k, q_out and k_out must have one type")
-        heads, kv_heads = self._heads(q, "q"), self._heads(k, "k")
-        qa, qs, dtype = _packed(q, q.shape[1], "q")
-        ka, ks, _ = _packed(k, k.shape[1], "k")
-        qo, qos, _ = _packed(q_out, q.shape[1], "q_out")
-        ko, kos, _ = _packed(k_out, k.shape[1], "k_out")
+        heads, kv_heads, tokens = self._heads(q_shape, "q"), self._heads(k_shape, "k"), q_shape[0]
+        qa, qs, dtype = _packed(q, q_shape[1], "q")
+        ka, ks, _ = _packed(k, k_shape[1], "k")
+        qo, qos, _ = _packed(q_out, q_shape[1], "q_out")
+        ko, kos, _ = _packed(k_out, k_shape[1], "k_out")
         at, n = _int_list(starts, "starts")
         if n < 1:
             raise ValueError("starts must hold one number more than there are sequences")
         pa = None
         if positions is not None:
             pa, m = _int_list(positions, "positions")
-            if m != q.shape[0]:
+            if m != tokens:
                 raise ValueError("positions must hold a number for each token")
-        d = self._rows(qa, ka, qo, ko, at, pa, n - 1, q.shape[0], heads, kv_heads, self.head_dim, qs, ks, qos, kos, dtype)
+        d = self._rows(qa, ka, qo, ko, at, pa, n - 1, tokens, heads, kv_heads, self.head_dim, qs, ks, qos, kos, dtype)
         self.ctx._check(self._lib.pimdl_rotate(self.ctx._h, self._desc, d))
 
 
@@ -239,9 +241,9 @@ class PagedCache:
             if q is not None:
                 if q_out is None or q.shape != q_out.shape or q.dtype != k.dtype or q_out.dtype != k.dtype or q.shape[:1] != k.shape[:1]:
                     raise ValueError("q and q_out must have one shape, and k's type and number of rows")
-                heads = rotary._heads(q, "q")
-                qa, qs, _ = _packed(q, q.shape[1], "q")
-                qo, qos, _ = _packed(q_out, q.shape[1], "q_out")
+                heads = rotary._heads(q.shape, "q")
+                qa, qs, _ = _packed(q, heads * self.head_dim, "q")
+                qo, qos, _ = _packed(q_out, heads * self.head_dim, "q_out")
             self.ctx._check(self._lib.pimdl_cache_append_rotary(self.ctx._h, self._of(layer), to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt, rotary._desc, depths,
                                                                 qa, qo, heads, qs, qos))
             return
