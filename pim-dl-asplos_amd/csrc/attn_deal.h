@@ -104,6 +104,14 @@ __device__ __forceinline__ DealRow deal_row(const AttnArgs& a, const Row& r)
     return d;
 }
 
+// Sums of units end at 2^31 - 1, which the host makes sure that rows with tokens of their own do not reach: starts that fall again, so that rows share tokens, could, and
+// the last rows get nothing then.
+__device__ __forceinline__ uint32_t add_units(uint32_t x, uint32_t y)
+{
+    const uint32_t sum = x + y;
+    return sum < 0x7fffffffu ? sum : 0x7fffffffu;
+}
+
 // Looks at every row of the batch (up to DEAL_BATCH, a thread each); returns all units.
 template <typename C>
 __device__ __forceinline__ uint32_t deal_units(const AttnArgs& a, typename Deal<C>::Shared& sh)
@@ -123,27 +131,28 @@ __device__ __forceinline__ uint32_t deal_units(const AttnArgs& a, typename Deal<
             sh.length[b] = r.length;
             mine[i] = deal_row<C>(a, r).units() * a.kv_heads;
         }
-        sum += mine[i];
+        sum = add_units(sum, mine[i]);
     }
     uint32_t x = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t y = __shfl_up(x, o);
-        if (lane >= (uint32_t)o) x += y;
+        if (lane >= (uint32_t)o) x = add_units(x, y);
     }
     if (lane == 63) sh.tmp[wave] = x;
     __syncthreads();
-    uint32_t before = x - sum, total = 0;
+    uint32_t before = __shfl_up(x, 1), total = 0;
+    if (lane == 0) before = 0;
 #pragma unroll
     for (uint32_t i = 0; i < D::WAVES; ++i) {
-        if (i < wave) before += sh.tmp[i];
-        total += sh.tmp[i];
+        if (i < wave) before = add_units(before, sh.tmp[i]);
+        total = add_units(total, sh.tmp[i]);
     }
 #pragma unroll
     for (uint32_t i = 0; i < EACH; ++i) {
         const uint32_t b = tid * EACH + i;
         if (b < a.batch) sh.unit[b] = before;
-        before += mine[i];
+        before = add_units(before, mine[i]);
     }
     if (tid == 0) sh.unit[a.batch] = total;
     __syncthreads();

@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256) void attention_deal_join_kernel(AttnArgs a, at
     constexpr uint32_t AHEAD = 8;
     const uint32_t tid = threadIdx.x, lanes = a.head_dim / 4, col = tid % lanes * 4, share = blockIdx.y, row = blockIdx.x * (256 / lanes) + tid / lanes;
     const attn::u32x4 size = part.joins[2 * share], where = part.joins[2 * share + 1];
-    const uint32_t count = size[0];
+    const uint32_t count = __builtin_amdgcn_readfirstlane(size[0]);
     if (row >= size[1] || tid / lanes >= 256 / lanes) return;
     float top = -__builtin_inff(), l = 0.0f;
     attn::f32x4 y = {0.f, 0.f, 0.f, 0.f};
@@ -348,11 +348,12 @@ __global__ __launch_bounds__(256) void attention_deal_join_kernel(AttnArgs a, at
         attn::f32x4 mlc[AHEAD], x[AHEAD];
 #pragma unroll
         for (uint32_t i = 0; i < AHEAD; ++i) {
-            const uint32_t s = s0 + i < count ? s0 + i : count - 1;
+            mlc[i] = x[i] = (attn::f32x4){-__builtin_inff(), 0.0f, 0.0f, 0.0f};
+            if (s0 + i >= count) continue;
+            const uint32_t s = s0 + i;
             const size_t at = (size_t)(s == 0 ? 2 * share + 1 : 2 * (share + s)) * block_rows + row;
             mlc[i] = part.mlc[at];
             x[i] = *reinterpret_cast<const attn::f32x4*>(part.o + at * a.head_dim + col);
-            if (s0 + i >= count) mlc[i][1] = 0.0f;
         }
         float up = top;
 #pragma unroll
