@@ -452,7 +452,7 @@ typedef struct pimdl_rotate_desc {
 PIMDL_API int pimdl_rotate(pimdl_ctx* ctx, const pimdl_rotary* rotary, const pimdl_rotate_desc* d);
 /* pimdl_cache_append with the keys turned on the way, by lengths[s] - n + i (the place of token i of the row's n), or, with `depths`,
  * lengths[s] - n + depths[t] (a tree's tokens; they are stored at place i all the same).  Queries ([tokens][q_stride], of the same type) are turned along into q_out,
- * which may be q with one stride for both; heads 0: none.  Queries are turned, by the numbers above, whether or not their keys have a place in the cache. */
+ * which may be q with one stride for both and overlaps nothing else; heads 0: none.  Queries are turned, by the numbers above, whether or not their keys have a place in the cache. */
 PIMDL_API int pimdl_cache_append_rotary(pimdl_ctx* ctx, const pimdl_paged_cache* cache, const int32_t* seqs,
                                         const int32_t* starts, uint32_t batch, uint32_t tokens, const void* k, const void* v,
                                         uint32_t kv_stride, uint32_t dtype, const pimdl_rotary* rotary, const int32_t* depths,
@@ -528,7 +528,8 @@ PIMDL_API int pimdl_pages_copy(pimdl_ctx* ctx, const pimdl_page_book* book, cons
  * first, move to the places from lengths[s] - n on, the sequence becomes lengths[s] - n + kept[b] long, and pages that it no longer needs are given back;
  * kept[b] is the branch's length.  A row is left as it is, with kept[b] = -1, where last[b] is no node of it or lacks its own bit in the masks, where it has more
  * nodes than the sequence has positions or the masks hold, where s is out of range or stands in the list before, where another sequence holds a page that would
- * be written or left partly filled (a fork made while the tree was there), and while *lacking is not 0, since the tree is not in the cache then. */
+ * be written or left partly filled (a fork made while the tree was there), and while *lacking is not 0, since the tree is not in the cache then.  kept overlaps none of the
+ * inputs. */
 PIMDL_API int pimdl_pages_accept(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_t* seqs, const int32_t* starts,
                                  uint32_t batch, uint32_t tokens, const pimdl_tree* tree, const int32_t* last, uint32_t row_bytes,
                                  int32_t* kept);

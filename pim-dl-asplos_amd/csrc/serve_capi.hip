@@ -380,6 +380,9 @@ int pimdl_pages_accept(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_
     if ((rc = check_batch(ctx, fn, starts, batch, tokens)) || (seqs && (rc = check_device(ctx, fn, "seqs", seqs, 4))) ||
         (rc = check_device(ctx, fn, "masks", tree->masks, 4)) || (rc = check_device(ctx, fn, "last", last, 4)) || (rc = check_device(ctx, fn, "kept", kept, 4)))
         return rc;
+    // several workgroups read a row's numbers, and the first to be done writes kept
+    for (const int32_t* in : {last, seqs, starts})
+        if (in && kept < in + batch + (in == starts) && in < kept + batch) return set_error(ctx, PIMDL_ERR_INVALID, "%s: kept must not overlap last, seqs or starts", fn);
     if ((rc = activate(ctx))) return rc;
     return launch_pages_accept(ctx, *book, seqs, starts, batch, tokens, *tree, last, row_bytes, kept);
 }

@@ -929,6 +929,18 @@ def test_wrong_calls_are_refused(ctx):
     assert torch.equal(c.k.view(torch.int16), before[0].view(torch.int16)) and torch.equal(c.tables, before[1])
 
 
+def test_accept_refuses_to_write_over_what_it_reads(ctx):
+    f, tree = Filled(ctx, 50, [40, 9], 2, 64, 16, "f16"), K.DraftTree(ctx, pimdl, 2)
+    before, both = f.cache.lengths.clone(), ints(-1, -1, 0, 1, 2)
+    last, mixed, starts, seqs = both[:2], both[1:3], starts_of([1, 1]), ints(0, 1)
+    for args in ((last, last, starts), (last, mixed, starts), (mixed, last, starts), (last, starts[:2], starts), (last, starts[1:], starts), (last, seqs, starts, seqs)):
+        with pytest.raises(pimdl.PimdlError, match="overlap"):
+            f.cache.accept(tree, *args)
+    torch.cuda.synchronize()
+    assert torch.equal(f.cache.lengths, before)
+    f.cache.accept(tree, last, both[2:4], starts)  # beside each other
+
+
 def test_calls_without_tokens_do_nothing(ctx):
     f, r = Filled(ctx, 50, [40, 9], 2, 64, 16, "f16"), rotary_of(ctx, 64, 64, "halves")
     book, tree, kept = Book(f.cache), K.DraftTree(ctx, pimdl, 0), ints(7, 7)
