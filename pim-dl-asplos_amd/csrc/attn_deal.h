@@ -12,14 +12,19 @@ namespace pimdl {
 namespace attn {
 
 constexpr uint32_t DEAL_BATCH = 512;  // rows of the batch that fit
-constexpr uint32_t DEAL_BLOCK = 16;   // units of a block without its tiles: its queries, the first keys' way and the results take 7 us with 64 rows, 13 with 256
-constexpr uint32_t DEAL_SHORT = 32;   // units of tiles up to which a block is not worth cutting
-constexpr uint32_t DEAL_LEAST = 24;   // units of a share, at least
-// Units of a tile of 64 keys by its block's groups of 32 rows: us / 0.5 as measured, one block of each size to every CU, 128 dims, bf16 (1.50, 1.57, 2.06, 2.17, 2.60, 2.70, 3.36, 3.42).
+// Units are a 14th of the time that a tile takes with 256 rows.  Measured, 40 sequences with blocks of 2 to 8 groups of 32 rows each, us a tile: of 64 keys 1.86, 2.13, 2.19, 2.57, 2.81,
+// 3.32, 3.54 (bf16, 128 dims), 1.11, 1.46, 1.53, 1.83, 1.91, 2.40, 2.47 (fp16, 64), 2.35, 3.08, 3.31, 4.00, 4.33, 5.44, 5.72 (fp32, 64); of 32 keys, which waves do not share, 2.25, 2.41, 2.54,
+// 3.30, 3.58, 3.72, 3.95 (fp32, 80), 3.18, 3.35, 3.59 (fp32, 128).
+template <int TILE>
 __device__ __forceinline__ uint32_t tile_units(uint32_t groups)
 {
-    return groups <= 2 ? 3 : groups <= 4 ? 4 : groups <= 6 ? 5 : 7;
+    if (TILE == 64) return groups + (groups > 6 ? 6 : 5);
+    return groups <= 4 ? 8 + groups / 3 : 10 + groups / 2;
 }
+constexpr uint32_t TILE_MOST = 8;     // units of a tile for each of a block's groups, at most
+constexpr uint32_t DEAL_BLOCK = 36;   // units of a block without its tiles: its queries, the first keys' way and the results (10 to 12, 5.5 to 7.4, 8 to 10, 7 to 9 and 6 to 9 us)
+constexpr uint32_t DEAL_SHORT = 64;   // units of tiles up to which a block is not worth cutting
+constexpr uint32_t DEAL_LEAST = 48;   // units of a share, at least
 
 // What the shares of one call leave: share w's sums of a block that began in an earlier share in slot 2 w, of one that goes on in a later share in slot 2 w + 1.
 struct DealPart {
@@ -99,8 +104,8 @@ __device__ __forceinline__ DealRow deal_row(const AttnArgs& a, const Row& r)
     d.blocks = (groups + each - 1) / each;  // (the last ones may have come out empty)
     d.rows = 32 * each;
     d.tiles = (uint32_t)(tiles > 0 ? tiles : 1);
-    d.whole = tile_units(each);
-    d.last = tile_units(groups - (d.blocks - 1) * each);
+    d.whole = tile_units<D::TILE>(each);
+    d.last = tile_units<D::TILE>(groups - (d.blocks - 1) * each);
     return d;
 }
 
