@@ -291,16 +291,15 @@ struct Step {
 
 // Tiles from .. to - 1 (at least one) for this workgroup's rows.  KG (key groups) 1: a wave takes all keys of a tile; 2: the 32 that `half` says, of 64.  While tile t's values
 // are worked on, the scores are tile t + 1's: K is a tile ahead of V in LDS, where it has three places and V two, and the next of both are on their way in
-// registers.  One barrier a tile.
+// registers.  One barrier a tile.  `ahead` has been asked for the first tile's pages.
 template <typename C, int KG>
 __device__ __forceinline__ void deal_tiles(const AttnArgs& a, const Row& r, uint32_t kh, Rows<C, 32>& w, const Span& span, int32_t from, int32_t to, int32_t all_hi, int64_t all_lo,
-                                           bool works, uint32_t half, typename Deal<C>::Shared& sh)
+                                           bool works, uint32_t half, Ahead<C, Deal<C>::TILE>& ahead, typename Deal<C>::Shared& sh)
 {
     typedef Deal<C> D;
     constexpr int TILE = D::TILE, STEPS = TILE / 32 / KG;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), mine = KG == 1 ? 0 : 32 * half;
     typename D::S sk, sv;
-    Ahead<C, TILE> ahead;
     Place at_k, at_v;
     auto key_of = [&](int32_t t) { return span.at(t) * TILE; };
     auto fetch_k = [&](typename D::S& x, int32_t t) __attribute__((always_inline)) {
@@ -317,7 +316,6 @@ __device__ __forceinline__ void deal_tiles(const AttnArgs& a, const Row& r, uint
         D::store(sv, sh.tile.v[buf], tid);
     };
     if (tid < 4) sh.bad[tid] = 0;
-    ahead.ask(a, r, key_of(from));
     uint32_t there0, there1 = ~0u, there2 = ~0u;  // of tiles t, t + 1 and t + 2
     {
         typename D::S first;
@@ -502,16 +500,18 @@ __global__ __launch_bounds__(Deal<C>::THREADS, Deal<C>::WAVES / 4) void attentio
         const uint32_t half = duty.half, mine = row0 + 32 * duty.group;
         const Span span = span_of<true>(a, r, row0, end - 1, D::TILE);  // (a part of the last block's: only its end may come earlier)
         const bool works = mine < end;
+        const int32_t until = to < span.total ? to : span.total;
+        Ahead<C, D::TILE> ahead;  // (on the way together with the queries)
+        if (from < until) ahead.ask(a, r, span.at(from) * D::TILE);
         Rows<C, 32> w;
         w.begin(a, r, kh, works ? mine : row0, rows);
         const int32_t all_hi = r.pos0 < 0 ? 0 : r.pos0;
         const int64_t all_lo = (int64_t)r.pos0 + (end - 1) / a.group - a.left;
-        const int32_t until = to < span.total ? to : span.total;
         __syncthreads();  // everybody is done with the block before
         if (from < until) {
             // (a barrier for each tile on either way)
-            if (D::TILE == 64 && duty.halves) deal_tiles<C, D::TILE / 32>(a, r, kh, w, span, from, until, all_hi, all_lo, works, half, sh);
-            else deal_tiles<C, 1>(a, r, kh, w, span, from, until, all_hi, all_lo, works, 0, sh);
+            if (D::TILE == 64 && duty.halves) deal_tiles<C, D::TILE / 32>(a, r, kh, w, span, from, until, all_hi, all_lo, works, half, ahead, sh);
+            else deal_tiles<C, 1>(a, r, kh, w, span, from, until, all_hi, all_lo, works, 0, ahead, sh);
             if (D::TILE == 64) deal_join_halves<C>(w, duty, sh);
         }
         if (half == 0 && mine + j < end) {
