@@ -2,6 +2,9 @@
 //
 // At position p the pair (a, b) of frequency f becomes (a cos pf - b sin pf, a sin pf + b cos pf): a token's angles are the same for all of its heads, so a
 // workgroup works out those of its tokens once, in LDS, while the heads' columns are on their way.
+//
+// HBM bounds it: 6 prompts of up to 4096 tokens, 32 heads over 8 of 128 dims, bf16, 343 MB, 68 to 70 us (5.0 TB/s; a copy of 4 GiB reaches 4.8); 12 on their way into the cache, values
+// too, 696 MB, 129 to 135.  A few tokens wait for memory three times over (starts; lengths and pages; frequencies), 5.2 and 6.4 us, and for the host, 9 us a call.
 #include <algorithm>
 #include <type_traits>
 
