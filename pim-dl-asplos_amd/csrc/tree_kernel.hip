@@ -75,8 +75,9 @@ int launch_build(Ctx* ctx, const int32_t* parents, const int32_t* starts, uint32
 // The branch is the set bits of its last node's mask, in order; its j-th node moves to place j, which is never behind its own.  A thread of the first launch owns a
 // part of a row (of one head, layer and pool) and moves that of every node in order, ACCEPT_AHEAD of them asked for before the first is stored: none of them is a place
 // that has been written, as later nodes lie behind all places up to their own.
-// Memory bounds it: the branches of 64 trees in 12 layers, 8 heads of 128, bf16, 158 MB, take 47 us (3.4 TB/s; a plain copy reaches 4.8), 16 rows ahead 48; the book
-// 4 us.  One branch alone waits for memory five times in a row: 6.6 us.
+// Memory bounds it, and the longest branch: those of 64 trees in 12 layers, 8 heads of 128, bf16, up to 82 rows that move, 158 MB, take 41 us (3.9 TB/s; a plain copy reaches 4.8), 16
+// rows ahead 40; in workgroups of 256 threads, half as many CUs to a branch, 48, of 64, each of which finds out the same, 44; the book 4 us.  One branch alone waits for memory five
+// times in a row: 6.4 us.
 // ------------------------------------------------------------------------------------------------------------
 struct AcceptArgs {
     const int32_t *seqs, *starts, *last, *lengths, *refs, *lacking, *tables;
@@ -90,10 +91,10 @@ struct AcceptPools {
     uint64_t page_bytes, layer_bytes;
 };
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));  // (an array of HIP's own uint4 would be in scratch)
-constexpr uint32_t ACCEPT_NODES = 1024, ACCEPT_AHEAD = 8;
+constexpr uint32_t ACCEPT_NODES = 1024, ACCEPT_AHEAD = 8, ACCEPT_THREADS = 128;
 
 template <typename T>
-__global__ __launch_bounds__(256) void pages_accept_kernel(AcceptArgs a, AcceptPools pl)
+__global__ __launch_bounds__(ACCEPT_THREADS) void pages_accept_kernel(AcceptArgs a, AcceptPools pl)
 {
     __shared__ uint64_t from[ACCEPT_NODES], to[ACCEPT_NODES];  // of the rows that move: first byte in a layer's buffer, of a page's first run
     __shared__ int32_t path[ACCEPT_NODES];
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(256) void pages_accept_kernel(AcceptArgs a, AcceptP
     const int64_t base = length - n;
     if (tid == 0 && (*a.lacking != 0 || !there || base < 0 || n > 32 * a.words || last < -1 || last >= (int32_t)n)) wrong = 1;
     if (a.seqs)
-        for (uint32_t i = tid; i < b; i += 256)
+        for (uint32_t i = tid; i < b; i += ACCEPT_THREADS)
             if (a.seqs[i] == s) wrong = 1;  // (who comes first)
     __syncthreads();
     if (wrong) {
@@ -139,13 +140,13 @@ __global__ __launch_bounds__(256) void pages_accept_kernel(AcceptArgs a, AcceptP
     __syncthreads();
     const uint32_t count = before[32];
     if (last >= 0)
-        for (uint32_t i = tid; i <= (uint32_t)last; i += 256) {
+        for (uint32_t i = tid; i <= (uint32_t)last; i += ACCEPT_THREADS) {
             const uint32_t word = word_of(i / 32), bit = 1u << (i & 31);
             if (word & bit) path[before[i / 32] + __popc(word & (bit - 1))] = (int32_t)i;
         }
     __syncthreads();
     if (tid == 0 && last >= 0 && (count == 0 || path[count - 1] != last)) wrong = 1;  // its own bit is not there
-    for (uint32_t j = tid; j < count; j += 256)
+    for (uint32_t j = tid; j < count; j += ACCEPT_THREADS)
         if (path[j] == (int32_t)j) atomicAdd(&unmoved, 1u);  // (the first ones: a node behind one that moves lies behind its place)
     __syncthreads();
     if (wrong) {
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(256) void pages_accept_kernel(AcceptArgs a, AcceptP
     const int32_t* const table = a.tables + (size_t)s * a.width;
     if (n) {
         const uint32_t p0 = (uint32_t)((base + unmoved) / a.page_tokens), p1 = (uint32_t)((base + count + a.page_tokens - 1) / a.page_tokens);
-        for (uint32_t p = p0 + tid; p < p1; p += 256) {
+        for (uint32_t p = p0 + tid; p < p1; p += ACCEPT_THREADS) {
             const int32_t page = table[p];
             if (page >= 0 && (uint32_t)page < a.pages && a.refs[page] > 1) wrong = 1;
         }
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(256) void pages_accept_kernel(AcceptArgs a, AcceptP
         const int32_t page = table[place / a.page_tokens];
         return page < 0 || (uint32_t)page >= a.pages ? -1 : (int64_t)(page * pl.page_bytes + place % a.page_tokens * pl.row_bytes);
     };
-    for (uint32_t j = unmoved + tid; j < count; j += 256) {
+    for (uint32_t j = unmoved + tid; j < count; j += ACCEPT_THREADS) {
         const int64_t f = byte_of(base + path[j]), t = byte_of(base + j);
         // (a row on no page is not there: what would move from it or to it stays)
         from[j - unmoved] = f < 0 || t < 0 ? 0 : (uint64_t)f;
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(256) void pages_accept_kernel(AcceptArgs a, AcceptP
     const uint32_t rows = count - unmoved, parts = pl.row_bytes / (uint32_t)sizeof(T);
     const uint64_t columns = (uint64_t)parts * pl.runs * pl.layers * pl.count, run_bytes = (uint64_t)a.page_tokens * pl.row_bytes;
     if (rows == 0) return;
-    for (uint64_t c = (uint64_t)blockIdx.x * 256 + tid; c < columns; c += (uint64_t)gridDim.x * 256) {
+    for (uint64_t c = (uint64_t)blockIdx.x * ACCEPT_THREADS + tid; c < columns; c += (uint64_t)gridDim.x * ACCEPT_THREADS) {
         const uint32_t part = (uint32_t)(c % parts), rest = (uint32_t)(c / parts), run = rest % pl.runs, slot = rest / pl.runs;
         char* const at = pl.at[slot / pl.layers] + (size_t)(slot % pl.layers) * pl.layer_bytes + run * run_bytes + (size_t)part * sizeof(T);
         for (uint32_t j0 = 0; j0 < rows; j0 += ACCEPT_AHEAD) {
@@ -215,12 +216,12 @@ __global__ __launch_bounds__(64) void pages_accept_book_kernel(AcceptArgs a, int
 template <typename T>
 int launch_accept(Ctx* ctx, const AcceptArgs& a, const AcceptPools& pl)
 {
-    // enough workgroups to fill the device twice, no more than there are columns
-    const uint64_t columns = (uint64_t)(pl.row_bytes / sizeof(T)) * pl.runs * pl.layers * pl.count, blocks = (columns + 255) / 256;
+    // workgroups enough for the device, no more than there are columns
+    const uint64_t columns = (uint64_t)(pl.row_bytes / sizeof(T)) * pl.runs * pl.layers * pl.count, blocks = (columns + ACCEPT_THREADS - 1) / ACCEPT_THREADS;
     if (columns > 0xffffffffu) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "pimdl_pages_accept: more parts of rows than 2^32");
     const uint64_t most = ((uint64_t)ctx->prop.multiProcessorCount * 16 + a.batch - 1) / a.batch;
     const uint32_t grid = (uint32_t)(blocks == 0 ? 1 : blocks < most ? blocks : most);
-    hipLaunchKernelGGL((pages_accept_kernel<T>), dim3(grid, a.batch), dim3(256), 0, ctx->stream, a, pl);
+    hipLaunchKernelGGL((pages_accept_kernel<T>), dim3(grid, a.batch), dim3(ACCEPT_THREADS), 0, ctx->stream, a, pl);
     return hip_check(ctx, hipGetLastError(), "pages_accept_kernel launch");
 }
 
