@@ -475,6 +475,92 @@ def test_dealt_blocks_of_short_sequences(ctx):
     dealt(tree_case(ctx, 8, [40, 64] * 30 + [1], [17, 0] * 30 + [3000], 8, 8, 64, 16, "f16", "f16"))
 
 
+def test_dealt_blocks_recorded_and_replayed(ctx):
+    """Lengths, borders of the batch, its list and its parents change from replay to replay, sequences that are not there among them; every replay against plain attention."""
+    heads, kv, hd, room = 16, 8, 64, 340
+    own, side = pimdl.Context(0), torch.cuda.Stream()
+    f = Filled(own, 60, [9000, 5033, 900, 70], kv, hd, 16, "f16")
+    full = f.cache.lengths.clone()
+    tree, starts, seqs, parents = K.DraftTree(own, pimdl, room, most=160), starts_of([100, 150, 60, 30]), ints(0, 1, 2, 3), forest([100, 150, 60, 30], 1)
+    q, out = randn(gen_of(61), room, heads * hd, dtype="f16"), torch.zeros(room, heads * hd, device="cuda", dtype=torch.float16)
+
+    def step():
+        tree.build(parents, starts)
+        f.cache.attend(0, q, out, starts, heads, seqs, left=6000, sinks=70, tree=tree)
+
+    torch.cuda.synchronize()
+    own.set_stream(side.cuda_stream)
+    with torch.cuda.stream(side):
+        step()  # sizes the scratch
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+        step()
+    dealt(own.last_attention())
+    for i, (counts, lengths, order) in enumerate([([100, 150, 60, 30], [9000, 5033, 900, 70], [0, 1, 2, 3]), ([1, 160, 9, 33], [8000, 4000, 60, 33], [2, 0, 3, 1]),
+                                                  ([0, 0, 150, 0], [9000, 5033, 900, 70], [0, 1, 2, 3]), ([33, 40, 50, 60], [40, 41, 50, 20], [3, 99, 0, -1]),
+                                                  ([64, 64, 64, 64], [0, 3, 64, 70], [3, 2, 1, 0]), ([100, 150, 60, 30], [9000, 5033, 900, 70], [1, 0, 1, 2])]):
+        torch.cuda.synchronize()
+        f.cache.lengths.copy_(torch.minimum(ints(*lengths), full))
+        starts.copy_(starts_of(counts))
+        seqs.copy_(ints(*order))
+        packed = forest(counts, 20 + i)
+        parents.fill_(7)
+        parents[:sum(counts)] = packed
+        q.copy_(randn(gen_of(70 + i), *q.shape, dtype="f16"))
+        out.fill_(-5.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out[sum(counts):] == -5.0).all(), i
+        at = 0
+        for c, s, p in zip(counts, order, split(packed, counts)):
+            length = min(lengths[s], int(full[s])) if 0 <= s < 4 else 0
+            k, v = (x[0][:length] for x in f.rows[s if 0 <= s < 4 else 0])
+            if c:
+                want, off, mass = reference_tree(q[at:at + c].reshape(c, heads, hd), k, v, p, 6000, 70, 1 / math.sqrt(hd))
+                check(out[at:at + c].reshape(c, heads, hd), want, off, mass, "f16")
+            at += c
+    own.close()
+
+
+@pytest.mark.parametrize("dtype,cache,hd", [("bf16", "bf16", 128), ("f16", "f16", 64), ("f32", "f32", 80), ("f32", "f16", 32), ("f32", "bf16", 96), ("f32", "f32", 64), ("f32", "bf16", 128)])
+def test_dealt_blocks_over_pages_that_are_not_there(ctx, dtype, cache, hd):
+    """... and past values that are not finite, which only those who see them get."""
+    counts, lengths, heads, kv = [90, 130, 33], [9000, 4100, 700], 16, 8
+    f, parents = Filled(ctx, 80, lengths, kv, hd, 16, cache), forest(counts, 81)
+    gone = [[3, 4, 5, 6, 300, 8950 // 16], [0, 1, (4100 - 130 + 20) // 16], list(range(30))]
+    for s, pages in enumerate(gone):
+        for i, page in enumerate(pages):
+            f.cache.tables[s, page] = (-1, 1 << 30, f.cache.k.shape[1])[i % 3]
+    tree, n = K.DraftTree(ctx, pimdl, sum(counts), most=130), sum(counts)
+    tree.build(parents, starts_of(counts))
+    q = randn(gen_of(82), n, heads * hd, dtype=dtype)
+    out = [torch.zeros_like(q) for _ in range(2)]
+    f.cache.attend(0, q, out[0], starts_of(counts), heads, tree=tree)
+    dealt(ctx.last_attention())
+    at = 0
+    for s, (c, p) in enumerate(zip(counts, split(parents, counts))):
+        k, v = (x[0] for x in f.rows[s])
+        want, off, mass = reference_tree(q[at:at + c].reshape(c, heads, hd), k, v, p, 1 << 40, 0, 1 / math.sqrt(hd), [j for j in range(lengths[s]) if j // 16 in gone[s]])
+        check(out[0][at:at + c].reshape(c, heads, hd), want, off, mass, dtype)
+        at += c
+    # node 77 of the second tree: its own value is infinite, for one key head; its key is NaN, for another
+    node, place = 77, 4100 - 130 + 77
+    page = int(f.cache.tables[1, place // 16])
+    f.cache.v[0, page, 2, place % 16, hd - 1] = float("inf")
+    f.cache.k[0, page, 5, place % 16, 0] = float("nan")
+    f.cache.attend(0, q, out[1], starts_of(counts), heads, tree=tree)
+    torch.cuda.synchronize()
+    of = [torch.from_numpy(kin_of(split(parents, counts)[1]))[:, node].nonzero()[:, 0].cuda() + 90, heads // kv]
+    a, b = (o.reshape(n, heads, hd).clone() for o in out)
+    assert not torch.isfinite(b[of[0], 2 * of[1]:3 * of[1], hd - 1]).any() and torch.isnan(b[of[0], 5 * of[1]:6 * of[1]]).all()
+    for o in (a, b):
+        o[of[0], 2 * of[1]:3 * of[1], hd - 1] = 0
+        o[of[0], 5 * of[1]:6 * of[1]] = 0
+    assert torch.equal(a, b)
+
+
 def test_more_words_than_nodes_change_nothing(ctx):
     for most in (40, 64, 65, 1024):
         tree_case(ctx, 5, [40, 3], [200, 300], 4, 2, 64, 16, "bf16", "bf16", most=most)
