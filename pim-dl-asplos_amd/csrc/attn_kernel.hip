@@ -411,7 +411,13 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     // 14.3 / 29.1 (8 x 16 over 1000); 2^15: 22.8 / 34.1 (64), 34.6 / 40.3 (8 x 8); 2^16: 51.4 / 36.6 (128), 58.5 / 46.3 (8 x 16), 34.8 / 48.5 (32 over
     // 16000); 2^17: 56.5 / 54.0 (64 over 16000), 95.5 / 56.0 (8 x 32).  Keys are counted by what a row of the table can hold, not by what it does: the
     // lengths are on the device.
-    const bool few = 16 * wide_items <= 3 * cus && (uint64_t)a.tokens * a.heads * keys <= cus << 15;
+    // Trees over 16-bit keys of more than 32 rows a sequence, on average: up to 2^16 scores a CU, in as many blocks as two on each CU.  At 2^15 25.2 / 43.7 (4 of 64 over 1000), 28.8 / 42.2
+    // (16 of 16 over 1000), 24.9 / 42.1 (2 of 128 over 1000); 2^15.6 26.2 / 36.2 (8 of 64 over 2000, 12 heads, fp32 over fp16); 2^16 29.1 / 35.4 (2 of 64 over 4000), 37.9 / 47.4 (8 of 32
+    // over 2000), 32.9 / 39.1 (8 of 16 over 4000, dealt out); 2^17 56.0 / 47.5 (64 over 16 000).  Of fewer rows 67.5 / 49.9 (64 of 4 over 1000), 48.0 / 32.1 (64 of 8 over 500); of more blocks 44.3
+    // / 38.2 (16 of 24 over 1000), 60.7 / 50.2 (64 of 9 over 500); over fp32 keys, dealt out, 56.1 / 51.8 (8 of 64 over 1000, 16 heads of 80).
+    const uint64_t scores = (uint64_t)a.tokens * a.heads * keys, tree_blocks = ((rows + a.batch - 1) / a.batch + attn::NARROW_ROWS - 1) / attn::NARROW_ROWS * a.batch * a.kv_heads;
+    const bool few = (16 * wide_items <= 3 * cus && scores <= cus << 15) ||
+                     (a.masks && a.cache_dtype != PIMDL_F32 && rows > 32ull * a.batch && scores <= cus << 16 && tree_blocks <= 2 * cus);
     p->narrow = a.paged || few;
     p->wide = !few && !(a.paged && a.tokens <= a.batch);
     p->by_slot = few && a.tokens > a.batch;
@@ -423,8 +429,11 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
         // Up to 1024 keys: no split, whose join costs more than it saves (32 heads over 8, bf16, one sequence of 777: 8.8 us, in three 11.3; of 1500
         // 12.3 and 11.3, of 2000 14.7 and 11.2).  Fewer items than half the CUs: every CU one workgroup, of at least 256 keys.  More: shares of at least 1024 keys, so that long sequences are dealt
         // out too.  us with shares of 512 / 1024 / 2048 keys for more items: 64 sequences of up to 8191 231 / 203 / 203, 32 of up to 4000, 12 heads,
-        // fp32 116 / 96 / 118; for fewer: two of 100 000 67 / 55 / 50 (one workgroup per CU), 32 of up to 16000 with one key head 52 / 44 / 41.
+        // fp32 116 / 96 / 118; for fewer: two of 100 000 67 / 55 / 50 (one workgroup per CU), 32 of up to 16000 with one key head 52 / 44 / 41.  Trees: none
+        // where every CU has a block of 16 rows (two of 64 nodes over 4000, 32 heads over 8, bf16, in one 29.1 us, two 35.6, three 42.4; four of 32 31.9, 37.0, 45.2), else no more than two a
+        // CU (four of 17 over 8000 in three 42.7, in seven 61.1).
         p->narrow_splits = (uint32_t)std::max<uint64_t>(1, keys <= 1024 ? 1 : 2 * items <= cus ? std::min<uint64_t>({(cus + items - 1) / items, keys / 256, 256})
+                                                                        : a.masks && p->by_slot ? std::min<uint64_t>(tree_blocks < cus ? 2 * cus / tree_blocks : 1, keys / 1024)
                                                                         : std::min<uint64_t>((8 * cus + items - 1) / items, keys / 1024));
     }
     // About two workgroups a CU, rounded up: registers leave room for two, or for one in fp32 above 80 dims and fp32 over 16 bits above 96, which the rule

@@ -475,6 +475,21 @@ def test_dealt_blocks_of_short_sequences(ctx):
     dealt(tree_case(ctx, 8, [40, 64] * 30 + [1], [17, 0] * 30 + [3000], 8, 8, 64, 16, "f16", "f16"))
 
 
+@pytest.mark.parametrize("batch,n,length,heads,kv,hd,dtype,cache,splits", [
+    (4, 64, 1000, 32, 8, 128, "bf16", "bf16", 1),     # two blocks on every CU
+    (2, 64, 4000, 32, 8, 128, "f16", "f16", 1),       # one, which is not split
+    (4, 17, 7600, 32, 8, 128, "bf16", "bf16", 3),     # fewer, split up to two a CU
+    (8, 60, 2000, 12, 12, 64, "f32", "f16", 1),
+    (3, 65, 1500, 8, 2, 96, "f32", "bf16", 3),        # 98 blocks, a CU each in thirds
+])
+def test_trees_in_blocks_of_sixteen_rows(ctx, batch, n, length, heads, kv, hd, dtype, cache, splits):
+    """Trees whose scores are few enough for a CU, for the many blocks' sake, with lengths from the tree alone to all that the table holds."""
+    lengths = [length if b == 0 else n + (length - n) * b // batch for b in range(batch)]
+    plan = tree_case(ctx, n, [n - b % 2 for b in range(batch)], lengths, heads, kv, hd, 16, dtype, cache, width=5)
+    want = dict(plain=0, wide=0, narrow=1, narrow_splits=splits, by_slot=1, join=int(splits > 1))
+    assert {k: plan[k] for k in want} == want, plan
+
+
 def test_dealt_blocks_recorded_and_replayed(ctx):
     """Lengths, borders of the batch, its list and its parents change from replay to replay, sequences that are not there among them; every replay against plain attention."""
     heads, kv, hd, room = 16, 8, 64, 340
