@@ -540,7 +540,8 @@ __global__ __launch_bounds__(Deal<C>::THREADS, Deal<C>::WAVES / 4) void attentio
             }
         }
         if (tid == 0 && from == 0 && to < most) {
-            part.joins[2 * share] = (u32x4){(first + each * (d.tiles - 1)) / per - share + 1, end - row0, 0, 0};
+            const uint32_t last = (first + each * (d.tiles - 1)) / per;
+            part.joins[2 * share] = (u32x4){(last < gridDim.x ? last : gridDim.x - 1) - share + 1, end - row0, 0, 0};  // (behind the last one: see add_units)
             part.joins[2 * share + 1] = (u32x4){r.first, row0, kh, 0};
         }
     }
