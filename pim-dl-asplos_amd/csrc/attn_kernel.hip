@@ -445,8 +445,8 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     // 214 / 224 / 225 / 236; three of 300 to 512 over up to 3000, 16 heads of 80, fp32, 144 / 118 / 125 / 124.
     if (p->wide) p->wide_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(2 * cus + wide_items - 1) / wide_items, keys / 512, 16}));
     // Trees of more than 32 rows a sequence, on average, and 16 tiles of 64 keys a CU: an even deal over the device's CUs, where the units of any lengths fit in 32 bits.  us a call, dealt / in
-    // blocks of 128 rows with equal splits: 32 sequences of 16 to 64 nodes over up to 8191 keys, 32 heads over 8, bf16, 235 / 307 (in four splits, the best, the kernels alone 272 + 28 of
-    // 312 + 26), two of 36 and 42 over 100 000 and 130 000, 16 heads over 2, fp16, 168 / 269; one of 16 over 64 000 66 / 123; four of 100 to 250 in a window of 1024, 16 heads of 80, fp32,
+    // blocks of 128 rows with equal splits: 32 sequences of 16 to 64 nodes over up to 8191 keys, 32 heads over 8, bf16, 228 / 307 (in four splits, the best, the kernels alone 272 + 28 of
+    // 312 + 26), two of 36 and 42 over 100 000 and 130 000, 16 heads over 2, fp16, 158 / 269; one of 16 over 64 000 66 / 123; four of 100 to 250 in a window of 1024, 16 heads of 80, fp32,
     // whose tiles count four times, 56 / 76 (in four splits 51 + 7 of 76 + 6).  At 16 tiles a CU both take the same (8 of 16 or of 32 nodes over 4000 41 / 40, 49 / 49; 16 of 16 over 2000 45 / 45), below it the deal's own 20 us
     // tell (one of 64 over 16 000 54 / 48; two of 128 over 2000 40 / 37), and few rows wait for memory in blocks of 16 (64 of 4 nodes over 2000 111 / 85; 32 of 8 over 1000 55 / 34).
     const uint64_t tiles_a_cu = (rows / 256 + a.batch) * a.kv_heads * (keys / 64 + 1) * (a.cache_dtype == PIMDL_F32 ? 4 : 1) / cus;
