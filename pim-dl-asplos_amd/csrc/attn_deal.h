@@ -225,9 +225,11 @@ struct Step {
     __device__ __forceinline__ void scores(Rows<C, 32>& w, uint32_t k, float* s, const float* old, float base, uint32_t lv)
     {
         u32x4 x[KS][C::NK];
+        uint32_t from = k + at_k;
+        asm("" : "+v"(from));  // (or sums with each step's place are kept in registers, and added to again)
         auto read_k = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int n = 0; n < C::NK; ++n) x[i][n] = *(LdsRow)(uintptr_t)(k + at_k + i * 32 + n * PIECE);
+            for (int n = 0; n < C::NK; ++n) x[i][n] = *(LdsRow)(uintptr_t)(from + i * 32 + n * PIECE);
         };
 #pragma unroll
         for (int i = 0; i < KAHEAD; ++i) read_k(i);
