@@ -480,6 +480,8 @@ def test_dealt_blocks_of_short_sequences(ctx):
     (2, 64, 4000, 32, 8, 128, "f16", "f16", 1),       # one, which is not split
     (4, 17, 7600, 32, 8, 128, "bf16", "bf16", 3),     # fewer, split up to two a CU
     (8, 60, 2000, 12, 12, 64, "f32", "f16", 1),
+    (16, 24, 2000, 16, 16, 80, "f32", "f16", 1),      # 24 rows to a key head, which no other query head reads
+    (16, 8, 4000, 32, 8, 64, "bf16", "bf16", 1),      # 32, of four heads of 64
     (3, 65, 1500, 8, 2, 96, "f32", "bf16", 3),        # 98 blocks, a CU each in thirds
 ])
 def test_trees_in_blocks_of_sixteen_rows(ctx, batch, n, length, heads, kv, hd, dtype, cache, splits):
