@@ -413,15 +413,18 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     // 14.3 / 29.1 (8 x 16 over 1000); 2^15: 22.8 / 34.1 (64), 34.6 / 40.3 (8 x 8); 2^16: 51.4 / 36.6 (128), 58.5 / 46.3 (8 x 16), 34.8 / 48.5 (32 over
     // 16000); 2^17: 56.5 / 54.0 (64 over 16000), 95.5 / 56.0 (8 x 32).  Keys are counted by what a row of the table can hold, not by what it does: the
     // lengths are on the device.
-    // Trees over 16-bit keys of more than 32 rows a sequence, on average, or 16 where heads share no keys or have up to 64 dims: up to 2^16 scores a CU, in as many blocks as two
-    // on each CU.  At 2^15 25.2 / 43.7 (4 of 64 over 1000), 28.8 / 42.2 (16 of 16 over 1000), 24.9 / 42.1 (2 of 128 over 1000); 2^15.6 26.2 / 36.2 (8 of 64 over 2000, 12 heads, fp32
+    // Trees of more than 32 rows a sequence, on average, or 16 where heads share no keys or have up to 64 dims, over fp32 keys of no more than 32: up to 2^16 scores a CU, in as many
+    // blocks as two on each CU.  At 2^15 25.2 / 43.7 (4 of 64 over 1000), 28.8 / 42.2 (16 of 16 over 1000), 24.9 / 42.1 (2 of 128 over 1000); 2^15.6 26.2 / 36.2 (8 of 64 over 2000, 12 heads, fp32
     // over fp16); 2^16 29.1 / 35.4 (2 of 64 over 4000), 37.9 / 47.4 (8 of 32 over 2000), 32.9 / 39.1 (8 of 16 over 4000, dealt out); 2^17 56.0 / 47.5 (64 over 16 000).  Of fewer rows
     // 67.5 / 49.9 (64 of 4 over 1000), 48.0 / 32.1 (64 of 8 over 500); of more blocks 44.3 / 38.2 (16 of 24 over 1000), 60.7 / 50.2 (64 of 9 over 500).  17 to 32 rows: 17.2 / 24.8 (16
     // of 32 over 1000, 16 heads of 64, fp16), 49.3 / 61.9 (8 of 32 over 4000, 16 of 128), 32.3 / 57.9 (4 of 32 over 8000, 16 of 80, fp32 over fp16), 31.2 / 39.3 (16 of 8 over 4000, 32
-    // over 8 of 64), but 25.5 / 20.9 (32 of 8 over 500, of 96) and 68.5 / 62.0 (16 of 8 over 4000, of 128).  Over fp32 keys, dealt out, 56.1 / 51.8 (8 of 64 over 1000, 16 heads of 80).
+    // over 8 of 64), but 25.5 / 20.9 (32 of 8 over 500, of 96) and 68.5 / 62.0 (16 of 8 over 4000, of 128).  fp32 keys: 58.3 / 71.1
+    // (16 of 24 over 2000, 12 heads of 64), 126 / 207 (8 of 32 over 4000, 16 of 128), 89 / 93 (of 80); more rows, dealt out, 83 / 47 (2 of 256 over 2000, 16 of 80), 46 / 38 (4 of 64 over
+    // 4000, 12 of 64).
     const uint64_t scores = (uint64_t)a.tokens * a.heads * keys, tree_blocks = ((rows + a.batch - 1) / a.batch + attn::NARROW_ROWS - 1) / attn::NARROW_ROWS * a.batch * a.kv_heads;
     const bool few = (16 * wide_items <= 3 * cus && scores <= cus << 15) ||
-                     (a.masks && a.cache_dtype != PIMDL_F32 && rows > (a.group == 1 || a.head_dim <= 64 ? 16ull : 32ull) * a.batch && scores <= cus << 16 && tree_blocks <= 2 * cus);
+                     (a.masks && rows > (a.group == 1 || a.head_dim <= 64 ? 16ull : 32ull) * a.batch && (a.cache_dtype != PIMDL_F32 || rows <= 32ull * a.batch) && scores <= cus << 16 &&
+                      tree_blocks <= 2 * cus);
     p->narrow = a.paged || few;
     p->wide = !few && !(a.paged && a.tokens <= a.batch);
     p->by_slot = few && a.tokens > a.batch;

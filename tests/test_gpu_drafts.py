@@ -482,6 +482,7 @@ def test_dealt_blocks_of_short_sequences(ctx):
     (8, 60, 2000, 12, 12, 64, "f32", "f16", 1),
     (16, 24, 2000, 16, 16, 80, "f32", "f16", 1),      # 24 rows to a key head, which no other query head reads
     (16, 8, 4000, 32, 8, 64, "bf16", "bf16", 1),      # 32, of four heads of 64
+    (8, 32, 4000, 16, 16, 128, "f32", "f32", 1),      # 32, of keys in fp32, where more are dealt out
     (3, 65, 1500, 8, 2, 96, "f32", "bf16", 3),        # 98 blocks, a CU each in thirds
 ])
 def test_trees_in_blocks_of_sixteen_rows(ctx, batch, n, length, heads, kv, hd, dtype, cache, splits):
