@@ -98,11 +98,11 @@ __global__ __launch_bounds__(ACCEPT_THREADS) void pages_accept_kernel(AcceptArgs
 {
     __shared__ uint64_t from[ACCEPT_NODES], to[ACCEPT_NODES];  // of the rows that move: first byte in a layer's buffer, of a page's first run
     __shared__ int32_t path[ACCEPT_NODES];
-    __shared__ uint32_t before[33], unmoved, wrong;
+    __shared__ uint32_t before[33], unmoved, wrong, others;  // others: have a page that this would change (a flag of its own: `wrong` may still be read then)
     const uint32_t tid = threadIdx.x, b = blockIdx.y;
     const int32_t s = a.seqs ? a.seqs[b] : (int32_t)b, last = a.last[b];
     const uint32_t first = clamped_start(a.starts, b, a.tokens), end = clamped_start(a.starts, b + 1, a.tokens), n = end > first ? end - first : 0;
-    if (tid == 0) unmoved = 0, wrong = 0;
+    if (tid == 0) unmoved = 0, wrong = 0, others = 0;
     __syncthreads();
     const bool there = s >= 0 && (uint32_t)s < a.seq_count;
     int64_t length = 0;
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(ACCEPT_THREADS) void pages_accept_kernel(AcceptArgs
         const uint32_t p0 = (uint32_t)((base + unmoved) / a.page_tokens), p1 = (uint32_t)((base + count + a.page_tokens - 1) / a.page_tokens);
         for (uint32_t p = p0 + tid; p < p1; p += ACCEPT_THREADS) {
             const int32_t page = table[p];
-            if (page >= 0 && (uint32_t)page < a.pages && a.refs[page] > 1) wrong = 1;
+            if (page >= 0 && (uint32_t)page < a.pages && a.refs[page] > 1) others = 1;
         }
     }
     auto byte_of = [&](int64_t place) -> int64_t {
@@ -172,8 +172,8 @@ __global__ __launch_bounds__(ACCEPT_THREADS) void pages_accept_kernel(AcceptArgs
         to[j - unmoved] = f < 0 || t < 0 ? ~0ull : (uint64_t)t;
     }
     __syncthreads();
-    if (blockIdx.x == 0 && tid == 0) a.kept[b] = wrong ? -1 : (int32_t)count;
-    if (wrong) return;
+    if (blockIdx.x == 0 && tid == 0) a.kept[b] = others ? -1 : (int32_t)count;
+    if (others) return;
     const uint32_t rows = count - unmoved, parts = pl.row_bytes / (uint32_t)sizeof(T);
     const uint64_t columns = (uint64_t)parts * pl.runs * pl.layers * pl.count, run_bytes = (uint64_t)a.page_tokens * pl.row_bytes;
     if (rows == 0) return;

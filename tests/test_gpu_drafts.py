@@ -821,6 +821,19 @@ def test_accept_does_not_write_on_pages_of_others(ctx):
     assert accept_case(ctx, cache, [48], [2], forest([48], 0, width=1), [20]) == [21]
 
 
+def test_accept_finds_a_page_of_others_wherever_it_lies(ctx):
+    """A page that another sequence holds, the first, a middle or the last one of 65 that rows would move to, each looked at by a thread of its own: the sequence is left
+    as it was, the one beside it is not."""
+    p = torch.cat([ints(-1, -1, *range(1, 1023)), forest([1024], 3, width=5)])
+    for place in (4, 35, 67, 68):
+        f = Filled(ctx, 8, [1100, 1100], 2, 64, 16, "bf16", layers=9)
+        f.cache.refs[f.cache.tables[0, place].long()] += 1
+        assert accept_case(ctx, f.cache, [1024, 1024], None, p, [1023, 1000])[0] == -1
+    f = Filled(ctx, 8, [1100, 1100], 2, 64, 16, "bf16", layers=9)
+    f.cache.refs[f.cache.tables[0, 3].long()] += 1  # (before all of them)
+    assert accept_case(ctx, f.cache, [1024, 1024], None, p, [1023, 1000])[0] == 1023
+
+
 def test_accept_of_pages_that_are_not_there(ctx):
     f = Filled(ctx, 4, [100, 64], 2, 64, 16, "f16", layers=2)
     f.cache.tables[0, 5], f.cache.tables[1, 0] = -1, 1 << 28
