@@ -2,7 +2,7 @@
 
 The reference recomputes whole sequences in every forward (inference-engine/src/host/transformer_layer.cpp:211-230) and has no
 cache; this is what a caller needs to feed a model its new tokens only.  Everything stays on the device, the bookkeeping included: once a cache is made no
-call here waits for the GPU, and a step (reserve, then per layer append and attend) can be recorded into a HIP graph.
+call here waits for the GPU (but see DraftTree.order), and a step (reserve, then per layer append and attend) can be recorded into a HIP graph.
 
     cache = PagedCache(ctx, pimdl, layers=12, pages=4096, kv_heads=12, head_dim=64, page_tokens=16, dtype="f16", seqs=64, max_len=2048)
     cache.reserve(seqs, counts)                      # room for counts[i] more positions of sequence seqs[i]
@@ -25,6 +25,7 @@ Drafts: the new tokens of a sequence may be a tree of candidates.  A step over t
 """
 import ctypes
 import math
+import weakref
 
 import torch
 
@@ -137,12 +138,24 @@ class DraftTree:
         if not masks.is_contiguous() or not depths.is_contiguous() or masks.device != depths.device:
             raise ValueError("masks and depths must be contiguous and on one GPU")
         self.ctx, self.masks, self.depths = ctx, masks, depths
+        self._readers = weakref.WeakSet()  # contexts that have read it and that nothing orders with its own
         self._lib, self._desc = pimdl.lib(), pimdl.TreeDesc(masks.data_ptr(), depths.data_ptr(), masks.shape[1])
 
     def check_tokens(self, tokens):
         """Refuses batches of more tokens than there is room for."""
         if tokens > self.masks.shape[0]:
             raise ValueError(f"{tokens} tokens: the tree has room for {self.masks.shape[0]}")
+
+    def order(self, ctx):
+        """Before calls of `ctx` that read the tree: refuses a context that runs on another stream than the tree's, where one of them was given (set_stream).  Where each has its
+        own, which nobody else can order, the host waits, here for `build` and there for these calls."""
+        if ctx.in_order_with(self.ctx):
+            return
+        if ctx.stream is not None or self.ctx.stream is not None:
+            raise ValueError("the tree's context runs on another stream than the cache's: nothing orders their calls")
+        if self.ctx._h:  # (not closed)
+            self.ctx.synchronize()
+        self._readers.add(ctx)
 
     def build(self, parents, starts):
         """Token t, the (t - starts[b])-th node of row b's tree, follows node parents[t] of that tree, or, with -1, what the sequence has in the cache; a parent stands before
@@ -152,6 +165,10 @@ class DraftTree:
         if m < 1:
             raise ValueError("starts must hold one number more than there are sequences")
         self.check_tokens(n)
+        for ctx in self._readers:
+            if ctx._h:
+                ctx.synchronize()
+        self._readers.clear()
         self.ctx._check(self._lib.pimdl_tree_build(self.ctx._h, pa, at, m - 1, n, self._desc.words, self._desc.masks, self._desc.depths))
 
 
@@ -236,6 +253,7 @@ class PagedCache:
             depths = None
             if tree is not None:
                 tree.check_tokens(k.shape[0])
+                tree.order(self.ctx)
                 depths = tree._desc.depths
             heads = qa = qo = qs = qos = 0
             if q is not None:
@@ -267,6 +285,7 @@ class PagedCache:
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
         if tree is not None:
             tree.check_tokens(q.shape[0])
+            tree.order(self.ctx)
             self.ctx._check(self._lib.pimdl_attention_tree(self.ctx._h, self._of(layer), to, at, batch, q.shape[0], tree._desc, qa, oa, heads, qs, os_, qt, left, sinks, scale))
             return
         self.ctx._check(self._lib.pimdl_attention_paged(self.ctx._h, self._of(layer), to, at, batch, q.shape[0], qa, oa, heads, qs, os_, qt, left, sinks, scale))
@@ -301,6 +320,7 @@ class PagedCache:
         ka, m = _int_list(kept, "kept")
         if n != batch or m != batch:
             raise ValueError("last and kept must hold a number for each sequence of the batch")
+        tree.order(self.ctx)
         self.ctx._check(self._lib.pimdl_pages_accept(self.ctx._h, self._book, to, at, batch, tree.masks.shape[0], tree._desc, la, self._row_bytes, ka))
 
     def compact(self):

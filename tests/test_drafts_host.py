@@ -151,3 +151,49 @@ def test_a_configuration_with_a_rotation(tmp_path, rotary, fine):
 def test_a_model_without_a_rotation_reads_as_before():
     p = T.TransformerParams.from_yaml(os.path.join(os.path.dirname(__file__), "golden", "transformer_small.yaml"))
     assert p.rotary is None and T.TransformerLayer.rotary is None
+
+
+def named_context(calls, name, stream=None):
+    c = context(stream)
+    c._h = name  # (of a context that is not closed)
+    c.synchronize = lambda: calls.append(name)
+    return c
+
+
+def uses_of(c, tree):
+    q, at = torch.zeros(2, 256), ints(0, 1, 2)
+    c._row_bytes = 128
+    return (lambda: c.append(0, q, q, at, rotary=rotary_of(), tree=tree), lambda: c.attend(0, q, torch.zeros(2, 256), at, 4, tree=tree),
+            lambda: c.accept(tree, ints(0, -1), ints(0, 0), at))
+
+
+@pytest.mark.parametrize("mine,its", [(5, 6), (5, None), (None, 6)])
+def test_a_tree_on_another_stream_than_the_caches_is_refused(mine, its):
+    c = cache_of(context(mine))
+    for call in uses_of(c, tree_of(ctx=context(its))):
+        with pytest.raises(ValueError, match="another stream"):
+            call()
+    assert c._lib.calls == []
+    for call in uses_of(c, tree_of(ctx=context(mine) if mine else c.ctx)):
+        call()
+    assert c._lib.calls == ["pimdl_cache_append_rotary", "pimdl_attention_tree", "pimdl_pages_accept"]
+
+
+def test_a_tree_between_two_contexts_with_streams_of_their_own(recorder):
+    """Nobody else can order them: what reads the tree waits for what has filled it, and what fills it again for all that have read it."""
+    log = []
+    ours, other, its = (named_context(log, n) for n in ("ours", "other", "its"))
+    tree, a, b = tree_of(ctx=its), cache_of(ours), cache_of(other)
+    recorder.calls = a._lib.calls = b._lib.calls = log
+    for c in (a, b):
+        for call in uses_of(c, tree):
+            call()
+    reads = ["its", "pimdl_cache_append_rotary", "its", "pimdl_attention_tree", "its", "pimdl_pages_accept"]
+    assert log == reads * 2
+    log.clear()
+    tree.build(ints(-1, 0), ints(0, 2))
+    assert sorted(log[:2]) == ["other", "ours"] and log[2:] == ["pimdl_tree_build"]
+    log.clear()
+    tree.build(ints(-1, 0), ints(0, 2))  # (nobody has read it since)
+    uses_of(cache_of(its), tree)[1]()    # its own context's
+    assert log == ["pimdl_tree_build"]

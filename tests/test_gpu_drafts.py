@@ -984,6 +984,34 @@ def test_two_contexts_draft_on_two_streams(ctx):
         c.close()
 
 
+def test_a_tree_of_another_context(ctx):
+    """Filled by one context and read by another, each on a stream of its own, with another forest every time; contexts on given streams that differ are refused."""
+    one, two = pimdl.Context(0), pimdl.Context(0)
+    f, counts = Filled(two, 33, [3000, 1100], 2, 64, 16, "f16"), [60, 1000]
+    tree, q, starts = K.DraftTree(one, pimdl, 1060, most=1024), randn(gen_of(7), 1060, 8 * 64), starts_of(counts)
+    forests, outs = [forest(counts, i, width=1 + 3 * i) for i in range(6)], [torch.zeros_like(q) for _ in range(6)]
+    torch.cuda.synchronize()
+    for p, out in zip(forests, outs):
+        tree.build(p, starts)
+        f.cache.attend(0, q, out, starts, 8, tree=tree)
+    torch.cuda.synchronize()
+    mine = K.DraftTree(two, pimdl, 1060, most=1024)
+    for p, out in zip(forests, outs):
+        mine.build(p, starts)
+        again = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        f.cache.attend(0, q, again, starts, 8, tree=mine)
+        torch.cuda.synchronize()
+        assert torch.equal(out, again)
+    two.set_stream(torch.cuda.Stream().cuda_stream)
+    with pytest.raises(ValueError, match="another stream"):
+        f.cache.attend(0, q, outs[0], starts, 8, tree=tree)
+    two.close()
+    tree.build(forests[0], starts)  # (a reader that is gone)
+    torch.cuda.synchronize()
+    one.close()
+
+
 def test_drafts_beyond_four_gigabytes(ctx):
     """Pages whose offsets do not fit in 32 bits, of bytes or of elements: written turned, attended to, moved."""
     kv, hd, pt, pages = 2, 128, 16, 700_000  # 8 KiB a page of 16 bits: 5.7 GB
