@@ -529,7 +529,7 @@ PIMDL_API int pimdl_pages_copy(pimdl_ctx* ctx, const pimdl_page_book* book, cons
  * kept[b] is the branch's length.  A row is left as it is, with kept[b] = -1, where last[b] is no node of it or lacks its own bit in the masks, where it has more
  * nodes than the sequence has positions or the masks hold, where s is out of range or stands in the list before, where another sequence holds a page that would
  * be written or left partly filled (a fork made while the tree was there), and while *lacking is not 0, since the tree is not in the cache then.  kept overlaps none of the
- * inputs. */
+ * inputs.  Without tokens (all n are 0) there need be no masks. */
 PIMDL_API int pimdl_pages_accept(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_t* seqs, const int32_t* starts,
                                  uint32_t batch, uint32_t tokens, const pimdl_tree* tree, const int32_t* last, uint32_t row_bytes,
                                  int32_t* kept);

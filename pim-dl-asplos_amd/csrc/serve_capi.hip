@@ -378,7 +378,7 @@ int pimdl_pages_accept(pimdl_ctx* ctx, const pimdl_page_book* book, const int32_
     if (batch == 0) return PIMDL_OK;
     if (batch > 16384) return set_error(ctx, PIMDL_ERR_UNSUPPORTED, "%s: a list of %u (up to 16384)", fn, batch);
     if ((rc = check_batch(ctx, fn, starts, batch, tokens)) || (seqs && (rc = check_device(ctx, fn, "seqs", seqs, 4))) ||
-        (rc = check_device(ctx, fn, "masks", tree->masks, 4)) || (rc = check_device(ctx, fn, "last", last, 4)) || (rc = check_device(ctx, fn, "kept", kept, 4)))
+        (tokens && (rc = check_device(ctx, fn, "masks", tree->masks, 4))) || (rc = check_device(ctx, fn, "last", last, 4)) || (rc = check_device(ctx, fn, "kept", kept, 4)))
         return rc;
     // several workgroups read a row's numbers, and the first to be done writes kept
     for (const int32_t* in : {last, seqs, starts})

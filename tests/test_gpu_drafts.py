@@ -1103,6 +1103,18 @@ def test_calls_without_tokens_do_nothing(ctx):
     book.same(f.cache)
 
 
+def test_accept_of_a_tree_without_tokens(ctx):
+    """As for a tree with room whose rows are empty: nothing moves, 0 are kept, and a row that cannot be done is still told."""
+    f, none, kept = Filled(ctx, 50, [40, 9], 2, 64, 16, "f16"), starts_of([0, 0]), ints(7, 7)
+    book = Book(f.cache)
+    for tree in (K.DraftTree(ctx, pimdl, 0), K.DraftTree(ctx, pimdl, 0, most=1024)):
+        for last, seqs, want in (((-1, -1), None, [0, 0]), ((-1, -1), (1, 1), [0, -1]), ((-1, 0), (0, 1), [0, -1]), ((-1, -1), (0, 2), [0, -1])):
+            f.cache.accept(tree, ints(*last), kept, none, None if seqs is None else ints(*seqs))
+            torch.cuda.synchronize()
+            assert kept.tolist() == want
+            book.same(f.cache)
+
+
 # ---------------------------------------------------------------------------------------------- the transformer
 
 def rotated_model(ctx, hd, heads, layers, seq_len, batch, rotary, window=None, fused=False):
