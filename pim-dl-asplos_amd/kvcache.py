@@ -243,18 +243,19 @@ class PagedCache:
     def append(self, layer, k, v, starts, seqs=None, rotary=None, q=None, q_out=None, tree=None):
         """New tokens' keys and values [tokens][kv_heads * head_dim] into the last positions of their sequences (whose room `reserve` has made).  With `rotary`
         the keys are turned by those positions on the way, and queries q [tokens][heads * head_dim], if any, into q_out (which may be q); with `tree` by the
-        positions that their nodes have (the draft's first one, and the node's depth on top)."""
+        positions that their nodes have (the draft's first one, and the node's depth on top).  Without `rotary` a tree changes nothing here."""
         if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
             raise ValueError("k and v must have one shape, stride and type")
         ka, ks, kt = _packed(k, self.kv_heads * self.head_dim, "k")
         to, at, batch = self._batch(starts, seqs)
+        if tree is not None:
+            tree.check_tokens(k.shape[0])
+            tree.order(self.ctx)
         if rotary is not None:
             rotary.check_fits(self)
-            depths = None
-            if tree is not None:
-                tree.check_tokens(k.shape[0])
-                tree.order(self.ctx)
-                depths = tree._desc.depths
+            depths = None if tree is None else tree._desc.depths
+            if q is None and q_out is not None:
+                raise ValueError("q_out without q: there are no queries to turn")
             heads = qa = qo = qs = qos = 0
             if q is not None:
                 if q_out is None or q.shape != q_out.shape or q.dtype != k.dtype or q_out.dtype != k.dtype or q.shape[:1] != k.shape[:1]:
@@ -265,7 +266,7 @@ class PagedCache:
             self.ctx._check(self._lib.pimdl_cache_append_rotary(self.ctx._h, self._of(layer), to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt, rotary._desc, depths,
                                                                 qa, qo, heads, qs, qos))
             return
-        if q is not None:
+        if q is not None or q_out is not None:
             raise ValueError("queries are turned by a rotary: none is given")
         self.ctx._check(self._lib.pimdl_cache_append(self.ctx._h, self._of(layer), to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt))
 

@@ -197,3 +197,15 @@ def test_a_tree_between_two_contexts_with_streams_of_their_own(recorder):
     tree.build(ints(-1, 0), ints(0, 2))  # (nobody has read it since)
     uses_of(cache_of(its), tree)[1]()    # its own context's
     assert log == ["pimdl_tree_build"]
+
+
+def test_append_drops_no_argument_in_silence():
+    c, x, q, at = cache_of(context()), torch.zeros(2, 256), torch.zeros(2, 512), ints(0, 1, 2)
+    tree = tree_of(2, ctx=c.ctx)
+    for kw, text in ((dict(rotary=rotary_of(), q_out=q), "no queries"), (dict(q_out=q), "none is given"), (dict(tree=tree_of(1, ctx=c.ctx)), "room for 1"),
+                     (dict(tree=tree_of(2, ctx=context(5))), "another stream")):
+        with pytest.raises(ValueError, match=text):
+            c.append(0, x, x, at, **kw)
+    assert c._lib.calls == []
+    c.append(0, x, x, at, tree=tree)  # (a tree's keys have the places of any others)
+    assert c._lib.calls == ["pimdl_cache_append"]
