@@ -433,7 +433,7 @@ typedef enum pimdl_rotary_pairs {
     PIMDL_PAIRS_NEIGHBOURS = 1  /* column 2 i with 2 i + 1 */
 } pimdl_rotary_pairs;
 typedef struct pimdl_rotary {
-    const double* freqs;     /* DEVICE [dims / 2]: radians a position, finite */
+    const double* freqs;     /* DEVICE [dims / 2]: radians a position; times a position below 2^52 in magnitude (an angle of 64 bits says nothing beyond) */
     uint32_t dims;           /* even, 2 .. head_dim: a head's columns from there on are left as they are */
     uint32_t pairs;          /* pimdl_rotary_pairs */
 } pimdl_rotary;

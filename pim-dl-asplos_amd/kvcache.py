@@ -54,7 +54,7 @@ class Rotary:
     """Turns queries and keys by their positions: at position p the pair (a, b) of a head's columns that belongs to frequency f becomes
     (a cos pf - b sin pf, a sin pf + b cos pf).  The first `dims` columns of a head turn (all of them by default), column i with i + dims / 2 (pairs="halves") or 2 i with
     2 i + 1 ("neighbours").  Frequency i is base^(-2 i / dims), or freqs[i] (float64 [dims / 2] on the device, radians a position): scaled ones for
-    longer contexts, say."""
+    longer contexts, say.  A position times a frequency is below 2^52 (positions below 2^31: frequencies up to 2^21, a base of 2^-21 or more)."""
 
     def __init__(self, ctx, pimdl, head_dim, base=10000.0, dims=None, pairs="halves", freqs=None):
         if pairs not in pimdl.PAIRS:
@@ -63,8 +63,8 @@ class Rotary:
             dims = head_dim if dims is None else dims
             if dims % 2 or not 2 <= dims <= head_dim:
                 raise ValueError(f"dims={dims} must be even, 2 .. head_dim={head_dim}")
-            if not (0 < base < math.inf):
-                raise ValueError(f"base={base} must be positive and finite")
+            if not 2.0 ** -21 <= base < math.inf:
+                raise ValueError(f"base={base} must be finite and 2^-21 or more")
             freqs = torch.tensor([float(base) ** (-i / dims) for i in range(0, dims, 2)], dtype=torch.float64, device=torch.device("cuda", torch.cuda.current_device()))
         if freqs.dim() != 1 or freqs.dtype != torch.float64 or not freqs.is_contiguous() or not 2 <= 2 * freqs.shape[0] <= head_dim:
             raise ValueError(f"freqs must be a contiguous float64 vector of 1 to {head_dim // 2}")

@@ -86,8 +86,8 @@ class TransformerParams:
         """rotary as what kvcache.Rotary takes"""
         base, dims, pairs = self.rotary
         base, dims = float(base), self.head_dim if dims is None else operator.index(dims)
-        if not 0 < base < math.inf or dims % 2 or not 2 <= dims <= self.head_dim or pairs not in ("halves", "neighbours"):
-            raise ValueError(f"rotary={self.rotary}: a positive base, an even number of columns up to head_dim={self.head_dim}, and 'halves' or 'neighbours'")
+        if not 2.0 ** -21 <= base < math.inf or dims % 2 or not 2 <= dims <= self.head_dim or pairs not in ("halves", "neighbours"):
+            raise ValueError(f"rotary={self.rotary}: a base of 2^-21 or more, an even number of columns up to head_dim={self.head_dim}, and 'halves' or 'neighbours'")
         return {"base": base, "dims": dims, "pairs": pairs}
 
     @classmethod

@@ -209,3 +209,16 @@ def test_append_drops_no_argument_in_silence():
     assert c._lib.calls == []
     c.append(0, x, x, at, tree=tree)  # (a tree's keys have the places of any others)
     assert c._lib.calls == ["pimdl_cache_append"]
+
+
+@pytest.mark.parametrize("base", [5e-324, 1e-310, 1e-300, 2.0 ** -30, -1.0])
+def test_bases_whose_angles_are_lost_are_refused(base):
+    """Frequencies beyond 2^21 radians a position take angles to where neighbouring doubles are a radian and more apart."""
+    with pytest.raises(ValueError, match="base"):
+        K.Rotary(context(), pimdl, 128, base=base)
+    p = params(hd=128)
+    p.rotary = (base, None, "halves")
+    with pytest.raises(ValueError, match="base"):
+        p.turns()
+    p.rotary = (2.0 ** -21, None, "halves")
+    assert p.turns()["base"] ** (-126 / 128) < 2.0 ** 21
