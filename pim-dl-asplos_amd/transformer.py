@@ -84,10 +84,14 @@ class TransformerParams:
 
     def turns(self):
         """rotary as what kvcache.Rotary takes"""
-        base, dims, pairs = self.rotary
-        base, dims = float(base), self.head_dim if dims is None else operator.index(dims)
+        wrong = ValueError(f"rotary={self.rotary}: [base, dims, pairs], a base of 2^-21 or more, an even number of columns up to head_dim={self.head_dim}, and 'halves' or 'neighbours'")
+        try:
+            base, dims, pairs = self.rotary
+            base, dims = float(base), self.head_dim if dims is None else operator.index(dims)
+        except (TypeError, ValueError):
+            raise wrong from None
         if not 2.0 ** -21 <= base < math.inf or dims % 2 or not 2 <= dims <= self.head_dim or pairs not in ("halves", "neighbours"):
-            raise ValueError(f"rotary={self.rotary}: a base of 2^-21 or more, an even number of columns up to head_dim={self.head_dim}, and 'halves' or 'neighbours'")
+            raise wrong
         return {"base": base, "dims": dims, "pairs": pairs}
 
     @classmethod
@@ -102,9 +106,10 @@ class TransformerParams:
             left, right, sinks = net["attention_window"]
             p.window = (None if left is None else int(left), None if right is None else int(right), int(sinks))
             p.borders()
-        if "rotary" in net:  # [base, dims, pairs]; dims null: all of a head
-            p.rotary = tuple(net["rotary"])
+        if net.get("rotary") is not None:  # [base, dims, pairs]; dims null: all of a head
+            p.rotary = net["rotary"]
             p.turns()
+            p.rotary = tuple(p.rotary)
         if p.head_num * p.head_dim != p.token_dim:
             raise ValueError("head_num * head_dim != token_dim")
         dims = {"qkv": (p.token_dim, 3 * p.token_dim), "o": (p.token_dim, p.token_dim),

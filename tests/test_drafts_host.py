@@ -222,3 +222,16 @@ def test_bases_whose_angles_are_lost_are_refused(base):
         p.turns()
     p.rotary = (2.0 ** -21, None, "halves")
     assert p.turns()["base"] ** (-126 / 128) < 2.0 ** 21
+
+
+@pytest.mark.parametrize("rotary", [10000.0, "halves", [1e4, 8.0, "halves"], [1e4, "8", "halves"], [[1e4], 8, "halves"], [1e4, 8, ["halves"]], {"base": 1e4}, []])
+def test_a_configuration_without_a_rotation_or_with_none_that_can_be(tmp_path, rotary):
+    cfg = yaml.safe_load(open(os.path.join(os.path.dirname(__file__), "golden", "transformer_small.yaml")))
+    path = tmp_path / "r.yaml"
+    cfg["network_params"]["rotary"] = None  # null: no rotation, as if it were not there
+    path.write_text(yaml.safe_dump(cfg))
+    assert T.TransformerParams.from_yaml(path).rotary is None
+    cfg["network_params"]["rotary"] = rotary
+    path.write_text(yaml.safe_dump(cfg))
+    with pytest.raises(ValueError, match="rotary="):
+        T.TransformerParams.from_yaml(path)
