@@ -102,7 +102,7 @@ class TransformerParams:
         net, ker = cfg["network_params"], cfg["kernel_params"]
         p = cls(int(net["seq_len"]), int(net["batch_size"]), int(net["head_num"]), int(net["head_dim"]),
                 int(net["token_dim"]), int(net["ffn_hidden_dim"]), int(net["layer_num"]))
-        if "attention_window" in net:  # [left, right, sinks]; null: no border on that side
+        if net.get("attention_window") is not None:  # [left, right, sinks]; null: no border on that side
             left, right, sinks = net["attention_window"]
             p.window = (None if left is None else int(left), None if right is None else int(right), int(sinks))
             p.borders()

@@ -188,6 +188,14 @@ def test_a_configuration_with_a_window_out_of_range_is_refused(tmp_path):
                 T.TransformerParams.from_yaml(path)
 
 
+def test_a_configuration_whose_window_is_null_has_none(tmp_path):
+    cfg = yaml.safe_load(open(os.path.join(os.path.dirname(__file__), "golden", "transformer_small.yaml")))
+    cfg["network_params"]["attention_window"] = None
+    path = tmp_path / "w.yaml"
+    path.write_text(yaml.safe_dump(cfg))
+    assert T.TransformerParams.from_yaml(path).window is None
+
+
 @pytest.mark.parametrize("layer", [-1, -2, 2, 7])
 def test_layers_that_are_not_there_are_refused(layer):
     c, x = cache_of(context()), torch.zeros(2, 256)
