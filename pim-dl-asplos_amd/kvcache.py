@@ -254,7 +254,7 @@ class PagedCache:
         if rotary is not None:
             rotary.check_fits(self)
             depths = None if tree is None else tree._desc.depths
-            if q is None and q_out is not None:
+            if q is None and q_out is not None and q_out.numel():  # (one without columns takes none)
                 raise ValueError("q_out without q: there are no queries to turn")
             heads = qa = qo = qs = qos = 0
             if q is not None:
@@ -266,7 +266,7 @@ class PagedCache:
             self.ctx._check(self._lib.pimdl_cache_append_rotary(self.ctx._h, self._of(layer), to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt, rotary._desc, depths,
                                                                 qa, qo, heads, qs, qos))
             return
-        if q is not None or q_out is not None:
+        if q is not None or (q_out is not None and q_out.numel()):
             raise ValueError("queries are turned by a rotary: none is given")
         self.ctx._check(self._lib.pimdl_cache_append(self.ctx._h, self._of(layer), to, at, batch, k.shape[0], ka, v.data_ptr(), ks, kt))
 

@@ -208,7 +208,8 @@ def test_append_drops_no_argument_in_silence():
             c.append(0, x, x, at, **kw)
     assert c._lib.calls == []
     c.append(0, x, x, at, tree=tree)  # (a tree's keys have the places of any others)
-    assert c._lib.calls == ["pimdl_cache_append"]
+    c.append(0, x, x, at, rotary=rotary_of(), q_out=q[:, :0])  # (no columns: nothing is dropped)
+    assert c._lib.calls == ["pimdl_cache_append", "pimdl_cache_append_rotary"]
 
 
 @pytest.mark.parametrize("base", [5e-324, 1e-310, 1e-300, 2.0 ** -30, -1.0])
