@@ -11,24 +11,10 @@
 // instructions, a third of them for the second piece of p, 142.  These are at work in 39 % of the SIMDs' cycles, others in 44 %, and mostly not at once: a product leaves the vector unit
 // to others for a part of its time only, 57 cycles for a product of 32 and its share of 9 others.  Shares end within 5 % of each other; a block's own 10 us come twice in most.
 #pragma once
+#include "attn_deal_units.h"
 
 namespace pimdl {
 namespace attn {
-
-constexpr uint32_t DEAL_BATCH = 512;  // rows of the batch that fit
-// Units are a 14th of the time that a tile takes with 256 rows.  Measured, 40 sequences with blocks of 2 to 8 groups of 32 rows each, us a tile: of 64 keys 1.86, 2.13, 2.19, 2.57, 2.81,
-// 3.32, 3.54 (bf16, 128 dims), 1.11, 1.46, 1.53, 1.83, 1.91, 2.40, 2.47 (fp16, 64), 2.35, 3.08, 3.31, 4.00, 4.33, 5.44, 5.72 (fp32, 64); of 32 keys, which waves do not share, 2.25, 2.41, 2.54,
-// 3.30, 3.58, 3.72, 3.95 (fp32, 80), 3.18, 3.35, 3.59 (fp32, 128).
-template <int TILE>
-__device__ __forceinline__ uint32_t tile_units(uint32_t groups)
-{
-    if (TILE == 64) return groups + (groups > 6 ? 6 : 5);
-    return groups <= 4 ? 8 + groups / 3 : 10 + groups / 2;
-}
-constexpr uint32_t TILE_MOST = 8;     // units of a tile for each of a block's groups, at most
-constexpr uint32_t DEAL_BLOCK = 36;   // units of a block without its tiles: its queries, the first keys' way and the results (10 to 12, 5.5 to 7.4, 8 to 10, 7 to 9 and 6 to 9 us)
-constexpr uint32_t DEAL_SHORT = 64;   // units of tiles up to which a block is not worth cutting
-constexpr uint32_t DEAL_LEAST = 48;   // units of a share, at least
 
 // What the shares of one call leave: share w's sums of a block that began in an earlier share in slot 2 w, of one that goes on in a later share in slot 2 w + 1.
 struct DealPart {
@@ -88,37 +74,13 @@ struct Deal {
 inline uint32_t deal_rows(bool alone) { return alone ? 128 : 256; }
 inline int32_t deal_tile(bool fp32_keys, uint32_t head_dim) { return fp32_keys && head_dim > 64 ? 32 : 64; }
 
-// Row b of the batch: blocks of its rows, equal ones as near as groups of 32 allow, and tiles of keys (a block without keys has one, so that somebody writes its zeros)
-struct DealRow {
-    uint32_t blocks, rows, tiles;  // rows: of a block but the last
-    uint32_t whole, last;          // units of a tile of a block, and of the last one
-    __device__ __forceinline__ uint32_t block_units(uint32_t each) const { return DEAL_BLOCK + each * tiles; }
-    __device__ __forceinline__ uint32_t units() const { return blocks ? (blocks - 1) * block_units(whole) + block_units(last) : 0; }  // of a key head
-};
 template <typename C>
 __device__ __forceinline__ DealRow deal_row(const AttnArgs& a, const Row& r)
 {
     typedef Deal<C> D;
-    DealRow d = {0, D::ROWS, 1, 1, 1};
-    if (r.n == 0) return d;
-    const uint32_t rows = r.n * a.group, groups = (rows + 31) / 32;
-    const int32_t tiles = span_of<true>(a, r, 0, rows - 1, D::TILE).total;
-    d.blocks = (rows + D::ROWS - 1) / D::ROWS;
-    const uint32_t each = (groups + d.blocks - 1) / d.blocks;
-    d.blocks = (groups + each - 1) / each;  // (the last ones may have come out empty)
-    d.rows = 32 * each;
-    d.tiles = (uint32_t)(tiles > 0 ? tiles : 1);
-    d.whole = tile_units<D::TILE>(each);
-    d.last = tile_units<D::TILE>(groups - (d.blocks - 1) * each);
-    return d;
-}
-
-// Sums of units end at 2^31 - 1, which the host makes sure that rows with tokens of their own do not reach: starts that fall again, so that rows share tokens, could, and
-// the last rows get nothing then.
-__device__ __forceinline__ uint32_t add_units(uint32_t x, uint32_t y)
-{
-    const uint32_t sum = x + y;
-    return sum < 0x7fffffffu ? sum : 0x7fffffffu;
+    if (r.n == 0) return {0, D::ROWS, 1, 1, 1};
+    const uint32_t rows = r.n * a.group;
+    return deal_row_of<D::TILE>(rows, D::ROWS, span_of<true>(a, r, 0, rows - 1, D::TILE).total);
 }
 
 // Looks at every row of the batch (up to DEAL_BATCH, a thread each); returns all units.
@@ -166,12 +128,6 @@ __device__ __forceinline__ uint32_t deal_units(const AttnArgs& a, typename Deal<
     if (tid == 0) sh.unit[a.batch] = total;
     __syncthreads();
     return total;
-}
-
-__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t shares)
-{
-    const uint32_t s = (total + shares - 1) / shares;
-    return s > DEAL_LEAST ? s : DEAL_LEAST;
 }
 
 // What a wave does with 32 keys, in two stretches of matrix instructions, each of which takes the time of several others: the scores of the NEXT 32 keys while
@@ -491,15 +447,10 @@ __global__ __launch_bounds__(Deal<C>::THREADS, Deal<C>::WAVES / 4) void attentio
         r.table = a.tables + (size_t)(r.length > 0 ? seq : 0) * a.table_width;  // (read where there are keys)
         const DealRow d = deal_row<C>(a, r);
         // the block that `unit` lies in, its first unit and those of its tiles
-        const uint32_t head_units = d.units(), of_row = __builtin_amdgcn_readfirstlane(sh.unit[b]), at = unit - of_row, kh = at / head_units, in_head = at - kh * head_units;
-        const uint32_t guess = in_head / d.block_units(d.whole), block = guess < d.blocks - 1 ? guess : d.blocks - 1;
-        const uint32_t each = block == d.blocks - 1 ? d.last : d.whole, begin = of_row + kh * head_units + block * d.block_units(d.whole), end_unit = begin + d.block_units(each);
-        // a tile is the share's that its first unit lies in, a short block's are all with the first one
-        const uint32_t first = begin + DEAL_BLOCK, step = each * d.tiles <= DEAL_SHORT ? each * d.tiles : each;
-        const uint32_t from_tile = unit > first ? (unit - first + step - 1) / step : 0, to_tile = stop > first ? (stop - first + step - 1) / step : 0;
-        const uint32_t tiles = step == each ? d.tiles : 1;
-        const int32_t most = (int32_t)d.tiles, from = from_tile < tiles ? (int32_t)from_tile : most, to = to_tile < tiles ? (int32_t)to_tile : most;
-        unit = end_unit < stop ? end_unit : stop;
+        const DealPiece p = deal_piece(d, __builtin_amdgcn_readfirstlane(sh.unit[b]), unit, stop);
+        const uint32_t kh = p.kh, block = p.block;
+        const int32_t most = (int32_t)d.tiles, from = p.from, to = p.to;
+        unit = p.end < stop ? p.end : stop;
         if (from >= to) continue;
         const uint32_t rows = r.n * a.group, row0 = block * d.rows, end = row0 + d.rows < rows ? row0 + d.rows : rows;
         const Duty duty = duty_of<C>(wave, (end - row0 + 31) / 32);
@@ -542,8 +493,7 @@ __global__ __launch_bounds__(Deal<C>::THREADS, Deal<C>::WAVES / 4) void attentio
             }
         }
         if (tid == 0 && from == 0 && to < most) {
-            const uint32_t last = (first + each * (d.tiles - 1)) / per;
-            part.joins[2 * share] = (u32x4){(last < gridDim.x ? last : gridDim.x - 1) - share + 1, end - row0, 0, 0};  // (behind the last one: see add_units)
+            part.joins[2 * share] = (u32x4){deal_shares(p, d.tiles, per, share, gridDim.x), end - row0, 0, 0};
             part.joins[2 * share + 1] = (u32x4){r.first, row0, kh, 0};
         }
     }

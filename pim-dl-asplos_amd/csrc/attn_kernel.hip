@@ -457,8 +457,8 @@ int make_plan(Ctx* ctx, const AttnArgs& a, attn::Plan* p)
     const uint64_t tiles_a_cu = (rows / 256 + a.batch) * a.kv_heads * (keys / 64 + 1) * (a.cache_dtype == PIMDL_F32 ? 4 : 1) / cus;
     if (a.masks && p->wide && a.batch <= attn::DEAL_BATCH && rows > 32ull * a.batch && tiles_a_cu >= 16) {
         const bool alone = (a.cache_dtype == PIMDL_F32 && a.head_dim > 80) || (a.dtype == PIMDL_F32 && a.head_dim > 96);  // (as PER_CU)
-        const uint64_t block_rows = attn::deal_rows(alone), groups = rows / 32 + a.batch;  // (of 32 rows, at most)
-        const uint64_t most_units = groups * a.kv_heads * (attn::TILE_MOST * (((uint64_t)a.table_width << a.page_shift) / attn::deal_tile(a.cache_dtype == PIMDL_F32, a.head_dim) + 1) + attn::DEAL_BLOCK);
+        const uint64_t block_rows = attn::deal_rows(alone);
+        const uint64_t most_units = attn::deal_most_units(rows, a.batch, a.kv_heads, (uint64_t)a.table_width << a.page_shift, attn::deal_tile(a.cache_dtype == PIMDL_F32, a.head_dim));
         if (most_units < 1ull << 31) {
             p->deal = (uint32_t)std::min<uint64_t>(cus, (most_units + attn::DEAL_LEAST - 1) / attn::DEAL_LEAST);
             p->deal_rows = (uint32_t)block_rows;
