@@ -285,7 +285,8 @@ def prepare(case, seed):
 # ------------------------------------------------------------------------------------------------ one pass
 
 def _ctx():
-    """One context for the process, on torch's stream, as a serving program holds it."""
+    """One context for the process, as a serving program holds it: on the stream that torch is on at the first pass, on which the program stays.  Torch's default stream has no
+    handle (0), and the context keeps its own stream then, which takes turns with the default one: so a pass that changes from torch's work to the library's, or back, waits for it."""
     global _package, _context, _pages
     if _context is None:
         root = os.getcwd()
