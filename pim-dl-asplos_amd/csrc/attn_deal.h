@@ -7,8 +7,8 @@
 // sequence's number of units and a sum over them.  A block that one share holds whole is written at once; of others every share leaves its sums, which
 // attention_deal_join_kernel joins.
 //
-// 32 sequences of 16 to 64 nodes over up to 8191 keys, 32 heads over 8 of 128 dims, bf16: 226 us at full clock, 250 once its power has brought that down; 574 MB alone would be 121 us, the matrix
-// instructions, a third of them for the second piece of p, 142.  These are at work in 39 % of the SIMDs' cycles, others in 44 %, and mostly not at once: a product leaves the vector unit
+// 32 sequences of 16 to 64 nodes over up to 8191 keys, 32 heads over 8 of 128 dims, bf16: 210 us once the clock has settled, after some hundred launches on end, 259 in the median of the first 40;
+// 574 MB alone would be 121 us, the matrix instructions, a third of them for the second piece of p, 142.  These are at work in 39 % of the SIMDs' cycles, others in 44 %, and mostly not at once: a product leaves the vector unit
 // to others for a part of its time only, 57 cycles for a product of 32 and its share of 9 others.  Shares end within 5 % of each other; a block's own 10 us come twice in most.
 #pragma once
 #include "attn_deal_units.h"
